@@ -246,6 +246,51 @@ typedef struct opure_attn_args {
 
 int opure_attn_decode_paged(opure_dev* dev, const opure_attn_args* a);
 
+/* ---- attention with a sliding window and sinks over the same paged cache.
+ *      Row j of sequence b, at position p = seq_len[b] + j, sees the positions
+ *      t <= p with t < sinks or t > p - window (window 0: every t <= p, as
+ *      opure_attn_decode_paged).  One row or a few a sequence (decoding, a
+ *      verify step) and a prompt's rows take the same call: rows up to
+ *      OPURE_MAX_PROMPT_ROWS, batch up to OPURE_MAX_BATCH_ROWS, every format
+ *      and head size of opure_attn_decode_paged.
+ *        What a row does not see does not reach it: masked K and V may hold
+ *      anything, NaN and infinities included, and pages that no row of a
+ *      sequence sees may be missing (-1), so a cache that only grows can
+ *      release them.  A page that a row sees and that is missing makes the row
+ *      NaN; a row whose every visible score is -inf gives 0.
+ *        `weights` (or NULL) accumulates what the positions got:
+ *      weights[b][h][t] += the softmax weights of position t summed over the
+ *      rows and the query heads of KV head h, in fp32 and in a fixed order
+ *      (positions that no row sees are left as they are).  Those sums are what
+ *      opure_kv_evict goes by; one layer's part of its [batch][n_layers]
+ *      [n_kv_heads][stride] array is weights + layer * n_kv_heads * stride with
+ *      weights_batch_stride = n_layers * n_kv_heads * stride.
+ *        pool and q are 16-byte aligned, out 8-byte.  The order of sums follows
+ *      the shape of the call (batch, rows, max_ctx, window, sinks and whether
+ *      there are weights): the same call gives the same bits, a row alone and
+ *      in a batch may differ in its last ones. */
+typedef struct opure_attn_window_args {
+    const opure_model* model; /* n_layers, n_heads, n_kv_heads, head_dim, attn_scale, afmt */
+    const opure_kv*    kv;
+    uint32_t           layer;
+    uint32_t           batch, rows;
+    const int32_t*     seq_len;     /* device [batch] */
+    uint32_t           max_ctx;     /* host upper bound on seq_len[b] + rows */
+    uint32_t           window;      /* positions a row sees up to its own, which counts; 0 = all */
+    uint32_t           sinks;       /* first positions that stay visible */
+    const void*        q;           /* [batch*rows][n_heads*head_dim] in afmt */
+    void*              out;         /* like q */
+    float*             weights;     /* device, or NULL */
+    uint32_t           weights_stride;        /* floats between KV heads, >= max_ctx */
+    uint64_t           weights_batch_stride;  /* floats between sequences */
+} opure_attn_window_args;
+
+/* Sizes the device's workspace for such a call (the pointers seq_len, q, out
+ * are not read; weights counts as wanted when not NULL); call it before
+ * capturing one into a graph. */
+int opure_attn_window_reserve(opure_dev* dev, const opure_attn_window_args* a);
+int opure_attn_window_paged(opure_dev* dev, const opure_attn_window_args* a);
+
 /* ---- acceptance ------------------------------------------------------- */
 /* Greedy: argmax per row (ties -> lowest index; the reference's ArgMaxMain,
  * Opure_ArgMax.usf:33-86, re-specified), longest matching draft prefix, then
@@ -328,6 +373,48 @@ typedef struct opure_rollback_args {
 } opure_rollback_args;
 
 int opure_kv_rollback(opure_dev* dev, const opure_rollback_args* a);
+
+/* ---- eviction from the paged cache by accumulated attention weight, in
+ *      place.  A sequence of n = seq_len[b] positions keeps sinks + recent +
+ *      heavy of them (all of them when it has no more): in every layer and KV
+ *      head its first `sinks`, its last `recent`, and of the others the `heavy`
+ *      with the largest scores of that layer and head (ties: the lowest
+ *      position; a NaN counts as larger than every number, -0 as 0).  The kept
+ *      positions move up, in order, to slots 0, 1, ...; layers and heads keep
+ *      different positions, and all the same number of them.
+ *        With `turn`, a key that moves from slot s to slot i is turned back by
+ *      RoPE over s - i positions (the model's table at row s - i, in fp32,
+ *      rounded once to the cache's format), so the kept keys stand at their new
+ *      positions and a verify or prompt step goes on at seq_len = new_seq_len.
+ *      That needs a table whose angles grow in proportion to the position and
+ *      rope_max_pos >= max_ctx.  Without it keys move as they are.
+ *        With `freed`, pages wholly past the kept positions are released as
+ *      opure_kv_rollback does (entry -> -1, id to freed[b][...]); without, they
+ *      stay in the row for the tokens to come.  A page that is missing among
+ *      the seq_len positions is OPURE_E_CAPACITY at the next sync, as is a
+ *      length past max_ctx or the table; what such a sequence's cache and
+ *      outputs then hold is not defined, but no access leaves the buffers. */
+typedef struct opure_evict_args {
+    const opure_model* model;        /* n_layers, n_kv_heads, head_dim, afmt; turn: rope_cos, rope_sin, rope_max_pos */
+    const opure_kv*    kv;           /* kv->page_table is updated in place (freed) */
+    uint32_t           batch;
+    const int32_t*     seq_len;      /* device [batch] */
+    uint32_t           max_ctx;      /* host upper bound on seq_len[b] */
+    const float*       scores;       /* device [batch][n_layers][n_kv_heads][scores_stride] */
+    uint32_t           scores_stride;/* floats, >= max_ctx */
+    uint32_t           sinks, recent, heavy;
+    uint32_t           turn;
+    int32_t*           kept;         /* device [batch][n_layers][n_kv_heads][sinks+recent+heavy]: the old positions
+                                      * in order, -1 after */
+    float*             scores_out;   /* the kept positions' scores in the layout of scores, 0 from there to seq_len;
+                                      * may be scores itself; or NULL */
+    int32_t*           new_seq_len;  /* device [batch], may be seq_len itself */
+    int32_t*           freed;        /* [batch][freed_stride] or NULL */
+    uint32_t           freed_stride; /* >= ceil(max_ctx / OPURE_PAGE_SIZE) */
+    int32_t*           n_freed;      /* [batch] or NULL */
+} opure_evict_args;
+
+int opure_kv_evict(opure_dev* dev, const opure_evict_args* a);
 
 /* ---- one verify step: embedding, every layer (RMSNorm -> fused QKV GEMV
  *      with RoPE and paged KV append -> paged attention -> o_proj + residual

@@ -116,6 +116,23 @@ bool prof_kernel_events(opure_dev* dev, hipEvent_t* start, hipEvent_t* stop);
 inline uint64_t align_up(uint64_t v, uint64_t a) { return (v + a - 1) / a * a; }
 inline uint32_t act_bytes(uint32_t afmt) { return afmt == OPURE_A_F32 ? 4u : 2u; }
 
+// The device handle's GPU as the current one for the length of a call: a
+// caller whose thread works on another GPU gets its own back.
+struct DeviceGuard {
+    int before = -1;
+    explicit DeviceGuard(const opure_dev* dev)
+    {
+        int now = -1;
+        if (hipGetDevice(&now) == hipSuccess && now != dev->ordinal && hipSetDevice(dev->ordinal) == hipSuccess) before = now;
+    }
+    ~DeviceGuard()
+    {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+    DeviceGuard(const DeviceGuard&) = delete;
+    DeviceGuard& operator=(const DeviceGuard&) = delete;
+};
+
 #define OPURE_HIP_TRY(expr)                                                  \
     do {                                                                     \
         hipError_t _e = (expr);                                              \

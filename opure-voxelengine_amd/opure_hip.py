@@ -73,6 +73,14 @@ class AttnArgs(C.Structure):
                 ("max_ctx", C.c_uint32), ("q", C.c_void_p), ("out", C.c_void_p)]
 
 
+class AttnWindowArgs(C.Structure):
+    _fields_ = [("model", C.POINTER(Model)), ("kv", C.POINTER(KV)), ("layer", C.c_uint32),
+                ("batch", C.c_uint32), ("rows", C.c_uint32), ("seq_len", C.c_void_p),
+                ("max_ctx", C.c_uint32), ("window", C.c_uint32), ("sinks", C.c_uint32), ("q", C.c_void_p),
+                ("out", C.c_void_p), ("weights", C.c_void_p), ("weights_stride", C.c_uint32),
+                ("weights_batch_stride", C.c_uint64)]
+
+
 class AcceptArgs(C.Structure):
     _fields_ = [("batch", C.c_uint32), ("k", C.c_uint32), ("vocab", C.c_uint32),
                 ("target_logits", C.c_void_p), ("draft_logits", C.c_void_p), ("drafts", C.c_void_p),
@@ -92,6 +100,15 @@ class RollbackArgs(C.Structure):
                 ("seq_len", C.c_void_p), ("accepted", C.c_void_p), ("new_seq_len", C.c_void_p),
                 ("freed", C.c_void_p), ("freed_stride", C.c_uint32), ("n_freed", C.c_void_p),
                 ("poison", C.c_uint32), ("poison_bits", C.c_uint32)]
+
+
+class EvictArgs(C.Structure):
+    _fields_ = [("model", C.POINTER(Model)), ("kv", C.POINTER(KV)), ("batch", C.c_uint32),
+                ("seq_len", C.c_void_p), ("max_ctx", C.c_uint32), ("scores", C.c_void_p),
+                ("scores_stride", C.c_uint32), ("sinks", C.c_uint32), ("recent", C.c_uint32),
+                ("heavy", C.c_uint32), ("turn", C.c_uint32), ("kept", C.c_void_p), ("scores_out", C.c_void_p),
+                ("new_seq_len", C.c_void_p), ("freed", C.c_void_p), ("freed_stride", C.c_uint32),
+                ("n_freed", C.c_void_p)]
 
 
 class VerifyArgs(C.Structure):
@@ -149,12 +166,15 @@ def _declare(L):
         "opure_gemv_batched_i8pc": ([vp, C.POINTER(GemvArgs)], i),
         "opure_gemv_batched_i4g128": ([vp, C.POINTER(GemvArgs)], i),
         "opure_attn_decode_paged": ([vp, C.POINTER(AttnArgs)], i),
+        "opure_attn_window_reserve": ([vp, C.POINTER(AttnWindowArgs)], i),
+        "opure_attn_window_paged": ([vp, C.POINTER(AttnWindowArgs)], i),
         "opure_accept_greedy": ([vp, C.POINTER(AcceptArgs)], i),
         "opure_accept_rejection": ([vp, C.POINTER(AcceptArgs)], i),
         "opure_accept_rejection_noalloc": ([vp, C.POINTER(AcceptArgs)], i),
         "opure_sample_rows": ([vp, C.POINTER(SampleArgs)], i),
         "opure_philox_uniform": ([vp, u64, vp, vp, u32, u32, vp], i),
         "opure_kv_rollback": ([vp, C.POINTER(RollbackArgs)], i),
+        "opure_kv_evict": ([vp, C.POINTER(EvictArgs)], i),
         "opure_verify_reserve": ([vp, C.POINTER(Model), u32, u32, u32], i),
         "opure_verify_step": ([vp, C.POINTER(VerifyArgs)], i),
         "opure_verify_layer": ([vp, C.POINTER(VerifyLayerArgs)], i),
