@@ -30,6 +30,7 @@ struct EvictParams {
     const float* cos;
     const float* sin;
     uint32_t n_layers, n_kv, hd, n_pages, max_pages, afmt, scores_stride, sinks, recent, heavy, keep, freed_stride, cap;
+    uint32_t new_len_now;         // no k_evict_finish follows: the selection writes the new lengths
     uint32_t* err;
 };
 
@@ -47,95 +48,144 @@ __device__ __forceinline__ uint32_t score_key(float f)
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Sums over 1,024 threads in thread order: the sum of those before this one,
-// and of all.
-__device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t* wsum, uint32_t& all)
+// Sums over 1,024 threads in thread order of two counts, packed low and high:
+// those before this thread's, and all.
+__device__ __forceinline__ uint64_t block_prefix(uint64_t v, uint64_t* wsum, uint64_t& all)
 {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    uint32_t x = v;
+    uint64_t x = v;
 #pragma unroll
     for (uint32_t o = 1; o < 64u; o <<= 1)
     {
-        const uint32_t y = __shfl_up(x, o);
+        const uint64_t y = __shfl_up(x, o);
         if (lane >= o) x += y;
     }
     __syncthreads();                                       // wsum of the call before is read
     if (lane == 63u) wsum[wave] = x;
     __syncthreads();
-    uint32_t before = 0;
+    uint64_t before = 0;
     all = 0;
 #pragma unroll
     for (uint32_t w = 0; w < 16u; ++w)
     {
-        const uint32_t s = wsum[w];
+        const uint64_t s = wsum[w];
         before += w < wave ? s : 0u;
         all += s;
     }
     return before + x - v;
 }
 
-// The kept positions of one (sequence, layer, KV head): the `heavy`-th largest
-// key by four counts of 8 bits each, then the positions above it and, from the
-// lowest on, as many equal to it as are missing, written in order.
+// The kept positions of one (sequence, layer, KV head).  First the `heavy`-th
+// largest key, by counts of its leading 11, next 11 and last 10 bits; then the
+// positions above it and, from the lowest on, as many equal to it as are
+// missing, in order.  A thread holds 8 consecutive scores in registers, so up to
+// 8,192 positions are read once and ordered by one prefix sum.
+constexpr uint32_t SEL = 8, SEL_BLOCK = 1024u * SEL;
+
 __global__ __launch_bounds__(1024) void k_evict_select(EvictParams p)
 {
-    __shared__ uint32_t hist[256], wsum[16], pick[2];
+    __shared__ uint32_t hist[2048], pick[2];
+    __shared__ uint64_t wsum[16];
     const uint32_t b = blockIdx.y, tid = threadIdx.x;
     const uint64_t plane = static_cast<uint64_t>(b) * p.n_layers * p.n_kv + blockIdx.x;
     const int32_t raw = p.seq_len[b];
     const uint32_t n = evict_len(p, b);
-    if (tid == 0u && blockIdx.x == 0u && (raw < 0 || static_cast<uint32_t>(raw) > p.cap)) p.err[ERR_POSITION] = 1u;
     const float* sc = p.scores + plane * p.scores_stride;
     int32_t* kept = p.kept + plane * p.keep;
     const uint32_t lo = p.sinks, hi = n > p.keep ? n - p.recent : 0u;   // candidates lo .. hi - 1
     const uint32_t count = min(n, p.keep);
+    if (tid == 0u && blockIdx.x == 0u)
+    {
+        if (raw < 0 || static_cast<uint32_t>(raw) > p.cap) p.err[ERR_POSITION] = 1u;
+        if (p.new_len_now)
+        {
+            p.new_len[b] = static_cast<int32_t>(count);
+            if (p.n_freed) p.n_freed[b] = 0;
+        }
+    }
     if (n <= p.keep)
     {
         for (uint32_t i = tid; i < p.keep; i += 1024u) kept[i] = i < n ? static_cast<int32_t>(i) : -1;
     }
     else
     {
-        uint32_t prefix = 0, need = p.heavy;               // the key's leading bits so far; how many still of its group
-        if (p.heavy)
-            for (int shift = 24; shift >= 0; shift -= 8)
+        uint32_t key[SEL];
+        auto load = [&](uint32_t t0) {
+#pragma unroll
+            for (uint32_t u = 0; u < SEL; ++u)
             {
-                if (tid < 256u) hist[tid] = 0u;
-                __syncthreads();
-                const uint32_t mask = shift == 24 ? 0u : 0xFFFFFFFFu << (shift + 8);
-                for (uint32_t t = lo + tid; t < hi; t += 1024u)
-                {
-                    const uint32_t k = score_key(sc[t]);
-                    if ((k & mask) == prefix) atomicAdd(&hist[(k >> shift) & 255u], 1u);
-                }
-                __syncthreads();
-                // how many keys of the group lie above each bin, from the top
-                uint32_t all;
-                const uint32_t h = tid < 256u ? hist[255u - tid] : 0u;
-                const uint32_t above = block_prefix(h, wsum, all);
-                if (tid < 256u && above < need && above + h >= need)
-                {
-                    pick[0] = 255u - tid;
-                    pick[1] = need - above;
-                }
-                __syncthreads();
-                prefix |= pick[0] << shift;
-                need = pick[1];
-                __syncthreads();
+                const uint32_t t = t0 + tid * SEL + u;
+                key[u] = t >= lo && t < hi ? score_key(sc[t]) : 0u;
             }
-        uint32_t out = 0, equal = 0;                       // kept so far; equal keys so far
-        for (uint32_t t0 = 0; t0 < n; t0 += 1024u)
+        };
+        load(0u);
+        uint32_t prefix = 0, need = p.heavy;               // the key's leading bits so far; how many still of its group
+        for (uint32_t step = 0; step < 3u && p.heavy; ++step)
         {
-            const uint32_t t = t0 + tid;
-            const bool fixed = t < n && (t < lo || t >= hi);
-            const uint32_t k = t >= lo && t < hi ? score_key(sc[t]) : 0u;
-            const bool cand = t >= lo && t < hi && p.heavy != 0u, eq = cand && k == prefix;
-            uint32_t all_eq, all;
-            const uint32_t eq_before = block_prefix(eq ? 1u : 0u, wsum, all_eq);
-            const bool stay = fixed || (cand && k > prefix) || (eq && equal + eq_before < need);
-            const uint32_t at = block_prefix(stay ? 1u : 0u, wsum, all);
-            if (stay) kept[out + at] = static_cast<int32_t>(t);
-            out += all;
-            equal += all_eq;
+            const uint32_t shift = step == 0u ? 21u : step == 1u ? 10u : 0u, bins = step == 2u ? 1024u : 2048u;
+            const uint32_t mask = step == 0u ? 0u : 0xFFFFFFFFu << (step == 1u ? 21u : 10u);
+            for (uint32_t i = tid; i < bins; i += 1024u) hist[i] = 0u;
+            __syncthreads();
+            for (uint32_t t0 = 0; t0 < hi; t0 += SEL_BLOCK)
+            {
+                if (n > SEL_BLOCK) load(t0);
+#pragma unroll
+                for (uint32_t u = 0; u < SEL; ++u)
+                {
+                    const uint32_t t = t0 + tid * SEL + u;
+                    if (t >= lo && t < hi && (key[u] & mask) == prefix) atomicAdd(&hist[(key[u] >> shift) & (bins - 1u)], 1u);
+                }
+            }
+            __syncthreads();
+            // how many keys of the group lie above each bin, from the top: two bins a thread, or one
+            const uint32_t per = bins / 1024u, top = bins - 1u - tid * per;
+            const uint32_t h0 = hist[top], h1 = per > 1u ? hist[top - 1u] : 0u;
+            uint64_t all;
+            const uint32_t above = static_cast<uint32_t>(block_prefix(h0 + h1, wsum, all));
+            if (above < need && above + h0 >= need)
+            {
+                pick[0] = top;
+                pick[1] = need - above;
+            }
+            else if (above + h0 < need && above + h0 + h1 >= need)
+            {
+                pick[0] = top - 1u;
+                pick[1] = need - above - h0;
+            }
+            __syncthreads();
+            prefix |= pick[0] << shift;
+            need = pick[1];
+            __syncthreads();
+        }
+        uint32_t out = 0, equal = 0;                       // kept and equal keys of the blocks before
+        for (uint32_t t0 = 0; t0 < n; t0 += SEL_BLOCK)
+        {
+            if (n > SEL_BLOCK) load(t0);
+            uint32_t sure = 0, eq = 0;                     // kept for certain; equal to the key
+#pragma unroll
+            for (uint32_t u = 0; u < SEL; ++u)
+            {
+                const uint32_t t = t0 + tid * SEL + u;
+                const bool cand = t >= lo && t < hi && p.heavy != 0u;
+                sure += t < n && (t < lo || t >= hi || (cand && key[u] > prefix)) ? 1u : 0u;
+                eq += cand && key[u] == prefix ? 1u : 0u;
+            }
+            uint64_t all;
+            const uint64_t at = block_prefix(static_cast<uint64_t>(sure) << 32 | eq, wsum, all);
+            uint32_t eq_before = equal + static_cast<uint32_t>(at);
+            uint32_t to = out + static_cast<uint32_t>(at >> 32) + min(eq_before, need) - min(equal, need);
+#pragma unroll
+            for (uint32_t u = 0; u < SEL; ++u)
+            {
+                const uint32_t t = t0 + tid * SEL + u;
+                const bool cand = t >= lo && t < hi && p.heavy != 0u, same = cand && key[u] == prefix;
+                const bool stay = t < n && (t < lo || t >= hi || (cand && key[u] > prefix) || (same && eq_before < need));
+                eq_before += same ? 1u : 0u;
+                if (stay) kept[to++] = static_cast<int32_t>(t);
+            }
+            const uint32_t eq_after = equal + static_cast<uint32_t>(all);
+            out += static_cast<uint32_t>(all >> 32) + min(eq_after, need) - min(equal, need);
+            equal = eq_after;
         }
     }
     if (p.scores_out)
@@ -154,60 +204,260 @@ __global__ __launch_bounds__(1024) void k_evict_select(EvictParams p)
     }
 }
 
-// Moves the K (y = 0) or V (y = 1) plane of one (sequence, layer, KV head): a
-// run of 16 kept positions at a time, all of them read before any is written.
+typedef uint32_t u4v __attribute__((ext_vector_type(4)));
+typedef float f4_t __attribute__((ext_vector_type(4)));
+
+constexpr uint32_t MOVE_CH = 16;                           // V channels a workgroup moves
+// positions a workgroup reads at a time: 16 KB either way
+template <int AF>
+constexpr uint32_t move_run() { return AF == OPURE_A_F32 ? 256u : 512u; }
+
+// a pair of a key's channels turned back by the angle of (c, s)
+template <int AF>
+__device__ __forceinline__ uint32_t turn_pair(uint32_t v, float c, float s)
+{
+    const float x = AF == OPURE_A_F16 ? f16_to_f32(static_cast<uint16_t>(v)) : bits_f(v << 16);
+    const float y = AF == OPURE_A_F16 ? f16_to_f32(static_cast<uint16_t>(v >> 16)) : bits_f(v & 0xFFFF0000u);
+    const float a = __fmaf_rn(x, c, __fmul_rn(y, s)), b = __fmaf_rn(y, c, -__fmul_rn(x, s));
+    return AF == OPURE_A_F16 ? static_cast<uint32_t>(f32_to_f16(a)) | static_cast<uint32_t>(f32_to_f16(b)) << 16
+                             : static_cast<uint32_t>(f32_to_bf16(a)) | static_cast<uint32_t>(f32_to_bf16(b)) << 16;
+}
+
+// Moves part of one (sequence, layer, KV head): 64 bytes of its K rows, or 16
+// channels of its V planes, from the first position that can move to the last.
+// Parts never meet, so all run at once; within one the runs go in order, a run's
+// loads issued before the run before it is written (no slot that a run writes is
+// read by a later one), with one barrier between a run's loads and its stores.
+//   K: four threads a position, 256 kept positions a run, each thread's kept
+// position, page and data fetched a run ahead of one another.
+//   V: a channel's positions lie side by side, so runs of source pages go whole
+// (their 32-byte rows hold a kept position nearly always) through LDS, rows of
+// one channel, and the kept ones are collected from there into 16-byte stores;
+// a group of positions that a run fills in part is stored by elements.
+template <int AF>
 __global__ __launch_bounds__(256) void k_evict_move(EvictParams p)
 {
-    const uint32_t b = blockIdx.z, layer = blockIdx.x / p.n_kv, kh = blockIdx.x - layer * p.n_kv, which = blockIdx.y;
-    const uint32_t n = evict_len(p, b), tid = threadIdx.x, hd = p.hd;
+    constexpr uint32_t EB = AF == OPURE_A_F32 ? 4u : 2u, RUN = move_run<AF>(), TPP = 16u / EB, PPC = 16u / TPP;
+    constexpr uint32_t ROW = RUN * EB + 16u;               // bytes of a channel's row in LDS, a piece of padding
+    __shared__ __align__(16) uint8_t rows[MOVE_CH * ROW];
+    __shared__ __align__(16) uint16_t from[RUN + 16u];     // the run's kept positions, from the run's first
+    __shared__ uint32_t cnt[4];
+    const uint32_t hd = p.hd, segk = (hd * EB + 63u) / 64u, segs = segk + hd / MOVE_CH;
+    const uint32_t b = blockIdx.y, head = blockIdx.x / segs, layer = head / p.n_kv, kh = head - layer * p.n_kv, tid = threadIdx.x;
+    uint32_t seg = blockIdx.x - head * segs;
+    const uint32_t n = evict_len(p, b);
     if (n <= p.keep) return;                               // every position stays where it is
-    const int32_t* kept = p.kept + (static_cast<uint64_t>(b) * p.n_layers * p.n_kv + blockIdx.x) * p.keep;
+    const int32_t* kept = p.kept + (static_cast<uint64_t>(b) * p.n_layers * p.n_kv + head) * p.keep;
     const int32_t* pt = p.page_table + static_cast<uint64_t>(b) * p.max_pages;
-    auto page = [&](uint32_t t) -> int32_t {
-        const int32_t pg = pt[t / OPURE_PAGE_SIZE];
-        if (pg >= 0 && static_cast<uint32_t>(pg) < p.n_pages) return pg;
-        p.err[ERR_POSITION] = 1u;
-        return -1;
-    };
-    for (uint32_t i0 = 0; i0 < p.keep; i0 += OPURE_PAGE_SIZE)
+    const uint64_t plane = static_cast<uint64_t>(OPURE_PAGE_SIZE) * hd * EB, page_bytes = 2ull * p.n_kv * plane;
+    uint8_t* base = static_cast<uint8_t*>(p.pool) + static_cast<uint64_t>(layer) * p.n_pages * page_bytes + kh * plane;
+    auto there = [&](int32_t pg) { return static_cast<uint32_t>(pg) < p.n_pages; };
+    if (seg < segk)
     {
-        // 16 positions x hd channels: up to 8 pairs of channels a thread
-        float x[8], y[8];
+        constexpr uint32_t U = 4;
+        const uint32_t piece = seg * 4u + (tid & 3u), tok = tid >> 2;
+        const bool mine = piece * 16u < hd * EB;
+        const bool turn = p.cos != nullptr;
+        auto kept_at = [&](uint32_t i) { return i < p.keep ? kept[i] : -1; };
+        // (source position or -1, its page, the slot's page) of this thread's positions of a run
+        int32_t s0[U], s1[U], ps[U], pd[U], qs[U], qd[U];
+        u4v data[U], next[U];
+        f4_t co[U], si[U], nco[U], nsi[U];
+        const uint32_t first = p.sinks / 256u * 256u;
+        auto pages = [&](uint32_t i0, const int32_t (&s)[U], int32_t (&a)[U], int32_t (&d)[U]) {
 #pragma unroll
-        for (uint32_t u = 0; u < 8; ++u)
-        {
-            const uint32_t e = tid + 256u * u, i = i0 + e % OPURE_PAGE_SIZE, c = e / OPURE_PAGE_SIZE;
-            x[u] = y[u] = 0.0f;
-            if (2u * c >= hd || i >= p.keep) continue;
-            const uint32_t s = static_cast<uint32_t>(kept[i]);
-            const int32_t pg = page(s);
-            if (pg < 0) continue;
-            const uint32_t d = 2u * c;
-            float k0 = load_act_rt(p.pool, kv_elem(layer, p.n_pages, pg, which, p.n_kv, kh, hd, s % OPURE_PAGE_SIZE, d), p.afmt);
-            float k1 = load_act_rt(p.pool, kv_elem(layer, p.n_pages, pg, which, p.n_kv, kh, hd, s % OPURE_PAGE_SIZE, d + 1u), p.afmt);
-            if (which == 0u && p.cos && s != i)
+            for (uint32_t u = 0; u < U; ++u)
             {
-                const float co = p.cos[static_cast<uint64_t>(s - i) * (hd / 2u) + c], si = p.sin[static_cast<uint64_t>(s - i) * (hd / 2u) + c];
-                const float r0 = __fmaf_rn(k0, co, __fmul_rn(k1, si)), r1 = __fmaf_rn(k1, co, -__fmul_rn(k0, si));
-                k0 = r0;
-                k1 = r1;
+                const uint32_t i = i0 + 64u * u + tok;
+                const bool moves = mine && s[u] > static_cast<int32_t>(i);
+                a[u] = moves ? pt[static_cast<uint32_t>(s[u]) / OPURE_PAGE_SIZE] : -1;
+                d[u] = moves ? pt[i / OPURE_PAGE_SIZE] : -1;
+                if (moves && !(there(a[u]) && there(d[u])))
+                {
+                    p.err[ERR_POSITION] = 1u;
+                    a[u] = d[u] = -1;
+                }
             }
-            x[u] = k0;
-            y[u] = k1;
-        }
-        __syncthreads();
+        };
+        auto load = [&](uint32_t i0, const int32_t (&s)[U], const int32_t (&a)[U], u4v (&x)[U], f4_t (&c)[U], f4_t (&sn)[U]) {
 #pragma unroll
-        for (uint32_t u = 0; u < 8; ++u)
+            for (uint32_t u = 0; u < U; ++u)
+            {
+                const uint32_t i = i0 + 64u * u + tok;
+                if (a[u] < 0) continue;
+                const uint32_t t = static_cast<uint32_t>(s[u]);
+                x[u] = *reinterpret_cast<const u4v*>(base + static_cast<uint32_t>(a[u]) * page_bytes + (t % OPURE_PAGE_SIZE) * (hd * EB) + piece * 16u);
+                if (turn)
+                {
+                    const uint64_t at = static_cast<uint64_t>(t - i) * (hd / 2u) + piece * (TPP / 2u);
+                    if constexpr (AF == OPURE_A_F32)
+                    {
+                        c[u][0] = p.cos[at], c[u][1] = p.cos[at + 1u];
+                        sn[u][0] = p.sin[at], sn[u][1] = p.sin[at + 1u];
+                    }
+                    else
+#pragma unroll
+                        for (uint32_t k = 0; k < 4; ++k)
+                        {
+                            c[u][k] = p.cos[at + k];
+                            sn[u][k] = p.sin[at + k];
+                        }
+                }
+            }
+        };
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u)
         {
-            const uint32_t e = tid + 256u * u, i = i0 + e % OPURE_PAGE_SIZE, c = e / OPURE_PAGE_SIZE;
-            if (2u * c >= hd || i >= p.keep || static_cast<uint32_t>(kept[i]) == i) continue;
-            const int32_t pg = page(i);
-            if (pg < 0) continue;
-            const uint32_t d = 2u * c;
-            store_act_rt(p.pool, kv_elem(layer, p.n_pages, pg, which, p.n_kv, kh, hd, i % OPURE_PAGE_SIZE, d), x[u], p.afmt);
-            store_act_rt(p.pool, kv_elem(layer, p.n_pages, pg, which, p.n_kv, kh, hd, i % OPURE_PAGE_SIZE, d + 1u), y[u], p.afmt);
+            s0[u] = kept_at(first + 64u * u + tok);
+            s1[u] = kept_at(first + 256u + 64u * u + tok);
+        }
+        pages(first, s0, ps, pd);
+        load(first, s0, ps, data, co, si);
+        pages(first + 256u, s1, qs, qd);
+        for (uint32_t i0 = first; i0 < p.keep; i0 += 256u)
+        {
+            int32_t s2[U], rs[U], rd[U];
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u) s2[u] = kept_at(i0 + 512u + 64u * u + tok);
+            load(i0 + 256u, s1, qs, next, nco, nsi);
+            __syncthreads();
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u)
+            {
+                if (ps[u] < 0) continue;
+                const uint32_t i = i0 + 64u * u + tok;
+                u4v x = data[u];
+                if (turn)
+                {
+                    if constexpr (AF == OPURE_A_F32)
+#pragma unroll
+                        for (uint32_t k = 0; k < 2; ++k)
+                        {
+                            const float a = bits_f(x[2 * k]), c = bits_f(x[2 * k + 1]);
+                            x[2 * k] = f_bits(__fmaf_rn(a, co[u][k], __fmul_rn(c, si[u][k])));
+                            x[2 * k + 1] = f_bits(__fmaf_rn(c, co[u][k], -__fmul_rn(a, si[u][k])));
+                        }
+                    else
+#pragma unroll
+                        for (uint32_t k = 0; k < 4; ++k) x[k] = turn_pair<AF>(x[k], co[u][k], si[u][k]);
+                }
+                *reinterpret_cast<u4v*>(base + static_cast<uint32_t>(pd[u]) * page_bytes + (i % OPURE_PAGE_SIZE) * (hd * EB) + piece * 16u) = x;
+            }
+            pages(i0 + 512u, s2, rs, rd);
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u)
+            {
+                s0[u] = s1[u];
+                s1[u] = s2[u];
+                ps[u] = qs[u];
+                pd[u] = qd[u];
+                qs[u] = rs[u];
+                qd[u] = rd[u];
+                data[u] = next[u];
+                co[u] = nco[u];
+                si[u] = nsi[u];
+            }
+        }
+        return;
+    }
+    // ---- V: 16 channels
+    seg -= segk;
+    constexpr uint32_t U = 4, PG = RUN / OPURE_PAGE_SIZE, PPP = MOVE_CH * PPC;   // pages a run; pieces a page
+    static_assert(PG * PPP == 256u * U, "a run is four pieces a thread");
+    uint8_t* vbase = base + p.n_kv * plane + static_cast<uint64_t>(seg) * MOVE_CH * OPURE_PAGE_SIZE * EB;
+    const uint32_t wave = tid >> 6, lane = tid & 63u;
+    u4v data[U];
+    int32_t pe[U];
+    auto entries = [&](uint32_t t0) {
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u)
+        {
+            const uint32_t t = t0 + (u * 256u + tid) / PPP * OPURE_PAGE_SIZE;
+            pe[u] = t < n ? pt[t / OPURE_PAGE_SIZE] : -1;
+            if (t < n && !there(pe[u]))
+            {
+                p.err[ERR_POSITION] = 1u;
+                pe[u] = -1;
+            }
+        }
+    };
+    auto load = [&] {
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u)
+            if (pe[u] >= 0)
+                data[u] = *reinterpret_cast<const u4v*>(vbase + static_cast<uint32_t>(pe[u]) * page_bytes + (u * 256u + tid) % PPP * 16u);
+    };
+    constexpr uint32_t KW = RUN / 256u;
+    int32_t kw[KW];
+    uint32_t t0 = p.sinks / RUN * RUN, i0 = t0;            // everything before the sinks' end stays in place
+    auto window = [&](uint32_t i) {
+#pragma unroll
+        for (uint32_t k = 0; k < KW; ++k) kw[k] = i + 256u * k + tid < p.keep ? kept[i + 256u * k + tid] : 0x7FFFFFFF;
+    };
+    window(i0);
+    entries(t0);
+    load();
+    entries(t0 + RUN);
+    for (; i0 < p.keep && t0 < n; t0 += RUN)
+    {
+        __syncthreads();                                   // the run before is collected
+        uint32_t c = 0;
+        const uint32_t d0 = i0 / OPURE_PAGE_SIZE;
+#pragma unroll
+        for (uint32_t k = 0; k < KW; ++k)
+        {
+            const bool in = static_cast<uint32_t>(kw[k]) < t0 + RUN;
+            c += static_cast<uint32_t>(__popcll(__ballot(in)));
+            if (in) from[i0 - d0 * OPURE_PAGE_SIZE + 256u * k + tid] = static_cast<uint16_t>(static_cast<uint32_t>(kw[k]) - t0);
+        }
+        if (lane == 0u) cnt[wave] = c;
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u)
+        {
+            const uint32_t e = u * 256u + tid, pg = e / PPP, ch = e % PPP / PPC, half = e % PPC;
+            *reinterpret_cast<u4v*>(rows + ch * ROW + (pg * PPC + half) * 16u) = data[u];
         }
         __syncthreads();
+        const uint32_t i1 = i0 + cnt[0] + cnt[1] + cnt[2] + cnt[3];
+        window(i1);
+        load();
+        entries(t0 + 2u * RUN);
+        if (i1 > i0)
+        {
+            const uint32_t d1 = (i1 - 1u) / OPURE_PAGE_SIZE;
+            for (uint32_t e = tid; e < (d1 - d0 + 1u) * PPP; e += 256u)
+            {
+                const uint32_t pg = d0 + e / PPP, ch = e % PPP / PPC, half = e % PPC, g0 = pg * OPURE_PAGE_SIZE + half * TPP;
+                const uint32_t a = max(g0, i0), z = min(g0 + TPP, i1);
+                if (a >= z) continue;
+                const uint16_t* f = from + (g0 - d0 * OPURE_PAGE_SIZE);
+                if (t0 + f[z - 1u - g0] == z - 1u) continue;   // the last one does not move, so none does
+                const int32_t to = pt[pg];
+                if (!there(to)) continue;                      // reported by the runs that read it
+                uint8_t* dst = vbase + static_cast<uint32_t>(to) * page_bytes + (ch * PPC + half) * 16u;
+                const uint8_t* row = rows + ch * ROW;
+                if (z - a == TPP)
+                {
+                    u4v x;
+                    if constexpr (EB == 4u)
+#pragma unroll
+                        for (uint32_t k = 0; k < 4; ++k) x[k] = *reinterpret_cast<const uint32_t*>(row + f[k] * 4u);
+                    else
+#pragma unroll
+                        for (uint32_t k = 0; k < 4; ++k)
+                            x[k] = static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(row + f[2 * k] * 2u)) |
+                                   static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(row + f[2 * k + 1] * 2u)) << 16;
+                    *reinterpret_cast<u4v*>(dst) = x;
+                }
+                else
+                    for (uint32_t i = a; i < z; ++i)
+                    {
+                        if constexpr (EB == 4u) reinterpret_cast<uint32_t*>(dst)[i - g0] = *reinterpret_cast<const uint32_t*>(row + f[i - g0] * 4u);
+                        else reinterpret_cast<uint16_t*>(dst)[i - g0] = *reinterpret_cast<const uint16_t*>(row + f[i - g0] * 2u);
+                    }
+            }
+        }
+        i0 = i1;
     }
 }
 
@@ -254,7 +504,7 @@ extern "C" int opure_kv_evict(opure_dev* dev, const opure_evict_args* a)
     OPURE_REQUIRE(kv->n_pages >= 1 && kv->max_pages_per_seq >= 1, OPURE_E_INVALID, "opure_kv_evict: the cache has no pages");
     OPURE_REQUIRE(a->batch >= 1 && a->batch <= OPURE_MAX_BATCH_ROWS, OPURE_E_CAPACITY, "opure_kv_evict: %u sequences outside 1..%d",
                   a->batch, OPURE_MAX_BATCH_ROWS);
-    OPURE_REQUIRE(static_cast<uint64_t>(m->n_layers) * m->n_kv_heads <= 0x7FFFFFu, OPURE_E_CAPACITY, "opure_kv_evict: %u layers x %u KV heads",
+    OPURE_REQUIRE(static_cast<uint64_t>(m->n_layers) * m->n_kv_heads <= 0x7FFFFu, OPURE_E_CAPACITY, "opure_kv_evict: %u layers x %u KV heads",
                   m->n_layers, m->n_kv_heads);
     const uint64_t slots = static_cast<uint64_t>(kv->max_pages_per_seq) * OPURE_PAGE_SIZE;
     OPURE_REQUIRE(a->max_ctx >= 1 && a->max_ctx <= slots && a->max_ctx <= 0x7FFFFFFFu, OPURE_E_CAPACITY,
@@ -295,11 +545,18 @@ extern "C" int opure_kv_evict(opure_dev* dev, const opure_evict_args* a)
     p.freed_stride = a->freed_stride;
     p.cap = a->max_ctx;
     p.err = dev->err;
+    // the other workgroups read seq_len and the table: what is written over them waits for a launch of its own
+    p.new_len_now = !a->freed && a->new_seq_len != a->seq_len ? 1u : 0u;
     const uint32_t planes = p.n_layers * p.n_kv;
     OPURE_LAUNCH(dev, k_evict_select, dim3(planes, a->batch), dim3(1024), 0, p);
     OPURE_LAUNCH_CHECK("k_evict_select");
-    OPURE_LAUNCH(dev, k_evict_move, dim3(planes, 2, a->batch), dim3(256), 0, p);
+    const uint32_t eb = act_bytes(p.afmt), segs = (p.hd * eb + 63u) / 64u + p.hd / MOVE_CH;
+    auto move = [&](auto k) { OPURE_LAUNCH(dev, k, dim3(planes * segs, a->batch), dim3(256), 0, p); };
+    if (p.afmt == OPURE_A_F32) move(&k_evict_move<OPURE_A_F32>);
+    else if (p.afmt == OPURE_A_F16) move(&k_evict_move<OPURE_A_F16>);
+    else move(&k_evict_move<OPURE_A_BF16>);
     OPURE_LAUNCH_CHECK("k_evict_move");
+    if (p.new_len_now) return OPURE_OK;
     OPURE_LAUNCH(dev, k_evict_finish, dim3(a->batch), dim3(64), 0, p);
     OPURE_LAUNCH_CHECK("k_evict_finish");
     return OPURE_OK;
