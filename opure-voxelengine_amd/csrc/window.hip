@@ -8,275 +8,13 @@
 //  out = sum w_t v_t, and weights[h][t] += w_t over the rows and the query heads
 //  of KV head h.
 // ============================================================================
-#include "internal.h"
+#include "window.h"
 
 #include <algorithm>
-#include <atomic>
 
-using namespace opure_dev_math;
+using namespace opure_win;
 
 namespace {
-
-struct WinParams {
-    const void* q;
-    void* out;
-    const void* pool;
-    const int32_t* page_table;
-    const int32_t* seq_len;
-    float* part_acc;     // [batch][n_kv][parts][Gq][hd]: a part's unnormalised output of each query row
-    float* part_ml;      // [batch][n_kv][parts][Gq][2]: its maximum (in powers of two) and sum
-    float* scores;       // with weights: [batch][n_kv][tiles][Gq][tile's positions], in powers of two
-    float* weights;
-    uint64_t weights_batch_stride;
-    uint32_t weights_stride;
-    uint32_t n_heads, n_kv, hd, rows, n_pages, max_pages, layer, afmt;
-    uint32_t window, sinks;       // window >= 1: 2^31 - 1 sees everything
-    uint32_t cap;                 // positions that may be read: min(max_ctx, the table's)
-    uint32_t parts, blocks;       // parts a (sequence, KV head, block of query rows); such blocks
-    uint32_t tiles;               // most tiles a sequence's rows see
-    uint32_t combine_rows;        // query rows of the call
-    uint32_t combine_wgs;         // k_win_join: its first workgroups join the parts, the others add the weights
-    float scale;
-    uint32_t* err;
-};
-
-// A sequence's positions: `ctx` before the rows, `total` that may be read.  A
-// negative length or one that passes the capacity is reported and clamped.
-struct WinSeq {
-    uint32_t ctx, total;
-};
-
-__device__ __forceinline__ WinSeq win_seq(const WinParams& p, int32_t len)
-{
-    WinSeq s;
-    s.ctx = len < 0 ? 0u : static_cast<uint32_t>(len);
-    s.total = min(s.ctx + p.rows, p.cap);
-    if ((len < 0 || s.ctx + p.rows > p.cap) && threadIdx.x == 0u && p.err) p.err[ERR_POSITION] = 1u;
-    return s;
-}
-
-__device__ __forceinline__ bool win_sees(const WinParams& p, uint32_t pos, uint32_t t)
-{
-    return t <= pos && (t < p.sinks || t + p.window > pos);
-}
-
-// the page of position t (t < total), or -1
-__device__ __forceinline__ int32_t win_page(const WinParams& p, const int32_t* pt, uint32_t t)
-{
-    const int32_t pg = pt[t / OPURE_PAGE_SIZE];
-    return pg >= 0 && static_cast<uint32_t>(pg) < p.n_pages ? pg : -1;
-}
-
-// One query row by one wave, exactly as the formulas say it: lanes over 64
-// positions for the scores, then over channels for the output; a position that
-// the row does not see is not read.  qs: the row in LDS (hd floats).
-__device__ void win_row(const WinParams& p, const float* qs, uint32_t b, uint32_t kh, uint32_t pos, uint32_t total,
-                        float& m, float& l, float (&o)[4])
-{
-    const uint32_t lane = threadIdx.x & 63u, hd = p.hd;
-    const int32_t* pt = p.page_table + static_cast<uint64_t>(b) * p.max_pages;
-    const uint32_t end = min(pos + 1u, total);
-    const uint32_t low = pos + 1u > p.window ? pos + 1u - p.window : 0u;   // the window's first position
-    m = -__builtin_huge_valf();
-    l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) o[i] = 0.0f;
-    for (uint32_t t0 = 0; t0 < end; t0 += 64u)
-    {
-        if (t0 >= p.sinks && t0 + 64u <= low)
-        {
-            t0 = low / 64u * 64u - 64u;                    // between the sinks and the window
-            continue;
-        }
-        const uint32_t t = t0 + lane;
-        const bool in = t < end && win_sees(p, pos, t);
-        const int32_t pg = in ? win_page(p, pt, t) : -1;
-        float s = -__builtin_huge_valf();
-        if (in && pg < 0) s = __builtin_nanf("");
-        if (in && pg >= 0)
-        {
-            const uint64_t at = kv_elem(p.layer, p.n_pages, static_cast<uint32_t>(pg), 0u, p.n_kv, kh, hd, t % OPURE_PAGE_SIZE, 0u);
-            float acc = 0.0f;
-            for (uint32_t d = 0; d < hd; ++d) acc = __fmaf_rn(qs[d], load_act_rt(p.pool, at + d, p.afmt), acc);
-            s = __fmul_rn(acc, p.scale);
-        }
-        const float mx = fmaxf(m, wave_max64(s));          // a NaN score leaves the maximum and reaches the sum
-        const float ms = mx == -__builtin_huge_valf() ? 0.0f : mx;
-        const float a = expf_ref(__fsub_rn(m, ms)), e = in ? expf_ref(__fsub_rn(s, ms)) : 0.0f;
-        m = mx;
-        l = __fmaf_rn(l, a, wave_sum64(e));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = __fmul_rn(o[i], a);
-        uint64_t left = __ballot(in && pg >= 0);
-        while (left)
-        {
-            const int k = __builtin_ctzll(left);
-            left &= left - 1u;
-            const float w = __shfl(e, k);
-            const uint32_t pk = static_cast<uint32_t>(__shfl(pg, k)), tk = t0 + static_cast<uint32_t>(k);
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-            {
-                const uint32_t d = lane + 64u * i;
-                if (d < hd)
-                    o[i] = __fmaf_rn(w, load_act_rt(p.pool, kv_elem(p.layer, p.n_pages, pk, 1u, p.n_kv, kh, hd, tk % OPURE_PAGE_SIZE, d),
-                                                    p.afmt), o[i]);
-            }
-        }
-    }
-}
-
-typedef uint32_t u4v __attribute__((ext_vector_type(4)));
-typedef float f4_t __attribute__((ext_vector_type(4)));
-typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
-
-constexpr float NEG_INF = -__builtin_huge_valf();
-
-// The tiles (TT positions each) that the rows at ctx .. ctx + rows - 1 see: the
-// sinks' first, then the window's.  Tile i of the list starts at position start(i).
-struct WinSpan {
-    uint32_t ns, w0, n;           // sink tiles, the window's first tile, tiles in all
-    __device__ __forceinline__ uint32_t tile(uint32_t i) const { return i < ns ? i : i - ns + w0; }
-};
-
-template <uint32_t TT>
-__device__ __forceinline__ WinSpan win_span(const WinParams& p, const WinSeq& sq, uint32_t first_pos, uint32_t end_pos)
-{
-    WinSpan s;
-    const uint32_t low = first_pos + 1u > p.window ? first_pos + 1u - p.window : 0u;
-    const uint32_t end = min(end_pos, sq.total);
-    const uint32_t last = (end + TT - 1u) / TT;
-    s.w0 = min(low / TT, last);
-    s.ns = min((min(p.sinks, end) + TT - 1u) / TT, s.w0);
-    s.n = s.ns + last - s.w0;
-    return s;
-}
-
-// Operands of S^T = K Q^T and O^T = V^T P^T by 16x16 matrix instructions, lane
-// (r = lane % 16, g = lane / 16).  A tile is 32 positions of a 16-bit cache, two
-// score blocks of 16: row r of block T is position 8 (r / 4) + r % 4 + 4 T, so
-// that a lane's scores are positions 8 g .. 8 g + 7, which is its operand P^T,
-// and its part of a V channel is 16 bytes.  In fp32 a tile is one page, row r is
-// position r, a lane's scores are positions 4 g .. 4 g + 3 and each of the four
-// takes a matrix instruction over 4 positions.
-template <int AF, int HD>
-struct WinTile {
-    static constexpr uint32_t EB = AF == OPURE_A_F32 ? 4u : 2u, TT = AF == OPURE_A_F32 ? 16u : 32u, NB = TT / 16u;
-    static constexpr uint32_t KS = AF == OPURE_A_F32 ? HD / 16u : (HD + 31u) / 32u, DT = HD / 16u, NS = 16u / EB;
-    static constexpr uint32_t PB = OPURE_PAGE_SIZE * HD * EB;   // bytes of a K or V plane
-    static constexpr bool HALF = AF != OPURE_A_F32 && HD % 32 != 0;   // the last step's upper channels are not there
-    u4v k[NB][KS], v[DT];
-
-    __device__ __forceinline__ static float part(u4v x, uint32_t i) { return __uint_as_float(x[i]); }
-    __device__ __forceinline__ void load_k(const uint8_t* a, const uint8_t* b, uint32_t r, uint32_t g)
-    {
-        const uint8_t* at = AF == OPURE_A_F32 || r < 8u ? a : b;
-        const uint32_t slot = AF == OPURE_A_F32 ? r : 8u * ((r >> 2) & 1u) + (r & 3u);
-        at += slot * (HD * EB) + 16u * g;
-#pragma unroll
-        for (uint32_t t = 0; t < NB; ++t)
-#pragma unroll
-            for (uint32_t s = 0; s < KS; ++s)
-            {
-                if (HALF && s + 1u == KS && g >= 2u) k[t][s] = u4v{0u, 0u, 0u, 0u};
-                else k[t][s] = *reinterpret_cast<const u4v*>(at + t * 4u * HD * EB + 64u * s);
-            }
-    }
-    __device__ __forceinline__ void load_v(const uint8_t* a, const uint8_t* b, uint32_t r, uint32_t g)
-    {
-        const uint8_t* at = AF == OPURE_A_F32 || g < 2u ? a : b;
-        at += r * (16u * EB) + (AF == OPURE_A_F32 ? g : (g & 1u)) * 16u;
-#pragma unroll
-        for (uint32_t d = 0; d < DT; ++d) v[d] = *reinterpret_cast<const u4v*>(at + d * 16u * 16u * EB);
-    }
-};
-
-template <int AF, int HD>
-__device__ __forceinline__ void win_load_q(const WinParams& p, uint64_t row, uint32_t g, u4v (&q)[WinTile<AF, HD>::KS])
-{
-    typedef WinTile<AF, HD> T;
-    const uint8_t* at = static_cast<const uint8_t*>(p.q) + row * (HD * T::EB) + 16u * g;
-#pragma unroll
-    for (uint32_t s = 0; s < T::KS; ++s)
-    {
-        if (T::HALF && s + 1u == T::KS && g >= 2u) q[s] = u4v{0u, 0u, 0u, 0u};
-        else q[s] = *reinterpret_cast<const u4v*>(at + 64u * s);
-    }
-}
-
-template <int AF>
-__device__ __forceinline__ f4_t win_mfma(u4v a, u4v b, f4_t c)
-{
-    if constexpr (AF == OPURE_A_F16)
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
-    else if constexpr (AF == OPURE_A_BF16)
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
-    else
-    {
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i)
-            c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[i]), __uint_as_float(b[i]), c, 0, 0, 0);
-        return c;
-    }
-}
-
-template <int AF>
-__device__ __forceinline__ uint32_t win_pack(float a, float b)
-{
-    typedef float f2v __attribute__((ext_vector_type(2)));
-    typedef _Float16 h2v __attribute__((ext_vector_type(2)));
-    typedef __bf16 b2v __attribute__((ext_vector_type(2)));
-    const f2v v = {a, b};
-    if constexpr (AF == OPURE_A_F16) return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, h2v));
-    else return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, b2v));
-}
-
-template <int AF>
-__device__ __forceinline__ float win_low(uint32_t v) { return AF == OPURE_A_F16 ? f16_to_f32(static_cast<uint16_t>(v)) : bits_f(v << 16); }
-template <int AF>
-__device__ __forceinline__ float win_high(uint32_t v) { return AF == OPURE_A_F16 ? f16_to_f32(static_cast<uint16_t>(v >> 16)) : bits_f(v & 0xFFFF0000u); }
-
-// elements n .. of a 16-byte piece of consecutive positions read 0
-template <int AF>
-__device__ __forceinline__ u4v win_tail(u4v v, uint32_t n)
-{
-#pragma unroll
-    for (uint32_t i = 0; i < 4; ++i)
-    {
-        if (AF == OPURE_A_F32) v[i] = i < n ? v[i] : 0u;
-        else v[i] = 2u * i + 1u < n ? v[i] : 2u * i < n ? v[i] & 0xFFFFu : 0u;
-    }
-    return v;
-}
-
-// One tile's scores of a block of query rows, in powers of two (scale log2 e q.k),
-// -inf where the row at `pos` does not see the position.
-template <int AF, int HD>
-__device__ __forceinline__ void win_scores(const WinParams& p, const WinTile<AF, HD>& tl, const u4v (&q)[WinTile<AF, HD>::KS], float c,
-                                           bool full, uint32_t t0, uint32_t g, uint32_t pos, uint32_t total,
-                                           float (&s)[WinTile<AF, HD>::NS])
-{
-    typedef WinTile<AF, HD> T;
-#pragma unroll
-    for (uint32_t t = 0; t < T::NB; ++t)
-    {
-        f4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (uint32_t k = 0; k < T::KS; ++k) acc = win_mfma<AF>(tl.k[t][k], q[k], acc);
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) s[4u * t + i] = __fmul_rn(acc[i], c);
-    }
-    if (!full)
-    {
-#pragma unroll
-        for (uint32_t i = 0; i < T::NS; ++i)
-        {
-            const uint32_t t = t0 + T::NS * g + i;
-            s[i] = t < total && win_sees(p, pos, t) ? s[i] : NEG_INF;
-        }
-    }
-}
 
 // Few query rows: a workgroup takes a part of the tiles that a sequence's rows
 // see, for 16 NT query rows of a KV head (row qi = j group + head), a wave every
@@ -527,6 +265,7 @@ __global__ __launch_bounds__(256) void k_win_join(WinParams p)
             for (uint32_t i = 0; i < 4; ++i)
                 if (lane + 64u * i < p.hd) o[i] = __fmaf_rn(wx, acc[lane + 64u * i], o[i]);
         }
+        if (p.lse && lane == 0u) p.lse[(static_cast<uint64_t>(b) * p.n_kv + kh) * Gq + qi] = win_lse(M, L);
         bool fine = true;
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i)
@@ -595,58 +334,31 @@ template <int AF, int HD, int NT>
 int win_split_launch(opure_dev* dev, const WinParams& p, uint32_t batch)
 {
     constexpr uint32_t lds = 4u * (HD / 16u) * NT * 64u * 16u + 4u * NT * 16u * 2u * 4u;
-    if constexpr (lds > 64u * 1024u)
-    {
-        static std::atomic<uint64_t> done{0};              // a bit a device
-        const uint64_t bit = 1ull << (dev->ordinal & 63);
-        if (!(done.load(std::memory_order_relaxed) & bit))
-            OPURE_HIP_TRY(hipFuncSetAttribute(reinterpret_cast<const void*>(&k_win_split<AF, HD, NT>),
-                                              hipFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(lds)));
-        done.fetch_or(bit, std::memory_order_relaxed);
-    }
+    static std::atomic<uint64_t> done{0};
+    const int rc = win_lds(dev, reinterpret_cast<const void*>(&k_win_split<AF, HD, NT>), lds, done);
+    if (rc) return rc;
     OPURE_LAUNCH(dev, (k_win_split<AF, HD, NT>), dim3(p.n_kv * p.parts * batch * p.blocks), dim3(256), lds, p);
     OPURE_LAUNCH_CHECK("k_win_split");
     return OPURE_OK;
 }
 
-template <int AF, int HD>
-int win_split_hd(opure_dev* dev, const WinParams& p, uint32_t batch, bool two)
-{
-    if constexpr (HD <= 128)
-        if (two) return win_split_launch<AF, HD, 2>(dev, p, batch);
-    return win_split_launch<AF, HD, 1>(dev, p, batch);
-}
-
 template <int AF>
 int win_split_any(opure_dev* dev, const WinParams& p, uint32_t batch, bool two)
 {
-    switch (p.hd / 16u)
-    {
-    case 1: return win_split_hd<AF, 16>(dev, p, batch, two);
-    case 2: return win_split_hd<AF, 32>(dev, p, batch, two);
-    case 3: return win_split_hd<AF, 48>(dev, p, batch, two);
-    case 4: return win_split_hd<AF, 64>(dev, p, batch, two);
-    case 5: return win_split_hd<AF, 80>(dev, p, batch, two);
-    case 6: return win_split_hd<AF, 96>(dev, p, batch, two);
-    case 7: return win_split_hd<AF, 112>(dev, p, batch, two);
-    case 8: return win_split_hd<AF, 128>(dev, p, batch, two);
-    case 9: return win_split_hd<AF, 144>(dev, p, batch, two);
-    case 10: return win_split_hd<AF, 160>(dev, p, batch, two);
-    case 11: return win_split_hd<AF, 176>(dev, p, batch, two);
-    case 12: return win_split_hd<AF, 192>(dev, p, batch, two);
-    case 13: return win_split_hd<AF, 208>(dev, p, batch, two);
-    case 14: return win_split_hd<AF, 224>(dev, p, batch, two);
-    case 15: return win_split_hd<AF, 240>(dev, p, batch, two);
-    default: return win_split_hd<AF, 256>(dev, p, batch, two);
-    }
+    return win_by_head(p.hd, [&](auto h) {
+        constexpr int HD = decltype(h)::value;
+        if constexpr (HD <= 128)
+            if (two) return win_split_launch<AF, HD, 2>(dev, p, batch);
+        return win_split_launch<AF, HD, 1>(dev, p, batch);
+    });
 }
 
 // How a call is split, and its workspace.
 struct WinPlan {
     uint32_t tt, tiles, blocks, parts;
-    bool two;
-    uint64_t acc, ml, scores;     // bytes
-    uint64_t bytes() const { return acc + ml + scores; }
+    bool prompt, two, stored;     // the prompt kernel; split: 32 query rows a workgroup; weights from stored scores
+    uint64_t acc, ml, scores, lse;   // bytes
+    uint64_t bytes() const { return acc + ml + scores + lse; }
 };
 
 WinPlan win_plan(const opure_dev* dev, const opure_attn_window_args* a)
@@ -658,15 +370,19 @@ WinPlan win_plan(const opure_dev* dev, const opure_attn_window_args* a)
     // tiles of any sequence of the call: its sinks', then the window's and the rows', which begin anywhere in a tile
     const uint64_t all = (a->max_ctx + w.tt - 1u) / w.tt, window = a->window ? a->window : 0x7FFFFFFFu;
     w.tiles = static_cast<uint32_t>(std::min<uint64_t>(all, (a->sinks + w.tt - 1ull) / w.tt + (window + a->rows + w.tt - 2ull) / w.tt + 1u));
+    const uint64_t rows = static_cast<uint64_t>(a->batch) * m->n_kv_heads * Gq;
+    w.prompt = m->afmt != OPURE_A_F32 && Gq >= 256u;
+    w.stored = a->weights && Gq <= 64u;
+    w.lse = a->weights && !w.stored ? opure_hip::align_up(rows * 4u, 256) : 0u;
+    if (w.prompt) return w;
     w.two = Gq > 16u && m->head_dim <= 128u;
     w.blocks = (Gq + (w.two ? 31u : 15u)) / (w.two ? 32u : 16u);
     const uint64_t groups = static_cast<uint64_t>(a->batch) * m->n_kv_heads * w.blocks;
     const uint64_t want = (4ull * n_cu + groups - 1u) / groups;
     w.parts = static_cast<uint32_t>(std::min<uint64_t>(want, std::min((w.tiles + 3u) / 4u, 64u)));
-    const uint64_t rows = static_cast<uint64_t>(a->batch) * m->n_kv_heads * Gq;
     w.acc = opure_hip::align_up(rows * w.parts * m->head_dim * 4u, 256);
     w.ml = opure_hip::align_up(rows * w.parts * 8u, 256);
-    w.scores = a->weights ? opure_hip::align_up(rows * w.tiles * w.tt * 4u, 256) : 0u;
+    w.scores = w.stored ? opure_hip::align_up(rows * w.tiles * w.tt * 4u, 256) : 0u;
     return w;
 }
 
@@ -740,7 +456,8 @@ extern "C" int opure_attn_window_paged(opure_dev* dev, const opure_attn_window_a
     p.seq_len = a->seq_len;
     p.part_acc = static_cast<float*>(dev->ws);
     p.part_ml = p.part_acc + w.acc / 4u;
-    p.scores = a->weights ? p.part_ml + w.ml / 4u : nullptr;
+    p.scores = w.stored ? p.part_ml + w.ml / 4u : nullptr;
+    p.lse = w.lse ? p.part_ml + (w.ml + w.scores) / 4u : nullptr;
     p.weights = a->weights;
     p.weights_stride = a->weights_stride;
     p.weights_batch_stride = a->weights_batch_stride;
@@ -762,13 +479,18 @@ extern "C" int opure_attn_window_paged(opure_dev* dev, const opure_attn_window_a
     p.tiles = w.tiles;
     p.combine_rows = a->batch * a->rows * p.n_heads;
     p.combine_wgs = (p.combine_rows + 3u) / 4u;
+    if (w.prompt)
+    {
+        rc = win_prompt_launch(dev, p, a->batch);
+        return rc || !p.lse ? rc : win_sums_launch(dev, p, a->batch, a->max_ctx);
+    }
     rc = p.afmt == OPURE_A_F32   ? win_split_any<OPURE_A_F32>(dev, p, a->batch, w.two)
          : p.afmt == OPURE_A_F16 ? win_split_any<OPURE_A_F16>(dev, p, a->batch, w.two)
                                  : win_split_any<OPURE_A_BF16>(dev, p, a->batch, w.two);
     if (rc) return rc;
-    const uint32_t sums = p.weights ? (w.tiles * w.tt + 255u) / 256u * p.n_kv * a->batch : 0u;
+    const uint32_t sums = p.scores ? (w.tiles * w.tt + 255u) / 256u * p.n_kv * a->batch : 0u;
     if (w.tt == 16u) OPURE_LAUNCH(dev, (k_win_join<16u>), dim3(p.combine_wgs + sums), dim3(256), 0, p);
     else OPURE_LAUNCH(dev, (k_win_join<32u>), dim3(p.combine_wgs + sums), dim3(256), 0, p);
     OPURE_LAUNCH_CHECK("k_win_join");
-    return OPURE_OK;
+    return p.lse ? win_sums_launch(dev, p, a->batch, a->max_ctx) : OPURE_OK;
 }

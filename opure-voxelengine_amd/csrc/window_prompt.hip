@@ -1,0 +1,410 @@
+// ============================================================================
+//  window_prompt.hip -- windowed attention of a prompt's rows, and the weights
+//  that the cached positions got from many rows.
+// ============================================================================
+#include "window.h"
+
+using namespace opure_win;
+
+namespace {
+
+typedef float f16_t __attribute__((ext_vector_type(16)));
+
+template <int AF>
+__device__ __forceinline__ f16_t mfma_32(u4v a, u4v b, f16_t c)
+{
+    if constexpr (AF == OPURE_A_F16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b), c, 0, 0, 0);
+}
+
+constexpr uint32_t PT = 64;                                // positions a tile
+template <int HD>
+constexpr uint32_t prompt_k_pieces() { return PT * (HD / 8u + 1u); }   // a padded row a position
+template <int HD>
+constexpr uint32_t prompt_v_pieces() { return (HD + 31u) / 32u * 32u * (PT / 8u + 1u); }   // a padded row a channel
+template <int HD>
+constexpr uint32_t prompt_lds() { return 2u * (prompt_k_pieces<HD>() + prompt_v_pieces<HD>()) * 16u; }
+
+// Many query rows: a workgroup takes 128 query rows (qi = j group + head) of a KV
+// head, 32 a wave, over tiles of 64 positions that the four waves share in LDS,
+// two stages deep, the next tile's loads in flight while one computes.  Products
+// are 32x32x16: S^T = K Q^T with a lane (q = lane % 32, h = lane / 32) holding 32
+// scores of one row, whose maximum and sum need one exchange between the halves;
+// K rows lie in LDS in the order (positions with bits 2 and 3 exchanged) that
+// makes a lane's scores 8 consecutive positions, its operand of O^T = V^T P^T.
+//   A row's output is scaled to a new maximum only where that passes the old one
+// by 2^8: the weights are then up to 2^8, which costs none of their bits.  They
+// enter the product rounded once to the cache's format (half a step, as the result
+// itself is): the matrix unit is what bounds a prompt, and a second product for
+// the rounding's rest would cost it half as much again.  fp16 weights are held
+// 2^6 higher, so that those down to 2^-20 of the largest keep their bits.
+template <int AF, int HD>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 128 ? 2 : 1))) void k_win_prompt(WinParams p)
+{
+    constexpr uint32_t KS = HD / 16u, DT = (HD + 31u) / 32u, P = HD / 8u, KROW = P + 1u, VROW = PT / 8u + 1u;
+    constexpr uint32_t N = 8u * HD, NP = (N + 255u) / 256u;   // 16-byte pieces of a tile's K (and of its V); a thread's
+    constexpr float UP = AF == OPURE_A_F16 ? 6.0f : 0.0f;
+    extern __shared__ __align__(16) uint8_t lds[];
+    u4v* const kt = reinterpret_cast<u4v*>(lds);
+    u4v* const vt = kt + 2u * prompt_k_pieces<HD>();
+    const uint32_t G = p.n_heads / p.n_kv, Gq = G * p.rows, nblk = (Gq + 127u) / 128u;
+    const uint32_t kh = blockIdx.x % p.n_kv, rest = blockIdx.x / p.n_kv, b = rest / nblk;
+    const uint32_t q0 = (nblk - 1u - (rest - b * nblk)) * 128u;   // the rows that see most first
+    const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63u, h = lane >> 5, r = lane & 31u;
+    const int32_t* pt = p.page_table + static_cast<uint64_t>(b) * p.max_pages;
+    const WinSeq sq = win_seq(p, p.seq_len[b]);
+    const uint32_t j0 = q0 / G, j1 = min(q0 + 127u, Gq - 1u) / G;
+    const WinSpan span = win_span<PT>(p, sq, sq.ctx + j0, sq.ctx + j1 + 1u);
+    // the wave's rows
+    const uint32_t w0 = min(q0 + 32u * wave, Gq - 1u), w1 = min(q0 + 32u * wave + 31u, Gq - 1u), qi = min(w0 + r, Gq - 1u);
+    const uint32_t j = qi / G, pos = sq.ctx + j, pos0 = sq.ctx + w0 / G, pos1 = sq.ctx + w1 / G;
+    const uint64_t row = (static_cast<uint64_t>(b) * p.rows + j) * p.n_heads + kh * G + (qi - j * G);
+    // scores in powers of two are c times the products: c >= 0, its sign goes to Q (and c = 0 to Q whole)
+    const float c = p.scale == 0.0f ? 1.0f : __fmul_rn(__builtin_fabsf(p.scale), 1.44269504088896340736f);
+    u4v q[KS];
+#pragma unroll
+    for (uint32_t s = 0; s < KS; ++s)
+    {
+        q[s] = *reinterpret_cast<const u4v*>(static_cast<const uint8_t*>(p.q) + row * (HD * 2u) + (2u * s + h) * 16u);
+        const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u, keep = p.scale == 0.0f ? 0u : ~0u;
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) q[s][i] = (q[s][i] ^ flip) & keep;
+    }
+    const uint64_t plane = static_cast<uint64_t>(OPURE_PAGE_SIZE) * HD * 2u, page_bytes = 2ull * p.n_kv * plane;
+    const uint8_t* base = static_cast<const uint8_t*>(p.pool) + static_cast<uint64_t>(p.layer) * p.n_pages * page_bytes + kh * plane;
+    const uint64_t vofs = p.n_kv * plane;
+
+    u4v kr[NP], vr[NP];
+    int32_t pe[NP], cur[NP];
+    auto entries = [&](uint32_t i) {
+        const uint32_t tile = span.tile(min(i, span.n - 1u));
+#pragma unroll
+        for (uint32_t u = 0; u < NP; ++u) pe[u] = pt[min(tile * 4u + (u * 256u + tid) / (2u * HD), p.max_pages - 1u)];
+    };
+    auto load = [&](uint32_t i) {
+        const uint32_t tile = span.tile(i);
+#pragma unroll
+        for (uint32_t u = 0; u < NP; ++u)
+        {
+            const uint32_t e = u * 256u + tid, pg = e / (2u * HD);
+            if (N % 256u != 0u && e >= N) continue;
+            cur[u] = (tile * 4u + pg) * OPURE_PAGE_SIZE < sq.total && static_cast<uint32_t>(pe[u]) < p.n_pages ? pe[u] : -1;
+            const uint8_t* at = base + static_cast<uint64_t>(cur[u] < 0 ? 0u : static_cast<uint32_t>(cur[u])) * page_bytes + (e - pg * 2u * HD) * 16u;
+            kr[u] = *reinterpret_cast<const u4v*>(at);
+            vr[u] = *reinterpret_cast<const u4v*>(at + vofs);
+        }
+    };
+    auto store = [&](uint32_t i) {
+        const uint32_t t0 = span.tile(i) * PT;
+        u4v* k = kt + (i & 1u) * prompt_k_pieces<HD>();
+        u4v* v = vt + (i & 1u) * prompt_v_pieces<HD>();
+        const uint32_t nan = AF == OPURE_A_F16 ? 0x7E007E00u : 0x7FC07FC0u;
+        const bool tail = t0 + PT > sq.total;
+#pragma unroll
+        for (uint32_t u = 0; u < NP; ++u)
+        {
+            const uint32_t e = u * 256u + tid, pg = e / (2u * HD), w = e - pg * 2u * HD;
+            if (N % 256u != 0u && e >= N) continue;
+            // positions without a page: NaN keys for the rows that see them, no values;
+            // slots past the sequence hold anything: values 0
+            u4v x = vr[u];
+            const uint32_t tv = t0 + pg * OPURE_PAGE_SIZE + (w & 1u) * 8u;
+            if (tail) x = win_tail<AF>(x, tv < sq.total ? sq.total - tv : 0u);
+            x = cur[u] < 0 ? u4v{0u, 0u, 0u, 0u} : x;
+            const uint32_t t = e / P, at = (t & ~12u) | ((t & 4u) << 1) | ((t & 8u) >> 1);
+            k[at * KROW + e % P] = cur[u] < 0 ? u4v{nan, nan, nan, nan} : kr[u];
+            v[(w >> 1) * VROW + pg * 2u + (w & 1u)] = x;
+        }
+    };
+
+    f16_t o[DT];
+    float m = NEG_INF, l = 0.0f;
+#pragma unroll
+    for (uint32_t d = 0; d < DT; ++d)
+#pragma unroll
+        for (uint32_t i = 0; i < 16; ++i) o[d][i] = 0.0f;
+    if constexpr (HD % 32 != 0)
+    {
+        // the last channel tile's upper half is not there: zeros
+        for (uint32_t e = tid; e < 2u * 16u * VROW; e += 256u)
+            vt[(e / (16u * VROW)) * prompt_v_pieces<HD>() + HD * VROW + e % (16u * VROW)] = u4v{0u, 0u, 0u, 0u};
+    }
+    if (span.n)
+    {
+        entries(0u);
+        load(0u);
+        entries(1u);
+    }
+    for (uint32_t i = 0; i < span.n; ++i)
+    {
+        store(i);
+        __syncthreads();
+        if (i + 1u < span.n)
+        {
+            load(i + 1u);
+            entries(i + 2u);
+        }
+        const uint32_t t0 = span.tile(i) * PT;
+        // nothing of the tile that a row of the wave sees
+        if (t0 > pos1 || (t0 >= p.sinks && t0 + PT - 1u + p.window <= pos0)) continue;
+        const u4v* k = kt + (i & 1u) * prompt_k_pieces<HD>();
+        const u4v* v = vt + (i & 1u) * prompt_v_pieces<HD>();
+        f16_t s[2];
+#pragma unroll
+        for (uint32_t t = 0; t < 2; ++t)
+        {
+#pragma unroll
+            for (uint32_t x = 0; x < 16; ++x) s[t][x] = 0.0f;
+#pragma unroll
+            for (uint32_t x = 0; x < KS; ++x) s[t] = mfma_32<AF>(k[(32u * t + r) * KROW + 2u * x + h], q[x], s[t]);
+        }
+        if (t0 + PT > min(pos0 + 1u, sq.total) || !(t0 + PT <= p.sinks || t0 + p.window > pos1))
+        {
+#pragma unroll
+            for (uint32_t t = 0; t < 2; ++t)
+#pragma unroll
+                for (uint32_t x = 0; x < 16; ++x)
+                {
+                    const uint32_t at = t0 + 32u * t + 16u * (x >> 3) + 8u * h + (x & 7u);
+                    s[t][x] = at < sq.total && win_sees(p, pos, at) ? s[t][x] : NEG_INF;
+                }
+        }
+        float mx = s[0][0];
+#pragma unroll
+        for (uint32_t x = 1; x < 32; ++x) mx = fmaxf(mx, s[x >> 4][x & 15u]);
+        mx = __fmul_rn(max_xor32(mx), c);
+        if (__any(mx > m + 8.0f))
+        {
+            const float mn = fmaxf(m, mx), a = __builtin_amdgcn_exp2f(__fsub_rn(m, mn == NEG_INF ? 0.0f : mn));
+            l = __fmul_rn(l, a);
+#pragma unroll
+            for (uint32_t d = 0; d < DT; ++d)
+#pragma unroll
+                for (uint32_t x = 0; x < 16; ++x) o[d][x] = __fmul_rn(o[d][x], a);
+            m = mn;
+        }
+        const float ms = m == NEG_INF ? 0.0f : m - UP;
+        float sum[2] = {0.0f, 0.0f};
+        u4v w[4];
+#pragma unroll
+        for (uint32_t t = 0; t < 2; ++t)
+#pragma unroll
+            for (uint32_t x = 0; x < 16; x += 2)
+            {
+                const float e0 = __builtin_amdgcn_exp2f(__fmaf_rn(s[t][x], c, -ms)), e1 = __builtin_amdgcn_exp2f(__fmaf_rn(s[t][x + 1], c, -ms));
+                sum[0] += e0;
+                sum[1] += e1;
+                w[2u * t + (x >> 3)][(x & 7u) / 2u] = win_pack<AF>(e0, e1);
+            }
+        l += sum[0] + sum[1];                              // this half's share
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u)
+#pragma unroll
+            for (uint32_t d = 0; d < DT; ++d) o[d] = mfma_32<AF>(v[(32u * d + r) * VROW + 2u * u + h], w[u], o[d]);
+    }
+    l = add_xor32(l);
+    const bool mine = q0 + 32u * wave + r < Gq;
+    if (p.lse && h == 0u && mine) p.lse[(static_cast<uint64_t>(b) * p.n_kv + kh) * Gq + qi] = win_lse(m - UP, l);
+    const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+    bool fine = true;
+    typedef uint32_t u2v __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (uint32_t d = 0; d < DT; ++d)
+#pragma unroll
+        for (uint32_t x = 0; x < 16; x += 4)
+        {
+            const uint32_t ch = 32u * d + 2u * x + 4u * h;
+            if (HD % 32 != 0 && ch >= HD) continue;
+            float y[4];
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k)
+            {
+                y[k] = __fmul_rn(o[d][x + k], inv);
+                fine = fine && __builtin_isfinite(y[k]);
+            }
+            if (mine)
+                *reinterpret_cast<u2v*>(static_cast<uint8_t*>(p.out) + (row * HD + ch) * 2u) = u2v{win_pack<AF>(y[0], y[1]), win_pack<AF>(y[2], y[3])};
+        }
+    // rows that are not finite, position by position (k_win_join's reason)
+    uint64_t bad = __ballot(!fine && mine);
+    bad = (bad | bad >> 32) & 0xFFFFFFFFull;
+    __syncthreads();                                       // the stages are done with
+    float* qs = reinterpret_cast<float*>(lds) + wave * 256u;
+    while (bad)
+    {
+        const uint32_t x = static_cast<uint32_t>(__builtin_ctzll(bad));
+        bad &= bad - 1u;
+        const uint32_t qx = w0 + x, jx = qx / G;
+        const uint64_t rx = ((static_cast<uint64_t>(b) * p.rows + jx) * p.n_heads + kh * G + (qx - jx * G)) * HD;
+        for (uint32_t d = lane; d < HD; d += 64u) qs[d] = load_act_rt(p.q, rx + d, p.afmt);
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        float mm, ll, oo[4];
+        win_row(p, qs, b, kh, sq.ctx + jx, sq.total, mm, ll, oo);
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i)
+            if (lane + 64u * i < HD) store_act_rt(p.out, rx + lane + 64u * i, ll == 0.0f ? 0.0f : __fdiv_rn(oo[i], ll), p.afmt);
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    }
+}
+
+// Weights from many rows: a workgroup takes 64 positions (32 of an fp32 cache) of
+// a (sequence, KV head), its eight waves every eighth block of 16 query rows that
+// see one of them.  A wave holds the positions' keys as operands, computes the
+// block's scores again and adds 2^(score - lse) to a sum a lane and position; the
+// lanes' and waves' sums are added in order.  To store the scores instead would
+// take as many bytes as K and V together from 64 query rows of a KV head on.
+template <int AF, int HD>
+__global__ __launch_bounds__(512) void k_win_sums(WinParams p)
+{
+    typedef WinTile<AF, HD> T;
+    constexpr uint32_t NS = T::NS, TILE = 2u * T::TT;
+    __shared__ float part[8][TILE];
+    const uint32_t kh = blockIdx.x % p.n_kv, rest = blockIdx.x / p.n_kv, b = rest % p.blocks, tile = rest / p.blocks;   // blocks: the batch
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, g = lane >> 4, r = lane & 15u;
+    const uint32_t G = p.n_heads / p.n_kv, Gq = G * p.rows, t0 = tile * TILE;
+    const int32_t* pt = p.page_table + static_cast<uint64_t>(b) * p.max_pages;
+    const WinSeq sq = win_seq(p, p.seq_len[b]);
+    // rows ja .. jz - 1 see a position of the tile
+    const uint32_t ja = t0 > sq.ctx ? t0 - sq.ctx : 0u;
+    const uint32_t jz = t0 < p.sinks ? p.rows : t0 + TILE - 1u + p.window > sq.ctx ? min(p.rows, t0 + TILE - 1u + p.window - sq.ctx) : 0u;
+    if (t0 >= sq.total || ja >= jz) return;                // whole workgroup
+    const uint64_t page_bytes = 2ull * p.n_kv * T::PB;
+    const uint8_t* base = static_cast<const uint8_t*>(p.pool) + static_cast<uint64_t>(p.layer) * p.n_pages * page_bytes + static_cast<uint64_t>(kh) * T::PB;
+    T tl[2];
+    bool whole = t0 + TILE <= sq.total;
+#pragma unroll
+    for (uint32_t x = 0; x < 2; ++x)
+    {
+        int32_t pg[2];
+#pragma unroll
+        for (uint32_t y = 0; y < T::NB; ++y)
+        {
+            const uint32_t t = t0 + x * T::TT + y * OPURE_PAGE_SIZE;
+            const int32_t e = t < sq.total ? pt[t / OPURE_PAGE_SIZE] : -1;
+            pg[y] = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(e) < p.n_pages ? e : -1);
+        }
+        if (T::NB == 1u) pg[1] = pg[0];
+        auto at = [&](int32_t e) { return base + static_cast<uint64_t>(e < 0 ? 0u : static_cast<uint32_t>(e)) * page_bytes; };
+        tl[x].load_k(at(pg[0]), at(pg[1]), r, g);
+        const uint32_t nan = AF == OPURE_A_F32 ? 0x7FC00000u : AF == OPURE_A_F16 ? 0x7E007E00u : 0x7FC07FC0u;
+        const bool gone = (T::NB > 1u && r >= 8u ? pg[1] : pg[0]) < 0;
+        whole = whole && pg[0] >= 0 && pg[1] >= 0;
+#pragma unroll
+        for (uint32_t t = 0; t < T::NB; ++t)
+#pragma unroll
+            for (uint32_t s = 0; s < T::KS; ++s) tl[x].k[t][s] = gone ? u4v{nan, nan, nan, nan} : tl[x].k[t][s];
+    }
+    const float c = __fmul_rn(p.scale, 1.44269504088896340736f);
+    float sum[2][NS];
+#pragma unroll
+    for (uint32_t x = 0; x < 2; ++x)
+#pragma unroll
+        for (uint32_t y = 0; y < NS; ++y) sum[x][y] = 0.0f;
+    const uint32_t qa = ja * G, qz = min(jz * G, Gq);
+    const float* lse = p.lse + (static_cast<uint64_t>(b) * p.n_kv + kh) * Gq;
+    u4v q[T::KS], nq[T::KS];
+    float ls, nls;
+    uint32_t jr, njr;
+    auto fetch = [&](uint32_t q0, u4v (&to)[T::KS], float& l, uint32_t& j) {
+        const uint32_t qi = min(q0 + r, Gq - 1u);
+        j = qi / G;
+        win_load_q<AF, HD>(p, (static_cast<uint64_t>(b) * p.rows + j) * p.n_heads + kh * G + (qi - j * G), g, to);
+        l = q0 + r < qz ? lse[qi] : __builtin_huge_valf();  // a row past the last: weight 0
+    };
+    uint32_t q0 = qa + 16u * wave;
+    if (q0 < qz) fetch(q0, q, ls, jr);
+    for (; q0 < qz; q0 += 128u)
+    {
+        if (q0 + 128u < qz) fetch(q0 + 128u, nq, nls, njr);
+        const uint32_t p0 = sq.ctx + q0 / G, p1 = sq.ctx + min(q0 + 15u, Gq - 1u) / G;
+        const bool full = whole && t0 + TILE <= p0 + 1u && (t0 + TILE <= p.sinks || t0 + p.window > p1);
+        const bool ragged = q0 + 16u > qz, past = q0 + r >= qz;
+#pragma unroll
+        for (uint32_t x = 0; x < 2; ++x)
+        {
+            float s[NS];
+            win_scores<AF, HD>(p, tl[x], q, c, full, t0 + x * T::TT, g, sq.ctx + jr, sq.total, s);
+#pragma unroll
+            for (uint32_t y = 0; y < NS; ++y) s[y] = __builtin_amdgcn_exp2f(__fsub_rn(s[y], ls));
+            if (!full || ragged)
+            {
+                // what a row does not see adds nothing, whatever the row's sum is
+#pragma unroll
+                for (uint32_t y = 0; y < NS; ++y)
+                {
+                    const uint32_t t = t0 + x * T::TT + NS * g + y;
+                    s[y] = !past && t < sq.total && win_sees(p, sq.ctx + jr, t) ? s[y] : 0.0f;
+                }
+            }
+#pragma unroll
+            for (uint32_t y = 0; y < NS; ++y) sum[x][y] += s[y];
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < T::KS; ++k) q[k] = nq[k];
+        ls = nls;
+        jr = njr;
+    }
+#pragma unroll
+    for (uint32_t x = 0; x < 2; ++x)
+#pragma unroll
+        for (uint32_t y = 0; y < NS; ++y)
+        {
+            const float v = row16_sum(sum[x][y]);
+            if (r == 0u) part[wave][x * T::TT + NS * g + y] = v;
+        }
+    __syncthreads();
+    const uint32_t t = t0 + threadIdx.x;
+    if (threadIdx.x >= TILE || t >= sq.total) return;
+    // seen by a row: the last one at or past the position that it still reaches
+    const uint32_t first = t > sq.ctx ? t - sq.ctx : 0u;
+    if (first >= p.rows || !win_sees(p, sq.ctx + first, t)) return;
+    float v = part[0][threadIdx.x];
+#pragma unroll
+    for (uint32_t w = 1; w < 8; ++w) v += part[w][threadIdx.x];
+    p.weights[b * p.weights_batch_stride + static_cast<uint64_t>(kh) * p.weights_stride + t] += v;
+}
+
+}  // namespace
+
+namespace opure_win {
+
+int win_prompt_launch(opure_dev* dev, const WinParams& p, uint32_t batch)
+{
+    const uint32_t Gq = p.n_heads / p.n_kv * p.rows;
+    auto go = [&](auto af) {
+        return win_by_head(p.hd, [&](auto h) {
+            constexpr int AF = decltype(af)::value, HD = decltype(h)::value;
+            static std::atomic<uint64_t> done{0};
+            const int rc = opure_win::win_lds(dev, reinterpret_cast<const void*>(&k_win_prompt<AF, HD>), prompt_lds<HD>(), done);
+            if (rc) return rc;
+            OPURE_LAUNCH(dev, (k_win_prompt<AF, HD>), dim3(p.n_kv * ((Gq + 127u) / 128u) * batch), dim3(256), prompt_lds<HD>(), p);
+            OPURE_LAUNCH_CHECK("k_win_prompt");
+            return OPURE_OK;
+        });
+    };
+    return p.afmt == OPURE_A_F16 ? go(std::integral_constant<int, OPURE_A_F16>{}) : go(std::integral_constant<int, OPURE_A_BF16>{});
+}
+
+int win_sums_launch(opure_dev* dev, const WinParams& p, uint32_t batch, uint32_t max_ctx)
+{
+    WinParams s = p;
+    s.blocks = batch;
+    const uint32_t tile = p.afmt == OPURE_A_F32 ? 32u : 64u;
+    auto go = [&](auto af) {
+        return win_by_head(p.hd, [&](auto h) {
+            constexpr int AF = decltype(af)::value, HD = decltype(h)::value;
+            OPURE_LAUNCH(dev, (k_win_sums<AF, HD>), dim3(p.n_kv * batch * ((max_ctx + tile - 1u) / tile)), dim3(512), 0, s);
+            OPURE_LAUNCH_CHECK("k_win_sums");
+            return OPURE_OK;
+        });
+    };
+    return p.afmt == OPURE_A_F32   ? go(std::integral_constant<int, OPURE_A_F32>{})
+           : p.afmt == OPURE_A_F16 ? go(std::integral_constant<int, OPURE_A_F16>{})
+                                   : go(std::integral_constant<int, OPURE_A_BF16>{});
+}
+
+}  // namespace opure_win
