@@ -19,8 +19,8 @@ struct WinParams {
     const void* pool;
     const int32_t* page_table;
     const int32_t* seq_len;
-    float* part_acc;     // [batch][n_kv][parts][Gq][hd]: a part's unnormalised output of each query row
-    float* part_ml;      // [batch][n_kv][parts][Gq][2]: its maximum (in powers of two) and sum
+    float* part_acc;     // [slot][block_rows][hd]: a part's unnormalised output of its block's query rows
+    float* part_ml;      // [slot][block_rows][2]: their maxima (in powers of two) and sums
     float* scores;       // with weights: [batch][n_kv][tiles][Gq][tile's positions], in powers of two
     float* lse;          // with weights summed by k_win_sums: [batch][n_kv][Gq], log2 of each row's sum of 2^score
     float* weights;
@@ -29,7 +29,9 @@ struct WinParams {
     uint32_t n_heads, n_kv, hd, rows, n_pages, max_pages, layer, afmt;
     uint32_t window, sinks;       // window >= 1: 2^31 - 1 sees everything
     uint32_t cap;                 // positions that may be read: min(max_ctx, the table's)
-    uint32_t parts, blocks;       // parts a (sequence, KV head, block of query rows); such blocks
+    uint32_t blocks, block_rows;  // blocks of query rows a (sequence, KV head), and the most rows in one
+    uint32_t two;                 // blocks of 32 query rows, not 16
+    uint32_t parts;               // parts of each (sequence, KV head, block): slot part + parts * its index
     uint32_t tiles;               // most tiles a sequence's rows see
     uint32_t combine_rows;        // query rows of the call
     uint32_t combine_wgs;         // k_win_join: its first workgroups join the parts, the others add the weights
@@ -128,6 +130,15 @@ typedef float f4_t __attribute__((ext_vector_type(4)));
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 
+// a 16-byte load; ONCE: of bytes that no other workgroup reads, kept out of the way of those in the caches
+template <bool ONCE>
+__device__ __forceinline__ u4v win_load(const uint8_t* p)
+{
+    const u4v* q = reinterpret_cast<const u4v*>(p);
+    if constexpr (ONCE) return __builtin_nontemporal_load(q);
+    else return *q;
+}
+
 constexpr float NEG_INF = -__builtin_huge_valf();
 
 // The tiles (TT positions each) that the rows at ctx .. ctx + rows - 1 see: the
@@ -166,6 +177,7 @@ struct WinTile {
     u4v k[NB][KS], v[DT];
 
     __device__ __forceinline__ static float part(u4v x, uint32_t i) { return __uint_as_float(x[i]); }
+    template <bool ONCE>
     __device__ __forceinline__ void load_k(const uint8_t* a, const uint8_t* b, uint32_t r, uint32_t g)
     {
         const uint8_t* at = AF == OPURE_A_F32 || r < 8u ? a : b;
@@ -177,15 +189,16 @@ struct WinTile {
             for (uint32_t s = 0; s < KS; ++s)
             {
                 if (HALF && s + 1u == KS && g >= 2u) k[t][s] = u4v{0u, 0u, 0u, 0u};
-                else k[t][s] = *reinterpret_cast<const u4v*>(at + t * 4u * HD * EB + 64u * s);
+                else k[t][s] = win_load<ONCE>(at + t * 4u * HD * EB + 64u * s);
             }
     }
+    template <bool ONCE>
     __device__ __forceinline__ void load_v(const uint8_t* a, const uint8_t* b, uint32_t r, uint32_t g)
     {
         const uint8_t* at = AF == OPURE_A_F32 || g < 2u ? a : b;
         at += r * (16u * EB) + (AF == OPURE_A_F32 ? g : (g & 1u)) * 16u;
 #pragma unroll
-        for (uint32_t d = 0; d < DT; ++d) v[d] = *reinterpret_cast<const u4v*>(at + d * 16u * 16u * EB);
+        for (uint32_t d = 0; d < DT; ++d) v[d] = win_load<ONCE>(at + d * 16u * 16u * EB);
     }
 };
 

@@ -16,6 +16,8 @@ using namespace opure_win;
 
 namespace {
 
+constexpr uint32_t MAX_PARTS = 64;                         // of a (sequence, KV head, block of query rows): a lane of the joining wave each
+
 // Few query rows: a workgroup takes a part of the tiles that a sequence's rows
 // see, for 16 NT query rows of a KV head (row qi = j group + head), a wave every
 // fourth tile with a running maximum, sum and output of its own in registers.
@@ -26,17 +28,18 @@ namespace {
 //   A probability enters its product as two 16-bit numbers (its rounding and the
 // rest: 16 bits of bf16, 22 of fp16): the products are not what bounds this.
 template <int AF, int HD, int NT>
-__global__ __launch_bounds__(256) void k_win_split(WinParams p)
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 2 ? 2 : 1))) void k_win_split(WinParams p)
 {
     typedef WinTile<AF, HD> T;
     constexpr uint32_t TT = T::TT, DT = T::DT, NS = T::NS;
     extern __shared__ __align__(16) uint8_t lds[];
     f4_t* cacc = reinterpret_cast<f4_t*>(lds);                            // [wave][DT][NT][64]
     float* cml = reinterpret_cast<float*>(lds + 4u * DT * NT * 64u * 16u);   // [wave][NT][16][2]
-    const uint32_t kh = blockIdx.x % p.n_kv, rest = blockIdx.x / p.n_kv, part = rest % p.parts;
-    const uint32_t b = rest / p.parts / p.blocks, blk = rest / p.parts - b * p.blocks;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, g = lane >> 4, r = lane & 15u;
-    const uint32_t G = p.n_heads / p.n_kv, Gq = G * p.rows, q0 = blk * 16u * NT;
+    const uint32_t G = p.n_heads / p.n_kv, Gq = G * p.rows;
+    // KV heads next to each other, then parts, blocks and sequences
+    const uint32_t kh = blockIdx.x % p.n_kv, rest = blockIdx.x / p.n_kv, part = rest % p.parts;
+    const uint32_t b = rest / p.parts / p.blocks, blk = rest / p.parts - b * p.blocks, q0 = blk * 16u * NT;
     const int32_t* pt = p.page_table + static_cast<uint64_t>(b) * p.max_pages;
     const int32_t len = p.seq_len[b];
     u4v q[NT][T::KS];
@@ -82,8 +85,8 @@ __global__ __launch_bounds__(256) void k_win_split(WinParams p)
         int32_t e = entry(i);
         int32_t pa = page(e, i, 0u), pb = T::NB > 1u ? page(e, i, 1u) : pa;
         auto at = [&](int32_t pg) { return kbase + static_cast<uint64_t>(pg < 0 ? 0u : static_cast<uint32_t>(pg)) * page_bytes; };
-        tl.load_k(at(pa), at(pb), r, g);
-        tl.load_v(at(pa) + vofs, at(pb) + vofs, r, g);
+        tl.template load_k<NT == 1>(at(pa), at(pb), r, g);
+        tl.template load_v<NT == 1>(at(pa) + vofs, at(pb) + vofs, r, g);
         e = entry(i + 4u);
         while (true)
         {
@@ -106,7 +109,7 @@ __global__ __launch_bounds__(256) void k_win_split(WinParams p)
             float s[NT][NS];
 #pragma unroll
             for (uint32_t n = 0; n < NT; ++n) win_scores<AF, HD>(p, tl, q[n], c, full, t0, g, sq.ctx + jr[n], sq.total, s[n]);
-            if (more) tl.load_k(at(na), at(nb), r, g);
+            if (more) tl.template load_k<NT == 1>(at(na), at(nb), r, g);
             if (p.scores)
 #pragma unroll
                 for (uint32_t n = 0; n < NT; ++n)
@@ -166,7 +169,7 @@ __global__ __launch_bounds__(256) void k_win_split(WinParams p)
                     o[d][n] = win_mfma<AF>(tl.v[d], hi[n], o[d][n]);
                 }
             if (!more) break;
-            tl.load_v(at(na) + vofs, at(nb) + vofs, r, g);
+            tl.template load_v<NT == 1>(at(na) + vofs, at(nb) + vofs, r, g);
             pa = na;
             pb = nb;
             i += 4u;
@@ -187,11 +190,11 @@ __global__ __launch_bounds__(256) void k_win_split(WinParams p)
         }
     }
     __syncthreads();
-    const uint64_t pbase = ((static_cast<uint64_t>(b) * p.n_kv + kh) * p.parts + part) * Gq;
+    const uint64_t pbase = (((static_cast<uint64_t>(b) * p.n_kv + kh) * p.blocks + blk) * p.parts + part) * p.block_rows;
 #pragma unroll
     for (uint32_t n = 0; n < NT; ++n)
     {
-        const uint32_t qi = q0 + 16u * n + r;
+        const uint32_t qi = 16u * n + r;                     // of the block
         float mw[4], w[4], M = NEG_INF, L = 0.0f;
 #pragma unroll
         for (uint32_t x = 0; x < 4; ++x)
@@ -205,7 +208,7 @@ __global__ __launch_bounds__(256) void k_win_split(WinParams p)
             w[x] = __builtin_amdgcn_exp2f(__fsub_rn(mw[x], M == NEG_INF ? 0.0f : M));
             L = __fmaf_rn(w[x], cml[((x * NT + n) * 16u + r) * 2u + 1u], L);
         }
-        if (qi >= Gq) continue;
+        if (q0 + qi >= Gq) continue;
         if (wave == 0u && g == 0u)
         {
             p.part_ml[(pbase + qi) * 2u] = M;
@@ -228,144 +231,223 @@ __global__ __launch_bounds__(256) void k_win_split(WinParams p)
     }
 }
 
-// A row's result from its parts' maxima and sums: lane x holds part x's weight.
-__device__ __forceinline__ void win_join(const WinParams& p, uint64_t pbase, uint32_t Gq, uint32_t qi, uint32_t lane, float& M, float& w, float& L)
+// A query row's maximum M and sum L over its parts, lane x holding part x's.
+__device__ __forceinline__ void win_total(float m, float l, uint32_t parts, uint32_t lane, float& M, float& w, float& L)
 {
-    const uint64_t at = (pbase + static_cast<uint64_t>(min(lane, p.parts - 1u)) * Gq + qi) * 2u;
-    const float m = p.part_ml[at], l = p.part_ml[at + 1u];
-    M = wave_max64(m);
-    w = lane < p.parts ? __builtin_amdgcn_exp2f(__fsub_rn(m, M == NEG_INF ? 0.0f : M)) : 0.0f;
-    L = wave_sum64(__fmul_rn(w, l));
+    M = wave_max64(lane < parts ? m : NEG_INF);
+    w = lane < parts ? __builtin_amdgcn_exp2f(__fsub_rn(m, M == NEG_INF ? 0.0f : M)) : 0.0f;
+    L = wave_sum64(lane < parts ? __fmul_rn(w, l) : 0.0f);
 }
 
-// Joins the parts, a wave a query row: lanes over the parts for the weights, over
-// channels for the output.  A row that is not finite is computed again position
+// Joins the parts: a workgroup a query row (WIDE: many parts, a wave every fourth
+// one) or four rows (a wave each); DPL channels a lane.  A lane takes a part's
+// maximum and sum, then channels.  Loads are unconditional (past the last part
+// the last one again, weight 0): the code stays small, and a launch this short
+// pays for every line of it.  A row that is not finite is computed again position
 // by position: a NaN or an infinity among the values of a position that the row
-// does not see meets weight 0 in the products above.  With weights, the launch's
-// other workgroups add them: a thread a position, over the query rows in order.
-template <uint32_t TT>
+// does not see meets weight 0 in the products above.  With scores, the launch's
+// other workgroups add the weights: PPT positions a thread (one where there are few),
+// over the query rows in order, 32 / PPT rows' maxima and sums at a time.
+template <uint32_t TT, bool WIDE, uint32_t DPL, uint32_t PPT>
 __global__ __launch_bounds__(256) void k_win_join(WinParams p)
 {
     __shared__ float sm[4][256];
-    const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63u, G = p.n_heads / p.n_kv, Gq = G * p.rows;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, G = p.n_heads / p.n_kv, Gq = G * p.rows;
+    const uint32_t shift = p.two ? 5u : 4u;                // a block's query rows
     if (blockIdx.x < p.combine_wgs)
     {
-        const uint64_t id = 4ull * blockIdx.x + wave;
-        if (id >= p.combine_rows) return;
-        const uint32_t head = static_cast<uint32_t>(id % p.n_heads), row = static_cast<uint32_t>(id / p.n_heads), b = row / p.rows, j = row - b * p.rows;
-        const uint32_t kh = head / G, qi = j * G + (head - kh * G);
-        const uint64_t pbase = (static_cast<uint64_t>(b) * p.n_kv + kh) * p.parts * Gq;
-        float M, w, L, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        win_join(p, pbase, Gq, qi, lane, M, w, L);
-        for (uint32_t x = 0; x < p.parts; ++x)
-        {
-            const float wx = __shfl(w, x);
-            const float* acc = p.part_acc + (pbase + static_cast<uint64_t>(x) * Gq + qi) * p.hd;
+        const uint32_t id = WIDE ? blockIdx.x : 4u * blockIdx.x + wave;
+        if (id >= p.combine_rows) return;                  // never with WIDE: the barrier below
+        const uint32_t row = id / p.n_heads, head = id - row * p.n_heads, b = row / p.rows, j = row - b * p.rows;
+        const uint32_t kh = head / G, qi = j * G + (head - kh * G), blk = qi >> shift, qb = qi - (blk << shift);
+        const uint32_t parts = p.parts, end = parts - 1u;
+        const uint64_t slot = ((static_cast<uint64_t>(b) * p.n_kv + kh) * p.blocks + blk) * parts;
+        const uint64_t ml = ((slot + min(lane, end)) * p.block_rows + qb) * 2u;
+        const float pm = p.part_ml[ml], pl = p.part_ml[ml + 1u];
+        constexpr uint32_t U = WIDE ? 8u : 4u, BY = WIDE ? 4u : 1u;
+        const uint32_t x0 = WIDE ? wave : 0u;
+        float v[U][DPL], o[DPL];
+        auto fetch = [&](uint32_t x) {
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i)
-                if (lane + 64u * i < p.hd) o[i] = __fmaf_rn(wx, acc[lane + 64u * i], o[i]);
+            for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+                for (uint32_t i = 0; i < DPL; ++i)
+                    v[u][i] = p.part_acc[((slot + min(x + BY * u, end)) * p.block_rows + qb) * p.hd + min(lane + 64u * i, p.hd - 1u)];
+        };
+        fetch(x0);
+        float M, w, L;
+        win_total(pm, pl, parts, lane, M, w, L);
+#pragma unroll
+        for (uint32_t i = 0; i < DPL; ++i) o[i] = 0.0f;
+        for (uint32_t x = x0; x < parts; x += BY * U)
+        {
+            if (x != x0) fetch(x);
+#pragma unroll
+            for (uint32_t u = 0; u < U; ++u)
+            {
+                const uint32_t y = x + BY * u;
+                const float wx = y < parts ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), min(y, 63u))) : 0.0f;
+#pragma unroll
+                for (uint32_t i = 0; i < DPL; ++i) o[i] = __fmaf_rn(wx, v[u][i], o[i]);
+            }
+        }
+        if constexpr (WIDE)
+        {
+#pragma unroll
+            for (uint32_t i = 0; i < DPL; ++i) sm[wave][lane + 64u * i] = o[i];
+            __syncthreads();
+            if (wave != 0u) return;
+#pragma unroll
+            for (uint32_t i = 0; i < DPL; ++i) o[i] = (sm[0][lane + 64u * i] + sm[1][lane + 64u * i]) + (sm[2][lane + 64u * i] + sm[3][lane + 64u * i]);
+            __builtin_amdgcn_wave_barrier();
         }
         if (p.lse && lane == 0u) p.lse[(static_cast<uint64_t>(b) * p.n_kv + kh) * Gq + qi] = win_lse(M, L);
         bool fine = true;
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i)
+        for (uint32_t i = 0; i < DPL; ++i)
         {
             o[i] = L == 0.0f ? 0.0f : __fdiv_rn(o[i], L);
-            fine = fine && __builtin_isfinite(o[i]);
+            fine = fine && (__builtin_isfinite(o[i]) || lane + 64u * i >= p.hd);
         }
-        const uint64_t at = (static_cast<uint64_t>(row) * p.n_heads + head) * p.hd;
+        const uint64_t at = static_cast<uint64_t>(id) * p.hd;
         if (!__all(fine))
         {
             for (uint32_t d = lane; d < p.hd; d += 64u) sm[wave][d] = load_act_rt(p.q, at + d, p.afmt);
             __builtin_amdgcn_wave_barrier();
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             const WinSeq sq = win_seq(p, p.seq_len[b]);
-            float m, l;
-            win_row(p, sm[wave], b, kh, sq.ctx + j, sq.total, m, l, o);
+            float m, l, x[4];
+            win_row(p, sm[wave], b, kh, sq.ctx + j, sq.total, m, l, x);
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) o[i] = l == 0.0f ? 0.0f : __fdiv_rn(o[i], l);
+            for (uint32_t i = 0; i < DPL; ++i) o[i] = l == 0.0f ? 0.0f : __fdiv_rn(x[i], l);
         }
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i)
+        for (uint32_t i = 0; i < DPL; ++i)
             if (lane + 64u * i < p.hd) store_act_rt(p.out, at + lane + 64u * i, o[i], p.afmt);
         return;
     }
-    // ---- weights: 256 positions of a (sequence, KV head)
-    const uint32_t per = (p.tiles * TT + 255u) / 256u, id = blockIdx.x - p.combine_wgs;
-    const uint32_t x = id % per, bh = id / per, kh = bh % p.n_kv, b = bh / p.n_kv;
+    // ---- weights: 256 PPT positions of a (sequence, KV head)
+    typedef float vec_t __attribute__((ext_vector_type(PPT)));
+    const uint32_t per = (p.tiles * TT + 256u * PPT - 1u) / (256u * PPT), id = blockIdx.x - p.combine_wgs;
+    const uint32_t bh = id / per, x = id - bh * per, b = bh / p.n_kv, kh = bh - b * p.n_kv;
     const WinSeq sq = win_seq(p, p.seq_len[b]);
     const WinSpan span = win_span<TT>(p, sq, sq.ctx, sq.ctx + p.rows);
-    if (x * 256u >= span.n * TT) return;                      // whole workgroup
-    const uint32_t at = x * 256u + threadIdx.x, i = at / TT, off = at - i * TT;
-    const uint32_t t = i < span.n ? span.tile(i) * TT + off : sq.total;
-    const bool in = t < sq.total;
-    const uint64_t pbase = static_cast<uint64_t>(bh) * p.parts * Gq;
-    const float* s = p.scores + ((static_cast<uint64_t>(bh) * p.tiles + (in ? i : 0u)) * Gq) * TT + off;
-    float sum = 0.0f;
-    bool any = false;
-    for (uint32_t c0 = 0; c0 < Gq; c0 += 128u)
+    if (x * 256u * PPT >= span.n * TT) return;                // whole workgroup
+    const uint32_t at = (x * 256u + threadIdx.x) * PPT, i = min(at / TT, span.n - 1u), off = at % TT;
+    const uint32_t t = at < span.n * TT ? span.tile(i) * TT + off : sq.total;
+    const float* s = p.scores + (static_cast<uint64_t>(bh) * p.tiles + i) * Gq * TT + off;
+    float sum[PPT];
+    bool any[PPT];
+#pragma unroll
+    for (uint32_t k = 0; k < PPT; ++k)
     {
-        const uint32_t n = min(128u, Gq - c0);
-        __syncthreads();
-        for (uint32_t y = wave; y < n; y += 4u)
-        {
-            float M, w, L;
-            win_join(p, pbase, Gq, c0 + y, lane, M, w, L);
-            if (lane == 0u)
+        sum[k] = 0.0f;
+        any[k] = false;
+    }
+    uint32_t j = 0, g = 0;                                    // the query row's row and head
+    constexpr uint32_t U = 8u / PPT, C = 4u * U;              // rows a wave; a turn
+    for (uint32_t c0 = 0; c0 < Gq; c0 += C)
+    {
+        vec_t v[C];
+        float pm[U], pl[U];
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u)
+            if (c0 + 4u * u < Gq)
             {
-                sm[0][y] = M == NEG_INF ? 0.0f : M;
-                sm[1][y] = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);
+                const uint32_t qi = min(c0 + 4u * u + wave, Gq - 1u), blk = qi >> shift;
+                const uint64_t slot = (static_cast<uint64_t>(bh) * p.blocks + blk) * p.parts + min(lane, p.parts - 1u);
+                const uint64_t ml = (slot * p.block_rows + (qi - (blk << shift))) * 2u;
+                pm[u] = p.part_ml[ml];
+                pl[u] = p.part_ml[ml + 1u];
             }
-        }
-        __syncthreads();
-        if (in)
-            for (uint32_t y = 0; y < n; ++y)
+#pragma unroll
+        for (uint32_t y = 0; y < C; ++y)
+            if (c0 + y < Gq) v[y] = *reinterpret_cast<const vec_t*>(s + static_cast<uint64_t>(c0 + y) * TT);
+        if (c0) __syncthreads();
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u)
+            if (c0 + 4u * u < Gq)
             {
-                const float v = s[static_cast<uint64_t>(c0 + y) * TT];
-                const bool sees = win_sees(p, sq.ctx + (c0 + y) / G, t);
-                any = any || sees;
-                sum += sees ? __fmul_rn(__builtin_amdgcn_exp2f(__fsub_rn(v, sm[0][y])), sm[1][y]) : 0.0f;
+                float M, w, L;
+                win_total(pm[u], pl[u], p.parts, lane, M, w, L);
+                if (lane == 0u)
+                {
+                    sm[0][4u * u + wave] = M == NEG_INF ? 0.0f : M;
+                    sm[1][4u * u + wave] = L == 0.0f ? 0.0f : __fdiv_rn(1.0f, L);
+                }
+            }
+        __syncthreads();
+#pragma unroll
+        for (uint32_t y = 0; y < C; ++y)
+            if (c0 + y < Gq)
+            {
+                const float m = sm[0][y], inv = sm[1][y];
+#pragma unroll
+                for (uint32_t k = 0; k < PPT; ++k)
+                {
+                    const bool sees = t + k < sq.total && win_sees(p, sq.ctx + j, t + k);
+                    any[k] = any[k] || sees;
+                    sum[k] += sees ? __fmul_rn(__builtin_amdgcn_exp2f(__fsub_rn(v[y][k], m)), inv) : 0.0f;
+                }
+                const bool wrap = g + 1u == G;
+                g = wrap ? 0u : g + 1u;
+                j += wrap ? 1u : 0u;
             }
     }
-    if (in && any) p.weights[b * p.weights_batch_stride + static_cast<uint64_t>(kh) * p.weights_stride + t] += sum;
+    float* to = p.weights + b * p.weights_batch_stride + static_cast<uint64_t>(kh) * p.weights_stride + t;
+#pragma unroll
+    for (uint32_t k = 0; k < PPT; ++k)
+        if (any[k]) to[k] += sum[k];
 }
 
-template <int AF, int HD, int NT>
-int win_split_launch(opure_dev* dev, const WinParams& p, uint32_t batch)
-{
-    constexpr uint32_t lds = 4u * (HD / 16u) * NT * 64u * 16u + 4u * NT * 16u * 2u * 4u;
-    static std::atomic<uint64_t> done{0};
-    const int rc = win_lds(dev, reinterpret_cast<const void*>(&k_win_split<AF, HD, NT>), lds, done);
-    if (rc) return rc;
-    OPURE_LAUNCH(dev, (k_win_split<AF, HD, NT>), dim3(p.n_kv * p.parts * batch * p.blocks), dim3(256), lds, p);
-    OPURE_LAUNCH_CHECK("k_win_split");
-    return OPURE_OK;
-}
+template <int HD, int NT>
+constexpr uint32_t win_split_lds() { return 4u * (HD / 16u) * NT * 64u * 16u + 4u * NT * 16u * 2u * 4u; }
 
-template <int AF>
-int win_split_any(opure_dev* dev, const WinParams& p, uint32_t batch, bool two)
+// f(kernel, dynamic LDS, workgroups of it that the device holds at a time) for a head size and format
+template <typename F>
+int win_split_kernel(opure_dev* dev, uint32_t afmt, uint32_t hd, bool two, F&& f)
 {
-    return win_by_head(p.hd, [&](auto h) {
-        constexpr int HD = decltype(h)::value;
-        if constexpr (HD <= 128)
-            if (two) return win_split_launch<AF, HD, 2>(dev, p, batch);
-        return win_split_launch<AF, HD, 1>(dev, p, batch);
-    });
+    auto one = [&](auto af, auto h, auto nt) {
+        constexpr int AF = decltype(af)::value, HD = decltype(h)::value, NT = decltype(nt)::value;
+        static std::atomic<uint64_t> done{0};
+        static std::atomic<int> a_cu{0};
+        auto* kernel = &k_win_split<AF, HD, NT>;
+        const int rc = win_lds(dev, reinterpret_cast<const void*>(kernel), win_split_lds<HD, NT>(), done);
+        if (rc) return rc;
+        int n = a_cu.load(std::memory_order_relaxed);
+        if (n == 0)
+        {
+            OPURE_HIP_TRY(hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, 256, win_split_lds<HD, NT>()));
+            n = std::max(n, 1);
+            a_cu.store(n, std::memory_order_relaxed);
+        }
+        return f(kernel, win_split_lds<HD, NT>(), static_cast<uint32_t>(n) * (dev->n_cu > 0 ? static_cast<uint32_t>(dev->n_cu) : 256u));
+    };
+    auto by_head = [&](auto af) {
+        return win_by_head(hd, [&](auto h) {
+            if constexpr (decltype(h)::value <= 128)
+                if (two) return one(af, h, std::integral_constant<int, 2>{});
+            return one(af, h, std::integral_constant<int, 1>{});
+        });
+    };
+    return afmt == OPURE_A_F32   ? by_head(std::integral_constant<int, OPURE_A_F32>{})
+           : afmt == OPURE_A_F16 ? by_head(std::integral_constant<int, OPURE_A_F16>{})
+                                 : by_head(std::integral_constant<int, OPURE_A_BF16>{});
 }
 
 // How a call is split, and its workspace.
 struct WinPlan {
-    uint32_t tt, tiles, blocks, parts;
-    bool prompt, two, stored;     // the prompt kernel; split: 32 query rows a workgroup; weights from stored scores
-    uint64_t acc, ml, scores, lse;   // bytes
+    uint32_t tt = 0, tiles = 0, blocks = 0, block_rows = 0, parts = 0;
+    bool prompt = false;                                 // the prompt kernel
+    bool two = false, stored = false, four = false;      // split: 32 query rows a workgroup; weights from stored scores, four positions a thread
+    uint64_t acc = 0, ml = 0, scores = 0, lse = 0;       // bytes
     uint64_t bytes() const { return acc + ml + scores + lse; }
 };
 
-WinPlan win_plan(const opure_dev* dev, const opure_attn_window_args* a)
+int win_plan(opure_dev* dev, const opure_attn_window_args* a, WinPlan& w)
 {
     const opure_model* m = a->model;
-    const uint32_t Gq = m->n_heads / m->n_kv_heads * a->rows, n_cu = dev->n_cu > 0 ? static_cast<uint32_t>(dev->n_cu) : 256u;
-    WinPlan w{};
+    const uint32_t Gq = m->n_heads / m->n_kv_heads * a->rows;
     w.tt = m->afmt == OPURE_A_F32 ? 16u : 32u;
     // tiles of any sequence of the call: its sinks', then the window's and the rows', which begin anywhere in a tile
     const uint64_t all = (a->max_ctx + w.tt - 1u) / w.tt, window = a->window ? a->window : 0x7FFFFFFFu;
@@ -374,16 +456,31 @@ WinPlan win_plan(const opure_dev* dev, const opure_attn_window_args* a)
     w.prompt = m->afmt != OPURE_A_F32 && Gq >= 256u;
     w.stored = a->weights && Gq <= 64u;
     w.lse = a->weights && !w.stored ? opure_hip::align_up(rows * 4u, 256) : 0u;
-    if (w.prompt) return w;
+    if (w.prompt) return OPURE_OK;
     w.two = Gq > 16u && m->head_dim <= 128u;
     w.blocks = (Gq + (w.two ? 31u : 15u)) / (w.two ? 32u : 16u);
+    w.block_rows = std::min(Gq, w.two ? 32u : 16u);
+    uint32_t room = 0;
+    const int rc = win_split_kernel(dev, m->afmt, m->head_dim, w.two, [&](auto, uint32_t, uint32_t n) {
+        room = n;
+        return OPURE_OK;
+    });
+    if (rc) return rc;
     const uint64_t groups = static_cast<uint64_t>(a->batch) * m->n_kv_heads * w.blocks;
-    const uint64_t want = (4ull * n_cu + groups - 1u) / groups;
-    w.parts = static_cast<uint32_t>(std::min<uint64_t>(want, std::min((w.tiles + 3u) / 4u, 64u)));
-    w.acc = opure_hip::align_up(rows * w.parts * m->head_dim * 4u, 256);
-    w.ml = opure_hip::align_up(rows * w.parts * 8u, 256);
+    // Parts of a group: as many as the device holds at a time, each of at least four tiles (one a wave), or of so many
+    // that the part's outputs, written and read again, stay a quarter of its keys and values (24 rows of 8B heads over
+    // 66 tiles: 16 parts 26.9 us, 11 24.9, 8 24.7); three times as many where a wave still has four tiles, which evens
+    // out ragged sequences (16 sequences of 2,000 to 8,000: 2 parts 91.5 us, 4 77.6, 12 73.4)
+    const uint32_t least = std::max(4u, w.block_rows / 4u);
+    const uint64_t fill = std::max<uint64_t>(1u, room / groups), more = std::min<uint64_t>(3ull * room / groups, w.tiles / 16u);
+    w.parts = static_cast<uint32_t>(std::min<uint64_t>(std::max(fill, more), std::min((w.tiles + least - 1u) / least, MAX_PARTS)));
+    const uint64_t wide = static_cast<uint64_t>(a->batch) * m->n_kv_heads * ((static_cast<uint64_t>(w.tiles) * w.tt + 1023u) / 1024u);
+    w.four = wide >= 2ull * (dev->n_cu > 0 ? static_cast<uint32_t>(dev->n_cu) : 256u);
+    const uint64_t slots = groups * w.parts * w.block_rows;
+    w.acc = opure_hip::align_up(slots * m->head_dim * 4u, 256);
+    w.ml = opure_hip::align_up(slots * 8u, 256);
     w.scores = w.stored ? opure_hip::align_up(rows * w.tiles * w.tt * 4u, 256) : 0u;
-    return w;
+    return OPURE_OK;
 }
 
 int win_validate(const opure_attn_window_args* a)
@@ -433,7 +530,9 @@ extern "C" int opure_attn_window_reserve(opure_dev* dev, const opure_attn_window
     const int rc = win_validate(a);
     if (rc) return rc;
     const DeviceGuard on(dev);
-    return ensure_workspace(dev, win_plan(dev, a).bytes());
+    WinPlan w;
+    const int rp = win_plan(dev, a, w);
+    return rp ? rp : ensure_workspace(dev, w.bytes());
 }
 
 extern "C" int opure_attn_window_paged(opure_dev* dev, const opure_attn_window_args* a)
@@ -445,7 +544,9 @@ extern "C" int opure_attn_window_paged(opure_dev* dev, const opure_attn_window_a
                       ((reinterpret_cast<uintptr_t>(a->seq_len) | reinterpret_cast<uintptr_t>(a->weights)) & 3u) == 0u,
                   OPURE_E_INVALID, "opure_attn_window_paged: q must be 16-byte aligned, out 8-byte, seq_len and weights 4-byte");
     const DeviceGuard on(dev);
-    const WinPlan w = win_plan(dev, a);
+    WinPlan w;
+    rc = win_plan(dev, a, w);
+    if (rc) return rc;
     rc = ensure_workspace(dev, w.bytes());
     if (rc) return rc;
     WinParams p{};
@@ -476,21 +577,45 @@ extern "C" int opure_attn_window_paged(opure_dev* dev, const opure_attn_window_a
     p.err = dev->err;
     p.parts = w.parts;
     p.blocks = w.blocks;
+    p.block_rows = w.block_rows;
+    p.two = w.two ? 1u : 0u;
     p.tiles = w.tiles;
     p.combine_rows = a->batch * a->rows * p.n_heads;
-    p.combine_wgs = (p.combine_rows + 3u) / 4u;
     if (w.prompt)
     {
         rc = win_prompt_launch(dev, p, a->batch);
         return rc || !p.lse ? rc : win_sums_launch(dev, p, a->batch, a->max_ctx);
     }
-    rc = p.afmt == OPURE_A_F32   ? win_split_any<OPURE_A_F32>(dev, p, a->batch, w.two)
-         : p.afmt == OPURE_A_F16 ? win_split_any<OPURE_A_F16>(dev, p, a->batch, w.two)
-                                 : win_split_any<OPURE_A_BF16>(dev, p, a->batch, w.two);
+    const uint32_t wgs = p.n_kv * w.parts * w.blocks * a->batch;
+    rc = win_split_kernel(dev, p.afmt, p.hd, w.two, [&](auto kernel, uint32_t lds, uint32_t) {
+        OPURE_LAUNCH(dev, kernel, dim3(wgs), dim3(256), lds, p);
+        OPURE_LAUNCH_CHECK("k_win_split");
+        return OPURE_OK;
+    });
     if (rc) return rc;
-    const uint32_t sums = p.scores ? (w.tiles * w.tt + 255u) / 256u * p.n_kv * a->batch : 0u;
-    if (w.tt == 16u) OPURE_LAUNCH(dev, (k_win_join<16u>), dim3(p.combine_wgs + sums), dim3(256), 0, p);
-    else OPURE_LAUNCH(dev, (k_win_join<32u>), dim3(p.combine_wgs + sums), dim3(256), 0, p);
+    const uint32_t sums = p.scores ? (w.tiles * w.tt + (w.four ? 1023u : 255u)) / (w.four ? 1024u : 256u) * p.n_kv * a->batch : 0u;
+    const bool wide = w.parts > 8u;
+    p.combine_wgs = wide ? p.combine_rows : (p.combine_rows + 3u) / 4u;
+    auto join = [&](auto tt, auto all, auto ppt) {
+        constexpr uint32_t TT = decltype(tt)::value, PPT = decltype(ppt)::value;
+        constexpr bool WIDE = decltype(all)::value;
+        const dim3 grid(p.combine_wgs + sums), block(256);
+        switch ((p.hd + 63u) / 64u)
+        {
+        case 1: OPURE_LAUNCH(dev, (k_win_join<TT, WIDE, 1, PPT>), grid, block, 0, p); break;
+        case 2: OPURE_LAUNCH(dev, (k_win_join<TT, WIDE, 2, PPT>), grid, block, 0, p); break;
+        case 3: OPURE_LAUNCH(dev, (k_win_join<TT, WIDE, 3, PPT>), grid, block, 0, p); break;
+        default: OPURE_LAUNCH(dev, (k_win_join<TT, WIDE, 4, PPT>), grid, block, 0, p); break;
+        }
+    };
+    typedef std::integral_constant<uint32_t, 1> One;
+    typedef std::integral_constant<uint32_t, 4> Four;
+    auto join_tt = [&](auto tt) {
+        if (w.four) wide ? join(tt, std::true_type{}, Four{}) : join(tt, std::false_type{}, Four{});
+        else wide ? join(tt, std::true_type{}, One{}) : join(tt, std::false_type{}, One{});
+    };
+    if (w.tt == 16u) join_tt(std::integral_constant<uint32_t, 16>{});
+    else join_tt(std::integral_constant<uint32_t, 32>{});
     OPURE_LAUNCH_CHECK("k_win_join");
     return p.lse ? win_sums_launch(dev, p, a->batch, a->max_ctx) : OPURE_OK;
 }

@@ -289,7 +289,7 @@ __global__ __launch_bounds__(512) void k_win_sums(WinParams p)
         }
         if (T::NB == 1u) pg[1] = pg[0];
         auto at = [&](int32_t e) { return base + static_cast<uint64_t>(e < 0 ? 0u : static_cast<uint32_t>(e)) * page_bytes; };
-        tl[x].load_k(at(pg[0]), at(pg[1]), r, g);
+        tl[x].template load_k<false>(at(pg[0]), at(pg[1]), r, g);
         const uint32_t nan = AF == OPURE_A_F32 ? 0x7FC00000u : AF == OPURE_A_F16 ? 0x7E007E00u : 0x7FC07FC0u;
         const bool gone = (T::NB > 1u && r >= 8u ? pg[1] : pg[0]) < 0;
         whole = whole && pg[0] >= 0 && pg[1] >= 0;
