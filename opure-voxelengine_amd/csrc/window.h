@@ -29,6 +29,7 @@ struct WinParams {
     uint32_t n_heads, n_kv, hd, rows, n_pages, max_pages, layer, afmt;
     uint32_t window, sinks;       // window >= 1: 2^31 - 1 sees everything
     uint32_t cap;                 // positions that may be read: min(max_ctx, the table's)
+    uint32_t batch;               // k_win_sums: sequences
     uint32_t blocks, block_rows;  // blocks of query rows a (sequence, KV head), and the most rows in one
     uint32_t two;                 // blocks of 32 query rows, not 16
     uint32_t parts;               // parts of each (sequence, KV head, block): slot part + parts * its index
@@ -295,6 +296,21 @@ __device__ __forceinline__ u4v win_tail(u4v v, uint32_t n)
     return v;
 }
 
+// What a row sees of the positions from `base` on, base + y being visible where
+// y <= end and (y < sinks or y >= low): y is a constant, so a mask is three
+// comparisons with one, and nothing of it has to be kept across a loop.
+struct WinMask {
+    int32_t end, sinks, low;
+    __device__ __forceinline__ WinMask(const WinParams& p, uint32_t pos, uint32_t total, uint32_t base)
+    {
+        const uint32_t first = pos + 1u > p.window ? pos + 1u - p.window : 0u;
+        end = static_cast<int32_t>(min(pos + 1u, total)) - 1 - static_cast<int32_t>(base);
+        sinks = static_cast<int32_t>(p.sinks) - static_cast<int32_t>(base);
+        low = static_cast<int32_t>(min(first, 0x7FFFFFFFu)) - static_cast<int32_t>(base);
+    }
+    __device__ __forceinline__ bool sees(int32_t y) const { return y <= end && (y < sinks || y >= low); }
+};
+
 // One tile's scores of a block of query rows, in powers of two (scale log2 e q.k),
 // -inf where the row at `pos` does not see the position.
 template <int AF, int HD>
@@ -314,12 +330,9 @@ __device__ __forceinline__ void win_scores(const WinParams& p, const WinTile<AF,
     }
     if (!full)
     {
+        const WinMask m(p, pos, total, t0 + T::NS * g);
 #pragma unroll
-        for (uint32_t i = 0; i < T::NS; ++i)
-        {
-            const uint32_t t = t0 + T::NS * g + i;
-            s[i] = t < total && win_sees(p, pos, t) ? s[i] : NEG_INF;
-        }
+        for (uint32_t i = 0; i < T::NS; ++i) s[i] = m.sees(static_cast<int32_t>(i)) ? s[i] : NEG_INF;
     }
 }
 
@@ -330,7 +343,8 @@ __device__ __forceinline__ float win_lse(float m, float l) { return l == 0.0f ? 
 // ---- window_prompt.hip
 // a prompt's rows in one launch (16-bit caches); with p.lse, what k_win_sums needs
 int win_prompt_launch(opure_dev* dev, const WinParams& p, uint32_t batch);
-// weights += from the cache, the queries and p.lse
-int win_sums_launch(opure_dev* dev, const WinParams& p, uint32_t batch, uint32_t max_ctx);
+// weights += from the cache, the queries and p.lse; scratch of win_sums_bytes (n_heads, n_kv, rows and cap are read)
+uint64_t win_sums_bytes(const WinParams& p, uint32_t batch);
+int win_sums_launch(opure_dev* dev, const WinParams& p, uint32_t batch, float* scratch);
 
 }  // namespace opure_win

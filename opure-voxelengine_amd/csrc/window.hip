@@ -440,8 +440,8 @@ struct WinPlan {
     uint32_t tt = 0, tiles = 0, blocks = 0, block_rows = 0, parts = 0;
     bool prompt = false;                                 // the prompt kernel
     bool two = false, stored = false, four = false;      // split: 32 query rows a workgroup; weights from stored scores, four positions a thread
-    uint64_t acc = 0, ml = 0, scores = 0, lse = 0;       // bytes
-    uint64_t bytes() const { return acc + ml + scores + lse; }
+    uint64_t acc = 0, ml = 0, scores = 0, lse = 0, sums = 0;   // bytes
+    uint64_t bytes() const { return acc + ml + scores + lse + sums; }
 };
 
 int win_plan(opure_dev* dev, const opure_attn_window_args* a, WinPlan& w)
@@ -456,6 +456,21 @@ int win_plan(opure_dev* dev, const opure_attn_window_args* a, WinPlan& w)
     w.prompt = m->afmt != OPURE_A_F32 && Gq >= 256u;
     w.stored = a->weights && Gq <= 64u;
     w.lse = a->weights && !w.stored ? opure_hip::align_up(rows * 4u, 256) : 0u;
+    if (w.lse)
+    {
+        WinParams p{};
+        p.n_heads = m->n_heads;
+        p.n_kv = m->n_kv_heads;
+        p.rows = a->rows;
+        p.cap = a->max_ctx;
+        w.sums = win_sums_bytes(p, a->batch);
+    }
+    // a launch's threads stay in 32 bits: 2^22 workgroups of up to 512
+    const uint64_t heads = static_cast<uint64_t>(a->batch) * m->n_kv_heads;
+    const uint64_t most = std::max<uint64_t>({rows / 4u, heads * ((Gq + 15u) / 16u),
+                                              a->weights ? heads * (a->max_ctx / 32u + 1u) * (w.lse ? (Gq + 511u) / 512u : 1u) / (w.lse ? 1u : 8u) : 0u});
+    OPURE_REQUIRE(most <= 1u << 22, OPURE_E_CAPACITY, "window attention: %u x %u rows of %u heads over max_ctx %u: too many workgroups",
+                  a->batch, a->rows, m->n_heads, a->max_ctx);
     if (w.prompt) return OPURE_OK;
     w.two = Gq > 16u && m->head_dim <= 128u;
     w.blocks = (Gq + (w.two ? 31u : 15u)) / (w.two ? 32u : 16u);
@@ -501,9 +516,9 @@ int win_validate(const opure_attn_window_args* a)
     OPURE_REQUIRE(a->batch >= 1 && a->batch <= OPURE_MAX_BATCH_ROWS && a->rows >= 1 && a->rows <= OPURE_MAX_PROMPT_ROWS,
                   OPURE_E_CAPACITY, "window attention: %u rows x %u sequences outside 1..%d x 1..%d", a->rows, a->batch,
                   OPURE_MAX_PROMPT_ROWS, OPURE_MAX_BATCH_ROWS);
-    // the launches' workgroups and the query rows' indexes stay in 32 bits
-    OPURE_REQUIRE(static_cast<uint64_t>(m->n_heads) * a->batch * a->rows <= 1u << 25 && static_cast<uint64_t>(m->n_kv_heads) * a->batch * (a->max_ctx / 64u + 1ull) <= 1u << 24,
-                  OPURE_E_CAPACITY, "window attention: %u x %u rows of %u heads, max_ctx %u", a->batch, a->rows, m->n_heads, a->max_ctx);
+    // the query rows' indexes stay in 32 bits
+    OPURE_REQUIRE(static_cast<uint64_t>(m->n_heads) * a->batch * a->rows <= 1u << 25, OPURE_E_CAPACITY,
+                  "window attention: %u x %u rows of %u heads", a->batch, a->rows, m->n_heads);
     const uint64_t slots = static_cast<uint64_t>(kv->max_pages_per_seq) * OPURE_PAGE_SIZE;
     OPURE_REQUIRE(a->max_ctx >= a->rows && a->max_ctx <= slots && a->max_ctx <= 0x7FFFFFFFu - OPURE_MAX_PROMPT_ROWS,
                   OPURE_E_CAPACITY, "window attention: max_ctx %u below %u rows or beyond the page table's %llu", a->max_ctx,
@@ -559,6 +574,7 @@ extern "C" int opure_attn_window_paged(opure_dev* dev, const opure_attn_window_a
     p.part_ml = p.part_acc + w.acc / 4u;
     p.scores = w.stored ? p.part_ml + w.ml / 4u : nullptr;
     p.lse = w.lse ? p.part_ml + (w.ml + w.scores) / 4u : nullptr;
+    float* const sums_at = w.lse ? p.lse + w.lse / 4u : nullptr;
     p.weights = a->weights;
     p.weights_stride = a->weights_stride;
     p.weights_batch_stride = a->weights_batch_stride;
@@ -584,7 +600,7 @@ extern "C" int opure_attn_window_paged(opure_dev* dev, const opure_attn_window_a
     if (w.prompt)
     {
         rc = win_prompt_launch(dev, p, a->batch);
-        return rc || !p.lse ? rc : win_sums_launch(dev, p, a->batch, a->max_ctx);
+        return rc || !p.lse ? rc : win_sums_launch(dev, p, a->batch, sums_at);
     }
     const uint32_t wgs = p.n_kv * w.parts * w.blocks * a->batch;
     rc = win_split_kernel(dev, p.afmt, p.hd, w.two, [&](auto kernel, uint32_t lds, uint32_t) {
@@ -617,5 +633,5 @@ extern "C" int opure_attn_window_paged(opure_dev* dev, const opure_attn_window_a
     if (w.tt == 16u) join_tt(std::integral_constant<uint32_t, 16>{});
     else join_tt(std::integral_constant<uint32_t, 32>{});
     OPURE_LAUNCH_CHECK("k_win_join");
-    return p.lse ? win_sums_launch(dev, p, a->batch, a->max_ctx) : OPURE_OK;
+    return p.lse ? win_sums_launch(dev, p, a->batch, sums_at) : OPURE_OK;
 }

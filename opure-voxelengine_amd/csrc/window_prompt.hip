@@ -40,19 +40,22 @@ constexpr uint32_t prompt_lds() { return 2u * (prompt_k_pieces<HD>() + prompt_v_
 // itself is): the matrix unit is what bounds a prompt, and a second product for
 // the rounding's rest would cost it half as much again.  fp16 weights are held
 // 2^6 higher, so that those down to 2^-20 of the largest keep their bits.
-template <int AF, int HD>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 128 ? 2 : 1))) void k_win_prompt(WinParams p)
+//   KG 2 (a grid that does not give every SIMD two waves): eight waves, two for
+// each 32 rows, one on the even tiles and one on the odd ones, merged at the end.
+template <int AF, int HD, int KG>
+__global__ __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(HD <= 128 ? 2 : 1))) void k_win_prompt(WinParams p)
 {
     constexpr uint32_t KS = HD / 16u, DT = (HD + 31u) / 32u, P = HD / 8u, KROW = P + 1u, VROW = PT / 8u + 1u;
     constexpr uint32_t N = 8u * HD, NP = (N + 255u) / 256u;   // 16-byte pieces of a tile's K (and of its V); a thread's
     constexpr float UP = AF == OPURE_A_F16 ? 6.0f : 0.0f;
     extern __shared__ __align__(16) uint8_t lds[];
-    u4v* const kt = reinterpret_cast<u4v*>(lds);
+    const uint32_t kg = KG > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0u;   // takes tiles kg, kg + KG, ...
+    u4v* const kt = reinterpret_cast<u4v*>(lds) + kg * (prompt_lds<HD>() / 16u);
     u4v* const vt = kt + 2u * prompt_k_pieces<HD>();
     const uint32_t G = p.n_heads / p.n_kv, Gq = G * p.rows, nblk = (Gq + 127u) / 128u;
     const uint32_t kh = blockIdx.x % p.n_kv, rest = blockIdx.x / p.n_kv, b = rest / nblk;
     const uint32_t q0 = (nblk - 1u - (rest - b * nblk)) * 128u;   // the rows that see most first
-    const uint32_t tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63u, h = lane >> 5, r = lane & 31u;
+    const uint32_t tid = threadIdx.x & 255u, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63u, h = lane >> 5, r = lane & 31u;
     const int32_t* pt = p.page_table + static_cast<uint64_t>(b) * p.max_pages;
     const WinSeq sq = win_seq(p, p.seq_len[b]);
     const uint32_t j0 = q0 / G, j1 = min(q0 + 127u, Gq - 1u) / G;
@@ -76,28 +79,32 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 128 ?
     const uint8_t* base = static_cast<const uint8_t*>(p.pool) + static_cast<uint64_t>(p.layer) * p.n_pages * page_bytes + kh * plane;
     const uint64_t vofs = p.n_kv * plane;
 
-    u4v kr[NP], vr[NP];
-    int32_t pe[NP], cur[NP];
+    // the loads of the next DEPTH tiles, a set of registers each
+    constexpr uint32_t DEPTH = HD <= 96 ? 2u : 1u;
+    u4v kr[DEPTH][NP], vr[DEPTH][NP];
+    int32_t pe[NP], cur[DEPTH][NP];
     auto entries = [&](uint32_t i) {
-        const uint32_t tile = span.tile(min(i, span.n - 1u));
+        const uint32_t tile = span.tile(min(i * KG + kg, span.n - 1u));
 #pragma unroll
         for (uint32_t u = 0; u < NP; ++u) pe[u] = pt[min(tile * 4u + (u * 256u + tid) / (2u * HD), p.max_pages - 1u)];
     };
-    auto load = [&](uint32_t i) {
-        const uint32_t tile = span.tile(i);
+    auto load = [&](uint32_t i, auto set) {
+        constexpr uint32_t D = decltype(set)::value;
+        const uint32_t tile = span.tile(i * KG + kg);
 #pragma unroll
         for (uint32_t u = 0; u < NP; ++u)
         {
             const uint32_t e = u * 256u + tid, pg = e / (2u * HD);
             if (N % 256u != 0u && e >= N) continue;
-            cur[u] = (tile * 4u + pg) * OPURE_PAGE_SIZE < sq.total && static_cast<uint32_t>(pe[u]) < p.n_pages ? pe[u] : -1;
-            const uint8_t* at = base + static_cast<uint64_t>(cur[u] < 0 ? 0u : static_cast<uint32_t>(cur[u])) * page_bytes + (e - pg * 2u * HD) * 16u;
-            kr[u] = *reinterpret_cast<const u4v*>(at);
-            vr[u] = *reinterpret_cast<const u4v*>(at + vofs);
+            cur[D][u] = (tile * 4u + pg) * OPURE_PAGE_SIZE < sq.total && static_cast<uint32_t>(pe[u]) < p.n_pages ? pe[u] : -1;
+            const uint8_t* at = base + static_cast<uint64_t>(cur[D][u] < 0 ? 0u : static_cast<uint32_t>(cur[D][u])) * page_bytes + (e - pg * 2u * HD) * 16u;
+            kr[D][u] = *reinterpret_cast<const u4v*>(at);
+            vr[D][u] = *reinterpret_cast<const u4v*>(at + vofs);
         }
     };
-    auto store = [&](uint32_t i) {
-        const uint32_t t0 = span.tile(i) * PT;
+    auto store = [&](uint32_t i, auto set) {
+        constexpr uint32_t D = decltype(set)::value;
+        const uint32_t t0 = span.tile(i * KG + kg) * PT;
         u4v* k = kt + (i & 1u) * prompt_k_pieces<HD>();
         u4v* v = vt + (i & 1u) * prompt_v_pieces<HD>();
         const uint32_t nan = AF == OPURE_A_F16 ? 0x7E007E00u : 0x7FC07FC0u;
@@ -109,12 +116,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 128 ?
             if (N % 256u != 0u && e >= N) continue;
             // positions without a page: NaN keys for the rows that see them, no values;
             // slots past the sequence hold anything: values 0
-            u4v x = vr[u];
+            u4v x = vr[D][u];
             const uint32_t tv = t0 + pg * OPURE_PAGE_SIZE + (w & 1u) * 8u;
             if (tail) x = win_tail<AF>(x, tv < sq.total ? sq.total - tv : 0u);
-            x = cur[u] < 0 ? u4v{0u, 0u, 0u, 0u} : x;
+            x = cur[D][u] < 0 ? u4v{0u, 0u, 0u, 0u} : x;
             const uint32_t t = e / P, at = (t & ~12u) | ((t & 4u) << 1) | ((t & 8u) >> 1);
-            k[at * KROW + e % P] = cur[u] < 0 ? u4v{nan, nan, nan, nan} : kr[u];
+            k[at * KROW + e % P] = cur[D][u] < 0 ? u4v{nan, nan, nan, nan} : kr[D][u];
             v[(w >> 1) * VROW + pg * 2u + (w & 1u)] = x;
         }
     };
@@ -131,27 +138,38 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 128 ?
         for (uint32_t e = tid; e < 2u * 16u * VROW; e += 256u)
             vt[(e / (16u * VROW)) * prompt_v_pieces<HD>() + HD * VROW + e % (16u * VROW)] = u4v{0u, 0u, 0u, 0u};
     }
-    if (span.n)
+    typedef std::integral_constant<uint32_t, 0> First;
+    typedef std::integral_constant<uint32_t, DEPTH - 1u> Second;
+    const uint32_t turns = (span.n + KG - 1u) / KG, own = (span.n + KG - 1u - kg) / KG;   // the workgroup's, and this half's tiles
+    if (own)
     {
         entries(0u);
-        load(0u);
+        load(0u, First{});
         entries(1u);
-    }
-    for (uint32_t i = 0; i < span.n; ++i)
-    {
-        store(i);
-        __syncthreads();
-        if (i + 1u < span.n)
+        if (DEPTH > 1u && own > 1u)
         {
-            load(i + 1u);
-            entries(i + 2u);
+            load(1u, Second{});
+            entries(2u);
         }
-        const uint32_t t0 = span.tile(i) * PT;
+    }
+    auto tile = [&](uint32_t i, auto set) {
+        if (KG == 1 || i < own) store(i, set);
+        __syncthreads();
+        if (KG > 1 && i >= own) return;
+        if (i + DEPTH < own)
+        {
+            load(i + DEPTH, set);
+            entries(i + DEPTH + 1u);
+        }
+        const uint32_t t0 = span.tile(i * KG + kg) * PT;
         // nothing of the tile that a row of the wave sees
-        if (t0 > pos1 || (t0 >= p.sinks && t0 + PT - 1u + p.window <= pos0)) continue;
+        if (t0 > pos1 || (t0 >= p.sinks && t0 + PT - 1u + p.window <= pos0)) return;
         const u4v* k = kt + (i & 1u) * prompt_k_pieces<HD>();
         const u4v* v = vt + (i & 1u) * prompt_v_pieces<HD>();
         f16_t s[2];
+        // the reads of the next key operand between the products of this one, and the products ahead of the other
+        // waves' vector work (8B prompt 183.5 -> 180.9 us, 1B 18.3 -> 18.1)
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (uint32_t t = 0; t < 2; ++t)
         {
@@ -160,16 +178,23 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 128 ?
 #pragma unroll
             for (uint32_t x = 0; x < KS; ++x) s[t] = mfma_32<AF>(k[(32u * t + r) * KROW + 2u * x + h], q[x], s[t]);
         }
+        __builtin_amdgcn_sched_group_barrier(0x100, KS, 0);
+#pragma unroll
+        for (uint32_t x = 0; x < KS; ++x)
+        {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, KS, 0);
+        __builtin_amdgcn_s_setprio(0);
         if (t0 + PT > min(pos0 + 1u, sq.total) || !(t0 + PT <= p.sinks || t0 + p.window > pos1))
         {
+            const WinMask mask(p, pos, sq.total, t0 + 8u * h);
 #pragma unroll
             for (uint32_t t = 0; t < 2; ++t)
 #pragma unroll
                 for (uint32_t x = 0; x < 16; ++x)
-                {
-                    const uint32_t at = t0 + 32u * t + 16u * (x >> 3) + 8u * h + (x & 7u);
-                    s[t][x] = at < sq.total && win_sees(p, pos, at) ? s[t][x] : NEG_INF;
-                }
+                    s[t][x] = mask.sees(static_cast<int32_t>(32u * t + 16u * (x >> 3) + (x & 7u))) ? s[t][x] : NEG_INF;
         }
         float mx = s[0][0];
 #pragma unroll
@@ -203,9 +228,46 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 128 ?
         for (uint32_t u = 0; u < 4; ++u)
 #pragma unroll
             for (uint32_t d = 0; d < DT; ++d) o[d] = mfma_32<AF>(v[(32u * d + r) * VROW + 2u * u + h], w[u], o[d]);
+    };
+    for (uint32_t i = 0; i < turns; i += DEPTH)
+    {
+        tile(i, First{});
+        if (DEPTH > 1u && i + 1u < turns) tile(i + 1u, Second{});
+    }
+    if constexpr (KG > 1)
+    {
+        // the odd tiles' results to the waves of the even ones: a lane hands over its own registers
+        __syncthreads();
+        f4_t* give = reinterpret_cast<f4_t*>(lds) + wave * (4u * DT + 1u) * 64u + lane;
+        if (kg)
+        {
+#pragma unroll
+            for (uint32_t d = 0; d < DT; ++d)
+#pragma unroll
+                for (uint32_t x = 0; x < 4; ++x) give[(4u * d + x) * 64u] = f4_t{o[d][4 * x], o[d][4 * x + 1], o[d][4 * x + 2], o[d][4 * x + 3]};
+            give[4u * DT * 64u] = f4_t{m, l, 0.0f, 0.0f};
+        }
+        __syncthreads();
+        if (!kg)
+        {
+            const f4_t ml = give[4u * DT * 64u];
+            const float mn = fmaxf(m, ml[0]), ms = mn == NEG_INF ? 0.0f : mn;
+            const float a = __builtin_amdgcn_exp2f(__fsub_rn(m, ms)), c2 = __builtin_amdgcn_exp2f(__fsub_rn(ml[0], ms));
+            l = __fmaf_rn(ml[1], c2, __fmul_rn(l, a));
+            m = mn;
+#pragma unroll
+            for (uint32_t d = 0; d < DT; ++d)
+#pragma unroll
+                for (uint32_t x = 0; x < 4; ++x)
+                {
+                    const f4_t v = give[(4u * d + x) * 64u];
+#pragma unroll
+                    for (uint32_t k = 0; k < 4; ++k) o[d][4 * x + k] = __fmaf_rn(v[k], c2, __fmul_rn(o[d][4 * x + k], a));
+                }
+        }
     }
     l = add_xor32(l);
-    const bool mine = q0 + 32u * wave + r < Gq;
+    const bool mine = kg == 0u && q0 + 32u * wave + r < Gq;
     if (p.lse && h == 0u && mine) p.lse[(static_cast<uint64_t>(b) * p.n_kv + kh) * Gq + qi] = win_lse(m - UP, l);
     const float inv = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
     bool fine = true;
@@ -231,7 +293,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 128 ?
     uint64_t bad = __ballot(!fine && mine);
     bad = (bad | bad >> 32) & 0xFFFFFFFFull;
     __syncthreads();                                       // the stages are done with
-    float* qs = reinterpret_cast<float*>(lds) + wave * 256u;
+    float* qs = reinterpret_cast<float*>(lds) + wave * 256u;   // the even half's: the others have no row
     while (bad)
     {
         const uint32_t x = static_cast<uint32_t>(__builtin_ctzll(bad));
@@ -252,26 +314,49 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 128 ?
 }
 
 // Weights from many rows: a workgroup takes 64 positions (32 of an fp32 cache) of
-// a (sequence, KV head), its eight waves every eighth block of 16 query rows that
-// see one of them.  A wave holds the positions' keys as operands, computes the
+// a (sequence, KV head) and a chunk of 512 query rows, its eight waves every
+// eighth block of 16 of those rows that see one of the positions.  A wave holds the positions' keys as operands, computes the
 // block's scores again and adds 2^(score - lse) to a sum a lane and position; the
 // lanes' and waves' sums are added in order.  To store the scores instead would
 // take as many bytes as K and V together from 64 query rows of a KV head on.
+//   With more than one chunk each leaves its sums in a place of its own, and
+// k_win_add adds them in order: the first positions of a prompt are seen by all of
+// its rows, which one workgroup took 30 us to walk through (1,024 rows of the 1B
+// shape).
+constexpr uint32_t SUM_ROWS = 512;
+
+// rows [ja, jz) of a chunk that see a position of [t0, t0 + n)
+__device__ __forceinline__ void sums_rows(const WinParams& p, const WinSeq& sq, uint32_t G, uint32_t chunk, uint32_t t0, uint32_t n,
+                                          uint32_t& qa, uint32_t& qz)
+{
+    const uint32_t ja = t0 > sq.ctx ? t0 - sq.ctx : 0u;
+    const uint32_t jz = t0 < p.sinks ? p.rows : t0 + n - 1u + p.window > sq.ctx ? min(p.rows, t0 + n - 1u + p.window - sq.ctx) : 0u;
+    qa = max(ja * G, chunk * SUM_ROWS);
+    qz = min(jz * G, (chunk + 1u) * SUM_ROWS);
+    if (t0 >= sq.total) qz = 0u;
+}
+
+constexpr uint32_t SUM_WAVES = 4;
+
 template <int AF, int HD>
-__global__ __launch_bounds__(512) void k_win_sums(WinParams p)
+__global__ __launch_bounds__(64 * SUM_WAVES) __attribute__((amdgpu_waves_per_eu(HD <= 64 ? 4 : HD <= 128 ? 2 : 1))) void k_win_sums(WinParams p)
 {
     typedef WinTile<AF, HD> T;
     constexpr uint32_t NS = T::NS, TILE = 2u * T::TT;
-    __shared__ float part[8][TILE];
-    const uint32_t kh = blockIdx.x % p.n_kv, rest = blockIdx.x / p.n_kv, b = rest % p.blocks, tile = rest / p.blocks;   // blocks: the batch
+    __shared__ float part[SUM_WAVES][TILE];
+    const uint32_t kh = blockIdx.x % p.n_kv, rest = blockIdx.x / p.n_kv, chunk = rest % p.parts, rest2 = rest / p.parts;
+    const uint32_t b = rest2 % p.batch, tile = rest2 / p.batch;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, g = lane >> 4, r = lane & 15u;
     const uint32_t G = p.n_heads / p.n_kv, Gq = G * p.rows, t0 = tile * TILE;
     const int32_t* pt = p.page_table + static_cast<uint64_t>(b) * p.max_pages;
-    const WinSeq sq = win_seq(p, p.seq_len[b]);
-    // rows ja .. jz - 1 see a position of the tile
-    const uint32_t ja = t0 > sq.ctx ? t0 - sq.ctx : 0u;
-    const uint32_t jz = t0 < p.sinks ? p.rows : t0 + TILE - 1u + p.window > sq.ctx ? min(p.rows, t0 + TILE - 1u + p.window - sq.ctx) : 0u;
-    if (t0 >= sq.total || ja >= jz) return;                // whole workgroup
+    // the length and the tile's page entries (a lane each) in one round trip
+    const int32_t len = p.seq_len[b];
+    const int32_t entries = pt[min(t0 / OPURE_PAGE_SIZE + (lane & (2u * T::NB - 1u)), p.max_pages - 1u)];
+    asm volatile("" ::: "memory");
+    const WinSeq sq = win_seq(p, len);
+    uint32_t qa, qz;
+    sums_rows(p, sq, G, chunk, t0, TILE, qa, qz);
+    if (qa >= qz) return;                                  // whole workgroup
     const uint64_t page_bytes = 2ull * p.n_kv * T::PB;
     const uint8_t* base = static_cast<const uint8_t*>(p.pool) + static_cast<uint64_t>(p.layer) * p.n_pages * page_bytes + static_cast<uint64_t>(kh) * T::PB;
     T tl[2];
@@ -283,9 +368,8 @@ __global__ __launch_bounds__(512) void k_win_sums(WinParams p)
 #pragma unroll
         for (uint32_t y = 0; y < T::NB; ++y)
         {
-            const uint32_t t = t0 + x * T::TT + y * OPURE_PAGE_SIZE;
-            const int32_t e = t < sq.total ? pt[t / OPURE_PAGE_SIZE] : -1;
-            pg[y] = __builtin_amdgcn_readfirstlane(static_cast<uint32_t>(e) < p.n_pages ? e : -1);
+            const int32_t e = __builtin_amdgcn_readlane(entries, x * T::NB + y);
+            pg[y] = t0 + x * T::TT + y * OPURE_PAGE_SIZE < sq.total && static_cast<uint32_t>(e) < p.n_pages ? e : -1;
         }
         if (T::NB == 1u) pg[1] = pg[0];
         auto at = [&](int32_t e) { return base + static_cast<uint64_t>(e < 0 ? 0u : static_cast<uint32_t>(e)) * page_bytes; };
@@ -293,60 +377,85 @@ __global__ __launch_bounds__(512) void k_win_sums(WinParams p)
         const uint32_t nan = AF == OPURE_A_F32 ? 0x7FC00000u : AF == OPURE_A_F16 ? 0x7E007E00u : 0x7FC07FC0u;
         const bool gone = (T::NB > 1u && r >= 8u ? pg[1] : pg[0]) < 0;
         whole = whole && pg[0] >= 0 && pg[1] >= 0;
+        if (pg[0] < 0 || pg[1] < 0)
 #pragma unroll
         for (uint32_t t = 0; t < T::NB; ++t)
 #pragma unroll
             for (uint32_t s = 0; s < T::KS; ++s) tl[x].k[t][s] = gone ? u4v{nan, nan, nan, nan} : tl[x].k[t][s];
     }
+    // the keys have arrived: the loop's waits are for the queries alone
+#pragma unroll
+    for (uint32_t x = 0; x < 2; ++x)
+#pragma unroll
+        for (uint32_t t = 0; t < T::NB; ++t)
+#pragma unroll
+            for (uint32_t s = 0; s < T::KS; ++s) asm volatile("" : "+v"(tl[x].k[t][s]));
     const float c = __fmul_rn(p.scale, 1.44269504088896340736f);
     float sum[2][NS];
 #pragma unroll
     for (uint32_t x = 0; x < 2; ++x)
 #pragma unroll
         for (uint32_t y = 0; y < NS; ++y) sum[x][y] = 0.0f;
-    const uint32_t qa = ja * G, qz = min(jz * G, Gq);
     const float* lse = p.lse + (static_cast<uint64_t>(b) * p.n_kv + kh) * Gq;
-    u4v q[T::KS], nq[T::KS];
-    float ls, nls;
-    uint32_t jr, njr;
+    // two blocks of rows a turn, the next turn's on their way (one where their operands are large)
+    constexpr uint32_t BLK = HD <= 128 ? 2u : 1u, EACH = 16u * SUM_WAVES, STEP = EACH * BLK;
+    u4v q[BLK][T::KS], nq[BLK][T::KS];
+    float ls[BLK], nls[BLK];
+    uint32_t jr[BLK], njr[BLK];
     auto fetch = [&](uint32_t q0, u4v (&to)[T::KS], float& l, uint32_t& j) {
         const uint32_t qi = min(q0 + r, Gq - 1u);
         j = qi / G;
         win_load_q<AF, HD>(p, (static_cast<uint64_t>(b) * p.rows + j) * p.n_heads + kh * G + (qi - j * G), g, to);
-        l = q0 + r < qz ? lse[qi] : __builtin_huge_valf();  // a row past the last: weight 0
+        l = lse[qi];
     };
     uint32_t q0 = qa + 16u * wave;
-    if (q0 < qz) fetch(q0, q, ls, jr);
-    for (; q0 < qz; q0 += 128u)
+    if (q0 < qz)
+#pragma unroll
+        for (uint32_t u = 0; u < BLK; ++u) fetch(q0 + EACH * u, q[u], ls[u], jr[u]);
+    for (; q0 < qz; q0 += STEP)
     {
-        if (q0 + 128u < qz) fetch(q0 + 128u, nq, nls, njr);
-        const uint32_t p0 = sq.ctx + q0 / G, p1 = sq.ctx + min(q0 + 15u, Gq - 1u) / G;
-        const bool full = whole && t0 + TILE <= p0 + 1u && (t0 + TILE <= p.sinks || t0 + p.window > p1);
-        const bool ragged = q0 + 16u > qz, past = q0 + r >= qz;
+        if (q0 + STEP < qz)
 #pragma unroll
-        for (uint32_t x = 0; x < 2; ++x)
+            for (uint32_t u = 0; u < BLK; ++u) fetch(q0 + STEP + EACH * u, nq[u], nls[u], njr[u]);
+#pragma unroll
+        for (uint32_t u = 0; u < BLK; ++u)
         {
-            float s[NS];
-            win_scores<AF, HD>(p, tl[x], q, c, full, t0 + x * T::TT, g, sq.ctx + jr, sq.total, s);
+            const uint32_t qb = q0 + EACH * u;
+            if (qb >= qz) break;
+            const uint32_t p0 = sq.ctx + qb / G, p1 = sq.ctx + min(qb + 15u, Gq - 1u) / G;
+            const bool full = whole && t0 + TILE <= p0 + 1u && (t0 + TILE <= p.sinks || t0 + p.window > p1);
+            const float of_row = qb + r < qz ? ls[u] : __builtin_huge_valf();   // a row past the last: weight 0
 #pragma unroll
-            for (uint32_t y = 0; y < NS; ++y) s[y] = __builtin_amdgcn_exp2f(__fsub_rn(s[y], ls));
-            if (!full || ragged)
+            for (uint32_t x = 0; x < 2; ++x)
             {
-                // what a row does not see adds nothing, whatever the row's sum is
+                float s[NS];
 #pragma unroll
-                for (uint32_t y = 0; y < NS; ++y)
+                for (uint32_t t = 0; t < T::NB; ++t)
                 {
-                    const uint32_t t = t0 + x * T::TT + NS * g + y;
-                    s[y] = !past && t < sq.total && win_sees(p, sq.ctx + jr, t) ? s[y] : 0.0f;
-                }
-            }
+                    f4_t acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (uint32_t y = 0; y < NS; ++y) sum[x][y] += s[y];
+                    for (uint32_t k = 0; k < T::KS; ++k) acc = win_mfma<AF>(tl[x].k[t][k], q[u][k], acc);
+#pragma unroll
+                    for (uint32_t i = 0; i < 4; ++i) s[4u * t + i] = __builtin_amdgcn_exp2f(__fmaf_rn(acc[i], c, -of_row));
+                }
+                if (!full)
+                {
+                    const WinMask m(p, sq.ctx + jr[u], sq.total, t0 + x * T::TT + NS * g);
+#pragma unroll
+                    for (uint32_t y = 0; y < NS; ++y) s[y] = m.sees(static_cast<int32_t>(y)) ? s[y] : 0.0f;
+                }
+#pragma unroll
+                for (uint32_t y = 0; y < NS; ++y) sum[x][y] += s[y];
+            }
         }
 #pragma unroll
-        for (uint32_t k = 0; k < T::KS; ++k) q[k] = nq[k];
-        ls = nls;
-        jr = njr;
+        for (uint32_t u = 0; u < BLK; ++u)
+        {
+#pragma unroll
+            for (uint32_t k = 0; k < T::KS; ++k) q[u][k] = nq[u][k];
+            ls[u] = nls[u];
+            jr[u] = njr[u];
+        }
     }
 #pragma unroll
     for (uint32_t x = 0; x < 2; ++x)
@@ -359,13 +468,41 @@ __global__ __launch_bounds__(512) void k_win_sums(WinParams p)
     __syncthreads();
     const uint32_t t = t0 + threadIdx.x;
     if (threadIdx.x >= TILE || t >= sq.total) return;
-    // seen by a row: the last one at or past the position that it still reaches
-    const uint32_t first = t > sq.ctx ? t - sq.ctx : 0u;
-    if (first >= p.rows || !win_sees(p, sq.ctx + first, t)) return;
     float v = part[0][threadIdx.x];
 #pragma unroll
-    for (uint32_t w = 1; w < 8; ++w) v += part[w][threadIdx.x];
+    for (uint32_t w = 1; w < SUM_WAVES; ++w) v += part[w][threadIdx.x];
+    if (p.parts > 1u)
+    {
+        p.part_acc[(static_cast<uint64_t>(b * p.n_kv + kh) * p.parts + chunk) * p.cap + t] = v;
+        return;
+    }
+    // seen by a row: by the first at or past the position, if by any
+    const uint32_t first = t > sq.ctx ? t - sq.ctx : 0u;
+    if (first >= p.rows || !win_sees(p, sq.ctx + first, t)) return;
     p.weights[b * p.weights_batch_stride + static_cast<uint64_t>(kh) * p.weights_stride + t] += v;
+}
+
+// the chunks' sums, a thread a position
+template <uint32_t TILE>
+__global__ __launch_bounds__(256) void k_win_add(WinParams p)
+{
+    const uint32_t G = p.n_heads / p.n_kv, kh = blockIdx.y, b = blockIdx.z, t = blockIdx.x * 256u + threadIdx.x;
+    const WinSeq sq = win_seq(p, p.seq_len[b]);
+    if (t >= sq.total) return;
+    const uint32_t first = t > sq.ctx ? t - sq.ctx : 0u;
+    if (first >= p.rows || !win_sees(p, sq.ctx + first, t)) return;
+    const float* part = p.part_acc + static_cast<uint64_t>(b * p.n_kv + kh) * p.parts * p.cap + t;
+    float* to = p.weights + b * p.weights_batch_stride + static_cast<uint64_t>(kh) * p.weights_stride + t;
+    const float old = *to;
+    float v = 0.0f;
+#pragma unroll 4
+    for (uint32_t chunk = 0; chunk < p.parts; ++chunk)
+    {
+        uint32_t qa, qz;
+        sums_rows(p, sq, G, chunk, t / TILE * TILE, TILE, qa, qz);
+        if (qa < qz) v += part[static_cast<uint64_t>(chunk) * p.cap];
+    }
+    *to = old + v;
 }
 
 }  // namespace
@@ -374,37 +511,58 @@ namespace opure_win {
 
 int win_prompt_launch(opure_dev* dev, const WinParams& p, uint32_t batch)
 {
-    const uint32_t Gq = p.n_heads / p.n_kv * p.rows;
+    const uint32_t Gq = p.n_heads / p.n_kv * p.rows, wgs = p.n_kv * ((Gq + 127u) / 128u) * batch;
+    const bool two = wgs <= static_cast<uint32_t>(dev->n_cu > 0 ? dev->n_cu : 256);   // 256: 21 us against 17 (1,024 causal rows); 360: 18.2 against 22.9
     auto go = [&](auto af) {
         return win_by_head(p.hd, [&](auto h) {
             constexpr int AF = decltype(af)::value, HD = decltype(h)::value;
-            static std::atomic<uint64_t> done{0};
-            const int rc = opure_win::win_lds(dev, reinterpret_cast<const void*>(&k_win_prompt<AF, HD>), prompt_lds<HD>(), done);
-            if (rc) return rc;
-            OPURE_LAUNCH(dev, (k_win_prompt<AF, HD>), dim3(p.n_kv * ((Gq + 127u) / 128u) * batch), dim3(256), prompt_lds<HD>(), p);
-            OPURE_LAUNCH_CHECK("k_win_prompt");
-            return OPURE_OK;
+            auto run = [&](auto groups) {
+                constexpr int KG = decltype(groups)::value;
+                static std::atomic<uint64_t> done{0};
+                const int rc = win_lds(dev, reinterpret_cast<const void*>(&k_win_prompt<AF, HD, KG>), KG * prompt_lds<HD>(), done);
+                if (rc) return rc;
+                OPURE_LAUNCH(dev, (k_win_prompt<AF, HD, KG>), dim3(wgs), dim3(256 * KG), KG * prompt_lds<HD>(), p);
+                OPURE_LAUNCH_CHECK("k_win_prompt");
+                return OPURE_OK;
+            };
+            if constexpr (HD <= 128)
+                if (two) return run(std::integral_constant<int, 2>{});
+            return run(std::integral_constant<int, 1>{});
         });
     };
     return p.afmt == OPURE_A_F16 ? go(std::integral_constant<int, OPURE_A_F16>{}) : go(std::integral_constant<int, OPURE_A_BF16>{});
 }
 
-int win_sums_launch(opure_dev* dev, const WinParams& p, uint32_t batch, uint32_t max_ctx)
+uint64_t win_sums_bytes(const WinParams& p, uint32_t batch)
+{
+    const uint64_t chunks = (static_cast<uint64_t>(p.n_heads / p.n_kv) * p.rows + SUM_ROWS - 1u) / SUM_ROWS;
+    return chunks > 1u ? static_cast<uint64_t>(batch) * p.n_kv * chunks * p.cap * 4u : 0u;
+}
+
+int win_sums_launch(opure_dev* dev, const WinParams& p, uint32_t batch, float* scratch)
 {
     WinParams s = p;
-    s.blocks = batch;
+    s.batch = batch;
+    s.parts = (p.n_heads / p.n_kv * p.rows + SUM_ROWS - 1u) / SUM_ROWS;
+    s.part_acc = scratch;
     const uint32_t tile = p.afmt == OPURE_A_F32 ? 32u : 64u;
     auto go = [&](auto af) {
         return win_by_head(p.hd, [&](auto h) {
             constexpr int AF = decltype(af)::value, HD = decltype(h)::value;
-            OPURE_LAUNCH(dev, (k_win_sums<AF, HD>), dim3(p.n_kv * batch * ((max_ctx + tile - 1u) / tile)), dim3(512), 0, s);
+            OPURE_LAUNCH(dev, (k_win_sums<AF, HD>), dim3(p.n_kv * batch * s.parts * ((p.cap + tile - 1u) / tile)), dim3(64 * SUM_WAVES), 0, s);
             OPURE_LAUNCH_CHECK("k_win_sums");
             return OPURE_OK;
         });
     };
-    return p.afmt == OPURE_A_F32   ? go(std::integral_constant<int, OPURE_A_F32>{})
-           : p.afmt == OPURE_A_F16 ? go(std::integral_constant<int, OPURE_A_F16>{})
-                                   : go(std::integral_constant<int, OPURE_A_BF16>{});
+    const int rc = p.afmt == OPURE_A_F32   ? go(std::integral_constant<int, OPURE_A_F32>{})
+                   : p.afmt == OPURE_A_F16 ? go(std::integral_constant<int, OPURE_A_F16>{})
+                                           : go(std::integral_constant<int, OPURE_A_BF16>{});
+    if (rc || s.parts == 1u) return rc;
+    const dim3 grid((p.cap + 255u) / 256u, p.n_kv, batch);
+    if (tile == 32u) OPURE_LAUNCH(dev, (k_win_add<32u>), grid, dim3(256), 0, s);
+    else OPURE_LAUNCH(dev, (k_win_add<64u>), grid, dim3(256), 0, s);
+    OPURE_LAUNCH_CHECK("k_win_add");
+    return OPURE_OK;
 }
 
 }  // namespace opure_win
