@@ -13,6 +13,8 @@
 // ============================================================================
 #include "internal.h"
 
+#include <type_traits>
+
 using namespace opure_dev_math;
 
 namespace {
@@ -48,52 +50,57 @@ __device__ __forceinline__ uint32_t score_key(float f)
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-// Sums over 1,024 threads in thread order of two counts, packed low and high:
-// those before this thread's, and all.
-__device__ __forceinline__ uint64_t block_prefix(uint64_t v, uint64_t* wsum, uint64_t& all)
+// Sums over W waves in thread order of a count: those before this thread's, and all.
+template <uint32_t W>
+__device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t* wsum, uint32_t& all)
 {
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6;
-    uint64_t x = v;
+    uint32_t x = v;
 #pragma unroll
     for (uint32_t o = 1; o < 64u; o <<= 1)
     {
-        const uint64_t y = __shfl_up(x, o);
+        const uint32_t y = __shfl_up(x, o);
         if (lane >= o) x += y;
     }
-    __syncthreads();                                       // wsum of the call before is read
     if (lane == 63u) wsum[wave] = x;
     __syncthreads();
-    uint64_t before = 0;
+    uint32_t before = 0;
     all = 0;
 #pragma unroll
-    for (uint32_t w = 0; w < 16u; ++w)
+    for (uint32_t w = 0; w < W; ++w)
     {
-        const uint64_t s = wsum[w];
+        const uint32_t s = wsum[w];
         before += w < wave ? s : 0u;
         all += s;
     }
     return before + x - v;
 }
 
-// The kept positions of one (sequence, layer, KV head).  First the `heavy`-th
-// largest key, by counts of its leading 11, next 11 and last 10 bits; then the
-// positions above it and, from the lowest on, as many equal to it as are
-// missing, in order.  A thread holds 8 consecutive scores in registers, so up to
-// 8,192 positions are read once and ordered by one prefix sum.
-constexpr uint32_t SEL = 8, SEL_BLOCK = 1024u * SEL;
+// The kept positions of one (sequence, layer, KV head), by 64 W threads.  First
+// the `heavy`-th largest key, by counts of its leading 11, next 11 and last 10
+// bits; then the positions above it and, from the lowest on, as many equal to it
+// as are missing, in order.  A thread holds 8 consecutive scores in registers, so
+// up to 512 W positions are read once, ordered by one prefix sum, and written with
+// their scores as they are found (all scores are read by then: scores_out may be
+// scores).  Bound by its chain of counts and barriers: as few waves as hold the
+// sequence (2,048 positions: 4 waves, where 16 took 13 us).
+constexpr uint32_t SEL = 8;
 
-__global__ __launch_bounds__(1024) void k_evict_select(EvictParams p)
+template <uint32_t W>
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W == 16 ? 8 : 4))) void k_evict_select(EvictParams p)
 {
-    __shared__ uint32_t hist[2048], pick[2];
-    __shared__ uint64_t wsum[16];
+    constexpr uint32_t T = 64u * W, BLOCK = T * SEL, BINS = 2048u, PER = BINS / T;
+    __shared__ uint32_t hist[BINS], pick[2], wsum[6][W];
     const uint32_t b = blockIdx.y, tid = threadIdx.x;
     const uint64_t plane = static_cast<uint64_t>(b) * p.n_layers * p.n_kv + blockIdx.x;
     const int32_t raw = p.seq_len[b];
-    const uint32_t n = evict_len(p, b);
     const float* sc = p.scores + plane * p.scores_stride;
+    const uint32_t n = raw < 0 ? 0u : min(static_cast<uint32_t>(raw), p.cap);
     int32_t* kept = p.kept + plane * p.keep;
+    float* so = p.scores_out ? p.scores_out + plane * p.scores_stride : nullptr;
     const uint32_t lo = p.sinks, hi = n > p.keep ? n - p.recent : 0u;   // candidates lo .. hi - 1
     const uint32_t count = min(n, p.keep);
+    const bool once = n <= BLOCK;
     if (tid == 0u && blockIdx.x == 0u)
     {
         if (raw < 0 || static_cast<uint32_t>(raw) > p.cap) p.err[ERR_POSITION] = 1u;
@@ -105,112 +112,135 @@ __global__ __launch_bounds__(1024) void k_evict_select(EvictParams p)
     }
     if (n <= p.keep)
     {
-        for (uint32_t i = tid; i < p.keep; i += 1024u) kept[i] = i < n ? static_cast<int32_t>(i) : -1;
+        for (uint32_t i = tid; i < p.keep; i += T) kept[i] = i < n ? static_cast<int32_t>(i) : -1;
+        if (so && so != sc)
+            for (uint32_t i = tid; i < n; i += T) so[i] = sc[i];
+        return;
     }
-    else
-    {
-        uint32_t key[SEL];
-        auto load = [&](uint32_t t0) {
+    float v[SEL];
+    auto load = [&](uint32_t t0) {
 #pragma unroll
-            for (uint32_t u = 0; u < SEL; ++u)
-            {
-                const uint32_t t = t0 + tid * SEL + u;
-                key[u] = t >= lo && t < hi ? score_key(sc[t]) : 0u;
-            }
-        };
-        load(0u);
-        uint32_t prefix = 0, need = p.heavy;               // the key's leading bits so far; how many still of its group
-        for (uint32_t step = 0; step < 3u && p.heavy; ++step)
+        for (uint32_t u = 0; u < SEL; ++u)
         {
-            const uint32_t shift = step == 0u ? 21u : step == 1u ? 10u : 0u, bins = step == 2u ? 1024u : 2048u;
-            const uint32_t mask = step == 0u ? 0u : 0xFFFFFFFFu << (step == 1u ? 21u : 10u);
-            for (uint32_t i = tid; i < bins; i += 1024u) hist[i] = 0u;
-            __syncthreads();
-            for (uint32_t t0 = 0; t0 < hi; t0 += SEL_BLOCK)
-            {
-                if (n > SEL_BLOCK) load(t0);
-#pragma unroll
-                for (uint32_t u = 0; u < SEL; ++u)
-                {
-                    const uint32_t t = t0 + tid * SEL + u;
-                    if (t >= lo && t < hi && (key[u] & mask) == prefix) atomicAdd(&hist[(key[u] >> shift) & (bins - 1u)], 1u);
-                }
-            }
-            __syncthreads();
-            // how many keys of the group lie above each bin, from the top: two bins a thread, or one
-            const uint32_t per = bins / 1024u, top = bins - 1u - tid * per;
-            const uint32_t h0 = hist[top], h1 = per > 1u ? hist[top - 1u] : 0u;
-            uint64_t all;
-            const uint32_t above = static_cast<uint32_t>(block_prefix(h0 + h1, wsum, all));
-            if (above < need && above + h0 >= need)
-            {
-                pick[0] = top;
-                pick[1] = need - above;
-            }
-            else if (above + h0 < need && above + h0 + h1 >= need)
-            {
-                pick[0] = top - 1u;
-                pick[1] = need - above - h0;
-            }
-            __syncthreads();
-            prefix |= pick[0] << shift;
-            need = pick[1];
-            __syncthreads();
+            const uint32_t t = t0 + tid * SEL + u;
+            v[u] = t < n ? sc[t] : 0.0f;
         }
-        uint32_t out = 0, equal = 0;                       // kept and equal keys of the blocks before
-        for (uint32_t t0 = 0; t0 < n; t0 += SEL_BLOCK)
-        {
-            if (n > SEL_BLOCK) load(t0);
-            uint32_t sure = 0, eq = 0;                     // kept for certain; equal to the key
+    };
+    load(0u);
+    uint32_t prefix = 0, need = p.heavy;                   // the key's leading bits so far; how many still of its group
 #pragma unroll
-            for (uint32_t u = 0; u < SEL; ++u)
-            {
-                const uint32_t t = t0 + tid * SEL + u;
-                const bool cand = t >= lo && t < hi && p.heavy != 0u;
-                sure += t < n && (t < lo || t >= hi || (cand && key[u] > prefix)) ? 1u : 0u;
-                eq += cand && key[u] == prefix ? 1u : 0u;
-            }
-            uint64_t all;
-            const uint64_t at = block_prefix(static_cast<uint64_t>(sure) << 32 | eq, wsum, all);
-            uint32_t eq_before = equal + static_cast<uint32_t>(at);
-            uint32_t to = out + static_cast<uint32_t>(at >> 32) + min(eq_before, need) - min(equal, need);
-#pragma unroll
-            for (uint32_t u = 0; u < SEL; ++u)
-            {
-                const uint32_t t = t0 + tid * SEL + u;
-                const bool cand = t >= lo && t < hi && p.heavy != 0u, same = cand && key[u] == prefix;
-                const bool stay = t < n && (t < lo || t >= hi || (cand && key[u] > prefix) || (same && eq_before < need));
-                eq_before += same ? 1u : 0u;
-                if (stay) kept[to++] = static_cast<int32_t>(t);
-            }
-            const uint32_t eq_after = equal + static_cast<uint32_t>(all);
-            out += static_cast<uint32_t>(all >> 32) + min(eq_after, need) - min(equal, need);
-            equal = eq_after;
-        }
-    }
-    if (p.scores_out)
+    for (uint32_t step = 0; step < 3u; ++step)
     {
-        float* so = p.scores_out + plane * p.scores_stride;
-        __syncthreads();                                   // the kept positions written, visible to the workgroup
-        for (uint32_t i0 = 0; i0 < count; i0 += 1024u)
+        if (p.heavy == 0u) break;
+        const uint32_t shift = step == 0u ? 21u : step == 1u ? 10u : 0u, bins = step == 2u ? 1024u : BINS;
+        const uint32_t mask = step == 0u ? 0u : 0xFFFFFFFFu << (step == 1u ? 21u : 10u);
+#pragma unroll
+        for (uint32_t i = 0; i < PER; ++i) hist[tid + T * i] = 0u;
+        __syncthreads();
+        for (uint32_t t0 = 0; t0 < hi; t0 += BLOCK)
         {
-            const uint32_t i = i0 + tid;
-            const float v = i < count ? sc[kept[i]] : 0.0f;
-            __syncthreads();                               // scores_out may be scores: read before written
-            if (i < count) so[i] = v;
+            if (!once) load(t0);
+#pragma unroll
+            for (uint32_t u = 0; u < SEL; ++u)
+            {
+                const uint32_t t = t0 + tid * SEL + u, key = score_key(v[u]);
+                if (t >= lo && t < hi && (key & mask) == prefix) atomicAdd(&hist[(key >> shift) & (bins - 1u)], 1u);
+            }
         }
         __syncthreads();
-        for (uint32_t i = count + tid; i < n; i += 1024u) so[i] = 0.0f;
+        // how many keys of the group lie above each of this thread's bins, from the top (the last step's upper bins are empty)
+        uint32_t h[PER], sum = 0, all;
+#pragma unroll
+        for (uint32_t i = 0; i < PER; ++i)
+        {
+            h[i] = hist[BINS - 1u - (tid * PER + i)];
+            sum += h[i];
+        }
+        uint32_t above = block_prefix<W>(sum, wsum[step], all);
+#pragma unroll
+        for (uint32_t i = 0; i < PER; ++i)
+        {
+            if (above < need && above + h[i] >= need)
+            {
+                pick[0] = BINS - 1u - (tid * PER + i);
+                pick[1] = need - above;
+            }
+            above += h[i];
+        }
+        __syncthreads();
+        prefix |= pick[0] << shift;
+        need = pick[1];
     }
+    uint32_t out = 0, equal = 0;                           // kept and equal keys of the blocks before
+    for (uint32_t t0 = 0; t0 < n; t0 += BLOCK)
+    {
+        if (!once) load(t0);
+        uint32_t sure = 0, eq = 0;                         // kept for certain; equal to the key
+#pragma unroll
+        for (uint32_t u = 0; u < SEL; ++u)
+        {
+            const uint32_t t = t0 + tid * SEL + u, key = score_key(v[u]);
+            const bool cand = t >= lo && t < hi && p.heavy != 0u;
+            sure += t < n && (t < lo || t >= hi || (cand && key > prefix)) ? 1u : 0u;
+            eq += cand && key == prefix ? 1u : 0u;
+        }
+        // a block's counts stay below 2^16: both in one sum
+        uint32_t all;
+        if (!once) __syncthreads();                        // wsum of the block before is read
+        const uint32_t at = block_prefix<W>(sure << 16 | eq, wsum[3], all);
+        uint32_t eq_before = equal + (at & 0xFFFFu);
+        uint32_t to = out + (at >> 16) + min(eq_before, need) - min(equal, need);
+#pragma unroll
+        for (uint32_t u = 0; u < SEL; ++u)
+        {
+            const uint32_t t = t0 + tid * SEL + u, key = score_key(v[u]);
+            const bool cand = t >= lo && t < hi && p.heavy != 0u, same = cand && key == prefix;
+            const bool stay = t < n && (t < lo || t >= hi || (cand && key > prefix) || (same && eq_before < need));
+            eq_before += same ? 1u : 0u;
+            if (stay)
+            {
+                kept[to] = static_cast<int32_t>(t);
+                if (so && once) so[to] = v[u];
+                ++to;
+            }
+        }
+        const uint32_t eq_after = equal + (all & 0xFFFFu);
+        out += (all >> 16) + min(eq_after, need) - min(equal, need);
+        equal = eq_after;
+    }
+    if (!so) return;
+    if (!once)
+    {
+        __syncthreads();                                   // the kept positions written, visible to the workgroup
+        for (uint32_t i0 = 0; i0 < count; i0 += T)
+        {
+            const uint32_t i = i0 + tid;
+            const float x = i < count ? sc[kept[i]] : 0.0f;
+            __syncthreads();                               // scores_out may be scores: read before written
+            if (i < count) so[i] = x;
+        }
+    }
+    for (uint32_t i = count + tid; i < n; i += T) so[i] = 0.0f;
 }
 
 typedef uint32_t u4v __attribute__((ext_vector_type(4)));
 typedef float f4_t __attribute__((ext_vector_type(4)));
 
-constexpr uint32_t MOVE_CH = 16;                           // V channels a workgroup moves
-// positions a workgroup reads at a time: 16 KB either way
-template <int AF>
-constexpr uint32_t move_run() { return AF == OPURE_A_F32 ? 256u : 512u; }
+// 16 bytes; ONCE: of a cache past the last-level cache, where nothing is met again before it is displaced
+template <bool ONCE>
+__device__ __forceinline__ u4v move_load(const uint8_t* p)
+{
+    const u4v* q = reinterpret_cast<const u4v*>(p);
+    if constexpr (ONCE) return __builtin_nontemporal_load(q);
+    else return *q;
+}
+template <bool ONCE>
+__device__ __forceinline__ void move_store(uint8_t* p, u4v x)
+{
+    u4v* q = reinterpret_cast<u4v*>(p);
+    if constexpr (ONCE) __builtin_nontemporal_store(x, q);
+    else *q = x;
+}
 
 // a pair of a key's channels turned back by the angle of (c, s)
 template <int AF>
@@ -223,26 +253,26 @@ __device__ __forceinline__ uint32_t turn_pair(uint32_t v, float c, float s)
                              : static_cast<uint32_t>(f32_to_bf16(a)) | static_cast<uint32_t>(f32_to_bf16(b)) << 16;
 }
 
-// Moves part of one (sequence, layer, KV head): 64 bytes of its K rows, or 16
+// Moves part of one (sequence, layer, KV head): 16 KP bytes of its K rows, or 16
 // channels of its V planes, from the first position that can move to the last.
 // Parts never meet, so all run at once; within one the runs go in order, a run's
 // loads issued before the run before it is written (no slot that a run writes is
 // read by a later one), with one barrier between a run's loads and its stores.
-//   K: four threads a position, 256 kept positions a run, each thread's kept
+//   K: KP threads a position, 1024 / KP kept positions a run, each thread's kept
 // position, page and data fetched a run ahead of one another.
 //   V: a channel's positions lie side by side, so runs of source pages go whole
 // (their 32-byte rows hold a kept position nearly always) through LDS, rows of
 // one channel, and the kept ones are collected from there into 16-byte stores;
 // a group of positions that a run fills in part is stored by elements.
-template <int AF>
+template <int AF, uint32_t KP, uint32_t CH, bool ONCE>
 __global__ __launch_bounds__(256) void k_evict_move(EvictParams p)
 {
-    constexpr uint32_t EB = AF == OPURE_A_F32 ? 4u : 2u, RUN = move_run<AF>(), TPP = 16u / EB, PPC = 16u / TPP;
+    constexpr uint32_t EB = AF == OPURE_A_F32 ? 4u : 2u, RUN = 16384u / (CH * EB), TPP = 16u / EB, PPC = 16u / TPP;
     constexpr uint32_t ROW = RUN * EB + 16u;               // bytes of a channel's row in LDS, a piece of padding
-    __shared__ __align__(16) uint8_t rows[MOVE_CH * ROW];
+    __shared__ __align__(16) uint8_t rows[CH * ROW];
     __shared__ __align__(16) uint16_t from[RUN + 16u];     // the run's kept positions, from the run's first
     __shared__ uint32_t cnt[4];
-    const uint32_t hd = p.hd, segk = (hd * EB + 63u) / 64u, segs = segk + hd / MOVE_CH;
+    const uint32_t hd = p.hd, segk = (hd * EB + 16u * KP - 1u) / (16u * KP), segs = segk + hd / CH;
     const uint32_t b = blockIdx.y, head = blockIdx.x / segs, layer = head / p.n_kv, kh = head - layer * p.n_kv, tid = threadIdx.x;
     uint32_t seg = blockIdx.x - head * segs;
     const uint32_t n = evict_len(p, b);
@@ -255,7 +285,8 @@ __global__ __launch_bounds__(256) void k_evict_move(EvictParams p)
     if (seg < segk)
     {
         constexpr uint32_t U = 4;
-        const uint32_t piece = seg * 4u + (tid & 3u), tok = tid >> 2;
+        constexpr uint32_t PASS = 256u / KP, KRUN = U * PASS;   // positions a pass; a run
+        const uint32_t piece = seg * KP + tid % KP, tok = tid / KP;
         const bool mine = piece * 16u < hd * EB;
         const bool turn = p.cos != nullptr;
         auto kept_at = [&](uint32_t i) { return i < p.keep ? kept[i] : -1; };
@@ -263,12 +294,12 @@ __global__ __launch_bounds__(256) void k_evict_move(EvictParams p)
         int32_t s0[U], s1[U], ps[U], pd[U], qs[U], qd[U];
         u4v data[U], next[U];
         f4_t co[U], si[U], nco[U], nsi[U];
-        const uint32_t first = p.sinks / 256u * 256u;
+        const uint32_t first = p.sinks / KRUN * KRUN;
         auto pages = [&](uint32_t i0, const int32_t (&s)[U], int32_t (&a)[U], int32_t (&d)[U]) {
 #pragma unroll
             for (uint32_t u = 0; u < U; ++u)
             {
-                const uint32_t i = i0 + 64u * u + tok;
+                const uint32_t i = i0 + PASS * u + tok;
                 const bool moves = mine && s[u] > static_cast<int32_t>(i);
                 a[u] = moves ? pt[static_cast<uint32_t>(s[u]) / OPURE_PAGE_SIZE] : -1;
                 d[u] = moves ? pt[i / OPURE_PAGE_SIZE] : -1;
@@ -283,10 +314,10 @@ __global__ __launch_bounds__(256) void k_evict_move(EvictParams p)
 #pragma unroll
             for (uint32_t u = 0; u < U; ++u)
             {
-                const uint32_t i = i0 + 64u * u + tok;
+                const uint32_t i = i0 + PASS * u + tok;
                 if (a[u] < 0) continue;
                 const uint32_t t = static_cast<uint32_t>(s[u]);
-                x[u] = *reinterpret_cast<const u4v*>(base + static_cast<uint32_t>(a[u]) * page_bytes + (t % OPURE_PAGE_SIZE) * (hd * EB) + piece * 16u);
+                x[u] = move_load<ONCE>(base + static_cast<uint32_t>(a[u]) * page_bytes + (t % OPURE_PAGE_SIZE) * (hd * EB) + piece * 16u);
                 if (turn)
                 {
                     const uint64_t at = static_cast<uint64_t>(t - i) * (hd / 2u) + piece * (TPP / 2u);
@@ -308,24 +339,24 @@ __global__ __launch_bounds__(256) void k_evict_move(EvictParams p)
 #pragma unroll
         for (uint32_t u = 0; u < U; ++u)
         {
-            s0[u] = kept_at(first + 64u * u + tok);
-            s1[u] = kept_at(first + 256u + 64u * u + tok);
+            s0[u] = kept_at(first + PASS * u + tok);
+            s1[u] = kept_at(first + KRUN + PASS * u + tok);
         }
         pages(first, s0, ps, pd);
         load(first, s0, ps, data, co, si);
-        pages(first + 256u, s1, qs, qd);
-        for (uint32_t i0 = first; i0 < p.keep; i0 += 256u)
+        pages(first + KRUN, s1, qs, qd);
+        for (uint32_t i0 = first; i0 < p.keep; i0 += KRUN)
         {
             int32_t s2[U], rs[U], rd[U];
 #pragma unroll
-            for (uint32_t u = 0; u < U; ++u) s2[u] = kept_at(i0 + 512u + 64u * u + tok);
-            load(i0 + 256u, s1, qs, next, nco, nsi);
+            for (uint32_t u = 0; u < U; ++u) s2[u] = kept_at(i0 + 2u * KRUN + PASS * u + tok);
+            load(i0 + KRUN, s1, qs, next, nco, nsi);
             __syncthreads();
 #pragma unroll
             for (uint32_t u = 0; u < U; ++u)
             {
                 if (ps[u] < 0) continue;
-                const uint32_t i = i0 + 64u * u + tok;
+                const uint32_t i = i0 + PASS * u + tok;
                 u4v x = data[u];
                 if (turn)
                 {
@@ -341,9 +372,9 @@ __global__ __launch_bounds__(256) void k_evict_move(EvictParams p)
 #pragma unroll
                         for (uint32_t k = 0; k < 4; ++k) x[k] = turn_pair<AF>(x[k], co[u][k], si[u][k]);
                 }
-                *reinterpret_cast<u4v*>(base + static_cast<uint32_t>(pd[u]) * page_bytes + (i % OPURE_PAGE_SIZE) * (hd * EB) + piece * 16u) = x;
+                move_store<ONCE>(base + static_cast<uint32_t>(pd[u]) * page_bytes + (i % OPURE_PAGE_SIZE) * (hd * EB) + piece * 16u, x);
             }
-            pages(i0 + 512u, s2, rs, rd);
+            pages(i0 + 2u * KRUN, s2, rs, rd);
 #pragma unroll
             for (uint32_t u = 0; u < U; ++u)
             {
@@ -362,9 +393,9 @@ __global__ __launch_bounds__(256) void k_evict_move(EvictParams p)
     }
     // ---- V: 16 channels
     seg -= segk;
-    constexpr uint32_t U = 4, PG = RUN / OPURE_PAGE_SIZE, PPP = MOVE_CH * PPC;   // pages a run; pieces a page
+    constexpr uint32_t U = 4, PG = RUN / OPURE_PAGE_SIZE, PPP = CH * PPC;   // pages a run; pieces a page
     static_assert(PG * PPP == 256u * U, "a run is four pieces a thread");
-    uint8_t* vbase = base + p.n_kv * plane + static_cast<uint64_t>(seg) * MOVE_CH * OPURE_PAGE_SIZE * EB;
+    uint8_t* vbase = base + p.n_kv * plane + static_cast<uint64_t>(seg) * CH * OPURE_PAGE_SIZE * EB;
     const uint32_t wave = tid >> 6, lane = tid & 63u;
     u4v data[U];
     int32_t pe[U];
@@ -385,7 +416,7 @@ __global__ __launch_bounds__(256) void k_evict_move(EvictParams p)
 #pragma unroll
         for (uint32_t u = 0; u < U; ++u)
             if (pe[u] >= 0)
-                data[u] = *reinterpret_cast<const u4v*>(vbase + static_cast<uint32_t>(pe[u]) * page_bytes + (u * 256u + tid) % PPP * 16u);
+                data[u] = move_load<ONCE>(vbase + static_cast<uint32_t>(pe[u]) * page_bytes + (u * 256u + tid) % PPP * 16u);
     };
     constexpr uint32_t KW = RUN / 256u;
     int32_t kw[KW];
@@ -447,7 +478,7 @@ __global__ __launch_bounds__(256) void k_evict_move(EvictParams p)
                         for (uint32_t k = 0; k < 4; ++k)
                             x[k] = static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(row + f[2 * k] * 2u)) |
                                    static_cast<uint32_t>(*reinterpret_cast<const uint16_t*>(row + f[2 * k + 1] * 2u)) << 16;
-                    *reinterpret_cast<u4v*>(dst) = x;
+                    move_store<ONCE>(dst, x);
                 }
                 else
                     for (uint32_t i = a; i < z; ++i)
@@ -548,13 +579,30 @@ extern "C" int opure_kv_evict(opure_dev* dev, const opure_evict_args* a)
     // the other workgroups read seq_len and the table: what is written over them waits for a launch of its own
     p.new_len_now = !a->freed && a->new_seq_len != a->seq_len ? 1u : 0u;
     const uint32_t planes = p.n_layers * p.n_kv;
-    OPURE_LAUNCH(dev, k_evict_select, dim3(planes, a->batch), dim3(1024), 0, p);
+    if (a->max_ctx <= 4u * 64u * SEL) OPURE_LAUNCH(dev, (k_evict_select<4>), dim3(planes, a->batch), dim3(256), 0, p);
+    else if (a->max_ctx <= 8u * 64u * SEL) OPURE_LAUNCH(dev, (k_evict_select<8>), dim3(planes, a->batch), dim3(512), 0, p);
+    else OPURE_LAUNCH(dev, (k_evict_select<16>), dim3(planes, a->batch), dim3(1024), 0, p);
     OPURE_LAUNCH_CHECK("k_evict_select");
-    const uint32_t eb = act_bytes(p.afmt), segs = (p.hd * eb + 63u) / 64u + p.hd / MOVE_CH;
-    auto move = [&](auto k) { OPURE_LAUNCH(dev, k, dim3(planes * segs, a->batch), dim3(256), 0, p); };
-    if (p.afmt == OPURE_A_F32) move(&k_evict_move<OPURE_A_F32>);
-    else if (p.afmt == OPURE_A_F16) move(&k_evict_move<OPURE_A_F16>);
-    else move(&k_evict_move<OPURE_A_BF16>);
+    const uint32_t row = p.hd * act_bytes(p.afmt);
+#ifndef SKP
+#define SKP 4
+#endif
+#ifndef SCH
+#define SCH 16
+#endif
+    const bool once = static_cast<uint64_t>(planes) * a->batch * a->max_ctx * row * 2u > 256u << 20;
+    auto move = [&](auto af) {
+        constexpr int AF = decltype(af)::value;
+        auto go = [&](auto kernel, uint32_t kp, uint32_t ch) {
+            OPURE_LAUNCH(dev, kernel, dim3(planes * ((row + 16u * kp - 1u) / (16u * kp) + p.hd / ch), a->batch), dim3(256), 0, p);
+        };
+        if (!once) go(&k_evict_move<AF, SKP, SCH, false>, SKP, SCH);
+        else if (row % 128u == 0u) go(&k_evict_move<AF, 8, 16, true>, 8u, 16u);
+        else go(&k_evict_move<AF, 4, 16, true>, 4u, 16u);
+    };
+    if (p.afmt == OPURE_A_F32) move(std::integral_constant<int, OPURE_A_F32>{});
+    else if (p.afmt == OPURE_A_F16) move(std::integral_constant<int, OPURE_A_F16>{});
+    else move(std::integral_constant<int, OPURE_A_BF16>{});
     OPURE_LAUNCH_CHECK("k_evict_move");
     if (p.new_len_now) return OPURE_OK;
     OPURE_LAUNCH(dev, k_evict_finish, dim3(a->batch), dim3(64), 0, p);
