@@ -11,8 +11,10 @@
 #include "window.h"
 
 #include <algorithm>
+#include <cmath>
 
 using namespace opure_win;
+using opure_hip::act_bytes;
 
 namespace {
 
@@ -444,6 +446,35 @@ struct WinPlan {
     uint64_t bytes() const { return acc + ml + scores + lse + sums; }
 };
 
+// Which kernels take a call, by what each would take (us, of what was measured on
+// 8 KV heads of 64 and 128 channels and 4 query heads each):
+//   k_win_prompt walks all tiles of 64 positions in one workgroup a 128 query rows:
+//     5 + 0.73 a tile (1.15 at 128 channels), times the workgroups a CU;
+//   k_win_split + k_win_join: 8.5, and 1 ns a tile of 32 positions, block of query
+//     rows and 100 channels.
+// Measured, prompt / split: 64 query rows of a KV head over 64 positions 6.3 / 8.6,
+// over 1,000 16.4 / 9.6, over 8,000 92.6 / 15.7; four sequences of 512 over 1,000
+// 18.8 / 30.7, over 8,000 95 / 97; 1,024 of 128 channels behind a window of 1,024
+// 29.2 / 26.3, four sequences 33.0 / 77.1.
+//   Weights from stored scores cost the join 0.17 a query row, computed again
+// (k_win_sums) about 3 and the keys once more at 2.5 TB/s.  Measured, stored /
+// computed again: 16 query rows over 64 positions 9.7 / 11.2, 64 18.0 / 11.9; four
+// sequences over 8,000 positions of 128 channels, 16 41.7 / 75.1, 64 81.1 / 92.4,
+// 128 139 / 124.
+void win_choose(const opure_dev* dev, const opure_attn_window_args* a, WinPlan& w)
+{
+    const opure_model* m = a->model;
+    const double G = m->n_heads / m->n_kv_heads, Gq = G * a->rows, hd = m->head_dim, cu = dev->n_cu > 0 ? dev->n_cu : 256;
+    const double heads = static_cast<double>(a->batch) * m->n_kv_heads, span = static_cast<double>(w.tiles) * w.tt;
+    const double wgs = heads * std::ceil(Gq / 128.0), window = a->window ? a->window : 2147483647.0;
+    const double prompt = 5.0 + std::max(1.0, wgs / cu) * std::ceil(std::min(span, a->sinks + window + 128.0 / G) / 64.0) * (0.31 + hd / 152.0);
+    const double split = 8.5 + heads * std::ceil(Gq / (Gq > 16.0 && hd <= 128.0 ? 32.0 : 16.0)) * w.tiles * hd * 1e-5;
+    const double store = 0.17 * Gq, again = 3.0 + heads * span * hd * act_bytes(m->afmt) / 2.5e6;
+    w.stored = a->weights && Gq <= 96.0 && store < again;
+    w.prompt = m->afmt != OPURE_A_F32 && prompt + (a->weights ? again : 0.0) < split + (a->weights ? std::min(store, again) : 0.0);
+    if (w.prompt) w.stored = false;
+}
+
 int win_plan(opure_dev* dev, const opure_attn_window_args* a, WinPlan& w)
 {
     const opure_model* m = a->model;
@@ -453,8 +484,7 @@ int win_plan(opure_dev* dev, const opure_attn_window_args* a, WinPlan& w)
     const uint64_t all = (a->max_ctx + w.tt - 1u) / w.tt, window = a->window ? a->window : 0x7FFFFFFFu;
     w.tiles = static_cast<uint32_t>(std::min<uint64_t>(all, (a->sinks + w.tt - 1ull) / w.tt + (window + a->rows + w.tt - 2ull) / w.tt + 1u));
     const uint64_t rows = static_cast<uint64_t>(a->batch) * m->n_kv_heads * Gq;
-    w.prompt = m->afmt != OPURE_A_F32 && Gq >= 256u;
-    w.stored = a->weights && Gq <= 64u;
+    win_choose(dev, a, w);
     w.lse = a->weights && !w.stored ? opure_hip::align_up(rows * 4u, 256) : 0u;
     if (w.lse)
     {
