@@ -549,6 +549,10 @@ extern "C" int opure_kv_evict(opure_dev* dev, const opure_evict_args* a)
     OPURE_REQUIRE(!a->freed || a->freed_stride >= (a->max_ctx + OPURE_PAGE_SIZE - 1u) / OPURE_PAGE_SIZE, OPURE_E_INVALID,
                   "opure_kv_evict: freed_stride %u below the pages of max_ctx %u", a->freed_stride, a->max_ctx);
     OPURE_REQUIRE((reinterpret_cast<uintptr_t>(kv->pool) & 15u) == 0u, OPURE_E_INVALID, "opure_kv_evict: pool must be 16-byte aligned");
+    OPURE_REQUIRE(((reinterpret_cast<uintptr_t>(a->scores) | reinterpret_cast<uintptr_t>(a->scores_out) | reinterpret_cast<uintptr_t>(a->kept) |
+                    reinterpret_cast<uintptr_t>(a->seq_len) | reinterpret_cast<uintptr_t>(a->new_seq_len) | reinterpret_cast<uintptr_t>(a->freed) |
+                    reinterpret_cast<uintptr_t>(a->n_freed) | reinterpret_cast<uintptr_t>(kv->page_table)) & 3u) == 0u, OPURE_E_INVALID,
+                  "opure_kv_evict: scores, kept, lengths and tables must be 4-byte aligned");
     const DeviceGuard on(dev);
     EvictParams p{};
     p.pool = kv->pool;

@@ -338,13 +338,15 @@ __global__ __launch_bounds__(256) void k_win_join(WinParams p)
     const uint32_t at = (x * 256u + threadIdx.x) * PPT, i = min(at / TT, span.n - 1u), off = at % TT;
     const uint32_t t = at < span.n * TT ? span.tile(i) * TT + off : sq.total;
     const float* s = p.scores + (static_cast<uint64_t>(bh) * p.tiles + i) * Gq * TT + off;
-    float sum[PPT];
+    float* to = p.weights + b * p.weights_batch_stride + static_cast<uint64_t>(kh) * p.weights_stride + t;
+    float sum[PPT], old[PPT];
     bool any[PPT];
 #pragma unroll
     for (uint32_t k = 0; k < PPT; ++k)
     {
         sum[k] = 0.0f;
         any[k] = false;
+        old[k] = t + k < sq.total ? to[k] : 0.0f;
     }
     uint32_t j = 0, g = 0;                                    // the query row's row and head
     constexpr uint32_t U = 8u / PPT, C = 4u * U;              // rows a wave; a turn
@@ -396,10 +398,9 @@ __global__ __launch_bounds__(256) void k_win_join(WinParams p)
                 j += wrap ? 1u : 0u;
             }
     }
-    float* to = p.weights + b * p.weights_batch_stride + static_cast<uint64_t>(kh) * p.weights_stride + t;
 #pragma unroll
     for (uint32_t k = 0; k < PPT; ++k)
-        if (any[k]) to[k] += sum[k];
+        if (any[k]) to[k] = old[k] + sum[k];
 }
 
 template <int HD, int NT>

@@ -130,12 +130,36 @@ def test_head_sizes(dev, hd, afmt, turn):
     check(dev, afmt, 2, 3, hd, [100, 3, 47, 161], 2, 21, 24, turn, seed=hd)
 
 
+@pytest.mark.parametrize("afmt", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd", list(range(16, 257, 16)))
+def test_caches_past_the_last_level_cache(dev, hd, afmt):
+    """What a cache could hold (max_ctx) decides how it is moved: 256 MB and more
+    whole lines at a time, here with few positions in it; 600 of them take several runs."""
+    say("evict large", hd, afmt)
+    eb = 4 if afmt == F32 else 2
+    extra = (300 << 20) // (2 * hd * eb * 2 * 2)
+    check(dev, afmt, 1, 2, hd, [600, 90], 3, 100, 130, hd % 32 == 0 and extra < 400000, seed=hd, extra=extra)
+
+
 @pytest.mark.parametrize("sinks,recent,heavy", [(0, 1, 0), (0, 0, 1), (1, 0, 0), (4, 30, 0), (0, 0, 50), (16, 16, 16), (5, 1, 250), (0, 299, 0),
                                                 (0, 0, 300), (100, 100, 99), (1000, 2, 3), (0, 40, 1)])
 def test_budgets(dev, sinks, recent, heavy):
     say("budget", sinks, recent, heavy)
     check(dev, F16, 1, 2, 64, [300, 0, 1, 16, 17, 299, 50], sinks, recent, heavy, seed=sinks)
     check(dev, BF16, 2, 1, 32, [300, 16], sinks, recent, heavy, seed=sinks, free=False, in_place=True, extra=40)
+
+
+@pytest.mark.parametrize("seed", range(40))
+def test_shapes_at_random(dev, seed):
+    r = np.random.default_rng(2000 + seed)
+    seq = [int(r.integers(0, int(2 ** r.uniform(3, 12.5)))) for _ in range(int(r.integers(1, 5)))]
+    keep = 1 + int(r.integers(0, max(seq) + 20))
+    sinks = int(r.integers(0, min(keep, 40) + 1))
+    recent = int(r.integers(0, keep - sinks + 1))
+    afmt, hd = int(r.integers(0, 3)), 16 * int(r.integers(1, 9))
+    say("evict random", seed, afmt, hd, seq, sinks, recent, keep)
+    check(dev, afmt, int(r.integers(1, 4)), int(r.integers(1, 4)), hd, [max(1, n) for n in seq], sinks, recent, keep - sinks - recent,
+          bool(r.integers(0, 2)), seed=seed, in_place=bool(r.integers(0, 2)), free=bool(r.integers(0, 2)), extra=int(r.choice([0, 5, 5000])))
 
 
 @pytest.mark.parametrize("n,keep", [(1024, 1000), (1025, 64), (2049, 1500), (5000, 1100), (9000, 4500), (20000, 300)])

@@ -22,14 +22,14 @@ def dev():
     d.close()
 
 
-def check(dev, afmt, heads, n_kv, hd, seq, rows, window, sinks, weights=False, layers=1, seed=0, edit=None, spread=1.5, max_ctx=None):
+def check(dev, afmt, heads, n_kv, hd, seq, rows, window, sinks, weights=False, layers=1, seed=0, edit=None, spread=1.5, max_ctx=None, scale=None):
     rng = np.random.default_rng(seed)
     layer = layers - 1
     cache = R.Cache(rng, afmt, layers, n_kv, hd, [n + rows for n in seq], cap=max_ctx)
     q = R.act_to_f32(R.f32_to_act(rng.standard_normal((len(seq), rows, heads, hd), dtype=np.float32) * np.float32(spread), afmt), afmt)
     if edit:
         edit(cache, q)
-    scale = hd ** -0.5
+    scale = hd ** -0.5 if scale is None else scale
     cap = max_ctx or max(seq) + rows
     w0 = rng.random((len(seq), layers, n_kv, cap + 5), dtype=np.float32) if weights else None
     c = R.Call(dev, cache, q, heads, seq, rows, window, sinks, scale, layer, cap, w0)
@@ -72,6 +72,53 @@ def check(dev, afmt, heads, n_kv, hd, seq, rows, window, sinks, weights=False, l
 def test_head_sizes(dev, hd, afmt, weights):
     say("head size", hd, afmt, weights)
     check(dev, afmt, 6, 2, hd, [0, 37, 150], 3, 50, 5, weights, seed=hd)
+
+
+SHAPES = {  # sequences, rows, heads: every way a call is run, at every head size
+    "one-block": ([900, 3, 511], 3, 6),                  # up to 16 query rows a KV head over a long cache
+    "two-blocks": ([1200, 40], 12, 6),                   # 36: blocks of 32
+    "prompt": ([70], 130, 4),                            # 260 over a short one
+    "wide": ([30, 0, 64, 5] * 20, 70, 8),                # 280 in 80 sequences: more workgroups than the device has CUs
+}
+
+
+@pytest.mark.parametrize("shape,afmt,weights", [(s, f, w) for s in SHAPES for f in (F32, F16, BF16) for w in (False, True)
+                                                if s != "wide" or not (w or f == F32)])   # there, as the prompt's
+@pytest.mark.parametrize("hd", list(range(16, 257, 16)))
+def test_every_kernel(dev, shape, hd, afmt, weights):
+    seq, rows, heads = SHAPES[shape]
+    say("kernel", shape, hd, afmt, weights)
+    check(dev, afmt, heads, 2, hd, seq, rows, 333 if shape != "wide" else 40, 6, weights, seed=hd)
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.11, 1.0, 3.0])
+@pytest.mark.parametrize("rows,n", [(2, 700), (90, 20)])
+def test_scales(dev, rows, n, scale):
+    """attn_scale of either sign, and 0, where every visible position weighs the same."""
+    say("scale", scale, rows)
+    for afmt in (F32, F16, BF16):
+        check(dev, afmt, 4, 2, 64, [n], rows, 50, 3, True, seed=rows, spread=0.3, scale=scale)
+
+
+@pytest.mark.parametrize("seed", range(60))
+def test_shapes_at_random(dev, seed):
+    r = np.random.default_rng(1000 + seed)
+    n_kv, G = int(r.choice([1, 2, 3, 5, 8])), int(r.choice([1, 2, 3, 4, 7, 8]))
+    afmt, hd = int(r.integers(0, 3)), 16 * int(r.integers(1, 17))
+    rows = int(r.choice([1, 1, 2, 5, 9, 16, 33, 70, 150]))
+    batch = int(r.integers(1, 6)) if rows < 33 else int(r.integers(1, 3))
+    most = int(2 ** r.uniform(3, 11))
+    seq = [int(r.integers(0, most)) for _ in range(batch)]
+    window, sinks = int(r.choice([0, 1, 15, 16, 63, 64, int(2 ** r.uniform(0, 11))])), int(r.choice([0, 0, 1, 4, 16, 33, 200]))
+    say("random", seed, afmt, n_kv, G, hd, seq, rows, window, sinks)
+    check(dev, afmt, n_kv * G, n_kv, hd, seq, rows, window, sinks, bool(r.integers(0, 2)), seed=seed,
+          max_ctx=max(seq) + rows + int(r.choice([0, 0, 7, 500])))
+
+
+def test_most_sequences(dev):
+    rng = np.random.default_rng(12)
+    check(dev, F16, 8, 2, 64, [int(n) for n in rng.integers(0, 400, 256)], 1, 100, 4, True)
+    check(dev, BF16, 4, 1, 32, [int(n) for n in rng.integers(0, 60, 256)], 3, 0, 0, False)
 
 
 @pytest.mark.parametrize("window,sinks", [(1, 0), (1, 1), (1, 40), (7, 0), (16, 4), (17, 3), (33, 16), (64, 70), (100, 0), (129, 33),

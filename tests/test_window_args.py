@@ -111,6 +111,9 @@ def test_evict_refusals(fake, kw, code):
 
 def test_evict_refuses_models_and_caches(fake):
     L, (at, m, kv, _) = H.lib(), fake
+    for name in ("scores", "scores_out", "kept", "seq_len", "new_seq_len", "freed", "n_freed"):
+        assert L.opure_kv_evict(at, C.byref(evict_args(fake, **{name: at + 2}))) == H.E_INVALID, name
+        assert b"aligned" in L.opure_last_error()
     assert L.opure_kv_evict(None, C.byref(evict_args(fake))) == H.E_INVALID
     assert L.opure_kv_evict(at, None) == H.E_INVALID
     for obj, what, value, code in ((m, "n_layers", 0, H.E_INVALID), (m, "n_kv_heads", 0, H.E_INVALID), (m, "head_dim", 40, H.E_UNSUPPORTED),
