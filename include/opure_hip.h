@@ -265,10 +265,15 @@ int opure_attn_decode_paged(opure_dev* dev, const opure_attn_args* a);
  *      opure_kv_evict goes by; one layer's part of its [batch][n_layers]
  *      [n_kv_heads][stride] array is weights + layer * n_kv_heads * stride with
  *      weights_batch_stride = n_layers * n_kv_heads * stride.
- *        pool and q are 16-byte aligned, out 8-byte.  The order of sums follows
- *      the shape of the call (batch, rows, max_ctx, window, sinks and whether
- *      there are weights): the same call gives the same bits, a row alone and
- *      in a batch may differ in its last ones. */
+ *        pool and q are 16-byte aligned, out 8-byte.  Scores, maxima and sums are
+ *      fp32; with a 16-bit cache a weight meets V as two 16-bit numbers where a
+ *      call has few query rows a KV head, and rounded once to the cache's
+ *      format where many share the work (off by half a step, as the result
+ *      itself).  Which, and the order of sums, follow the shape of the call
+ *      (batch, rows, max_ctx, window, sinks and whether there are weights): the
+ *      same call gives the same bits, a row alone and in a batch may differ in
+ *      its last ones.  A length below 0 or past max_ctx is OPURE_E_CAPACITY at
+ *      the next sync; positions past max_ctx are neither read nor weighed. */
 typedef struct opure_attn_window_args {
     const opure_model* model; /* n_layers, n_heads, n_kv_heads, head_dim, attn_scale, afmt */
     const opure_kv*    kv;
@@ -390,8 +395,10 @@ int opure_kv_rollback(opure_dev* dev, const opure_rollback_args* a);
  *      rope_max_pos >= max_ctx.  Without it keys move as they are.
  *        With `freed`, pages wholly past the kept positions are released as
  *      opure_kv_rollback does (entry -> -1, id to freed[b][...]); without, they
- *      stay in the row for the tokens to come.  A page that is missing among
- *      the seq_len positions is OPURE_E_CAPACITY at the next sync, as is a
+ *      stay in the row for the tokens to come (entries of freed[b] past
+ *      n_freed[b] are left as they are).  No page is in the table twice: a cache
+ *      whose sequences share a prefix's pages cannot be evicted in place.  A
+ *      page that is missing among the seq_len positions is OPURE_E_CAPACITY at the next sync, as is a
  *      length past max_ctx or the table; what such a sequence's cache and
  *      outputs then hold is not defined, but no access leaves the buffers. */
 typedef struct opure_evict_args {

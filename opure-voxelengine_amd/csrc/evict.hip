@@ -83,7 +83,7 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t* wsum, uin
 // up to 512 W positions are read once, ordered by one prefix sum, and written with
 // their scores as they are found (all scores are read by then: scores_out may be
 // scores).  Bound by its chain of counts and barriers: as few waves as hold the
-// sequence (2,048 positions: 4 waves, where 16 took 13 us).
+// sequence (128 heads of 2,048 positions: 9 us with 4 waves, 13 with 16).
 constexpr uint32_t SEL = 8;
 
 template <uint32_t W>
@@ -253,7 +253,7 @@ __device__ __forceinline__ uint32_t turn_pair(uint32_t v, float c, float s)
                              : static_cast<uint32_t>(f32_to_bf16(a)) | static_cast<uint32_t>(f32_to_bf16(b)) << 16;
 }
 
-// Moves part of one (sequence, layer, KV head): 16 KP bytes of its K rows, or 16
+// Moves part of one (sequence, layer, KV head): 16 KP bytes of its K rows, or CH
 // channels of its V planes, from the first position that can move to the last.
 // Parts never meet, so all run at once; within one the runs go in order, a run's
 // loads issued before the run before it is written (no slot that a run writes is
@@ -264,6 +264,14 @@ __device__ __forceinline__ uint32_t turn_pair(uint32_t v, float c, float s)
 // (their 32-byte rows hold a kept position nearly always) through LDS, rows of
 // one channel, and the kept ones are collected from there into 16-byte stores;
 // a group of positions that a run fills in part is stored by elements.
+//   Bound by the cache's bytes: 32 layers of 3 sequences of 3,500 to 8,000
+// positions cut to 2,504 (8 KV heads of 128) read K where it is kept, V whole and
+// write both, 2.6 GB in 635 us, 4.0 TB/s (a copy reaches 4.65); 16 layers of 2,048
+// positions halved (heads of 64), 84 MB in 22 us.
+//   A cache past the last-level cache (256 MB) moves K in whole 128-byte lines,
+// which two parts on two XCDs would each fetch, and with accesses that do not stay
+// in the caches: 64-byte parts 790 us, lines 730, and streaming 679 for the first;
+// the second takes 34 us with 64-byte parts, 39 with lines, 44 streaming.
 template <int AF, uint32_t KP, uint32_t CH, bool ONCE>
 __global__ __launch_bounds__(256) void k_evict_move(EvictParams p)
 {
@@ -588,19 +596,13 @@ extern "C" int opure_kv_evict(opure_dev* dev, const opure_evict_args* a)
     else OPURE_LAUNCH(dev, (k_evict_select<16>), dim3(planes, a->batch), dim3(1024), 0, p);
     OPURE_LAUNCH_CHECK("k_evict_select");
     const uint32_t row = p.hd * act_bytes(p.afmt);
-#ifndef SKP
-#define SKP 4
-#endif
-#ifndef SCH
-#define SCH 16
-#endif
     const bool once = static_cast<uint64_t>(planes) * a->batch * a->max_ctx * row * 2u > 256u << 20;
     auto move = [&](auto af) {
         constexpr int AF = decltype(af)::value;
         auto go = [&](auto kernel, uint32_t kp, uint32_t ch) {
             OPURE_LAUNCH(dev, kernel, dim3(planes * ((row + 16u * kp - 1u) / (16u * kp) + p.hd / ch), a->batch), dim3(256), 0, p);
         };
-        if (!once) go(&k_evict_move<AF, SKP, SCH, false>, SKP, SCH);
+        if (!once) go(&k_evict_move<AF, 4, 16, false>, 4u, 16u);
         else if (row % 128u == 0u) go(&k_evict_move<AF, 8, 16, true>, 8u, 16u);
         else go(&k_evict_move<AF, 4, 16, true>, 4u, 16u);
     };

@@ -29,6 +29,10 @@ constexpr uint32_t MAX_PARTS = 64;                         // of a (sequence, KV
 // set of registers.  The four waves are merged in LDS, the parts by k_win_join.
 //   A probability enters its product as two 16-bit numbers (its rounding and the
 // rest: 16 bits of bf16, 22 of fp16): the products are not what bounds this.
+//   32 sequences of 1,024 to 16,384 positions behind a window of 4,096 (8 KV heads
+// of 128) read 412 MB in 76 us, 5.4 TB/s; reads alone of such scattered 4 KB planes
+// reach 5.8.  One row over 1,000 positions of heads of 64 takes 4.4 us, a chain of
+// round trips (length, page entries, keys and values) rather than bytes.
 template <int AF, int HD, int NT>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 2 ? 2 : 1))) void k_win_split(WinParams p)
 {
@@ -245,11 +249,15 @@ __device__ __forceinline__ void win_total(float m, float l, uint32_t parts, uint
 // one) or four rows (a wave each); DPL channels a lane.  A lane takes a part's
 // maximum and sum, then channels.  Loads are unconditional (past the last part
 // the last one again, weight 0): the code stays small, and a launch this short
-// pays for every line of it.  A row that is not finite is computed again position
+// pays for every line of it (3.5 us for one row of 32 heads in 9 parts, 7.2 with
+// each load under its test).  A row that is not finite is computed again position
 // by position: a NaN or an infinity among the values of a position that the row
 // does not see meets weight 0 in the products above.  With scores, the launch's
-// other workgroups add the weights: PPT positions a thread (one where there are few),
-// over the query rows in order, 32 / PPT rows' maxima and sums at a time.
+// other workgroups add the weights: PPT positions a thread (one where there are
+// few), over the query rows in order, 32 / PPT rows' maxima and sums at a time.
+//   A launch of its own: joining in the workgroup that arrives last needs fences
+// across the XCDs, which cost more than the launch (one row over 1,000 positions
+// 7.9 us in two launches, 9.5 in one; the 32 sequences above 78 and 433).
 template <uint32_t TT, bool WIDE, uint32_t DPL, uint32_t PPT>
 __global__ __launch_bounds__(256) void k_win_join(WinParams p)
 {

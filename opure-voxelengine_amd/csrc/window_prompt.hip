@@ -40,6 +40,11 @@ constexpr uint32_t prompt_lds() { return 2u * (prompt_k_pieces<HD>() + prompt_v_
 // itself is): the matrix unit is what bounds a prompt, and a second product for
 // the rounding's rest would cost it half as much again.  fp16 weights are held
 // 2^6 higher, so that those down to 2^-20 of the largest keep their bits.
+//   Bound by the matrix and vector units together, which overlap little (36% and
+// 43% of the clocks): 2,048 rows of 32 heads of 128 over 4,096 positions each take
+// 160 to 170 us, 810 to 860 TFLOP/s, where a library product of 8,192 x 8,192
+// matrices reaches 1,133; 1,437 rows of 32 heads of 64 behind a window of 512, ten
+// tiles a workgroup, 18 us.
 //   KG 2 (a grid that does not give every SIMD two waves): eight waves, two for
 // each 32 rows, one on the even tiles and one on the odd ones, merged at the end.
 template <int AF, int HD, int KG>
@@ -314,16 +319,20 @@ __global__ __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(HD <= 
 }
 
 // Weights from many rows: a workgroup takes 64 positions (32 of an fp32 cache) of
-// a (sequence, KV head) and a chunk of 512 query rows, its eight waves every
-// eighth block of 16 of those rows that see one of the positions.  A wave holds the positions' keys as operands, computes the
-// block's scores again and adds 2^(score - lse) to a sum a lane and position; the
-// lanes' and waves' sums are added in order.  To store the scores instead would
-// take as many bytes as K and V together from 64 query rows of a KV head on.
+// a (sequence, KV head) and a chunk of 1,536 query rows, its four waves every
+// fourth block of 16 of those rows that see one of the positions.  A wave holds
+// the positions' keys as operands, computes the block's scores again and adds
+// 2^(score - lse) to a sum a lane and position; the lanes' and waves' sums are
+// added in order.
 //   With more than one chunk each leaves its sums in a place of its own, and
 // k_win_add adds them in order: the first positions of a prompt are seen by all of
 // its rows, which one workgroup took 30 us to walk through (1,024 rows of the 1B
-// shape).
-constexpr uint32_t SUM_ROWS = 512;
+// shape; 16 in chunks).  Bound there by its first loads and by the exponentials,
+// 16 clocks each on a SIMD.  Whole calls with chunks of 512, 1,024, 1,536, 2,048
+// and 4,096: that prompt 38.4, 35.7, 36.2, 37.3, 46.6 us; 2,048 rows 82.3, 81.8,
+// 74.4, 80.6, 81.7; 2,048 rows of 128 channels behind a window of 4,096 375, 345,
+// 334, 345, 318.
+constexpr uint32_t SUM_ROWS = 1536;
 
 // rows [ja, jz) of a chunk that see a position of [t0, t0 + n)
 __device__ __forceinline__ void sums_rows(const WinParams& p, const WinSeq& sq, uint32_t G, uint32_t chunk, uint32_t t0, uint32_t n,
@@ -339,7 +348,7 @@ __device__ __forceinline__ void sums_rows(const WinParams& p, const WinSeq& sq, 
 constexpr uint32_t SUM_WAVES = 4;
 
 template <int AF, int HD>
-__global__ __launch_bounds__(64 * SUM_WAVES) __attribute__((amdgpu_waves_per_eu(HD <= 64 ? 4 : HD <= 128 ? 2 : 1))) void k_win_sums(WinParams p)
+__global__ __launch_bounds__(64 * SUM_WAVES) __attribute__((amdgpu_waves_per_eu(HD <= 64 && AF != OPURE_A_F32 ? 4 : HD <= 128 ? 2 : 1))) void k_win_sums(WinParams p)
 {
     typedef WinTile<AF, HD> T;
     constexpr uint32_t NS = T::NS, TILE = 2u * T::TT;
@@ -512,7 +521,8 @@ namespace opure_win {
 int win_prompt_launch(opure_dev* dev, const WinParams& p, uint32_t batch)
 {
     const uint32_t Gq = p.n_heads / p.n_kv * p.rows, wgs = p.n_kv * ((Gq + 127u) / 128u) * batch;
-    const bool two = wgs <= static_cast<uint32_t>(dev->n_cu > 0 ? dev->n_cu : 256);   // 256: 21 us against 17 (1,024 causal rows); 360: 18.2 against 22.9
+    // KG 1 against 2: 256 workgroups (1,024 causal rows) 21 against 17 us, 360 18.2 against 22.9
+    const bool two = wgs <= static_cast<uint32_t>(dev->n_cu > 0 ? dev->n_cu : 256);
     auto go = [&](auto af) {
         return win_by_head(p.hd, [&](auto h) {
             constexpr int AF = decltype(af)::value, HD = decltype(h)::value;
