@@ -284,7 +284,7 @@ typedef struct opure_attn_window_args {
     uint32_t           window;      /* positions a row sees up to its own, which counts; 0 = all */
     uint32_t           sinks;       /* first positions that stay visible */
     const void*        q;           /* [batch*rows][n_heads*head_dim] in afmt */
-    void*              out;         /* like q */
+    void*              out;         /* like q, and apart from it */
     float*             weights;     /* device, or NULL */
     uint32_t           weights_stride;        /* floats between KV heads, >= max_ctx */
     uint64_t           weights_batch_stride;  /* floats between sequences */

@@ -90,7 +90,7 @@ template <uint32_t W>
 __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W == 16 ? 8 : 4))) void k_evict_select(EvictParams p)
 {
     constexpr uint32_t T = 64u * W, BLOCK = T * SEL, BINS = 2048u, PER = BINS / T;
-    __shared__ uint32_t hist[BINS], pick[2], wsum[6][W];
+    __shared__ uint32_t hist[BINS], pick[3], wsum[4][W];
     const uint32_t b = blockIdx.y, tid = threadIdx.x;
     const uint64_t plane = static_cast<uint64_t>(b) * p.n_layers * p.n_kv + blockIdx.x;
     const int32_t raw = p.seq_len[b];
@@ -164,12 +164,20 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W == 16 
             {
                 pick[0] = BINS - 1u - (tid * PER + i);
                 pick[1] = need - above;
+                pick[2] = h[i];
             }
             above += h[i];
         }
         __syncthreads();
         prefix |= pick[0] << shift;
         need = pick[1];
+        if (step < 2u && need == pick[2])
+        {
+            // the whole group stays: all keys from its lowest on (no key is 0)
+            --prefix;
+            need = 0;
+            break;
+        }
     }
     uint32_t out = 0, equal = 0;                           // kept and equal keys of the blocks before
     for (uint32_t t0 = 0; t0 < n; t0 += BLOCK)

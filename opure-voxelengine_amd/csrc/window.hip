@@ -597,6 +597,9 @@ extern "C" int opure_attn_window_paged(opure_dev* dev, const opure_attn_window_a
     OPURE_REQUIRE((reinterpret_cast<uintptr_t>(a->q) & 15u) == 0u && (reinterpret_cast<uintptr_t>(a->out) & 7u) == 0u &&
                       ((reinterpret_cast<uintptr_t>(a->seq_len) | reinterpret_cast<uintptr_t>(a->weights)) & 3u) == 0u,
                   OPURE_E_INVALID, "opure_attn_window_paged: q must be 16-byte aligned, out 8-byte, seq_len and weights 4-byte");
+    const uint64_t bytes = static_cast<uint64_t>(a->batch) * a->rows * a->model->n_heads * a->model->head_dim * act_bytes(a->model->afmt);
+    const uintptr_t q = reinterpret_cast<uintptr_t>(a->q), out = reinterpret_cast<uintptr_t>(a->out);
+    OPURE_REQUIRE(q + bytes <= out || out + bytes <= q, OPURE_E_INVALID, "opure_attn_window_paged: out overlaps q");
     const DeviceGuard on(dev);
     WinPlan w;
     rc = win_plan(dev, a, w);

@@ -242,6 +242,29 @@ def test_captured_and_replayed(dev):
     e.done()
 
 
+def test_offsets_past_32_bits(dev):
+    """A pool whose last pages lie past 2^32 bytes (and elements)."""
+    rng = np.random.default_rng(6)
+    n_kv, hd, n = 8, 128, 150
+    cache = R.Cache(rng, F16, 1, n_kv, hd, [n])
+    scores = rng.random((1, 1, n_kv, n), dtype=np.float32)
+    e = Evict(dev, cache, [n], scores, 4, 30, 40, True)
+    page_bytes = 2 * n_kv * 16 * hd * 2
+    big = (5 << 31) // page_bytes
+    pool = dev.alloc(big * page_bytes)
+    first = big - cache.n_pages
+    dev.write(pool, cache.pool, first * page_bytes)
+    dev.write(e.table, np.where(cache.table >= 0, cache.table + first, -1).astype(np.int32))
+    e.kv.pool, e.kv.n_pages = int(pool), big
+    e.run()
+    got = dev.download(pool, np.uint16, cache.pool.shape, first * page_bytes)
+    small = Evict(dev, cache, [n], scores, 4, 30, 40, True).run()
+    assert np.array_equal(got, small.get()["pool"]) and np.array_equal(e.get()["kept"], small.get()["kept"])
+    e.done()
+    small.done()
+    pool.free()
+
+
 @pytest.mark.parametrize("wfmt,afmt,bar", [(O.W_F32, O.A_F32, 1e-4), (O.W_I8PC, O.A_F16, 2e-2), (O.W_I4G128, O.A_BF16, 2e-2)],
                          ids=["f32", "i8-f16", "i4-bf16"])
 def test_prompt_weights_eviction_and_on(dev, wfmt, afmt, bar):

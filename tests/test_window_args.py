@@ -97,6 +97,14 @@ def test_window_refuses_models_and_caches(fake):
         assert b"aligned" in L.opure_last_error()
 
 
+def test_window_refuses_out_over_q(fake):
+    L, at = H.lib(), fake[0]
+    size = 2 * 4 * 8 * 64 * 2
+    for off in (0, 16, size - 16, -size + 16):
+        assert L.opure_attn_window_paged(at, C.byref(window_args(fake, q=at + 65536, out=at + 65536 + off))) == H.E_INVALID
+        assert b"overlaps" in L.opure_last_error()
+
+
 EVICT = [(dict(seq_len=None), H.E_INVALID), (dict(scores=None), H.E_INVALID), (dict(kept=None), H.E_INVALID), (dict(new_seq_len=None), H.E_INVALID),
          (dict(model=None), H.E_INVALID), (dict(kv=None), H.E_INVALID), (dict(batch=0), H.E_CAPACITY), (dict(batch=257), H.E_CAPACITY),
          (dict(max_ctx=0), H.E_CAPACITY), (dict(max_ctx=65, scores_stride=65), H.E_CAPACITY), (dict(scores_stride=63), H.E_INVALID),
