@@ -79,15 +79,19 @@ __device__ __forceinline__ uint32_t block_prefix(uint32_t v, uint32_t* wsum, uin
 // The kept positions of one (sequence, layer, KV head), by 64 W threads.  First
 // the `heavy`-th largest key, by counts of its leading 11, next 11 and last 10
 // bits; then the positions above it and, from the lowest on, as many equal to it
-// as are missing, in order.  A thread holds 8 consecutive scores in registers, so
-// up to 512 W positions are read once, ordered by one prefix sum, and written with
-// their scores as they are found (all scores are read by then: scores_out may be
-// scores).  Bound by its chain of counts and barriers: as few waves as hold the
-// sequence (128 heads of 2,048 positions: 9 us with 4 waves, 13 with 16).
-constexpr uint32_t SEL = 8;
+// as are missing, in order.  A group that stays whole ends the counting.  A thread
+// holds 4 consecutive scores in registers, so up to 256 W positions are read once,
+// ordered by one prefix sum, and written with their scores as they are found (all
+// scores are read by then: scores_out may be scores); longer sequences are read
+// again, a block of 256 W at a time.  Bound by its chain of counts and barriers: a
+// whole call of 128 small heads of 2,048 positions takes 20.8 us with 8 waves of 4
+// scores a thread, 22.7 with 4 waves of 8 or 16 of 4.  More positions than a block
+// and heads that leave CUs idle take 16 waves: 128 heads of 4,000 are 33.9 us, 38.5
+// with 8, while 768 heads of 3,500 to 8,000 lose 6 us of 608 to them.
+constexpr uint32_t SEL = 4;
 
 template <uint32_t W>
-__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W == 16 ? 8 : 4))) void k_evict_select(EvictParams p)
+__global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W / 2))) void k_evict_select(EvictParams p)
 {
     constexpr uint32_t T = 64u * W, BLOCK = T * SEL, BINS = 2048u, PER = BINS / T;
     __shared__ uint32_t hist[BINS], pick[3], wsum[4][W];
@@ -266,24 +270,27 @@ __device__ __forceinline__ uint32_t turn_pair(uint32_t v, float c, float s)
 // Parts never meet, so all run at once; within one the runs go in order, a run's
 // loads issued before the run before it is written (no slot that a run writes is
 // read by a later one), with one barrier between a run's loads and its stores.
-//   K: KP threads a position, 1024 / KP kept positions a run, each thread's kept
-// position, page and data fetched a run ahead of one another.
+//   K: KP threads a position, 1,024 / KP kept positions a run (768 with ONCE), each
+// thread's kept position, page and data fetched a run ahead of one another.
 //   V: a channel's positions lie side by side, so runs of source pages go whole
 // (their 32-byte rows hold a kept position nearly always) through LDS, rows of
 // one channel, and the kept ones are collected from there into 16-byte stores;
 // a group of positions that a run fills in part is stored by elements.
 //   Bound by the cache's bytes: 32 layers of 3 sequences of 3,500 to 8,000
 // positions cut to 2,504 (8 KV heads of 128) read K where it is kept, V whole and
-// write both, 2.6 GB in 635 us, 4.0 TB/s (a copy reaches 4.65); 16 layers of 2,048
+// write both, 2.6 GB in 576 us, 4.4 TB/s (a copy reaches 4.65); 16 layers of 2,048
 // positions halved (heads of 64), 84 MB in 22 us.
 //   A cache past the last-level cache (256 MB) moves K in whole 128-byte lines,
 // which two parts on two XCDs would each fetch, and with accesses that do not stay
-// in the caches: 64-byte parts 790 us, lines 730, and streaming 679 for the first;
-// the second takes 34 us with 64-byte parts, 39 with lines, 44 streaming.
+// in the caches: the first's call takes 790 us with 64-byte parts, 730 with lines,
+// 668 streaming; 629 with V's channels by 32, a page's 1,024 bytes together (640
+// with runs of twice the length, 730 with 64 channels), and 613 with K's runs of 96
+// positions, at whose registers a fourth workgroup fits a CU.  The second's takes
+// 34 us with 64-byte parts, 39 with lines, 44 streaming, 32 with the shorter runs.
 template <int AF, uint32_t KP, uint32_t CH, bool ONCE>
 __global__ __launch_bounds__(256) void k_evict_move(EvictParams p)
 {
-    constexpr uint32_t EB = AF == OPURE_A_F32 ? 4u : 2u, RUN = 16384u / (CH * EB), TPP = 16u / EB, PPC = 16u / TPP;
+    constexpr uint32_t EB = AF == OPURE_A_F32 ? 4u : 2u, RUN = 1024u / EB, TPP = 16u / EB, PPC = 16u / TPP;
     constexpr uint32_t ROW = RUN * EB + 16u;               // bytes of a channel's row in LDS, a piece of padding
     __shared__ __align__(16) uint8_t rows[CH * ROW];
     __shared__ __align__(16) uint16_t from[RUN + 16u];     // the run's kept positions, from the run's first
@@ -300,7 +307,7 @@ __global__ __launch_bounds__(256) void k_evict_move(EvictParams p)
     auto there = [&](int32_t pg) { return static_cast<uint32_t>(pg) < p.n_pages; };
     if (seg < segk)
     {
-        constexpr uint32_t U = 4;
+        constexpr uint32_t U = ONCE ? 3 : 4;
         constexpr uint32_t PASS = 256u / KP, KRUN = U * PASS;   // positions a pass; a run
         const uint32_t piece = seg * KP + tid % KP, tok = tid / KP;
         const bool mine = piece * 16u < hd * EB;
@@ -407,10 +414,10 @@ __global__ __launch_bounds__(256) void k_evict_move(EvictParams p)
         }
         return;
     }
-    // ---- V: 16 channels
+    // ---- V: CH channels
     seg -= segk;
-    constexpr uint32_t U = 4, PG = RUN / OPURE_PAGE_SIZE, PPP = CH * PPC;   // pages a run; pieces a page
-    static_assert(PG * PPP == 256u * U, "a run is four pieces a thread");
+    constexpr uint32_t U = CH / 4u, PG = RUN / OPURE_PAGE_SIZE, PPP = CH * PPC;   // pages a run; pieces a page
+    static_assert(PG * PPP == 256u * U, "a run is U pieces a thread");
     uint8_t* vbase = base + p.n_kv * plane + static_cast<uint64_t>(seg) * CH * OPURE_PAGE_SIZE * EB;
     const uint32_t wave = tid >> 6, lane = tid & 63u;
     u4v data[U];
@@ -599,8 +606,7 @@ extern "C" int opure_kv_evict(opure_dev* dev, const opure_evict_args* a)
     // the other workgroups read seq_len and the table: what is written over them waits for a launch of its own
     p.new_len_now = !a->freed && a->new_seq_len != a->seq_len ? 1u : 0u;
     const uint32_t planes = p.n_layers * p.n_kv;
-    if (a->max_ctx <= 4u * 64u * SEL) OPURE_LAUNCH(dev, (k_evict_select<4>), dim3(planes, a->batch), dim3(256), 0, p);
-    else if (a->max_ctx <= 8u * 64u * SEL) OPURE_LAUNCH(dev, (k_evict_select<8>), dim3(planes, a->batch), dim3(512), 0, p);
+    if (a->max_ctx <= 8u * 64u * SEL || planes * a->batch > 256u) OPURE_LAUNCH(dev, (k_evict_select<8>), dim3(planes, a->batch), dim3(512), 0, p);
     else OPURE_LAUNCH(dev, (k_evict_select<16>), dim3(planes, a->batch), dim3(1024), 0, p);
     OPURE_LAUNCH_CHECK("k_evict_select");
     const uint32_t row = p.hd * act_bytes(p.afmt);
@@ -611,7 +617,7 @@ extern "C" int opure_kv_evict(opure_dev* dev, const opure_evict_args* a)
             OPURE_LAUNCH(dev, kernel, dim3(planes * ((row + 16u * kp - 1u) / (16u * kp) + p.hd / ch), a->batch), dim3(256), 0, p);
         };
         if (!once) go(&k_evict_move<AF, 4, 16, false>, 4u, 16u);
-        else if (row % 128u == 0u) go(&k_evict_move<AF, 8, 16, true>, 8u, 16u);
+        else if (row % 128u == 0u) go(&k_evict_move<AF, 8, 32, true>, 8u, 32u);
         else go(&k_evict_move<AF, 4, 16, true>, 4u, 16u);
     };
     if (p.afmt == OPURE_A_F32) move(std::integral_constant<int, OPURE_A_F32>{});

@@ -168,6 +168,13 @@ def test_long(dev, n, keep):
     check(dev, F16, 1, 2, 32, [n, n // 3], 4, keep // 3, keep - 4 - keep // 3, seed=n, in_place=n % 2 == 0)
 
 
+@pytest.mark.parametrize("in_place", [False, True], ids=["apart", "in place"])
+def test_long_of_many_heads(dev, in_place):
+    """More heads than CUs, whose selection takes its sequences in blocks of 2,048."""
+    say("evict long, many heads", in_place)
+    check(dev, BF16, 33, 4, 16, [5000, 4096, 2049], 4, 300, 800, seed=7, in_place=in_place)
+
+
 def test_scores_of_every_kind(dev):
     """Ties (the lowest positions stay), negative scores, zeros of both signs,
     infinities, NaN, denormal numbers, values that share their leading bits."""
