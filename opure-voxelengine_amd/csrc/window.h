@@ -30,6 +30,7 @@ struct WinParams {
     uint32_t window, sinks;       // window >= 1: 2^31 - 1 sees everything
     uint32_t cap;                 // positions that may be read: min(max_ctx, the table's)
     uint32_t batch;               // k_win_sums: sequences
+    uint32_t sum_rows;            // k_win_sums: query rows a chunk
     uint32_t blocks, block_rows;  // blocks of query rows a (sequence, KV head), and the most rows in one
     uint32_t two;                 // blocks of 32 query rows, not 16
     uint32_t parts;               // parts of each (sequence, KV head, block): slot part + parts * its index
@@ -343,8 +344,8 @@ __device__ __forceinline__ float win_lse(float m, float l) { return l == 0.0f ? 
 // ---- window_prompt.hip
 // a prompt's rows in one launch (16-bit caches); with p.lse, what k_win_sums needs
 int win_prompt_launch(opure_dev* dev, const WinParams& p, uint32_t batch);
-// weights += from the cache, the queries and p.lse; scratch of win_sums_bytes (n_heads, n_kv, rows and cap are read)
-uint64_t win_sums_bytes(const WinParams& p, uint32_t batch);
+// weights += from the cache, the queries and p.lse; scratch of win_sums_bytes (n_heads, n_kv, rows, afmt and cap are read)
+uint64_t win_sums_bytes(const opure_dev* dev, const WinParams& p, uint32_t batch);
 int win_sums_launch(opure_dev* dev, const WinParams& p, uint32_t batch, float* scratch);
 
 }  // namespace opure_win

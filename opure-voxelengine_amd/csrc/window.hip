@@ -502,7 +502,8 @@ int win_plan(opure_dev* dev, const opure_attn_window_args* a, WinPlan& w)
         p.n_kv = m->n_kv_heads;
         p.rows = a->rows;
         p.cap = a->max_ctx;
-        w.sums = win_sums_bytes(p, a->batch);
+        p.afmt = m->afmt;
+        w.sums = win_sums_bytes(dev, p, a->batch);
     }
     // a launch's threads stay in 32 bits: 2^22 workgroups of up to 512
     const uint64_t heads = static_cast<uint64_t>(a->batch) * m->n_kv_heads;

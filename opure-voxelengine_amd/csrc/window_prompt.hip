@@ -319,7 +319,7 @@ __global__ __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(HD <= 
 }
 
 // Weights from many rows: a workgroup takes 64 positions (32 of an fp32 cache) of
-// a (sequence, KV head) and a chunk of 1,536 query rows, its four waves every
+// a (sequence, KV head) and a chunk of query rows, its four waves every
 // fourth block of 16 of those rows that see one of the positions.  A wave holds
 // the positions' keys as operands, computes the block's scores again and adds
 // 2^(score - lse) to a sum a lane and position; the lanes' and waves' sums are
@@ -331,8 +331,16 @@ __global__ __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(HD <= 
 // 16 clocks each on a SIMD.  Whole calls with chunks of 512, 1,024, 1,536, 2,048
 // and 4,096: that prompt 38.4, 35.7, 36.2, 37.3, 46.6 us; 2,048 rows 82.3, 81.8,
 // 74.4, 80.6, 81.7; 2,048 rows of 128 channels behind a window of 4,096 375, 345,
-// 334, 345, 318.
-constexpr uint32_t SUM_ROWS = 1536;
+// 334, 345, 318.  Where chunks of 1,536 do not give every CU a workgroup, which
+// walks its rows alone, they are of 512 (whole calls with 1,536 / 512: 2,008 rows of
+// 4 heads of 64 behind a window of 20 34.8 / 24.9, 512 rows of 32 heads 28.7 / 23.1,
+// 400 of 12 heads of 112 in fp32 54.8 / 41.9; but with 400 workgroups 66.3 / 75.0).
+uint32_t sums_chunk(const opure_dev* dev, const WinParams& p, uint32_t batch)
+{
+    const uint32_t Gq = p.n_heads / p.n_kv * p.rows, tile = p.afmt == OPURE_A_F32 ? 32u : 64u;
+    const uint64_t wgs = static_cast<uint64_t>(p.n_kv) * batch * ((p.cap + tile - 1u) / tile) * ((Gq + 1535u) / 1536u);
+    return wgs <= static_cast<uint32_t>(dev->n_cu > 0 ? dev->n_cu : 256) ? 512u : 1536u;
+}
 
 // rows [ja, jz) of a chunk that see a position of [t0, t0 + n)
 __device__ __forceinline__ void sums_rows(const WinParams& p, const WinSeq& sq, uint32_t G, uint32_t chunk, uint32_t t0, uint32_t n,
@@ -340,8 +348,8 @@ __device__ __forceinline__ void sums_rows(const WinParams& p, const WinSeq& sq, 
 {
     const uint32_t ja = t0 > sq.ctx ? t0 - sq.ctx : 0u;
     const uint32_t jz = t0 < p.sinks ? p.rows : t0 + n - 1u + p.window > sq.ctx ? min(p.rows, t0 + n - 1u + p.window - sq.ctx) : 0u;
-    qa = max(ja * G, chunk * SUM_ROWS);
-    qz = min(jz * G, (chunk + 1u) * SUM_ROWS);
+    qa = max(ja * G, chunk * p.sum_rows);
+    qz = min(jz * G, (chunk + 1u) * p.sum_rows);
     if (t0 >= sq.total) qz = 0u;
 }
 
@@ -543,9 +551,10 @@ int win_prompt_launch(opure_dev* dev, const WinParams& p, uint32_t batch)
     return p.afmt == OPURE_A_F16 ? go(std::integral_constant<int, OPURE_A_F16>{}) : go(std::integral_constant<int, OPURE_A_BF16>{});
 }
 
-uint64_t win_sums_bytes(const WinParams& p, uint32_t batch)
+uint64_t win_sums_bytes(const opure_dev* dev, const WinParams& p, uint32_t batch)
 {
-    const uint64_t chunks = (static_cast<uint64_t>(p.n_heads / p.n_kv) * p.rows + SUM_ROWS - 1u) / SUM_ROWS;
+    const uint32_t rows = sums_chunk(dev, p, batch);
+    const uint64_t chunks = (static_cast<uint64_t>(p.n_heads / p.n_kv) * p.rows + rows - 1u) / rows;
     return chunks > 1u ? static_cast<uint64_t>(batch) * p.n_kv * chunks * p.cap * 4u : 0u;
 }
 
@@ -553,7 +562,8 @@ int win_sums_launch(opure_dev* dev, const WinParams& p, uint32_t batch, float* s
 {
     WinParams s = p;
     s.batch = batch;
-    s.parts = (p.n_heads / p.n_kv * p.rows + SUM_ROWS - 1u) / SUM_ROWS;
+    s.sum_rows = sums_chunk(dev, p, batch);
+    s.parts = (p.n_heads / p.n_kv * p.rows + s.sum_rows - 1u) / s.sum_rows;
     s.part_acc = scratch;
     const uint32_t tile = p.afmt == OPURE_A_F32 ? 32u : 64u;
     auto go = [&](auto af) {
