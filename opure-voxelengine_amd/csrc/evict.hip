@@ -270,8 +270,8 @@ __device__ __forceinline__ uint32_t turn_pair(uint32_t v, float c, float s)
 // Parts never meet, so all run at once; within one the runs go in order, a run's
 // loads issued before the run before it is written (no slot that a run writes is
 // read by a later one), with one barrier between a run's loads and its stores.
-//   K: KP threads a position, 1,024 / KP kept positions a run (768 with ONCE), each
-// thread's kept position, page and data fetched a run ahead of one another.
+//   K: KP threads a position, 256 KU / KP kept positions a run, each thread's kept
+// position, page and data fetched a run ahead of one another.
 //   V: a channel's positions lie side by side, so runs of source pages go whole
 // (their 32-byte rows hold a kept position nearly always) through LDS, rows of
 // one channel, and the kept ones are collected from there into 16-byte stores;
@@ -280,14 +280,18 @@ __device__ __forceinline__ uint32_t turn_pair(uint32_t v, float c, float s)
 // positions cut to 2,504 (8 KV heads of 128) read K where it is kept, V whole and
 // write both, 2.6 GB in 576 us, 4.4 TB/s (a copy reaches 4.65); 16 layers of 2,048
 // positions halved (heads of 64), 84 MB in 22 us.
+//   KU: long runs keep more in flight a workgroup, short ones more workgroups a CU.
+// Four where all workgroups fit at a time, three a CU (16 KV heads of 8,000 positions
+// 61 us, 72 with one; the 16 layers 28.5, 29.7), else one (240 heads of 160 positions
+// of 256 channels 33 -> 20 us, 256 heads of 1,000 of 128 53 -> 43).
 //   A cache past the last-level cache (256 MB) moves K in whole 128-byte lines,
 // which two parts on two XCDs would each fetch, and with accesses that do not stay
-// in the caches: the first's call takes 790 us with 64-byte parts, 730 with lines,
+// in the caches: the 32 layers' call takes 790 us with 64-byte parts, 730 with lines,
 // 668 streaming; 629 with V's channels by 32, a page's 1,024 bytes together (640
-// with runs of twice the length, 730 with 64 channels), and 613 with K's runs of 96
-// positions, at whose registers a fourth workgroup fits a CU.  The second's takes
-// 34 us with 64-byte parts, 39 with lines, 44 streaming, 32 with the shorter runs.
-template <int AF, uint32_t KP, uint32_t CH, bool ONCE>
+// with runs of twice the length, 730 with 64 channels), and 608 with KU 3 (1: 648, or
+// 614 with 16 channels).  The 16 layers' takes 34 us with 64-byte parts, 39 with
+// lines, 44 streaming.
+template <int AF, uint32_t KP, uint32_t KU, uint32_t CH, bool ONCE>
 __global__ __launch_bounds__(256) void k_evict_move(EvictParams p)
 {
     constexpr uint32_t EB = AF == OPURE_A_F32 ? 4u : 2u, RUN = 1024u / EB, TPP = 16u / EB, PPC = 16u / TPP;
@@ -307,8 +311,7 @@ __global__ __launch_bounds__(256) void k_evict_move(EvictParams p)
     auto there = [&](int32_t pg) { return static_cast<uint32_t>(pg) < p.n_pages; };
     if (seg < segk)
     {
-        constexpr uint32_t U = ONCE ? 3 : 4;
-        constexpr uint32_t PASS = 256u / KP, KRUN = U * PASS;   // positions a pass; a run
+        constexpr uint32_t U = KU, PASS = 256u / KP, KRUN = U * PASS;   // positions a pass; a run
         const uint32_t piece = seg * KP + tid % KP, tok = tid / KP;
         const bool mine = piece * 16u < hd * EB;
         const bool turn = p.cos != nullptr;
@@ -616,9 +619,11 @@ extern "C" int opure_kv_evict(opure_dev* dev, const opure_evict_args* a)
         auto go = [&](auto kernel, uint32_t kp, uint32_t ch) {
             OPURE_LAUNCH(dev, kernel, dim3(planes * ((row + 16u * kp - 1u) / (16u * kp) + p.hd / ch), a->batch), dim3(256), 0, p);
         };
-        if (!once) go(&k_evict_move<AF, 4, 16, false>, 4u, 16u);
-        else if (row % 128u == 0u) go(&k_evict_move<AF, 8, 32, true>, 8u, 32u);
-        else go(&k_evict_move<AF, 4, 16, true>, 4u, 16u);
+        const uint64_t wgs = static_cast<uint64_t>(planes) * ((row + 63u) / 64u + p.hd / 16u) * a->batch;
+        if (!once && wgs <= 3u * static_cast<uint32_t>(dev->n_cu > 0 ? dev->n_cu : 256)) go(&k_evict_move<AF, 4, 4, 16, false>, 4u, 16u);
+        else if (!once) go(&k_evict_move<AF, 4, 1, 16, false>, 4u, 16u);
+        else if (row % 128u == 0u) go(&k_evict_move<AF, 8, 3, 32, true>, 8u, 32u);
+        else go(&k_evict_move<AF, 4, 1, 16, true>, 4u, 16u);
     };
     if (p.afmt == OPURE_A_F32) move(std::integral_constant<int, OPURE_A_F32>{});
     else if (p.afmt == OPURE_A_F16) move(std::integral_constant<int, OPURE_A_F16>{});

@@ -168,6 +168,15 @@ def test_long(dev, n, keep):
     check(dev, F16, 1, 2, 32, [n, n // 3], 4, keep // 3, keep - 4 - keep // 3, seed=n, in_place=n % 2 == 0)
 
 
+@pytest.mark.parametrize("afmt", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("hd", list(range(16, 257, 16)))
+def test_more_parts_than_fit_at_a_time(dev, hd, afmt):
+    """Four a CU of 64 bytes of a key or 16 channels of V: shorter runs of keys."""
+    say("evict many parts", hd, afmt)
+    parts = -(-hd * (4 if afmt == F32 else 2) // 64) + hd // 16
+    check(dev, afmt, -(-1024 // (6 * parts)), 2, hd, [161, 300, 40], 1, 30, 60, seed=hd)
+
+
 @pytest.mark.parametrize("in_place", [False, True], ids=["apart", "in place"])
 def test_long_of_many_heads(dev, in_place):
     """More heads than CUs, whose selection takes its sequences in blocks of 2,048."""
