@@ -266,13 +266,11 @@ int opure_attn_decode_paged(opure_dev* dev, const opure_attn_args* a);
  *      [n_kv_heads][stride] array is weights + layer * n_kv_heads * stride with
  *      weights_batch_stride = n_layers * n_kv_heads * stride.
  *        pool and q are 16-byte aligned, out 8-byte.  Scores, maxima and sums are
- *      fp32; with a 16-bit cache a weight meets V as two 16-bit numbers where a
- *      call has few query rows a KV head, and rounded once to the cache's
- *      format where many share the work (off by half a step, as the result
- *      itself).  Which, and the order of sums, follow the shape of the call
- *      (batch, rows, max_ctx, window, sinks and whether there are weights): the
- *      same call gives the same bits, a row alone and in a batch may differ in
- *      its last ones.  A length below 0 or past max_ctx is OPURE_E_CAPACITY at
+ *      fp32; with a 16-bit cache a weight meets V as two numbers of the format,
+ *      its rounding and the rest (16 bits of it in bf16, 22 in fp16).  The order
+ *      of sums follows the shape of the call (batch, rows, max_ctx, window,
+ *      sinks and whether there are weights): the same call gives the same bits,
+ *      a row alone and in a batch may differ in its last ones.  A length below 0 or past max_ctx is OPURE_E_CAPACITY at
  *      the next sync; positions past max_ctx are neither read nor weighed. */
 typedef struct opure_attn_window_args {
     const opure_model* model; /* n_layers, n_heads, n_kv_heads, head_dim, attn_scale, afmt */

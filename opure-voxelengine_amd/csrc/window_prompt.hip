@@ -35,11 +35,13 @@ constexpr uint32_t prompt_lds() { return 2u * (prompt_k_pieces<HD>() + prompt_v_
 // K rows lie in LDS in the order (positions with bits 2 and 3 exchanged) that
 // makes a lane's scores 8 consecutive positions, its operand of O^T = V^T P^T.
 //   A row's output is scaled to a new maximum only where that passes the old one
-// by 2^8: the weights are then up to 2^8, which costs none of their bits.  They
-// enter the product rounded once to the cache's format (half a step, as the result
-// itself is): the matrix unit is what bounds a prompt, and a second product for
-// the rounding's rest would cost it half as much again.  fp16 weights are held
-// 2^6 higher, so that those down to 2^-20 of the largest keep their bits.
+// by 2^8: the weights are then up to 2^8, which costs none of their bits.  A weight
+// enters the product as two 16-bit numbers, as in k_win_split (2^-16 of it is lost in
+// bf16, 2^-22 in fp16; the result's own rounding is 2^-8, 2^-11): the second product
+// costs the 8B prompt 162 -> 209 us and the 1B one 18.1 -> 20.3, rounding the weights
+// once left its results 1.4 times as far from the exact ones as one rounding at the
+// end.  fp16 weights are held 2^6 higher, so that the smallest steps are small
+// against the row's largest weight.
 //   Bound by the matrix and vector units together, which overlap little (36% and
 // 43% of the clocks): 2,048 rows of 32 heads of 128 over 4,096 positions each take
 // 160 to 170 us, 810 to 860 TFLOP/s, where a library product of 8,192 x 8,192
@@ -217,22 +219,38 @@ __global__ __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(HD <= 
         }
         const float ms = m == NEG_INF ? 0.0f : m - UP;
         float sum[2] = {0.0f, 0.0f};
-        u4v w[4];
-#pragma unroll
-        for (uint32_t t = 0; t < 2; ++t)
-#pragma unroll
-            for (uint32_t x = 0; x < 16; x += 2)
-            {
-                const float e0 = __builtin_amdgcn_exp2f(__fmaf_rn(s[t][x], c, -ms)), e1 = __builtin_amdgcn_exp2f(__fmaf_rn(s[t][x + 1], c, -ms));
-                sum[0] += e0;
-                sum[1] += e1;
-                w[2u * t + (x >> 3)][(x & 7u) / 2u] = win_pack<AF>(e0, e1);
-            }
-        l += sum[0] + sum[1];                              // this half's share
 #pragma unroll
         for (uint32_t u = 0; u < 4; ++u)
+        {
+            u4v w, rest;
 #pragma unroll
-            for (uint32_t d = 0; d < DT; ++d) o[d] = mfma_32<AF>(v[(32u * d + r) * VROW + 2u * u + h], w[u], o[d]);
+            for (uint32_t x = 0; x < 4; ++x)
+            {
+                const float s0 = s[u >> 1][8u * (u & 1u) + 2u * x], s1 = s[u >> 1][8u * (u & 1u) + 2u * x + 1u];
+                const float e0 = __builtin_amdgcn_exp2f(__fmaf_rn(s0, c, -ms)), e1 = __builtin_amdgcn_exp2f(__fmaf_rn(s1, c, -ms));
+                sum[0] += e0;
+                sum[1] += e1;
+                w[x] = win_pack<AF>(e0, e1);
+                rest[x] = win_pack<AF>(__fsub_rn(e0, win_low<AF>(w[x])), __fsub_rn(e1, win_high<AF>(w[x])));
+            }
+            u4v vx[DT];
+#pragma unroll
+            for (uint32_t d = 0; d < DT; ++d) vx[d] = v[(32u * d + r) * VROW + 2u * u + h];
+#pragma unroll
+            for (uint32_t d = 0; d < DT; ++d) o[d] = mfma_32<AF>(vx[d], rest, o[d]);
+#pragma unroll
+            for (uint32_t d = 0; d < DT; ++d) o[d] = mfma_32<AF>(vx[d], w, o[d]);
+        }
+        l += sum[0] + sum[1];                              // this half's share
+        // the next 16 positions' weights between the products of these
+        __builtin_amdgcn_sched_group_barrier(0x002, 40, 0);
+#pragma unroll
+        for (uint32_t x = 0; x < 6u * DT; ++x)
+        {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 20u / DT, 0);
+        }
+        __builtin_amdgcn_sched_group_barrier(0x008, 2u * DT, 0);
     };
     for (uint32_t i = 0; i < turns; i += DEPTH)
     {

@@ -1,0 +1,69 @@
+"""What opure_attn_window_paged promises beyond its definition's values: weights
+that meet V with their rounding's rest, in every kernel."""
+import numpy as np
+import pytest
+
+import opure_hip as H
+import window_ref as R
+from gpu_util import say
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = H.A_F32, H.A_F16, H.A_BF16
+
+
+@pytest.fixture(scope="module")
+def dev():
+    d = H.Dev(0)
+    yield d
+    d.close()
+
+
+def sizes(cache, seq, q, heads, rows, window, sinks, scale):
+    """Sum of w |v| of every output and sum of |v| over what its row sees, in 64 bits."""
+    G = heads // cache.n_kv
+    mag, flat = np.zeros(q.shape), np.zeros(q.shape)
+    for b, n0 in enumerate(seq):
+        n = n0 + rows
+        m = R.sees(n0, rows, n, window, sinks)
+        for h in range(heads):
+            k, v = (cache.get(b, 0, h // G, i, n).astype(np.float64) for i in (0, 1))
+            s = np.where(m, q[b, :, h].astype(np.float64) @ k.T * scale, -np.inf)
+            e = np.exp(s - s.max(1, keepdims=True))
+            mag[b, :, h] = e / e.sum(1, keepdims=True) @ np.abs(v)
+            flat[b, :, h] = m @ np.abs(v)
+    return mag, flat
+
+
+# rows, sequences, window, and which positions' V are not 0 (about twelve a window, so that
+# roundings of single weights show): 4 query rows a KV head and 36 behind a long window, a
+# prompt of few workgroups and of many
+KERNELS = {"decode": (1, [900, 1300, 750], 700, 60), "verify": (9, [900, 20], 700, 60), "prompt": (130, [50], 12, 1),
+           "prompts": (260, [30, 5] * 20, 12, 1)}
+
+
+@pytest.mark.parametrize("afmt,hd", [(F16, 64), (BF16, 64), (F16, 128), (BF16, 128), (F16, 80), (BF16, 208)])
+@pytest.mark.parametrize("kernel", KERNELS)
+def test_weights_keep_their_rest(dev, kernel, afmt, hd):
+    """A weight of a 16-bit cache meets V as two numbers of its format: its rounding, off by
+    at most half a step u, and the rest, rounded by as much: u^2 of the weight in all (and in
+    fp16 half of the smallest step, 2^-25, where the row's largest weight is 1 or more).  So
+    the bound of the definition's test without its one rounding of the weights."""
+    rows, seq, window, every = KERNELS[kernel]
+    say("rest", kernel, afmt, hd)
+    rng = np.random.default_rng(hd + rows)
+    heads, n_kv, sinks, scale = 8, 2, 2, hd ** -0.5
+    cache = R.Cache(rng, afmt, 1, n_kv, hd, [n + rows for n in seq])
+    for b, n in enumerate(seq):
+        x = rng.standard_normal((1, 2, n_kv, n + rows, hd), dtype=np.float32)
+        x[0, 1, :, np.arange(n + rows) % every != 0] = 0
+        cache.put(b, slice(0, n + rows), x)
+    q = R.act_to_f32(R.f32_to_act(rng.standard_normal((len(seq), rows, heads, hd), dtype=np.float32) * np.float32(0.5), afmt), afmt)
+    ref, tol, _, _ = R.attention(cache, 0, q, heads, seq, rows, window, sinks, scale)
+    mag, flat = sizes(cache, seq, q, heads, rows, window, sinks, scale)
+    u = R.HALF_STEP[afmt]
+    tol = tol - u * mag + u * u * mag + (2.0 ** -25 * flat if afmt == F16 else 0)
+    c = R.Call(dev, cache, q, heads, seq, rows, window, sinks, scale).run()
+    off = np.abs(c.result() - ref)
+    c.free()
+    assert not (off > tol).any(), (int((off > tol).sum()), float((off - tol).max()))
