@@ -456,15 +456,17 @@ struct WinPlan {
 };
 
 // Which kernels take a call, by what each would take (us, of what was measured on
-// 8 KV heads of 64 and 128 channels and 4 query heads each):
+// 8 KV heads of 64, 128 and 192 channels and 4 of 256, 2 or 4 query heads each):
 //   k_win_prompt walks all tiles of 64 positions in one workgroup a 128 query rows:
-//     5 + 0.73 a tile (1.15 at 128 channels), times the workgroups a CU;
-//   k_win_split + k_win_join: 8.5, and 1 ns a tile of 32 positions, block of query
-//     rows and 100 channels.
-// Measured, prompt / split: 64 query rows of a KV head over 64 positions 6.3 / 8.6,
-// over 1,000 16.4 / 9.6, over 8,000 92.6 / 15.7; four sequences of 512 over 1,000
-// 18.8 / 30.7, over 8,000 95 / 97; 1,024 of 128 channels behind a window of 1,024
-// 29.2 / 26.3, four sequences 33.0 / 77.1.
+//     3 + channels / 32, and a tile 0.4 + channels / 125 (past 128 channels, without
+//     two waves a row block, channels / 60), times the workgroups a CU;
+//   k_win_split + k_win_join: 7 + channels / 100, 1.1 ns a tile of 32 positions, block
+//     of query rows and 100 channels, and 0.3 a query row and 100,000 channels of it.
+// Measured, prompt / split: 64 query rows of a KV head over 64 positions 5.8 / 7.6 (of
+// 128 channels 8.4 / 8.5, of 256 12.0 / 9.3), over 1,000 19.1 / 8.3, over 8,000 115.6 /
+// 13.1; four sequences of 512 over 1,000 21.4 / 16.5, of 1,024 24.9 / 50.3; 1,024 of
+// 128 channels behind a window of 1,024 33.4 / 25.5, over 1,000 in four sequences
+// 40.3 / 74.8.  Of 184 such calls it takes the slower one in 6, by 1.5 us at most.
 //   Weights from stored scores cost the join 0.17 a query row, computed again
 // (k_win_sums) about 3 and the keys once more at 2.5 TB/s.  Measured, stored /
 // computed again: 16 query rows over 64 positions 9.7 / 11.2, 64 18.0 / 11.9; four
@@ -476,8 +478,9 @@ void win_choose(const opure_dev* dev, const opure_attn_window_args* a, WinPlan& 
     const double G = m->n_heads / m->n_kv_heads, Gq = G * a->rows, hd = m->head_dim, cu = dev->n_cu > 0 ? dev->n_cu : 256;
     const double heads = static_cast<double>(a->batch) * m->n_kv_heads, span = static_cast<double>(w.tiles) * w.tt;
     const double wgs = heads * std::ceil(Gq / 128.0), window = a->window ? a->window : 2147483647.0;
-    const double prompt = 5.0 + std::max(1.0, wgs / cu) * std::ceil(std::min(span, a->sinks + window + 128.0 / G) / 64.0) * (0.31 + hd / 152.0);
-    const double split = 8.5 + heads * std::ceil(Gq / (Gq > 16.0 && hd <= 128.0 ? 32.0 : 16.0)) * w.tiles * hd * 1e-5;
+    const double prompt = 3.0 + hd / 32.0 + std::max(1.0, wgs / cu) * std::ceil(std::min(span, a->sinks + window + 128.0 / G) / 64.0) *
+                                                (hd <= 128.0 ? 0.4 + hd / 125.0 : hd / 60.0);
+    const double split = 7.0 + hd / 100.0 + heads * hd * (std::ceil(Gq / (Gq > 16.0 && hd <= 128.0 ? 32.0 : 16.0)) * w.tiles * 1.1e-5 + Gq * 3e-6);
     const double store = 0.17 * Gq, again = 3.0 + heads * span * hd * act_bytes(m->afmt) / 2.5e6;
     w.stored = a->weights && Gq <= 96.0 && store < again;
     w.prompt = m->afmt != OPURE_A_F32 && prompt + (a->weights ? again : 0.0) < split + (a->weights ? std::min(store, again) : 0.0);
