@@ -290,7 +290,11 @@ typedef struct opure_attn_window_args {
 
 /* Sizes the device's workspace for such a call (the pointers seq_len, q, out
  * are not read; weights counts as wanted when not NULL); call it before
- * capturing one into a graph. */
+ * capturing one into a graph.  It follows how that call is run, and a call of
+ * fewer rows, sequences or positions can need more: reserve each shape that
+ * will be captured.  Without weights it is about 64 MiB or twice the bytes of q
+ * in fp32 at most; with them as much again as the keys of the positions that
+ * are seen take in the layer, or 64 MiB. */
 int opure_attn_window_reserve(opure_dev* dev, const opure_attn_window_args* a);
 int opure_attn_window_paged(opure_dev* dev, const opure_attn_window_args* a);
 

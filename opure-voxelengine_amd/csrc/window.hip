@@ -467,11 +467,13 @@ struct WinPlan {
 // 13.1; four sequences of 512 over 1,000 21.4 / 16.5, of 1,024 24.9 / 50.3; 1,024 of
 // 128 channels behind a window of 1,024 33.4 / 25.5, over 1,000 in four sequences
 // 40.3 / 74.8.  Of 184 such calls it takes the slower one in 6, by 1.5 us at most.
-//   Weights from stored scores cost the join 0.17 a query row, computed again
-// (k_win_sums) about 3 and the keys once more at 2.5 TB/s.  Measured, stored /
-// computed again: 16 query rows over 64 positions 9.7 / 11.2, 64 18.0 / 11.9; four
-// sequences over 8,000 positions of 128 channels, 16 41.7 / 75.1, 64 81.1 / 92.4,
-// 128 139 / 124.
+//   Weights from stored scores cost the join 0.2 a query row, or its scores' 8 bytes a
+// position, written and read, at 5.3 TB/s; computed again (k_win_sums) they cost 2 +
+// channels / 64 and the keys once more at 2.5 TB/s.  Measured, stored / computed again:
+// 16 query rows over 500 positions of 64 channels 9.9 / 11.4, 64 20.4 / 13.0, 64 over
+// 4,000 in 16 sequences 104 / 87; of 128 channels 22.2 / 16.0, 141 / 177, of 256 22.0 /
+// 19.9, 229 / 250.  Stored scores are workspace too: past 64 MB no more than the keys
+// that they save reading, and no more rows than the 96 that were measured.
 void win_choose(const opure_dev* dev, const opure_attn_window_args* a, WinPlan& w)
 {
     const opure_model* m = a->model;
@@ -481,8 +483,9 @@ void win_choose(const opure_dev* dev, const opure_attn_window_args* a, WinPlan& 
     const double prompt = 3.0 + hd / 32.0 + std::max(1.0, wgs / cu) * std::ceil(std::min(span, a->sinks + window + 128.0 / G) / 64.0) *
                                                 (hd <= 128.0 ? 0.4 + hd / 125.0 : hd / 60.0);
     const double split = 7.0 + hd / 100.0 + heads * hd * (std::ceil(Gq / (Gq > 16.0 && hd <= 128.0 ? 32.0 : 16.0)) * w.tiles * 1.1e-5 + Gq * 3e-6);
-    const double store = 0.17 * Gq, again = 3.0 + heads * span * hd * act_bytes(m->afmt) / 2.5e6;
-    w.stored = a->weights && Gq <= 96.0 && store < again;
+    const double keys = heads * span * hd * act_bytes(m->afmt), scores = heads * span * 4.0 * Gq;
+    const double store = std::max(0.2 * Gq, 2.0 * scores / 5.3e6), again = 2.0 + hd / 64.0 + keys / 2.5e6;
+    w.stored = a->weights && Gq <= 96.0 && store < again && scores <= std::max(67108864.0, keys);
     w.prompt = m->afmt != OPURE_A_F32 && prompt + (a->weights ? again : 0.0) < split + (a->weights ? std::min(store, again) : 0.0);
     if (w.prompt) w.stored = false;
 }

@@ -1,5 +1,7 @@
 """What opure_attn_window_paged promises beyond its definition's values: weights
 that meet V with their rounding's rest, in every kernel."""
+import ctypes as C
+
 import numpy as np
 import pytest
 
@@ -67,3 +69,28 @@ def test_weights_keep_their_rest(dev, kernel, afmt, hd):
     off = np.abs(c.result() - ref)
     c.free()
     assert not (off > tol).any(), (int((off > tol).sum()), float((off - tol).max()))
+
+
+@pytest.mark.parametrize("afmt,heads,n_kv,hd", [(F16, 32, 8, 64), (BF16, 32, 8, 128), (F32, 9, 3, 64), (F16, 64, 8, 16)])
+@pytest.mark.parametrize("batch,rows,ctx", [(1, 1, 131072), (16, 24, 16000), (256, 12, 2000), (64, 4, 16000), (4, 256, 30000), (1, 2048, 60000)])
+def test_workspace_is_bounded(afmt, heads, n_kv, hd, batch, rows, ctx):
+    """What a call with weights asks of the workspace: no more than the keys of its
+    positions take in the layer, or 64 MiB, beside what it takes without weights."""
+    say("workspace", afmt, heads, n_kv, hd, batch, rows, ctx)
+    model = H.Model()
+    model.n_layers, model.n_heads, model.n_kv_heads, model.head_dim, model.afmt, model.attn_scale = 1, heads, n_kv, hd, afmt, 0.1
+    kv = H.KV(4096, 1 << 20, R.PAGE, 4096, (ctx + rows + 15) // 16)
+    need = []
+    for weights in (None, 4096):
+        d = H.Dev(0)
+        a = H.AttnWindowArgs(C.pointer(model), C.pointer(kv), 0, batch, rows, None, ctx + rows, 0, 0, None, None, weights, ctx + rows,
+                             n_kv * (ctx + rows))
+        H.check(H.lib().opure_attn_window_reserve(d.h, C.byref(a)))
+        ptr, size = C.c_void_p(), C.c_uint64()
+        H.check(H.lib().opure_debug_workspace(d.h, C.byref(ptr), C.byref(size)))
+        need.append(size.value)
+        d.close()
+    eb = 4 if afmt == F32 else 2
+    keys, q = batch * n_kv * (ctx + rows + 31) * hd * eb, batch * rows * heads * hd * 4
+    assert need[0] <= max(64 << 20, 2 * q) + (1 << 20)
+    assert need[1] <= max(64 << 20, 2 * q) + max(64 << 20, keys) + (1 << 20), (need[1] >> 20, keys >> 20)
