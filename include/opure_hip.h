@@ -252,7 +252,10 @@ int opure_attn_decode_paged(opure_dev* dev, const opure_attn_args* a);
  *      opure_attn_decode_paged).  One row or a few a sequence (decoding, a
  *      verify step) and a prompt's rows take the same call: rows up to
  *      OPURE_MAX_PROMPT_ROWS, batch up to OPURE_MAX_BATCH_ROWS, every format
- *      and head size of opure_attn_decode_paged.
+ *      and head size of opure_attn_decode_paged.  batch x rows x n_heads past
+ *      2^25, or a launch of 2^24 workgroups (with weights about 2^30 of batch x
+ *      n_kv_heads x max_ctx, fewer where a KV head has more than 1,536 query
+ *      rows), is OPURE_E_CAPACITY.
  *        What a row does not see does not reach it: masked K and V may hold
  *      anything, NaN and infinities included, and pages that no row of a
  *      sequence sees may be missing (-1), so a cache that only grows can

@@ -346,6 +346,7 @@ __device__ __forceinline__ float win_lse(float m, float l) { return l == 0.0f ? 
 int win_prompt_launch(opure_dev* dev, const WinParams& p, uint32_t batch);
 // weights += from the cache, the queries and p.lse; scratch of win_sums_bytes (n_heads, n_kv, rows, afmt and cap are read)
 uint64_t win_sums_bytes(const opure_dev* dev, const WinParams& p, uint32_t batch);
+uint64_t win_sums_workgroups(const opure_dev* dev, const WinParams& p, uint32_t batch);
 int win_sums_launch(opure_dev* dev, const WinParams& p, uint32_t batch, float* scratch);
 
 }  // namespace opure_win

@@ -501,6 +501,7 @@ int win_plan(opure_dev* dev, const opure_attn_window_args* a, WinPlan& w)
     const uint64_t rows = static_cast<uint64_t>(a->batch) * m->n_kv_heads * Gq;
     win_choose(dev, a, w);
     w.lse = a->weights && !w.stored ? opure_hip::align_up(rows * 4u, 256) : 0u;
+    uint64_t most = 0;                                   // workgroups of the call's largest launch
     if (w.lse)
     {
         WinParams p{};
@@ -510,14 +511,16 @@ int win_plan(opure_dev* dev, const opure_attn_window_args* a, WinPlan& w)
         p.cap = a->max_ctx;
         p.afmt = m->afmt;
         w.sums = win_sums_bytes(dev, p, a->batch);
+        most = win_sums_workgroups(dev, p, a->batch);
     }
-    // a launch's threads stay in 32 bits: 2^22 workgroups of up to 512
+    // a launch's threads, 256 a workgroup, stay in 32 bits
+    auto fits = [&](uint64_t wgs) {
+        OPURE_REQUIRE(std::max(wgs, most) < 1u << 24, OPURE_E_CAPACITY,
+                      "window attention: %u x %u rows of %u heads over max_ctx %u: too many workgroups", a->batch, a->rows, m->n_heads, a->max_ctx);
+        return OPURE_OK;
+    };
     const uint64_t heads = static_cast<uint64_t>(a->batch) * m->n_kv_heads;
-    const uint64_t most = std::max<uint64_t>({rows / 4u, heads * ((Gq + 15u) / 16u),
-                                              a->weights ? heads * (a->max_ctx / 32u + 1u) * (w.lse ? (Gq + 511u) / 512u : 1u) / (w.lse ? 1u : 8u) : 0u});
-    OPURE_REQUIRE(most <= 1u << 22, OPURE_E_CAPACITY, "window attention: %u x %u rows of %u heads over max_ctx %u: too many workgroups",
-                  a->batch, a->rows, m->n_heads, a->max_ctx);
-    if (w.prompt) return OPURE_OK;
+    if (w.prompt) return fits(heads * ((Gq + 127u) / 128u));
     w.two = Gq > 16u && m->head_dim <= 128u;
     w.blocks = (Gq + (w.two ? 31u : 15u)) / (w.two ? 32u : 16u);
     w.block_rows = std::min(Gq, w.two ? 32u : 16u);
@@ -527,7 +530,7 @@ int win_plan(opure_dev* dev, const opure_attn_window_args* a, WinPlan& w)
         return OPURE_OK;
     });
     if (rc) return rc;
-    const uint64_t groups = static_cast<uint64_t>(a->batch) * m->n_kv_heads * w.blocks;
+    const uint64_t groups = heads * w.blocks;
     // Parts of a group: as many as the device holds at a time, each of at least four tiles (one a wave), or of so many
     // that the part's outputs, written and read again, stay a quarter of its keys and values (24 rows of 8B heads over
     // 66 tiles: 16 parts 26.9 us, 11 24.9, 8 24.7); three times as many where a wave still has four tiles, which evens
@@ -535,13 +538,15 @@ int win_plan(opure_dev* dev, const opure_attn_window_args* a, WinPlan& w)
     const uint32_t least = std::max(4u, w.block_rows / 4u);
     const uint64_t fill = std::max<uint64_t>(1u, room / groups), more = std::min<uint64_t>(3ull * room / groups, w.tiles / 16u);
     w.parts = static_cast<uint32_t>(std::min<uint64_t>(std::max(fill, more), std::min((w.tiles + least - 1u) / least, MAX_PARTS)));
-    const uint64_t wide = static_cast<uint64_t>(a->batch) * m->n_kv_heads * ((static_cast<uint64_t>(w.tiles) * w.tt + 1023u) / 1024u);
+    const uint64_t wide = heads * ((static_cast<uint64_t>(w.tiles) * w.tt + 1023u) / 1024u);
     w.four = wide >= 2ull * (dev->n_cu > 0 ? static_cast<uint32_t>(dev->n_cu) : 256u);
     const uint64_t slots = groups * w.parts * w.block_rows;
     w.acc = opure_hip::align_up(slots * m->head_dim * 4u, 256);
     w.ml = opure_hip::align_up(slots * 8u, 256);
     w.scores = w.stored ? opure_hip::align_up(rows * w.tiles * w.tt * 4u, 256) : 0u;
-    return OPURE_OK;
+    // the join's: a row a workgroup or four, and with stored scores 1,024 positions or 256
+    const uint64_t join = (w.parts > 8u ? rows : (rows + 3u) / 4u) + (w.stored ? (w.four ? wide : 4u * wide) : 0u);
+    return fits(std::max(groups * w.parts, join));
 }
 
 int win_validate(const opure_attn_window_args* a)

@@ -576,6 +576,13 @@ uint64_t win_sums_bytes(const opure_dev* dev, const WinParams& p, uint32_t batch
     return chunks > 1u ? static_cast<uint64_t>(batch) * p.n_kv * chunks * p.cap * 4u : 0u;
 }
 
+uint64_t win_sums_workgroups(const opure_dev* dev, const WinParams& p, uint32_t batch)
+{
+    const uint32_t rows = sums_chunk(dev, p, batch), tile = p.afmt == OPURE_A_F32 ? 32u : 64u;
+    const uint64_t chunks = (static_cast<uint64_t>(p.n_heads / p.n_kv) * p.rows + rows - 1u) / rows;
+    return static_cast<uint64_t>(p.n_kv) * batch * chunks * ((p.cap + tile - 1u) / tile);
+}
+
 int win_sums_launch(opure_dev* dev, const WinParams& p, uint32_t batch, float* scratch)
 {
     WinParams s = p;

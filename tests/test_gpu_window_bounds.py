@@ -8,6 +8,7 @@ import pytest
 import opure_hip as H
 import window_ref as R
 from gpu_util import say
+from test_gpu_window import check
 
 pytestmark = pytest.mark.gpu
 
@@ -94,3 +95,28 @@ def test_workspace_is_bounded(afmt, heads, n_kv, hd, batch, rows, ctx):
     keys, q = batch * n_kv * (ctx + rows + 31) * hd * eb, batch * rows * heads * hd * 4
     assert need[0] <= max(64 << 20, 2 * q) + (1 << 20)
     assert need[1] <= max(64 << 20, 2 * q) + max(64 << 20, keys) + (1 << 20), (need[1] >> 20, keys >> 20)
+
+
+def reserve(dev, afmt, heads, n_kv, hd, batch, rows, ctx, window=0, weights=True):
+    model = H.Model()
+    model.n_layers, model.n_heads, model.n_kv_heads, model.head_dim, model.afmt, model.attn_scale = 1, heads, n_kv, hd, afmt, 0.1
+    kv = H.KV(4096, 1 << 20, R.PAGE, 4096, (ctx + 15) // 16)
+    a = H.AttnWindowArgs(C.pointer(model), C.pointer(kv), 0, batch, rows, None, ctx, window, 0, None, None, 4096 if weights else None, ctx,
+                         n_kv * ctx)
+    return H.lib().opure_attn_window_reserve(dev.h, C.byref(a))
+
+
+def test_large_calls_are_refused_where_a_launch_cannot_be(dev):
+    """Launches of up to 2^24 workgroups are taken, larger ones refused."""
+    say("large calls")
+    assert reserve(dev, F16, 32, 8, 64, 32, 2048, 32768) == H.OK       # 0.8 million workgroups
+    assert reserve(dev, F16, 64, 8, 64, 256, 2048, 4096, 512, False) == H.OK
+    assert reserve(dev, F16, 64, 8, 64, 256, 2048, 65536) == H.E_CAPACITY
+    assert b"workgroups" in H.lib().opure_last_error()
+    assert reserve(dev, F16, 65, 5, 64, 256, 2048, 4096, 512, False) == H.E_CAPACITY
+
+
+def test_more_than_four_million_workgroups(dev):
+    """A max_ctx of 2^26 for 4,800 query rows: 2^22 workgroups over the positions, of which a few have any."""
+    say("2^22 workgroups")
+    check(dev, F16, 16, 1, 32, [50], 300, 100, 3, True, max_ctx=1 << 26)
