@@ -114,6 +114,14 @@ __global__ __launch_bounds__(64 * W) __attribute__((amdgpu_waves_per_eu(W / 2)))
             if (p.n_freed) p.n_freed[b] = 0;
         }
     }
+    if (blockIdx.x == 0u)
+    {
+        // every page of the sequence, also those that the move has no need to read
+        const int32_t* pt = p.page_table + static_cast<uint64_t>(b) * p.max_pages;
+        bool gone = false;
+        for (uint32_t i = tid; i * OPURE_PAGE_SIZE < n; i += T) gone = gone || static_cast<uint32_t>(pt[i]) >= p.n_pages;
+        if (gone) p.err[ERR_POSITION] = 1u;
+    }
     if (n <= p.keep)
     {
         for (uint32_t i = tid; i < p.keep; i += T) kept[i] = i < n ? static_cast<int32_t>(i) : -1;

@@ -1,0 +1,42 @@
+"""What opure_kv_evict promises beyond its definition's values: every missing page is reported."""
+import numpy as np
+import pytest
+
+import opure_hip as H
+import window_ref as R
+from gpu_util import say
+from test_gpu_evict import Evict, check
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = H.A_F32, H.A_F16, H.A_BF16
+
+
+@pytest.fixture(scope="module")
+def dev():
+    d = H.Dev(0)
+    yield d
+    d.close()
+
+
+@pytest.mark.parametrize("seq,budget,page", [([40, 30], (4, 30, 30), 1),       # nothing to evict
+                                             ([1300, 20], (600, 300, 300), 0),  # before the sinks' last run
+                                             ([3000, 20], (2, 0, 40), 180),     # far behind the last kept position
+                                             ([3000, 1600], (700, 2, 3), 187)])
+@pytest.mark.parametrize("afmt", [F32, F16], ids=["f32", "f16"])
+def test_every_missing_page_is_reported(dev, afmt, seq, budget, page):
+    """Also of a sequence that keeps all its positions, and where no position moves."""
+    say("missing page", afmt, seq, budget, page)
+    rng = np.random.default_rng(page)
+    for value in (-1, 1 << 30):
+        cache = R.Cache(rng, afmt, 1, 2, 32, seq)
+        scores = rng.random((2, 1, 2, max(seq)), dtype=np.float32)
+        scores[..., 200:] *= 0.001                              # the heavy ones lie in front
+        cache.table[0, page] = value
+        e = Evict(dev, cache, seq, scores, *budget, True)
+        with pytest.raises(H.OpureError) as err:
+            e.run()
+        assert err.value.code == H.E_CAPACITY
+        e.done()
+    # pages past a sequence's positions are not its pages: missing in every shorter row of the table
+    check(dev, afmt, 1, 2, 32, seq, *budget)
