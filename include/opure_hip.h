@@ -285,7 +285,7 @@ typedef struct opure_attn_window_args {
     uint32_t           window;      /* positions a row sees up to its own, which counts; 0 = all */
     uint32_t           sinks;       /* first positions that stay visible */
     const void*        q;           /* [batch*rows][n_heads*head_dim] in afmt */
-    void*              out;         /* like q, and apart from it */
+    void*              out;         /* like q; apart from everything else, as weights is */
     float*             weights;     /* device, or NULL */
     uint32_t           weights_stride;        /* floats between KV heads, >= max_ctx */
     uint64_t           weights_batch_stride;  /* floats between sequences */
@@ -405,7 +405,10 @@ int opure_kv_rollback(opure_dev* dev, const opure_rollback_args* a);
  *      whose sequences share a prefix's pages cannot be evicted in place.  A
  *      page that is missing among the seq_len positions is OPURE_E_CAPACITY at the next sync, as is a
  *      length past max_ctx or the table; what such a sequence's cache and
- *      outputs then hold is not defined, but no access leaves the buffers. */
+ *      outputs then hold is not defined, but no access leaves the buffers.
+ *        What is written lies apart from everything else that the call takes,
+ *      but for scores_out at scores (or with its rows between those of scores)
+ *      and new_seq_len at seq_len: OPURE_E_INVALID otherwise. */
 typedef struct opure_evict_args {
     const opure_model* model;        /* n_layers, n_kv_heads, head_dim, afmt; turn: rope_cos, rope_sin, rope_max_pos */
     const opure_kv*    kv;           /* kv->page_table is updated in place (freed) */

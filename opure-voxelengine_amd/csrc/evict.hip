@@ -556,6 +556,46 @@ __global__ __launch_bounds__(64) void k_evict_finish(EvictParams p)
 
 using namespace opure_hip;
 
+namespace {
+
+// What the call writes lies apart from everything else that it takes, but for
+// scores_out at scores and new_seq_len at seq_len.
+int evict_apart(const opure_evict_args* a, uint64_t keep)
+{
+    const opure_model* m = a->model;
+    const opure_kv* kv = a->kv;
+    const uint64_t planes = static_cast<uint64_t>(m->n_layers) * m->n_kv_heads, rows = a->batch * planes;
+    const uint64_t scores = ((rows - 1u) * a->scores_stride + a->max_ctx) * 4u, lens = a->batch * 4u;
+    const uint64_t freed = (static_cast<uint64_t>(a->batch - 1u) * a->freed_stride + (a->max_ctx + OPURE_PAGE_SIZE - 1u) / OPURE_PAGE_SIZE) * 4u;
+    enum { POOL, TABLE, KEPT, SCORES, SCORES_OUT, LEN, NEW_LEN, FREED, N_FREED, PARTS };
+    const struct { const char* name; const void* at; uint64_t bytes; bool written; } part[PARTS] = {
+        {"pool", kv->pool, planes * kv->n_pages * 2u * OPURE_PAGE_SIZE * m->head_dim * act_bytes(m->afmt), true},
+        {"page_table", kv->page_table, static_cast<uint64_t>(a->batch) * kv->max_pages_per_seq * 4u, a->freed != nullptr},
+        {"kept", a->kept, rows * keep * 4u, true},
+        {"scores", a->scores, scores, false},
+        {"scores_out", a->scores_out, scores, true},
+        {"seq_len", a->seq_len, lens, false},
+        {"new_seq_len", a->new_seq_len, lens, true},
+        {"freed", a->freed, freed, true},
+        {"n_freed", a->n_freed, lens, true}};
+    // scores_out between the rows of scores: the nearest two decide
+    const int64_t d = a->scores_out ? a->scores_out - a->scores : 0, stride = a->scores_stride, last = static_cast<int64_t>(rows) - 1;
+    bool meet = false;
+    for (int64_t k = -(d / stride) - 1; k <= -(d / stride) + 1; ++k)
+        meet = meet || (k >= -last && k <= last && d + k * stride < a->max_ctx && d + k * stride > -static_cast<int64_t>(a->max_ctx));
+    for (int x = 0; x < PARTS; ++x)
+        for (int y = x + 1; y < PARTS; ++y)
+        {
+            if (!(part[x].written || part[y].written) || !overlaps(part[x].at, part[x].bytes, part[y].at, part[y].bytes)) continue;
+            if (x == SCORES && y == SCORES_OUT && (d == 0 || !meet)) continue;
+            if (x == LEN && y == NEW_LEN && part[x].at == part[y].at) continue;
+            return set_error(OPURE_E_INVALID, "opure_kv_evict: %s overlaps %s", part[y].name, part[x].name);
+        }
+    return OPURE_OK;
+}
+
+}  // namespace
+
 extern "C" int opure_kv_evict(opure_dev* dev, const opure_evict_args* a)
 {
     OPURE_REQUIRE(dev && a && a->model && a->kv && a->kv->pool && a->kv->page_table && a->seq_len && a->scores && a->kept &&
@@ -587,6 +627,8 @@ extern "C" int opure_kv_evict(opure_dev* dev, const opure_evict_args* a)
                     reinterpret_cast<uintptr_t>(a->seq_len) | reinterpret_cast<uintptr_t>(a->new_seq_len) | reinterpret_cast<uintptr_t>(a->freed) |
                     reinterpret_cast<uintptr_t>(a->n_freed) | reinterpret_cast<uintptr_t>(kv->page_table)) & 3u) == 0u, OPURE_E_INVALID,
                   "opure_kv_evict: scores, kept, lengths and tables must be 4-byte aligned");
+    const int rc = evict_apart(a, keep);
+    if (rc) return rc;
     const DeviceGuard on(dev);
     EvictParams p{};
     p.pool = kv->pool;

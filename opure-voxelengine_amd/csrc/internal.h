@@ -114,6 +114,11 @@ int  prof_end(opure_dev* dev);
 // nothing is being timed
 bool prof_kernel_events(opure_dev* dev, hipEvent_t* start, hipEvent_t* stop);
 inline uint64_t align_up(uint64_t v, uint64_t a) { return (v + a - 1) / a * a; }
+inline bool overlaps(const void* a, uint64_t a_bytes, const void* b, uint64_t b_bytes)
+{
+    const uint64_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x && y && x < y + b_bytes && y < x + a_bytes;
+}
 inline uint32_t act_bytes(uint32_t afmt) { return afmt == OPURE_A_F32 ? 4u : 2u; }
 
 // The device handle's GPU as the current one for the length of a call: a

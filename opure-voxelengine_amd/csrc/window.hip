@@ -609,9 +609,18 @@ extern "C" int opure_attn_window_paged(opure_dev* dev, const opure_attn_window_a
     OPURE_REQUIRE((reinterpret_cast<uintptr_t>(a->q) & 15u) == 0u && (reinterpret_cast<uintptr_t>(a->out) & 7u) == 0u &&
                       ((reinterpret_cast<uintptr_t>(a->seq_len) | reinterpret_cast<uintptr_t>(a->weights)) & 3u) == 0u,
                   OPURE_E_INVALID, "opure_attn_window_paged: q must be 16-byte aligned, out 8-byte, seq_len and weights 4-byte");
-    const uint64_t bytes = static_cast<uint64_t>(a->batch) * a->rows * a->model->n_heads * a->model->head_dim * act_bytes(a->model->afmt);
-    const uintptr_t q = reinterpret_cast<uintptr_t>(a->q), out = reinterpret_cast<uintptr_t>(a->out);
-    OPURE_REQUIRE(q + bytes <= out || out + bytes <= q, OPURE_E_INVALID, "opure_attn_window_paged: out overlaps q");
+    const opure_model* m = a->model;
+    const uint64_t bytes = static_cast<uint64_t>(a->batch) * a->rows * m->n_heads * m->head_dim * act_bytes(m->afmt);
+    const uint64_t cache = static_cast<uint64_t>(m->n_layers) * a->kv->n_pages * 2u * m->n_kv_heads * OPURE_PAGE_SIZE * m->head_dim * act_bytes(m->afmt);
+    const uint64_t table = static_cast<uint64_t>(a->batch) * a->kv->max_pages_per_seq * 4u;
+    const uint64_t spread = ((a->batch - 1u) * a->weights_batch_stride + static_cast<uint64_t>(m->n_kv_heads - 1u) * a->weights_stride + a->max_ctx) * 4u;
+    OPURE_REQUIRE(!overlaps(a->out, bytes, a->q, bytes), OPURE_E_INVALID, "opure_attn_window_paged: out overlaps q");
+    OPURE_REQUIRE(!overlaps(a->out, bytes, a->kv->pool, cache) && !overlaps(a->out, bytes, a->kv->page_table, table) &&
+                      !overlaps(a->out, bytes, a->seq_len, a->batch * 4u), OPURE_E_INVALID, "opure_attn_window_paged: out overlaps the cache");
+    OPURE_REQUIRE(!overlaps(a->weights, spread, a->q, bytes) && !overlaps(a->weights, spread, a->out, bytes) &&
+                      !overlaps(a->weights, spread, a->kv->pool, cache) && !overlaps(a->weights, spread, a->kv->page_table, table) &&
+                      !overlaps(a->weights, spread, a->seq_len, a->batch * 4u),
+                  OPURE_E_INVALID, "opure_attn_window_paged: weights overlaps q, out or the cache");
     const DeviceGuard on(dev);
     WinPlan w;
     rc = win_plan(dev, a, w);

@@ -1,4 +1,5 @@
-"""What opure_kv_evict promises beyond its definition's values: every missing page is reported."""
+"""What opure_kv_evict promises beyond its definition's values: every missing page is reported,
+and scores_out may lie between the rows of scores."""
 import numpy as np
 import pytest
 
@@ -40,3 +41,23 @@ def test_every_missing_page_is_reported(dev, afmt, seq, budget, page):
         e.done()
     # pages past a sequence's positions are not its pages: missing in every shorter row of the table
     check(dev, afmt, 1, 2, 32, seq, *budget)
+
+
+def test_scores_out_between_the_rows_of_scores(dev):
+    rng = np.random.default_rng(1)
+    n = 300
+    cache = R.Cache(rng, F16, 2, 2, 32, [n, 200])
+    scores = rng.random((2, 2, 2, 2 * n), dtype=np.float32)
+    apart = Evict(dev, cache, [n, 200], scores, 2, 40, 50, True).run()
+    e = Evict(dev, cache, [n, 200], scores, 2, 40, 50, True, with_scores=False)
+    e.args.scores_out = int(e.scores) + 4 * n
+    e.run()
+    got = dev.download(e.scores, np.float32, scores.shape)
+    want = apart.get()
+    assert np.array_equal(got[..., :n], scores[..., :n])
+    for b, length in enumerate((n, 200)):
+        assert np.array_equal(got[b, ..., n:n + length], want["scores"][b, ..., :length])
+        assert np.array_equal(got[b, ..., n + length:], scores[b, ..., n + length:])
+    assert np.array_equal(e.get()["kept"], want["kept"]) and np.array_equal(e.get()["pool"], want["pool"])
+    e.done()
+    apart.done()
