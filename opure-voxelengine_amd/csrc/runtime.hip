@@ -27,6 +27,7 @@ int set_error(int code, const char* fmt, ...)
 
 int hip_fail(hipError_t e, const char* what)
 {
+    (void)hipGetLastError();                               // reported here: the next launch's check does not find it again
     const int code = (e == hipErrorOutOfMemory || e == hipErrorMemoryAllocation) ? OPURE_E_OOM : OPURE_E_HIP;
     return set_error(code, "%s failed: %s (%d)", what, hipGetErrorString(e), static_cast<int>(e));
 }
@@ -54,13 +55,24 @@ int ensure_workspace(opure_dev* dev, uint64_t bytes)
                       "opure_verify_reserve (opure_attn_window_reserve) before capturing", (unsigned long long)dev->ws_bytes,
                       (unsigned long long)bytes);
         OPURE_HIP_TRY(hipStreamSynchronize(dev->stream));
+        void* ws = nullptr;
+        hipError_t e = hipMalloc(&ws, bytes);
+        if (e != hipSuccess && dev->ws && !dev->live_graphs)
+        {
+            // there may be room without the old one; if not, the handle gets one of its size again
+            const uint64_t old = dev->ws_bytes;
+            OPURE_HIP_TRY(hipFree(dev->ws));
+            dev->ws = nullptr;
+            dev->ws_bytes = 0;
+            e = hipMalloc(&ws, bytes);
+            if (e != hipSuccess && hipMalloc(&dev->ws, old) == hipSuccess) dev->ws_bytes = old;
+        }
+        if (e != hipSuccess) return hip_fail(e, "allocating the workspace");
         // a captured graph may still point into the old workspace: keep it until
         // the last graph is destroyed
         if (dev->ws && dev->live_graphs) dev->retired_ws.push_back(dev->ws);
         else if (dev->ws) OPURE_HIP_TRY(hipFree(dev->ws));
-        dev->ws = nullptr;
-        dev->ws_bytes = 0;
-        OPURE_HIP_TRY(hipMalloc(&dev->ws, bytes));
+        dev->ws = ws;
         dev->ws_bytes = bytes;
     }
     return OPURE_OK;

@@ -120,3 +120,37 @@ def test_more_than_four_million_workgroups(dev):
     """A max_ctx of 2^26 for 4,800 query rows: 2^22 workgroups over the positions, of which a few have any."""
     say("2^22 workgroups")
     check(dev, F16, 16, 1, 32, [50], 300, 100, 3, True, max_ctx=1 << 26)
+
+
+@pytest.mark.parametrize("captured", [False, True])
+def test_a_workspace_that_cannot_be_had(captured):
+    """A call whose workspace is larger than the memory (scores of 2^33 positions, 512 GiB) is
+    OPURE_E_OOM; the handle keeps the workspace that it had, and its next calls run."""
+    say("no room", captured)
+    d = H.Dev(0)
+    rng = np.random.default_rng(3)
+    cache = R.Cache(rng, F16, 1, 2, 64, [500])
+    q = R.act_to_f32(R.f32_to_act(rng.standard_normal((1, 1, 8, 64), dtype=np.float32), F16), F16)
+    c = R.Call(d, cache, q, 8, [499], 1, 0, 0, 0.125, weights=np.zeros((1, 1, 2, 500), np.float32)).run()
+    first, size, ptr, after = c.result(), C.c_uint64(), C.c_void_p(), C.c_uint64()
+    H.check(H.lib().opure_debug_workspace(d.h, C.byref(ptr), C.byref(size)))
+    if captured:
+        d.graph_begin()
+        c.run(sync=False)
+        g = d.graph_end()
+    for _ in range(2):
+        assert reserve(d, F16, 128, 32, 64, 256, 4, 1 << 20) == H.E_OOM
+        H.check(H.lib().opure_debug_workspace(d.h, C.byref(ptr), C.byref(after)))
+        assert after.value == size.value and ptr.value
+    if not captured:
+        d.graph_begin()
+        c.run(sync=False)                                   # no reserve in between
+        g = d.graph_end()
+    for run in (c.run, lambda: d.graph_launch(g)):
+        d.write(c.out, np.zeros(first.size, np.uint16))
+        run()
+        d.sync()
+        assert np.array_equal(first.view(np.uint32), c.result().view(np.uint32))
+    d.graph_destroy(g)
+    c.free()
+    d.close()
