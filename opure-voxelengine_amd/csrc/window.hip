@@ -29,11 +29,16 @@ constexpr uint32_t MAX_PARTS = 64;                         // of a (sequence, KV
 // set of registers.  The four waves are merged in LDS, the parts by k_win_join.
 //   A probability enters its product as two 16-bit numbers (its rounding and the
 // rest: 16 bits of bf16, 22 of fp16): the products are not what bounds this.
+//   ONCE: a KV head's rows are one block, so nobody else reads its bytes, and they are
+// loaded past the caches' usual order.  More blocks meet each other's: past 128
+// channels, in blocks of 16, streaming / not: 16 rows of 64 heads of 256 over 8,000
+// positions 88.0 / 58.9 us, 12 of 16 heads of 160 in 8 sequences of 4,000 46.5 / 32.2,
+// an fp32 prompt of 2,048 rows of 4 heads of 256 231 / 211.
 //   32 sequences of 1,024 to 16,384 positions behind a window of 4,096 (8 KV heads
 // of 128) read 412 MB in 76 us, 5.4 TB/s; reads alone of such scattered 4 KB planes
 // reach 5.8.  One row over 1,000 positions of heads of 64 takes 4.4 us, a chain of
 // round trips (length, page entries, keys and values) rather than bytes.
-template <int AF, int HD, int NT>
+template <int AF, int HD, int NT, bool ONCE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 2 ? 2 : 1))) void k_win_split(WinParams p)
 {
     typedef WinTile<AF, HD> T;
@@ -91,8 +96,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 2 ? 2
         int32_t e = entry(i);
         int32_t pa = page(e, i, 0u), pb = T::NB > 1u ? page(e, i, 1u) : pa;
         auto at = [&](int32_t pg) { return kbase + static_cast<uint64_t>(pg < 0 ? 0u : static_cast<uint32_t>(pg)) * page_bytes; };
-        tl.template load_k<NT == 1>(at(pa), at(pb), r, g);
-        tl.template load_v<NT == 1>(at(pa) + vofs, at(pb) + vofs, r, g);
+        tl.template load_k<ONCE>(at(pa), at(pb), r, g);
+        tl.template load_v<ONCE>(at(pa) + vofs, at(pb) + vofs, r, g);
         e = entry(i + 4u);
         while (true)
         {
@@ -115,7 +120,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 2 ? 2
             float s[NT][NS];
 #pragma unroll
             for (uint32_t n = 0; n < NT; ++n) win_scores<AF, HD>(p, tl, q[n], c, full, t0, g, sq.ctx + jr[n], sq.total, s[n]);
-            if (more) tl.template load_k<NT == 1>(at(na), at(nb), r, g);
+            if (more) tl.template load_k<ONCE>(at(na), at(nb), r, g);
             if (p.scores)
 #pragma unroll
                 for (uint32_t n = 0; n < NT; ++n)
@@ -175,7 +180,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 2 ? 2
                     o[d][n] = win_mfma<AF>(tl.v[d], hi[n], o[d][n]);
                 }
             if (!more) break;
-            tl.template load_v<NT == 1>(at(na) + vofs, at(nb) + vofs, r, g);
+            tl.template load_v<ONCE>(at(na) + vofs, at(nb) + vofs, r, g);
             pa = na;
             pb = nb;
             i += 4u;
@@ -416,13 +421,14 @@ constexpr uint32_t win_split_lds() { return 4u * (HD / 16u) * NT * 64u * 16u + 4
 
 // f(kernel, dynamic LDS, workgroups of it that the device holds at a time) for a head size and format
 template <typename F>
-int win_split_kernel(opure_dev* dev, uint32_t afmt, uint32_t hd, bool two, F&& f)
+int win_split_kernel(opure_dev* dev, uint32_t afmt, uint32_t hd, bool two, bool once, F&& f)
 {
-    auto one = [&](auto af, auto h, auto nt) {
+    auto one = [&](auto af, auto h, auto nt, auto alone) {
         constexpr int AF = decltype(af)::value, HD = decltype(h)::value, NT = decltype(nt)::value;
+        constexpr bool ONCE = decltype(alone)::value;
         static std::atomic<uint64_t> done{0};
         static std::atomic<int> a_cu{0};
-        auto* kernel = &k_win_split<AF, HD, NT>;
+        auto* kernel = &k_win_split<AF, HD, NT, ONCE>;
         const int rc = win_lds(dev, reinterpret_cast<const void*>(kernel), win_split_lds<HD, NT>(), done);
         if (rc) return rc;
         int n = a_cu.load(std::memory_order_relaxed);
@@ -437,8 +443,11 @@ int win_split_kernel(opure_dev* dev, uint32_t afmt, uint32_t hd, bool two, F&& f
     auto by_head = [&](auto af) {
         return win_by_head(hd, [&](auto h) {
             if constexpr (decltype(h)::value <= 128)
-                if (two) return one(af, h, std::integral_constant<int, 2>{});
-            return one(af, h, std::integral_constant<int, 1>{});
+            {
+                if (two) return one(af, h, std::integral_constant<int, 2>{}, std::false_type{});
+            }
+            else if (!once) return one(af, h, std::integral_constant<int, 1>{}, std::false_type{});
+            return one(af, h, std::integral_constant<int, 1>{}, std::true_type{});
         });
     };
     return afmt == OPURE_A_F32   ? by_head(std::integral_constant<int, OPURE_A_F32>{})
@@ -525,7 +534,7 @@ int win_plan(opure_dev* dev, const opure_attn_window_args* a, WinPlan& w)
     w.blocks = (Gq + (w.two ? 31u : 15u)) / (w.two ? 32u : 16u);
     w.block_rows = std::min(Gq, w.two ? 32u : 16u);
     uint32_t room = 0;
-    const int rc = win_split_kernel(dev, m->afmt, m->head_dim, w.two, [&](auto, uint32_t, uint32_t n) {
+    const int rc = win_split_kernel(dev, m->afmt, m->head_dim, w.two, w.blocks == 1u, [&](auto, uint32_t, uint32_t n) {
         room = n;
         return OPURE_OK;
     });
@@ -666,7 +675,7 @@ extern "C" int opure_attn_window_paged(opure_dev* dev, const opure_attn_window_a
         return rc || !p.lse ? rc : win_sums_launch(dev, p, a->batch, sums_at);
     }
     const uint32_t wgs = p.n_kv * w.parts * w.blocks * a->batch;
-    rc = win_split_kernel(dev, p.afmt, p.hd, w.two, [&](auto kernel, uint32_t lds, uint32_t) {
+    rc = win_split_kernel(dev, p.afmt, p.hd, w.two, w.blocks == 1u, [&](auto kernel, uint32_t lds, uint32_t) {
         OPURE_LAUNCH(dev, kernel, dim3(wgs), dim3(256), lds, p);
         OPURE_LAUNCH_CHECK("k_win_split");
         return OPURE_OK;
