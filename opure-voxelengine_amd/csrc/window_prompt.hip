@@ -71,16 +71,22 @@ __global__ __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(HD <= 
     const uint32_t w0 = min(q0 + 32u * wave, Gq - 1u), w1 = min(q0 + 32u * wave + 31u, Gq - 1u), qi = min(w0 + r, Gq - 1u);
     const uint32_t j = qi / G, pos = sq.ctx + j, pos0 = sq.ctx + w0 / G, pos1 = sq.ctx + w1 / G;
     const uint64_t row = (static_cast<uint64_t>(b) * p.rows + j) * p.n_heads + kh * G + (qi - j * G);
-    // scores in powers of two are c times the products: c >= 0, its sign goes to Q (and c = 0 to Q whole)
+    // scores in powers of two are c times the products: c >= 0, its sign goes to Q, and with c = 0 Q is 0 (NaN where it is
+    // not finite: 0 times that)
     const float c = p.scale == 0.0f ? 1.0f : __fmul_rn(__builtin_fabsf(p.scale), 1.44269504088896340736f);
+    constexpr uint32_t EXP = AF == OPURE_A_F16 ? 0x7C00u : 0x7F80u, QNAN = AF == OPURE_A_F16 ? 0x7E00u : 0x7FC0u;
     u4v q[KS];
 #pragma unroll
     for (uint32_t s = 0; s < KS; ++s)
     {
         q[s] = *reinterpret_cast<const u4v*>(static_cast<const uint8_t*>(p.q) + row * (HD * 2u) + (2u * s + h) * 16u);
-        const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u, keep = p.scale == 0.0f ? 0u : ~0u;
+        const uint32_t flip = p.scale < 0.0f ? 0x80008000u : 0u;
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) q[s][i] = (q[s][i] ^ flip) & keep;
+        for (uint32_t i = 0; i < 4; ++i)
+        {
+            const uint32_t x = q[s][i], none = ((x & EXP) == EXP ? QNAN : 0u) | ((x >> 16 & EXP) == EXP ? QNAN << 16 : 0u);
+            q[s][i] = p.scale == 0.0f ? none : x ^ flip;
+        }
     }
     const uint64_t plane = static_cast<uint64_t>(OPURE_PAGE_SIZE) * HD * 2u, page_bytes = 2ull * p.n_kv * plane;
     const uint8_t* base = static_cast<const uint8_t*>(p.pool) + static_cast<uint64_t>(p.layer) * p.n_pages * page_bytes + kh * plane;

@@ -154,3 +154,20 @@ def test_a_workspace_that_cannot_be_had(captured):
     d.graph_destroy(g)
     c.free()
     d.close()
+
+
+@pytest.mark.parametrize("weights", [False, True], ids=["", "weights"])
+@pytest.mark.parametrize("scale", [0.0, 0.125, -0.2])
+@pytest.mark.parametrize("afmt", [F32, F16, BF16], ids=["f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,n", [(3, 900), (12, 900), (70, 40), (300, 10)])
+def test_queries_that_are_not_finite(dev, rows, n, afmt, scale, weights):
+    """NaN and infinities in a query are its own row's and head's: NaN there (also with a scale of 0), the others exact."""
+    say("queries", rows, n, afmt, scale, weights)
+
+    def edit(cache, q):
+        q[0, 0, 0, 3], q[0, rows - 1, 1, 63], q[0, rows // 2, 2, 17] = np.nan, np.inf, -np.inf
+
+    got = check(dev, afmt, 4, 2, 64, [n], rows, 600, 3, weights, seed=rows, edit=edit, spread=0.5, scale=scale)
+    assert np.isnan(got[0, 0, 0]).all() and np.isfinite(got[0, :, 3]).all()
+    if scale == 0:
+        assert np.isnan(got[0, rows - 1, 1]).all() and np.isnan(got[0, rows // 2, 2]).all()
