@@ -61,3 +61,27 @@ def test_scores_out_between_the_rows_of_scores(dev):
     assert np.array_equal(e.get()["kept"], want["kept"]) and np.array_equal(e.get()["pool"], want["pool"])
     e.done()
     apart.done()
+
+
+def test_scores_past_32_bits(dev):
+    """Scores whose six planes lie 2^30 elements apart."""
+    say("scores past 32 bits")
+    rng = np.random.default_rng(2)
+    n, stride = 250, (1 << 30) + 3
+    cache = R.Cache(rng, BF16, 3, 2, 32, [n])
+    scores = rng.random((1, 3, 2, n), dtype=np.float32)
+    near = Evict(dev, cache, [n], scores, 2, 40, 50, True, in_place=True).run()
+    far = dev.alloc((5 * stride + n) * 4)
+    for plane in range(6):
+        dev.write(far, scores.reshape(6, n)[plane], plane * stride * 4)
+    e = Evict(dev, cache, [n], scores, 2, 40, 50, True)
+    e.args.scores = e.args.scores_out = int(far)
+    e.args.scores_stride = stride
+    e.run()
+    got, want = e.get(), near.get()
+    assert np.array_equal(got["kept"], want["kept"]) and np.array_equal(got["pool"], want["pool"])
+    for plane in range(6):
+        assert np.array_equal(dev.download(far, np.float32, (n,), plane * stride * 4), want["scores"].reshape(6, n)[plane])
+    e.done()
+    near.done()
+    far.free()

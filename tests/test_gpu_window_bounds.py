@@ -171,3 +171,46 @@ def test_queries_that_are_not_finite(dev, rows, n, afmt, scale, weights):
     assert np.isnan(got[0, 0, 0]).all() and np.isfinite(got[0, :, 3]).all()
     if scale == 0:
         assert np.isnan(got[0, rows - 1, 1]).all() and np.isnan(got[0, rows // 2, 2]).all()
+
+
+# batch, max_ctx, window: calls whose weights are added four positions a thread (at least two
+# workgroups a CU of 1,024 positions): with up to 8 parts a KV head, and with more
+FOUR = {"few parts": (64, 1111, 0), "windowed": (64, 3001, 1100), "many parts": (10, 7007, 0)}
+
+
+@pytest.mark.parametrize("group,rows", [(3, 3), (5, 2), (1, 16), (17, 1), (7, 3)])
+@pytest.mark.parametrize("afmt,hd", [(F32, 64), (F32, 128), (F32, 192), (F32, 256), (F16, 64), (BF16, 128), (F16, 192), (BF16, 256)])
+@pytest.mark.parametrize("form", FOUR)
+def test_weights_four_positions_a_thread(dev, form, afmt, hd, group, rows):
+    """9 to 21 query rows a KV head: several turns of the eight that a workgroup adds at a time, the last one not full."""
+    batch, cap, window = FOUR[form]
+    say("four", form, afmt, hd, group, rows)
+    rng = np.random.default_rng(hd + group)
+    seq = [int(n) for n in rng.integers(0, 60, batch)]
+    seq[3], seq[batch // 2] = cap - rows, cap // 3                # two long ones
+    check(dev, afmt, 8 * group, 8, hd, seq, rows, window, 5 if window else 0, True, seed=hd, max_ctx=cap)
+
+
+def test_weights_past_32_bits(dev):
+    """Sums whose heads and sequences lie 2^31 and 2^32 elements apart."""
+    say("weights past 32 bits")
+    rng = np.random.default_rng(14)
+    for rows, seq, heads in ((2, [300, 41], 4), (90, [33, 0], 4)):
+        cache = R.Cache(rng, F16, 1, 2, 64, [n + rows for n in seq])
+        q = R.act_to_f32(R.f32_to_act(rng.standard_normal((2, rows, heads, 64), dtype=np.float32), F16), F16)
+        c = R.Call(dev, cache, q, heads, seq, rows, 50, 4, 0.125)
+        stride, batch = (1 << 31) + 7, (1 << 32) + 1000
+        far = dev.alloc((batch + stride + 1000) * 4)
+        c.args.weights, c.args.weights_stride, c.args.weights_batch_stride = int(far), stride, batch
+        ref, tol, ws, wt = R.attention(cache, 0, q, heads, seq, rows, 50, 4, 0.125)
+        for b in range(2):
+            for h in range(2):
+                dev.write(far, np.zeros(1000, np.float32), (b * batch + h * stride) * 4)
+        c.run()
+        assert (np.abs(c.result() - ref) <= tol).all()
+        for b, n in enumerate(seq):
+            for h in range(2):
+                got = dev.download(far, np.float32, (1000,), (b * batch + h * stride) * 4)
+                assert (np.abs(got[:n + rows] - ws[b][h]) <= wt[b][h] + 2.0 ** -23 * ws[b][h]).all() and (got[n + rows:] == 0).all()
+        c.free()
+        far.free()
