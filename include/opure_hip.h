@@ -284,7 +284,8 @@ typedef struct opure_attn_window_args {
     uint32_t           max_ctx;     /* host upper bound on seq_len[b] + rows */
     uint32_t           window;      /* positions a row sees up to its own, which counts; 0 = all */
     uint32_t           sinks;       /* first positions that stay visible */
-    const void*        q;           /* [batch*rows][n_heads*head_dim] in afmt */
+    const void*        q;           /* [batch*rows][n_heads*head_dim] in afmt; not in the device's workspace
+                                     * (opure_debug_workspace), nor out and weights */
     void*              out;         /* like q; apart from everything else, as weights is */
     float*             weights;     /* device, or NULL */
     uint32_t           weights_stride;        /* floats between KV heads, >= max_ctx */

@@ -630,6 +630,10 @@ extern "C" int opure_attn_window_paged(opure_dev* dev, const opure_attn_window_a
                       !overlaps(a->weights, spread, a->kv->pool, cache) && !overlaps(a->weights, spread, a->kv->page_table, table) &&
                       !overlaps(a->weights, spread, a->seq_len, a->batch * 4u),
                   OPURE_E_INVALID, "opure_attn_window_paged: weights overlaps q, out or the cache");
+    // the call's parts and scores go to the workspace, which may also move
+    OPURE_REQUIRE(!overlaps(dev->ws, dev->ws_bytes, a->q, bytes) && !overlaps(dev->ws, dev->ws_bytes, a->out, bytes) &&
+                      !overlaps(dev->ws, dev->ws_bytes, a->weights, spread),
+                  OPURE_E_INVALID, "opure_attn_window_paged: q, out or weights in the device's workspace");
     const DeviceGuard on(dev);
     WinPlan w;
     rc = win_plan(dev, a, w);

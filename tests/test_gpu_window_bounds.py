@@ -214,3 +214,24 @@ def test_weights_past_32_bits(dev):
                 assert (np.abs(got[:n + rows] - ws[b][h]) <= wt[b][h] + 2.0 ** -23 * ws[b][h]).all() and (got[n + rows:] == 0).all()
         c.free()
         far.free()
+
+
+@pytest.mark.parametrize("what", ["q", "out", "weights"])
+def test_buffers_in_the_workspace_are_refused(dev, what):
+    """The call writes its parts there, and a larger one replaces it."""
+    say("in the workspace", what)
+    rng = np.random.default_rng(5)
+    cache = R.Cache(rng, F16, 1, 2, 64, [700])
+    q = R.act_to_f32(R.f32_to_act(rng.standard_normal((1, 1, 8, 64), dtype=np.float32), F16), F16)
+    c = R.Call(dev, cache, q, 8, [699], 1, 0, 0, 0.125, weights=np.zeros((1, 1, 2, 700), np.float32)).run()
+    ptr, size = C.c_void_p(), C.c_uint64()
+    H.check(H.lib().opure_debug_workspace(dev.h, C.byref(ptr), C.byref(size)))
+    for at in (ptr.value, ptr.value + size.value - 256):
+        old = getattr(c.args, what)
+        setattr(c.args, what, at)
+        with pytest.raises(H.OpureError) as e:
+            c.run()
+        assert e.value.code == H.E_INVALID and "workspace" in str(e.value)
+        setattr(c.args, what, old)
+    c.run()
+    c.free()
