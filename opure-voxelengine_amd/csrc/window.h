@@ -144,7 +144,7 @@ __device__ __forceinline__ u4v win_load(const uint8_t* p)
 constexpr float NEG_INF = -__builtin_huge_valf();
 
 // The tiles (TT positions each) that the rows at ctx .. ctx + rows - 1 see: the
-// sinks' first, then the window's.  Tile i of the list starts at position start(i).
+// sinks' first, then the window's.  Tile i of the list starts at position TT tile(i).
 struct WinSpan {
     uint32_t ns, w0, n;           // sink tiles, the window's first tile, tiles in all
     __device__ __forceinline__ uint32_t tile(uint32_t i) const { return i < ns ? i : i - ns + w0; }
@@ -178,7 +178,6 @@ struct WinTile {
     static constexpr bool HALF = AF != OPURE_A_F32 && HD % 32 != 0;   // the last step's upper channels are not there
     u4v k[NB][KS], v[DT];
 
-    __device__ __forceinline__ static float part(u4v x, uint32_t i) { return __uint_as_float(x[i]); }
     template <bool ONCE>
     __device__ __forceinline__ void load_k(const uint8_t* a, const uint8_t* b, uint32_t r, uint32_t g)
     {

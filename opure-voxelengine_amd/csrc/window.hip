@@ -419,7 +419,8 @@ __global__ __launch_bounds__(256) void k_win_join(WinParams p)
 template <int HD, int NT>
 constexpr uint32_t win_split_lds() { return 4u * (HD / 16u) * NT * 64u * 16u + 4u * NT * 16u * 2u * 4u; }
 
-// f(kernel, dynamic LDS, workgroups of it that the device holds at a time) for a head size and format
+// f(kernel, dynamic LDS, workgroups of it that the device holds at a time) for a head size and format.
+// What a CU holds is asked once a kernel: it is the same on every device that the code is built for.
 template <typename F>
 int win_split_kernel(opure_dev* dev, uint32_t afmt, uint32_t hd, bool two, bool once, F&& f)
 {
