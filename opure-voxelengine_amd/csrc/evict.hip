@@ -286,7 +286,8 @@ __device__ __forceinline__ uint32_t turn_pair(uint32_t v, float c, float s)
 // a group of positions that a run fills in part is stored by elements.
 //   Bound by the cache's bytes: 32 layers of 3 sequences of 3,500 to 8,000
 // positions cut to 2,504 (8 KV heads of 128) read K where it is kept, V whole and
-// write both, 2.6 GB in 576 us, 4.4 TB/s (a copy reaches 4.65); 16 layers of 2,048
+// write both, 2.6 GB in 576 us, 4.5 TB/s (copies of 4 GiB reach 4.6 to 4.8, of 1 GiB
+// 5.4); 16 layers of 2,048
 // positions halved (heads of 64), 84 MB in 22 us.
 //   KU: long runs keep more in flight a workgroup, short ones more workgroups a CU.
 // Four where all workgroups fit at a time, three a CU (16 KV heads of 8,000 positions

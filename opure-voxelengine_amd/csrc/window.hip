@@ -28,15 +28,16 @@ constexpr uint32_t MAX_PARTS = 64;                         // of a (sequence, KV
 // about a tile (16 KB at 128 channels) in flight all the time without a second
 // set of registers.  The four waves are merged in LDS, the parts by k_win_join.
 //   A probability enters its product as two 16-bit numbers (its rounding and the
-// rest: 16 bits of bf16, 22 of fp16): the products are not what bounds this.
+// rest: 16 bits in bf16, so that 2^-16 of it is lost where the result's own rounding
+// is 2^-8, and 22 in fp16, against 2^-11): the products are not what bounds this.
 //   ONCE: a KV head's rows are one block, so nobody else reads its bytes, and they are
 // loaded past the caches' usual order.  More blocks meet each other's: past 128
 // channels, in blocks of 16, streaming / not: 16 rows of 64 heads of 256 over 8,000
 // positions 88.0 / 58.9 us, 12 of 16 heads of 160 in 8 sequences of 4,000 46.5 / 32.2,
 // an fp32 prompt of 2,048 rows of 4 heads of 256 231 / 211.
 //   32 sequences of 1,024 to 16,384 positions behind a window of 4,096 (8 KV heads
-// of 128) read 412 MB in 76 us, 5.4 TB/s; reads alone of such scattered 4 KB planes
-// reach 5.8.  One row over 1,000 positions of heads of 64 takes 4.4 us, a chain of
+// of 128) read 412 MB in 75 us, 5.5 TB/s; reads alone of scattered 2 KB planes reach
+// 5.8.  One row over 1,000 positions of heads of 64 takes 4.4 us, a chain of
 // round trips (length, page entries, keys and values) rather than bytes.
 template <int AF, int HD, int NT, bool ONCE>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 2 ? 2 : 1))) void k_win_split(WinParams p)

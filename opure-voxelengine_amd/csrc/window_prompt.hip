@@ -42,11 +42,11 @@ constexpr uint32_t prompt_lds() { return 2u * (prompt_k_pieces<HD>() + prompt_v_
 // once left its results 1.4 times as far from the exact ones as one rounding at the
 // end.  fp16 weights are held 2^6 higher, so that the smallest steps are small
 // against the row's largest weight.
-//   Bound by the matrix and vector units together, which overlap little (36% and
-// 43% of the clocks): 2,048 rows of 32 heads of 128 over 4,096 positions each take
-// 160 to 170 us, 810 to 860 TFLOP/s, where a library product of 8,192 x 8,192
-// matrices reaches 1,133; 1,437 rows of 32 heads of 64 behind a window of 512, ten
-// tiles a workgroup, 18 us.
+//   Bound by the matrix and vector units together, each busy in half of the clocks:
+// 2,048 rows of 32 heads of 128 over 4,096 positions each take 208 us, 660 TFLOP/s of
+// the formulas and 990 of the products done, where a library product of 8,192 x 8,192
+// matrices reaches 1,133 to 1,160; 1,437 rows of 32 heads of 64 behind a window of 512,
+// ten tiles a workgroup, 20.5 us.
 //   KG 2 (a grid that does not give every SIMD two waves): eight waves, two for
 // each 32 rows, one on the even tiles and one on the odd ones, merged at the end.
 template <int AF, int HD, int KG>
@@ -181,7 +181,7 @@ __global__ __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(HD <= 
         const u4v* v = vt + (i & 1u) * prompt_v_pieces<HD>();
         f16_t s[2];
         // the reads of the next key operand between the products of this one, and the products ahead of the other
-        // waves' vector work (8B prompt 183.5 -> 180.9 us, 1B 18.3 -> 18.1)
+        // waves' vector work (with one product a weight: 8B prompt 183.5 -> 180.9 us, 1B 18.3 -> 18.1)
         __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (uint32_t t = 0; t < 2; ++t)
@@ -353,11 +353,11 @@ __global__ __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(HD <= 
 // its rows, which one workgroup took 30 us to walk through (1,024 rows of the 1B
 // shape; 16 in chunks).  Bound there by its first loads and by the exponentials,
 // 16 clocks each on a SIMD.  Whole calls with chunks of 512, 1,024, 1,536, 2,048
-// and 4,096: that prompt 38.4, 35.7, 36.2, 37.3, 46.6 us; 2,048 rows 82.3, 81.8,
-// 74.4, 80.6, 81.7; 2,048 rows of 128 channels behind a window of 4,096 375, 345,
-// 334, 345, 318.  Where chunks of 1,536 do not give every CU a workgroup, which
+// and 4,096: that prompt 41.4, 38.9, 39.3, 40.7, 50.0 us; 2,048 rows 90.5, 90.0,
+// 82.5, 88.8, 89.9; 2,048 rows of 128 channels behind a window of 4,096 414, 386,
+// 375, 390, 364.  Where chunks of 1,536 do not give every CU a workgroup, which
 // walks its rows alone, they are of 512 (whole calls with 1,536 / 512: 2,008 rows of
-// 4 heads of 64 behind a window of 20 34.8 / 24.9, 512 rows of 32 heads 28.7 / 23.1,
+// 4 heads of 64 behind a window of 20 34.8 / 24.9, 512 rows of 32 heads 30.0 / 24.9,
 // 400 of 12 heads of 112 in fp32 54.8 / 41.9; but with 400 workgroups 66.3 / 75.0).
 uint32_t sums_chunk(const opure_dev* dev, const WinParams& p, uint32_t batch)
 {
@@ -553,7 +553,8 @@ namespace opure_win {
 int win_prompt_launch(opure_dev* dev, const WinParams& p, uint32_t batch)
 {
     const uint32_t Gq = p.n_heads / p.n_kv * p.rows, wgs = p.n_kv * ((Gq + 127u) / 128u) * batch;
-    // KG 1 against 2: 256 workgroups (1,024 causal rows) 21 against 17 us, 360 18.2 against 22.9
+    // KG 1 against 2: 256 workgroups (1,024 causal rows) 24.8 against 20.4 us, 360 behind a window of 512 19.0 against
+    // 25.7, 512 23.9 against 28.5 (512 causal ones 47.2 against 42.5)
     const bool two = wgs <= static_cast<uint32_t>(dev->n_cu > 0 ? dev->n_cu : 256);
     auto go = [&](auto af) {
         return win_by_head(p.hd, [&](auto h) {
