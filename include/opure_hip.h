@@ -254,8 +254,8 @@ int opure_attn_decode_paged(opure_dev* dev, const opure_attn_args* a);
  *      OPURE_MAX_PROMPT_ROWS, batch up to OPURE_MAX_BATCH_ROWS, every format
  *      and head size of opure_attn_decode_paged.  batch x rows x n_heads past
  *      2^25, or a launch of 2^24 workgroups (with weights about 2^30 of batch x
- *      n_kv_heads x max_ctx, fewer where a KV head has more than 1,536 query
- *      rows), is OPURE_E_CAPACITY.
+ *      n_kv_heads x max_ctx, 2^29 in fp32, fewer where a KV head has more than
+ *      1,536 query rows), is OPURE_E_CAPACITY.
  *        What a row does not see does not reach it: masked K and V may hold
  *      anything, NaN and infinities included, and pages that no row of a
  *      sequence sees may be missing (-1), so a cache that only grows can
@@ -273,8 +273,9 @@ int opure_attn_decode_paged(opure_dev* dev, const opure_attn_args* a);
  *      its rounding and the rest (16 bits of it in bf16, 22 in fp16).  The order
  *      of sums follows the shape of the call (batch, rows, max_ctx, window,
  *      sinks and whether there are weights): the same call gives the same bits,
- *      a row alone and in a batch may differ in its last ones.  A length below 0 or past max_ctx is OPURE_E_CAPACITY at
- *      the next sync; positions past max_ctx are neither read nor weighed. */
+ *      a row alone and in a batch may differ in its last ones.  A length below 0
+ *      or past max_ctx is OPURE_E_CAPACITY at the next sync; positions past
+ *      max_ctx are neither read nor weighed. */
 typedef struct opure_attn_window_args {
     const opure_model* model; /* n_layers, n_heads, n_kv_heads, head_dim, attn_scale, afmt */
     const opure_kv*    kv;
@@ -297,8 +298,9 @@ typedef struct opure_attn_window_args {
  * capturing one into a graph.  It follows how that call is run, and a call of
  * fewer rows, sequences or positions can need more: reserve each shape that
  * will be captured.  Without weights it is about 64 MiB or twice the bytes of q
- * in fp32 at most; with them as much again as the keys of the positions that
- * are seen take in the layer, or 64 MiB. */
+ * in fp32 at most.  With them few rows add up to the bytes that the keys of the
+ * positions take in the layer, or 64 MiB; many rows add 4 bytes for each
+ * position, KV head and 1,536 of its query rows. */
 int opure_attn_window_reserve(opure_dev* dev, const opure_attn_window_args* a);
 int opure_attn_window_paged(opure_dev* dev, const opure_attn_window_args* a);
 

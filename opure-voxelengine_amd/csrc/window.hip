@@ -30,11 +30,11 @@ constexpr uint32_t MAX_PARTS = 64;                         // of a (sequence, KV
 //   A probability enters its product as two 16-bit numbers (its rounding and the
 // rest: 16 bits in bf16, so that 2^-16 of it is lost where the result's own rounding
 // is 2^-8, and 22 in fp16, against 2^-11): the products are not what bounds this.
-//   ONCE: a KV head's rows are one block, so nobody else reads its bytes, and they are
-// loaded past the caches' usual order.  More blocks meet each other's: past 128
-// channels, in blocks of 16, streaming / not: 16 rows of 64 heads of 256 over 8,000
-// positions 88.0 / 58.9 us, 12 of 16 heads of 160 in 8 sequences of 4,000 46.5 / 32.2,
-// an fp32 prompt of 2,048 rows of 4 heads of 256 231 / 211.
+//   ONCE: at most 16 query rows a KV head, so no other workgroup reads its bytes, and
+// the loads stream.  Past 128 channels more rows are more blocks of 16, which find
+// each other's bytes in the caches (streaming / not: 16 rows of 64 heads of 256 over
+// 8,000 positions 88.0 / 58.9 us, 12 of 16 heads of 160 in 8 sequences of 4,000 46.5 /
+// 32.2, an fp32 prompt of 2,048 rows of 4 heads of 256 231 / 211).
 //   32 sequences of 1,024 to 16,384 positions behind a window of 4,096 (8 KV heads
 // of 128) read 412 MB in 75 us, 5.5 TB/s; reads alone of scattered 2 KB planes reach
 // 5.8.  One row over 1,000 positions of heads of 64 takes 4.4 us, a chain of
@@ -497,7 +497,7 @@ void win_choose(const opure_dev* dev, const opure_attn_window_args* a, WinPlan& 
     const double keys = heads * span * hd * act_bytes(m->afmt), scores = heads * span * 4.0 * Gq;
     const double store = std::max(0.2 * Gq, 2.0 * scores / 5.3e6), again = 2.0 + hd / 64.0 + keys / 2.5e6;
     w.stored = a->weights && Gq <= 96.0 && store < again && scores <= std::max(67108864.0, keys);
-    w.prompt = m->afmt != OPURE_A_F32 && prompt + (a->weights ? again : 0.0) < split + (a->weights ? std::min(store, again) : 0.0);
+    w.prompt = m->afmt != OPURE_A_F32 && prompt + (a->weights ? again : 0.0) < split + (w.stored ? store : a->weights ? again : 0.0);
     if (w.prompt) w.stored = false;
 }
 

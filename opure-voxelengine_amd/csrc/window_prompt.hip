@@ -248,7 +248,7 @@ __global__ __launch_bounds__(256 * KG) __attribute__((amdgpu_waves_per_eu(HD <= 
             for (uint32_t d = 0; d < DT; ++d) o[d] = mfma_32<AF>(vx[d], w, o[d]);
         }
         l += sum[0] + sum[1];                              // this half's share
-        // the next 16 positions' weights between the products of these
+        // the next 16 positions' weights between the products of these (1B prompt 21.4 -> 20.3 us, 8B the same)
         __builtin_amdgcn_sched_group_barrier(0x002, 40, 0);
 #pragma unroll
         for (uint32_t x = 0; x < 6u * DT; ++x)
