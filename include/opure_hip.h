@@ -40,6 +40,17 @@
  *                            a V plane channel-major [head_dim][page_size] (so V^T
  *                            tiles of 8 tokens are one 16-byte load); page_table
  *                            int32[batch][max_pages_per_seq] (-1 = none)
+ *   4-bit KV pool            (OPURE_KV_I4, every activation format) [n_layers][n_pages]
+ *                            [n_kv_heads] blocks of 640 ng bytes, ng = ceil(head_dim / 32)
+ *                            groups of 32 channels of one token with a scale and a base:
+ *                              K codes  uint32 [j 4][token 16][ng], channels 32 g + 8 j +
+ *                                       2 n + h at bit 16 h + 4 n
+ *                              V codes  uint32 [j 4][c 16][ng], channels 32 g + 16 T + c of
+ *                                       the tokens 4 j + 2 m + h at bit 16 h + 8 T + 4 m
+ *                              K        fp16 [token 16][ng][scale, base]
+ *                              V        fp16 [j 4][ng][scale, base][token 4 j ..]
+ *                            A code c stands for the fp16 number nearest to
+ *                            scale (16 + c) + base.  5 bits a channel.
  *   rope table               float cos[max_pos][head_dim/2], sin[...] (interleaved
  *                            pairs (2p, 2p+1), Opure_RoPE.usf:7-10)
  */
@@ -71,6 +82,7 @@ enum { OPURE_W_F32 = 0, OPURE_W_I8PC = 1, OPURE_W_I4G128 = 2 };
 enum { OPURE_A_F32 = 0, OPURE_A_F16 = 1, OPURE_A_BF16 = 2 };
 enum { OPURE_ROPE_GPU = 0, OPURE_ROPE_CPUREF = 1 };
 enum { OPURE_EPI_STORE = 0, OPURE_EPI_RESIDUAL = 1, OPURE_EPI_SWIGLU = 2 };
+enum { OPURE_KV_ACT = 0, OPURE_KV_I4 = 1 };   /* the cache in the model's activation format, or in 4 bits */
 enum { OPURE_ACCEPT_NONE = 0, OPURE_ACCEPT_GREEDY = 1, OPURE_ACCEPT_REJECTION = 2 };
 
 typedef struct opure_dev opure_dev;
@@ -304,6 +316,83 @@ typedef struct opure_attn_window_args {
 int opure_attn_window_reserve(opure_dev* dev, const opure_attn_window_args* a);
 int opure_attn_window_paged(opure_dev* dev, const opure_attn_window_args* a);
 
+/* ---- rows of queries, keys and values that a program computed itself (its own
+ *      projections, adapters, opure_gemv_batched_* with OPURE_EPI_STORE), for a
+ *      layer of the paged cache: what the verify step's fused QKV product does
+ *      behind its sums.  Row j of sequence b stands at position seq_len[b] + j.
+ *        With `rotate`, q and k are turned to their positions by the model's RoPE
+ *      table (rope_max_pos >= max_ctx) in fp32, products and sums rounded as the
+ *      fused product does: the same numbers give the same bits.  Without it they
+ *      are taken as they are.  q (or NULL, with q_out) goes to q_out in the model's
+ *      format, k and v to the layer's pages: in that format, or quantised to 4 bits
+ *      straight from fp32.
+ *        4 bits (OPURE_KV_I4): of a token's 32 channels scale = fp16((hi - lo) / 15),
+ *      base = fp16(lo - 16 scale), codes to the nearest value, so a value is off by
+ *      half a scale and base's and the value's roundings to fp16 at most; magnitudes
+ *      past 2^14 are held as 2^14; a group with a NaN or an infinity reads NaN.
+ *        row_count (or NULL: all) gives each sequence's rows that are there, 0 to
+ *      `rows` (what lies outside counts as the nearest): the others of a padded
+ *      batch are not read and nothing of them is written, q_out's rows included.
+ *        Slots of other tokens keep their bits.  A page that two sequences share must
+ *      not be among those written.  A row past max_ctx, or a negative length, is
+ *      OPURE_E_CAPACITY at the next sync and nothing of it is written; a missing page
+ *      likewise, and then the row's q_out is.  What is written lies apart from
+ *      everything else that the call takes, but for q_out at a contiguous q of the
+ *      model's format (turned in place).  The call uses no workspace. */
+typedef struct opure_kv_append_args {
+    const opure_model* model;     /* n_layers, n_heads (with q), n_kv_heads, head_dim, afmt; rotate: rope_cos, rope_sin, rope_max_pos */
+    const opure_kv*    kv;        /* pool in kvfmt */
+    uint32_t           kvfmt;     /* OPURE_KV_* */
+    uint32_t           layer;
+    uint32_t           batch, rows;  /* up to OPURE_MAX_BATCH_ROWS x OPURE_MAX_PROMPT_ROWS */
+    const int32_t*     seq_len;   /* device [batch] */
+    uint32_t           max_ctx;   /* host upper bound on seq_len[b] + the sequence's rows */
+    const int32_t*     row_count; /* device [batch] or NULL */
+    uint32_t           rotate;
+    uint32_t           xfmt;      /* of q, k and v: OPURE_A_F32 or the model's */
+    const void*        q;         /* [batch*rows] rows of n_heads*head_dim, or NULL */
+    const void*        k;         /* [batch*rows] rows of n_kv_heads*head_dim */
+    const void*        v;
+    uint32_t           q_stride, k_stride, v_stride;   /* elements between rows; rows and pointers 16-byte aligned */
+    void*              q_out;     /* [batch*rows][n_heads*head_dim] in the model's format, or NULL */
+} opure_kv_append_args;
+
+int opure_kv_append(opure_dev* dev, const opure_kv_append_args* a);
+/* Bytes of a pool of n_pages pages in kvfmt (n_layers, n_kv_heads, head_dim, afmt are read). */
+int opure_kv_pool_bytes(const opure_model* model, uint32_t kvfmt, uint32_t n_pages, uint64_t* bytes);
+
+/* ---- attention over a 4-bit cache (OPURE_KV_I4): one row or a few a sequence
+ *      (decoding, a verify step) and a prompt's rows, with or without a window and
+ *      sinks: the rows, what they see, missing pages, rows of -inf, lengths and
+ *      limits are opure_attn_window_paged's, without its weights.  q and out are in
+ *      the model's format, any of the three.
+ *        The codes' values are fp16 numbers and meet the queries as such; scores,
+ *      maxima and sums are fp32.  A query row enters as fp16 numbers of a power of
+ *      two of it (fp32 rows as two each, 22 bits), a softmax weight as one fp16
+ *      number (bf16 models) or two (its rounding and the rest, 22 bits).  The same
+ *      call gives the same bits; a row alone and in a batch may differ in its last
+ *      ones.
+ *        opure_kv_rollback without poison and the page tables work on such a cache as
+ *      on any other; opure_verify_step, opure_prompt_step, the other attention calls
+ *      and opure_kv_evict read a cache in the model's format. */
+typedef struct opure_attn_kv4_args {
+    const opure_model* model; /* n_layers, n_heads, n_kv_heads, head_dim, attn_scale, afmt */
+    const opure_kv*    kv;    /* pool in OPURE_KV_I4 */
+    uint32_t           layer;
+    uint32_t           batch, rows;
+    const int32_t*     seq_len;     /* device [batch] */
+    uint32_t           max_ctx;     /* host upper bound on seq_len[b] + rows */
+    uint32_t           window;      /* positions a row sees up to its own, which counts; 0 = all */
+    uint32_t           sinks;       /* first positions that stay visible */
+    const void*        q;           /* [batch*rows][n_heads*head_dim] in afmt, 16-byte aligned, not in the device's workspace, nor out */
+    void*              out;         /* like q, 8-byte aligned, apart from everything else */
+} opure_attn_kv4_args;
+
+/* Sizes the device's workspace for such a call (seq_len, q and out are not read),
+ * before capturing it into a graph: reserve each shape that will be captured. */
+int opure_attn_kv4_reserve(opure_dev* dev, const opure_attn_kv4_args* a);
+int opure_attn_kv4_paged(opure_dev* dev, const opure_attn_kv4_args* a);
+
 /* ---- acceptance ------------------------------------------------------- */
 /* Greedy: argmax per row (ties -> lowest index; the reference's ArgMaxMain,
  * Opure_ArgMax.usf:33-86, re-specified), longest matching draft prefix, then
@@ -360,6 +449,38 @@ typedef struct opure_sample_args {
 } opure_sample_args;
 
 int opure_sample_rows(opure_dev* dev, const opure_sample_args* a);
+
+/* ---- log probabilities of given tokens, entropy and the most probable tokens of
+ *      each row of logits, for p = softmax(logits / temperature):
+ *        logprob[r]  log p(tokens[r])
+ *        entropy[r]  - sum p log p (a token of probability 0 adds 0)
+ *        top_tokens[r][0..top), top_logprobs  the tokens of the largest logits, the
+ *                    largest first, ties to the lowest token; a NaN counts as larger
+ *                    than every number, -0 as 0
+ *      One pass over the logits, sums in fp32 and in a fixed order.  A row with a NaN
+ *      or a +inf, or with nothing but -inf, has NaN for its log probabilities and its
+ *      entropy.  A token outside the vocabulary is OPURE_E_INVALID at the next sync and
+ *      reads NaN.  tokens with logprob, entropy, and top's two arrays may each be left
+ *      out; something is asked for.  top <= vocab, top <= OPURE_MAX_TOP. */
+#define OPURE_MAX_TOP 64
+#define OPURE_MAX_LOGPROB_ROWS 65535
+typedef struct opure_logprobs_args {
+    uint32_t       rows, vocab;      /* rows <= OPURE_MAX_LOGPROB_ROWS, vocab <= 2^24 */
+    const float*   logits;           /* [rows] rows of vocab, 16-byte aligned or not */
+    uint32_t       logits_stride;    /* floats between rows, >= vocab */
+    float          temperature;      /* > 0; 1: the logits as they are */
+    const int32_t* tokens;           /* device [rows], or NULL with logprob */
+    float*         logprob;          /* device [rows] or NULL */
+    float*         entropy;          /* device [rows] or NULL */
+    uint32_t       top;              /* 0: none */
+    int32_t*       top_tokens;       /* device [rows][top] or NULL (top 0) */
+    float*         top_logprobs;     /* device [rows][top] or NULL (top 0) */
+} opure_logprobs_args;
+
+/* Sizes the device's workspace for such a call (only rows, vocab and top are read),
+ * before capturing it into a graph. */
+int opure_logprobs_reserve(opure_dev* dev, const opure_logprobs_args* a);
+int opure_logprobs(opure_dev* dev, const opure_logprobs_args* a);
 
 /* Philox4x32-10 test hook: out[i] = word 0 of Philox(seed; pos[i], seq[i], stream, 0). */
 int opure_philox_uniform(opure_dev* dev, uint64_t seed, const uint32_t* pos, const uint32_t* seq,

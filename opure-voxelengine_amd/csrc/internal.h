@@ -281,6 +281,9 @@ int      attn_prompt_launch(opure_dev* dev, const opure_model* m, const opure_kv
 int      attn_launch(opure_dev* dev, const opure_model* m, const opure_kv* kv, uint32_t layer, uint32_t batch,
                      uint32_t rows, const int32_t* seq_len, uint32_t max_ctx, const void* q, void* out, float* part);
 
+// ---- the cache's formats (append.hip): bytes of a pool
+uint64_t kv_pool_bytes(const opure_model* m, uint32_t kvfmt, uint32_t n_pages);
+
 // ---- acceptance and rollback (accept.hip) ----------------------------------
 uint32_t argmax_parts(uint32_t vocab);
 uint64_t accept_ws_bytes(uint32_t batch, uint32_t k, uint32_t vocab, uint32_t mode);

@@ -1,0 +1,712 @@
+// ============================================================================
+//  kv4_attn.hip -- attention over the 4-bit paged cache (kv4.h), with a sliding
+//  window and first positions that stay visible or without.
+//
+//  Row j of a sequence, at position p = seq_len + j, sees t <= p with t < sinks or
+//  t > p - window:  s_t = scale q.k_t,  w_t = exp(s_t - m) / sum exp(s - m),
+//  out = sum w_t v_t.
+// ============================================================================
+#include "kv4.h"
+#include "window.h"
+
+#include <algorithm>
+
+using namespace opure_win;
+using namespace opure_kv4;
+using opure_hip::act_bytes;
+
+namespace {
+
+constexpr uint32_t MAX_PARTS = 64;                         // of a (sequence, KV head, block of query rows): a lane of the joining wave each
+constexpr float LOG2E = 1.44269504088896340736f;
+// Weights are held times 2^14, which fp16 still has: what fp16 loses at its small end then lies 2^38 below a row's
+// largest weight.
+constexpr float P_SHIFT = 14.0f;
+
+typedef u4v u4a __attribute__((aligned(4)));
+typedef uint32_t u2v __attribute__((ext_vector_type(2)));
+typedef u2v u2a __attribute__((aligned(4)));
+
+// N consecutive words, 4-byte aligned
+template <uint32_t N, bool ONCE>
+__device__ __forceinline__ void load_words(const uint32_t* p, uint32_t (&w)[N])
+{
+    auto get = [](auto* q) {
+        if constexpr (ONCE) return __builtin_nontemporal_load(q);
+        else return *q;
+    };
+    constexpr uint32_t Q = N / 4u * 4u;
+#pragma unroll
+    for (uint32_t i = 0; i < Q; i += 4u)
+    {
+        const u4v v = get(reinterpret_cast<const u4a*>(p + i));
+#pragma unroll
+        for (uint32_t x = 0; x < 4; ++x) w[i + x] = v[x];
+    }
+    if constexpr ((N & 2u) != 0u)
+    {
+        const u2v v = get(reinterpret_cast<const u2a*>(p + Q));
+        w[Q] = v[0];
+        w[Q + 1u] = v[1];
+    }
+    if constexpr ((N & 1u) != 0u) w[N - 1u] = get(p + N - 1u);
+}
+
+// Two pages of a KV head, positions 16 x + 0..15 of page x: lane (r, g) has K codes
+// of token r and channels 8 g of each group, and V codes of channels r and 16 + r of
+// each group and the tokens 4 g .. 4 g + 3.
+template <int HD, bool ONCE>
+struct Kv4Tile {
+    static constexpr uint32_t NG = groups(HD);
+    uint32_t kw[2][NG], ks[2][NG], vw[2][NG];
+    u4v vs[2][NG];                                         // [scale 0 1, scale 2 3, base 0 1, base 2 3]
+    __device__ __forceinline__ void load_k(const uint8_t* a, const uint8_t* b, uint32_t lane)
+    {
+#pragma unroll
+        for (uint32_t x = 0; x < 2; ++x)
+        {
+            const uint32_t* at = reinterpret_cast<const uint32_t*>(x ? b : a);
+            load_words<NG, ONCE>(at + lane * NG, kw[x]);
+            load_words<NG, ONCE>(at + k_scales(NG) / 4u + (lane & 15u) * NG, ks[x]);
+        }
+    }
+    __device__ __forceinline__ void load_v(const uint8_t* a, const uint8_t* b, uint32_t lane)
+    {
+#pragma unroll
+        for (uint32_t x = 0; x < 2; ++x)
+        {
+            const uint8_t* at = x ? b : a;
+            load_words<NG, ONCE>(reinterpret_cast<const uint32_t*>(at + v_codes(NG)) + lane * NG, vw[x]);
+#pragma unroll
+            for (uint32_t p = 0; p < NG; ++p) vs[x][p] = win_load<ONCE>(at + v_scales(NG) + ((lane >> 4) * NG + p) * 16u);
+        }
+    }
+    // group p of page x as fp16 numbers
+    __device__ __forceinline__ u4v k(uint32_t x, uint32_t p) const
+    {
+        const half2_t sb = pair(ks[x][p]), s = {sb[0], sb[0]}, b = {sb[1], sb[1]};
+        const uint32_t w = kw[x][p];
+        return u4v{values(codes<0>(w), s, b), values(codes<1>(w), s, b), values(codes<2>(w), s, b), values(codes<3>(w), s, b)};
+    }
+    // channels 32 p + 16 T + r of both pages' tokens
+    template <int T>
+    __device__ __forceinline__ u4v v(uint32_t p) const
+    {
+        u4v o;
+#pragma unroll
+        for (uint32_t x = 0; x < 2; ++x)
+        {
+            o[2 * x] = values(codes<2 * T>(vw[x][p]), pair(vs[x][p][0]), pair(vs[x][p][2]));
+            o[2 * x + 1] = values(codes<2 * T + 1>(vw[x][p]), pair(vs[x][p][1]), pair(vs[x][p][3]));
+        }
+        return o;
+    }
+};
+
+__device__ __forceinline__ f4_t mfma(u4v a, u4v b, f4_t c)
+{
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+}
+
+// A query row in fp16: of an fp16 model as it is, else times the power of two that
+// puts its largest magnitude just below 2^9 (bf16's 8 bits fit, and what fp16 cannot
+// hold of its small numbers is 2^-34 of the largest); an fp32 row is the sum of two.
+// Returns the factor of its scores in powers of two.
+template <int AF, int HD>
+__device__ __forceinline__ float load_query(const WinParams& p, uint64_t row, uint32_t g, u4v (&q)[AF == OPURE_A_F32 ? 2 : 1][groups(HD)])
+{
+    constexpr uint32_t NG = groups(HD);
+    constexpr bool HALF = HD % 32 != 0;
+    const float c = __fmul_rn(p.scale, LOG2E);
+    if constexpr (AF == OPURE_A_F16)
+    {
+        const uint8_t* at = static_cast<const uint8_t*>(p.q) + row * (HD * 2u) + 16u * g;
+#pragma unroll
+        for (uint32_t s = 0; s < NG; ++s) q[0][s] = HALF && s + 1u == NG && g >= 2u ? u4v{0u, 0u, 0u, 0u} : *reinterpret_cast<const u4v*>(at + 64u * s);
+        return c;
+    }
+    else
+    {
+        float x[NG][8], top = 0.0f;
+#pragma unroll
+        for (uint32_t s = 0; s < NG; ++s)
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i)
+            {
+                const bool there = !(HALF && s + 1u == NG && g >= 2u);
+                x[s][i] = there ? load_act<AF>(p.q, row * HD + 32u * s + 8u * g + i) : 0.0f;
+                top = fmaxf(top, __builtin_isfinite(x[s][i]) ? __builtin_fabsf(x[s][i]) : 0.0f);
+            }
+        const int e = __builtin_amdgcn_frexp_expf(max_xor32(max_xor16(top))) - 9;
+#pragma unroll
+        for (uint32_t s = 0; s < NG; ++s)
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i)
+            {
+                const float y0 = __builtin_ldexpf(x[s][2 * i], -e), y1 = __builtin_ldexpf(x[s][2 * i + 1], -e);
+                q[0][s][i] = win_pack<OPURE_A_F16>(y0, y1);
+                if constexpr (AF == OPURE_A_F32)
+                    q[1][s][i] = win_pack<OPURE_A_F16>(__fsub_rn(y0, win_low<OPURE_A_F16>(q[0][s][i])), __fsub_rn(y1, win_high<OPURE_A_F16>(q[0][s][i])));
+            }
+        return __builtin_ldexpf(c, e);
+    }
+}
+
+// One query row by one wave, exactly as the formulas say it; a position that the
+// row does not see is not read.  qs: the row in LDS (hd floats).
+__device__ inline void kv4_row(const WinParams& p, const float* qs, uint32_t b, uint32_t kh, uint32_t pos, uint32_t total, float& l, float (&o)[4])
+{
+    const uint32_t lane = threadIdx.x & 63u, hd = p.hd, ng = groups(hd);
+    const int32_t* pt = p.page_table + static_cast<uint64_t>(b) * p.max_pages;
+    const uint8_t* pool = static_cast<const uint8_t*>(p.pool);
+    const uint32_t end = min(pos + 1u, total), low = pos + 1u > p.window ? pos + 1u - p.window : 0u;
+    float m = NEG_INF;
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) o[i] = 0.0f;
+    for (uint32_t t0 = 0; t0 < end; t0 += 64u)
+    {
+        if (t0 >= p.sinks && t0 + 64u <= low)
+        {
+            t0 = low / 64u * 64u - 64u;                    // between the sinks and the window
+            continue;
+        }
+        const uint32_t t = t0 + lane;
+        const bool in = t < end && win_sees(p, pos, t);
+        const int32_t pg = in ? win_page(p, pt, t) : -1;
+        float s = in ? __builtin_nanf("") : NEG_INF;
+        if (pg >= 0)
+        {
+            const uint8_t* at = pool + block_at(p.layer, p.n_pages, static_cast<uint32_t>(pg), p.n_kv, kh, ng);
+            float acc = 0.0f;
+            for (uint32_t d = 0; d < hd; ++d) acc = __fmaf_rn(qs[d], k_value(at, ng, t % OPURE_PAGE_SIZE, d), acc);
+            s = __fmul_rn(acc, p.scale);
+        }
+        const float mx = fmaxf(m, wave_max64(s));          // a NaN score leaves the maximum and reaches the sum
+        const float ms = mx == NEG_INF ? 0.0f : mx;
+        const float a = expf_ref(__fsub_rn(m, ms)), e = in ? expf_ref(__fsub_rn(s, ms)) : 0.0f;
+        m = mx;
+        l = __fmaf_rn(l, a, wave_sum64(e));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = __fmul_rn(o[i], a);
+        uint64_t left = __ballot(in && pg >= 0);
+        while (left)
+        {
+            const int k = __builtin_ctzll(left);
+            left &= left - 1u;
+            const float w = __shfl(e, k);
+            const uint32_t pk = static_cast<uint32_t>(__shfl(pg, k)), tk = t0 + static_cast<uint32_t>(k);
+            const uint8_t* at = pool + block_at(p.layer, p.n_pages, pk, p.n_kv, kh, ng);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+            {
+                const uint32_t d = lane + 64u * i;
+                if (d < hd) o[i] = __fmaf_rn(w, v_value(at, ng, tk % OPURE_PAGE_SIZE, d), o[i]);
+            }
+        }
+    }
+}
+
+// A workgroup takes a part of the tiles that a sequence's rows see, for 16 NT query
+// rows of a KV head (row qi = j group + head), a wave every fourth tile of 32
+// positions with a running maximum, sum and output of its own in registers.  Lane
+// (r, g) holds scores of query row r and the tokens 4 g .. 4 g + 3 of both pages,
+// which is its operand P^T in the order that the V codes have.  Each tile's words are
+// asked for when the last one's are used up.  The four waves are merged in LDS, the
+// parts by k_kv4_join.
+template <int AF, int HD, int NT, bool ONCE>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 2 ? 2 : 1))) void k_kv4_split(WinParams p)
+{
+    typedef Kv4Tile<HD, ONCE> T;
+    constexpr uint32_t TT = 32u, DT = HD / 16u, NG = T::NG, QT = AF == OPURE_A_F32 ? 2u : 1u;
+    constexpr bool REST = AF != OPURE_A_BF16;              // a weight's rounding rest counts: bf16 results are rounded 2^3 more coarsely than a weight
+    extern __shared__ __align__(16) uint8_t lds[];
+    f4_t* cacc = reinterpret_cast<f4_t*>(lds);                            // [wave][DT][NT][64]
+    float* cml = reinterpret_cast<float*>(lds + 4u * DT * NT * 64u * 16u);   // [wave][NT][16][2]
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, g = lane >> 4, r = lane & 15u;
+    const uint32_t G = p.n_heads / p.n_kv, Gq = G * p.rows;
+    // KV heads next to each other, then parts, blocks and sequences
+    const uint32_t kh = blockIdx.x % p.n_kv, rest = blockIdx.x / p.n_kv, part = rest % p.parts;
+    const uint32_t b = rest / p.parts / p.blocks, blk = rest / p.parts - b * p.blocks, q0 = blk * 16u * NT;
+    const int32_t* pt = p.page_table + static_cast<uint64_t>(b) * p.max_pages;
+    const int32_t len = p.seq_len[b];
+    const WinSeq sq = win_seq(p, len);
+    u4v q[NT][QT][NG];
+    uint32_t jr[NT];
+    float c[NT];
+#pragma unroll
+    for (uint32_t n = 0; n < NT; ++n)
+    {
+        const uint32_t qi = min(q0 + 16u * n + r, Gq - 1u);
+        jr[n] = qi / G;
+        c[n] = load_query<AF, HD>(p, (static_cast<uint64_t>(b) * p.rows + jr[n]) * p.n_heads + kh * G + (qi - jr[n] * G), g, q[n]);
+    }
+    const uint32_t j0 = q0 / G, j1 = min(q0 + 16u * NT - 1u, Gq - 1u) / G;    // the block's first and last row
+    const WinSpan span = win_span<TT>(p, sq, sq.ctx + j0, sq.ctx + j1 + 1u);
+    const uint32_t first = static_cast<uint32_t>(static_cast<uint64_t>(span.n) * part / p.parts);
+    const uint32_t last = static_cast<uint32_t>(static_cast<uint64_t>(span.n) * (part + 1u) / p.parts);
+    const uint32_t page_bytes = p.n_kv * (BLOCK * NG);
+    const uint8_t* base = static_cast<const uint8_t*>(p.pool) + block_at(p.layer, p.n_pages, 0u, p.n_kv, kh, NG);
+
+    f4_t o[DT][NT];
+    float m[NT], l[NT];
+#pragma unroll
+    for (uint32_t n = 0; n < NT; ++n)
+    {
+        m[n] = NEG_INF;
+        l[n] = 0.0f;
+#pragma unroll
+        for (uint32_t d = 0; d < DT; ++d) o[d][n] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    // pages of tile i of the list: -1 past the sequence, missing or not in the pool
+    auto entry = [&](uint32_t i) { return pt[min(span.tile(min(i, span.n - 1u)) * 2u + (lane & 1u), p.max_pages - 1u)]; };
+    auto page = [&](int32_t e, uint32_t i, uint32_t which) -> int32_t {
+        const int32_t pg = __builtin_amdgcn_readlane(e, which);
+        return (span.tile(i) * 2u + which) * OPURE_PAGE_SIZE < sq.total && static_cast<uint32_t>(pg) < p.n_pages ? pg : -1;
+    };
+    T tl;
+    uint32_t i = first + wave;
+    if (i < last)
+    {
+        int32_t e = entry(i);
+        int32_t pa = page(e, i, 0u), pb = page(e, i, 1u);
+        auto at = [&](int32_t pg) { return base + static_cast<uint64_t>(pg < 0 ? 0u : static_cast<uint32_t>(pg)) * page_bytes; };
+        tl.load_k(at(pa), at(pb), lane);
+        tl.load_v(at(pa), at(pb), lane);
+        e = entry(i + 4u);
+        while (true)
+        {
+            const uint32_t t0 = span.tile(i) * TT;
+            const bool more = i + 4u < last;
+            const int32_t na = more ? page(e, i + 4u, 0u) : pa, nb = more ? page(e, i + 4u, 1u) : pb;
+            if (more) e = entry(i + 8u);
+            if (pa < 0 || pb < 0)
+            {
+                // positions without a page: NaN keys for the rows that see them
+#pragma unroll
+                for (uint32_t s = 0; s < NG; ++s)
+                {
+                    tl.ks[0][s] = pa < 0 ? 0x7E007E00u : tl.ks[0][s];
+                    tl.ks[1][s] = pb < 0 ? 0x7E007E00u : tl.ks[1][s];
+                }
+            }
+            f4_t acc[2][NT];
+#pragma unroll
+            for (uint32_t x = 0; x < 2; ++x)
+#pragma unroll
+                for (uint32_t n = 0; n < NT; ++n) acc[x][n] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (uint32_t s = 0; s < NG; ++s)
+#pragma unroll
+                for (uint32_t x = 0; x < 2; ++x)
+                {
+                    const u4v k = tl.k(x, s);
+#pragma unroll
+                    for (uint32_t n = 0; n < NT; ++n)
+#pragma unroll
+                        for (uint32_t z = 0; z < QT; ++z) acc[x][n] = mfma(k, q[n][z][s], acc[x][n]);
+                }
+            if (more) tl.load_k(at(na), at(nb), lane);
+            // every row sees every position
+            const bool full = t0 + TT <= min(sq.ctx + j0 + 1u, sq.total) && (t0 + TT <= p.sinks || t0 + p.window > sq.ctx + j1);
+            u4v hi[NT], lo[NT];
+#pragma unroll
+            for (uint32_t n = 0; n < NT; ++n)
+            {
+                float s[8];
+#pragma unroll
+                for (uint32_t y = 0; y < 8; ++y) s[y] = __fmul_rn(acc[y >> 2][n][y & 3u], c[n]);
+                if (!full)
+                {
+                    const WinMask mask(p, sq.ctx + jr[n], sq.total, t0 + 4u * g);
+#pragma unroll
+                    for (uint32_t y = 0; y < 8; ++y) s[y] = mask.sees(static_cast<int32_t>(16u * (y >> 2) + (y & 3u))) ? s[y] : NEG_INF;
+                }
+                float mx = s[0];
+#pragma unroll
+                for (uint32_t y = 1; y < 8; ++y) mx = fmaxf(mx, s[y]);
+                mx = fmaxf(m[n], max_xor32(max_xor16(mx)));
+                const float ms = mx == NEG_INF ? 0.0f : mx, a = __builtin_amdgcn_exp2f(__fsub_rn(m[n], ms)), down = __fsub_rn(ms, P_SHIFT);
+                m[n] = mx;
+                float sum = 0.0f;
+#pragma unroll
+                for (uint32_t y = 0; y < 8; ++y)
+                {
+                    s[y] = __builtin_amdgcn_exp2f(__fsub_rn(s[y], down));
+                    sum += s[y];
+                }
+                l[n] = __fmaf_rn(l[n], a, sum);                // this lane's share of the row's sum
+#pragma unroll
+                for (uint32_t d = 0; d < DT; ++d)
+#pragma unroll
+                    for (uint32_t y = 0; y < 4; ++y) o[d][n][y] = __fmul_rn(o[d][n][y], a);
+#pragma unroll
+                for (uint32_t y = 0; y < 4; ++y)
+                {
+                    hi[n][y] = win_pack<OPURE_A_F16>(s[2 * y], s[2 * y + 1]);
+                    if constexpr (REST)
+                        lo[n][y] = win_pack<OPURE_A_F16>(__fsub_rn(s[2 * y], win_low<OPURE_A_F16>(hi[n][y])), __fsub_rn(s[2 * y + 1], win_high<OPURE_A_F16>(hi[n][y])));
+                }
+            }
+            if (t0 + TT > sq.total || pa < 0 || pb < 0)
+            {
+                // slots past the sequence and pages that are not there hold anything: 0
+#pragma unroll
+                for (uint32_t x = 0; x < 2; ++x)
+                {
+                    const uint32_t t = t0 + 16u * x + 4u * g, n = (x ? pb : pa) < 0 || t >= sq.total ? 0u : min(sq.total - t, 4u);
+                    const uint32_t m0 = n >= 2u ? 0xFFFFFFFFu : n == 1u ? 0xFFFFu : 0u, m1 = n >= 4u ? 0xFFFFFFFFu : n == 3u ? 0xFFFFu : 0u;
+#pragma unroll
+                    for (uint32_t s = 0; s < NG; ++s) tl.vs[x][s] &= u4v{m0, m1, m0, m1};
+                }
+            }
+#pragma unroll
+            for (uint32_t d = 0; d < DT; ++d)
+            {
+                const u4v v = d & 1u ? tl.template v<1>(d >> 1) : tl.template v<0>(d >> 1);
+#pragma unroll
+                for (uint32_t n = 0; n < NT; ++n)
+                {
+                    if constexpr (REST) o[d][n] = mfma(v, lo[n], o[d][n]);
+                    o[d][n] = mfma(v, hi[n], o[d][n]);
+                }
+            }
+            if (!more) break;
+            tl.load_v(at(na), at(nb), lane);
+            pa = na;
+            pb = nb;
+            i += 4u;
+        }
+    }
+    // ---- the waves' results through LDS, merged in wave order: wave w takes
+    //      channel tiles w, w + 4, ... of every block
+#pragma unroll
+    for (uint32_t n = 0; n < NT; ++n)
+    {
+        l[n] = add_xor32(add_xor16(l[n]));
+#pragma unroll
+        for (uint32_t d = 0; d < DT; ++d) cacc[((wave * DT + d) * NT + n) * 64u + lane] = o[d][n];
+        if (g == 0u)
+        {
+            cml[((wave * NT + n) * 16u + r) * 2u] = m[n];
+            cml[((wave * NT + n) * 16u + r) * 2u + 1u] = l[n];
+        }
+    }
+    __syncthreads();
+    const uint64_t pbase = (((static_cast<uint64_t>(b) * p.n_kv + kh) * p.blocks + blk) * p.parts + part) * p.block_rows;
+#pragma unroll
+    for (uint32_t n = 0; n < NT; ++n)
+    {
+        const uint32_t qi = 16u * n + r;                     // of the block
+        float mw[4], w[4], M = NEG_INF, L = 0.0f;
+#pragma unroll
+        for (uint32_t x = 0; x < 4; ++x)
+        {
+            mw[x] = cml[((x * NT + n) * 16u + r) * 2u];
+            M = fmaxf(M, mw[x]);
+        }
+#pragma unroll
+        for (uint32_t x = 0; x < 4; ++x)
+        {
+            w[x] = __builtin_amdgcn_exp2f(__fsub_rn(mw[x], M == NEG_INF ? 0.0f : M));
+            L = __fmaf_rn(w[x], cml[((x * NT + n) * 16u + r) * 2u + 1u], L);
+        }
+        if (q0 + qi >= Gq) continue;
+        if (wave == 0u && g == 0u)
+        {
+            p.part_ml[(pbase + qi) * 2u] = M;
+            p.part_ml[(pbase + qi) * 2u + 1u] = L;
+        }
+        for (uint32_t d = wave; d < DT; d += 4u)
+        {
+            f4_t acc = cacc[(d * NT + n) * 64u + lane];
+#pragma unroll
+            for (uint32_t y = 0; y < 4; ++y) acc[y] = __fmul_rn(w[0], acc[y]);
+#pragma unroll
+            for (uint32_t x = 1; x < 4; ++x)
+            {
+                const f4_t v = cacc[((x * DT + d) * NT + n) * 64u + lane];
+#pragma unroll
+                for (uint32_t y = 0; y < 4; ++y) acc[y] = __fmaf_rn(w[x], v[y], acc[y]);
+            }
+            *reinterpret_cast<f4_t*>(p.part_acc + (pbase + qi) * HD + 16u * d + 4u * g) = acc;
+        }
+    }
+}
+
+// Joins the parts: a workgroup a query row (WIDE: many parts, a wave every fourth
+// one) or four rows (a wave each); DPL channels a lane.  A row that is not finite is
+// computed again position by position: a NaN among the values of a position that the
+// row does not see meets weight 0 in the products above.
+template <bool WIDE, uint32_t DPL>
+__global__ __launch_bounds__(256) void k_kv4_join(WinParams p)
+{
+    __shared__ float sm[4][256];
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, G = p.n_heads / p.n_kv;
+    const uint32_t shift = p.two ? 5u : 4u;                // a block's query rows
+    const uint32_t id = WIDE ? blockIdx.x : 4u * blockIdx.x + wave;
+    if (id >= p.combine_rows) return;                      // never with WIDE: the barrier below
+    const uint32_t row = id / p.n_heads, head = id - row * p.n_heads, b = row / p.rows, j = row - b * p.rows;
+    const uint32_t kh = head / G, qi = j * G + (head - kh * G), blk = qi >> shift, qb = qi - (blk << shift);
+    const uint32_t parts = p.parts, end = parts - 1u;
+    const uint64_t slot = ((static_cast<uint64_t>(b) * p.n_kv + kh) * p.blocks + blk) * parts;
+    const uint64_t ml = ((slot + min(lane, end)) * p.block_rows + qb) * 2u;
+    const float pm = p.part_ml[ml], pl = p.part_ml[ml + 1u];
+    constexpr uint32_t U = WIDE ? 8u : 4u, BY = WIDE ? 4u : 1u;
+    const uint32_t x0 = WIDE ? wave : 0u;
+    float v[U][DPL], o[DPL];
+    auto fetch = [&](uint32_t x) {
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+            for (uint32_t i = 0; i < DPL; ++i)
+                v[u][i] = p.part_acc[((slot + min(x + BY * u, end)) * p.block_rows + qb) * p.hd + min(lane + 64u * i, p.hd - 1u)];
+    };
+    fetch(x0);
+    const float M = wave_max64(lane < parts ? pm : NEG_INF);
+    const float w = lane < parts ? __builtin_amdgcn_exp2f(__fsub_rn(pm, M == NEG_INF ? 0.0f : M)) : 0.0f;
+    const float L = wave_sum64(lane < parts ? __fmul_rn(w, pl) : 0.0f);
+#pragma unroll
+    for (uint32_t i = 0; i < DPL; ++i) o[i] = 0.0f;
+    for (uint32_t x = x0; x < parts; x += BY * U)
+    {
+        if (x != x0) fetch(x);
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u)
+        {
+            const uint32_t y = x + BY * u;
+            const float wx = y < parts ? __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), min(y, 63u))) : 0.0f;
+#pragma unroll
+            for (uint32_t i = 0; i < DPL; ++i) o[i] = __fmaf_rn(wx, v[u][i], o[i]);
+        }
+    }
+    if constexpr (WIDE)
+    {
+#pragma unroll
+        for (uint32_t i = 0; i < DPL; ++i) sm[wave][lane + 64u * i] = o[i];
+        __syncthreads();
+        if (wave != 0u) return;
+#pragma unroll
+        for (uint32_t i = 0; i < DPL; ++i) o[i] = (sm[0][lane + 64u * i] + sm[1][lane + 64u * i]) + (sm[2][lane + 64u * i] + sm[3][lane + 64u * i]);
+        __builtin_amdgcn_wave_barrier();
+    }
+    bool fine = true;
+#pragma unroll
+    for (uint32_t i = 0; i < DPL; ++i)
+    {
+        o[i] = L == 0.0f ? 0.0f : __fdiv_rn(o[i], L);
+        fine = fine && (__builtin_isfinite(o[i]) || lane + 64u * i >= p.hd);
+    }
+    const uint64_t at = static_cast<uint64_t>(id) * p.hd;
+    if (!__all(fine))
+    {
+        for (uint32_t d = lane; d < p.hd; d += 64u) sm[wave][d] = load_act_rt(p.q, at + d, p.afmt);
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const WinSeq sq = win_seq(p, p.seq_len[b]);
+        float l, x[4];
+        kv4_row(p, sm[wave], b, kh, sq.ctx + j, sq.total, l, x);
+#pragma unroll
+        for (uint32_t i = 0; i < DPL; ++i) o[i] = l == 0.0f ? 0.0f : __fdiv_rn(x[i], l);
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < DPL; ++i)
+        if (lane + 64u * i < p.hd) store_act_rt(p.out, at + lane + 64u * i, o[i], p.afmt);
+}
+
+template <int HD, int NT>
+constexpr uint32_t split_lds() { return 4u * (HD / 16u) * NT * 64u * 16u + 4u * NT * 16u * 2u * 4u; }
+
+// f(kernel, dynamic LDS, workgroups of it that the device holds at a time) for a head size and format.
+// What a CU holds is asked once a kernel: it is the same on every device that the code is built for.
+template <typename F>
+int split_kernel(opure_dev* dev, uint32_t afmt, uint32_t hd, bool two, bool once, F&& f)
+{
+    auto one = [&](auto af, auto h, auto nt, auto alone) {
+        constexpr int AF = decltype(af)::value, HD = decltype(h)::value, NT = decltype(nt)::value;
+        constexpr bool ONCE = decltype(alone)::value;
+        static std::atomic<uint64_t> done{0};
+        static std::atomic<int> a_cu{0};
+        auto* kernel = &k_kv4_split<AF, HD, NT, ONCE>;
+        const int rc = win_lds(dev, reinterpret_cast<const void*>(kernel), split_lds<HD, NT>(), done);
+        if (rc) return rc;
+        int n = a_cu.load(std::memory_order_relaxed);
+        if (n == 0)
+        {
+            OPURE_HIP_TRY(hipOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, 256, split_lds<HD, NT>()));
+            n = std::max(n, 1);
+            a_cu.store(n, std::memory_order_relaxed);
+        }
+        return f(kernel, split_lds<HD, NT>(), static_cast<uint32_t>(n) * (dev->n_cu > 0 ? static_cast<uint32_t>(dev->n_cu) : 256u));
+    };
+    auto by_head = [&](auto af) {
+        return win_by_head(hd, [&](auto h) {
+            if constexpr (decltype(h)::value <= 128)
+            {
+                if (two) return one(af, h, std::integral_constant<int, 2>{}, std::false_type{});
+            }
+            else if (!once) return one(af, h, std::integral_constant<int, 1>{}, std::false_type{});
+            return one(af, h, std::integral_constant<int, 1>{}, std::true_type{});
+        });
+    };
+    return afmt == OPURE_A_F32   ? by_head(std::integral_constant<int, OPURE_A_F32>{})
+           : afmt == OPURE_A_F16 ? by_head(std::integral_constant<int, OPURE_A_F16>{})
+                                 : by_head(std::integral_constant<int, OPURE_A_BF16>{});
+}
+
+// How a call is split, and its workspace.
+struct Kv4Plan {
+    uint32_t tiles = 0, blocks = 0, block_rows = 0, parts = 0;
+    bool two = false;
+    uint64_t acc = 0, ml = 0;                            // bytes
+    uint64_t bytes() const { return acc + ml; }
+};
+
+int kv4_plan(opure_dev* dev, const opure_attn_kv4_args* a, Kv4Plan& w)
+{
+    const opure_model* m = a->model;
+    const uint32_t Gq = m->n_heads / m->n_kv_heads * a->rows;
+    // tiles of any block of rows: its sinks', then the window's and the rows', which begin anywhere in a tile
+    const uint64_t all = (a->max_ctx + 31u) / 32u, window = a->window ? a->window : 0x7FFFFFFFu;
+    w.tiles = static_cast<uint32_t>(std::min<uint64_t>(all, (a->sinks + 31ull) / 32u + (window + a->rows + 30ull) / 32u + 1u));
+    w.two = Gq > 16u && m->head_dim <= 128u;
+    w.blocks = (Gq + (w.two ? 31u : 15u)) / (w.two ? 32u : 16u);
+    w.block_rows = std::min(Gq, w.two ? 32u : 16u);
+    uint32_t room = 0;
+    const int rc = split_kernel(dev, m->afmt, m->head_dim, w.two, w.blocks == 1u, [&](auto, uint32_t, uint32_t n) {
+        room = n;
+        return OPURE_OK;
+    });
+    if (rc) return rc;
+    const uint64_t heads = static_cast<uint64_t>(a->batch) * m->n_kv_heads, groups = heads * w.blocks, rows = heads * Gq;
+    // Parts of a group: as many as the device holds at a time, each of at least four tiles, one a wave
+    const uint32_t least = std::max(4u, w.block_rows / 4u);
+    const uint64_t fill = std::max<uint64_t>(1u, room / groups), more = std::min<uint64_t>(3ull * room / groups, w.tiles / 16u);
+    w.parts = static_cast<uint32_t>(std::min<uint64_t>(std::max(fill, more), std::min((w.tiles + least - 1u) / least, MAX_PARTS)));
+    const uint64_t slots = groups * w.parts * w.block_rows;
+    w.acc = opure_hip::align_up(slots * m->head_dim * 4u, 256);
+    w.ml = opure_hip::align_up(slots * 8u, 256);
+    const uint64_t join = w.parts > 8u ? rows : (rows + 3u) / 4u;
+    // a launch's threads, 256 a workgroup, stay in 32 bits
+    OPURE_REQUIRE(std::max(groups * w.parts, join) < 1u << 24, OPURE_E_CAPACITY,
+                  "4-bit attention: %u x %u rows of %u heads over max_ctx %u: too many workgroups", a->batch, a->rows, m->n_heads, a->max_ctx);
+    return OPURE_OK;
+}
+
+int kv4_validate(const opure_attn_kv4_args* a)
+{
+    OPURE_REQUIRE(a && a->model && a->kv && a->kv->pool && a->kv->page_table, OPURE_E_INVALID, "4-bit attention: null argument, model or cache");
+    const opure_model* m = a->model;
+    const opure_kv* kv = a->kv;
+    OPURE_REQUIRE(m->n_kv_heads >= 1 && m->n_heads >= 1 && m->n_heads % m->n_kv_heads == 0, OPURE_E_INVALID,
+                  "4-bit attention: n_heads %u %% n_kv_heads %u != 0", m->n_heads, m->n_kv_heads);
+    OPURE_REQUIRE(m->head_dim >= 16 && m->head_dim <= 256 && m->head_dim % 16 == 0, OPURE_E_UNSUPPORTED,
+                  "4-bit attention: head_dim %u not in 16..256 step 16", m->head_dim);
+    OPURE_REQUIRE(m->afmt <= OPURE_A_BF16, OPURE_E_INVALID, "4-bit attention: bad activation format");
+    OPURE_REQUIRE(kv->page_size == OPURE_PAGE_SIZE, OPURE_E_UNSUPPORTED, "4-bit attention: page_size must be %d", OPURE_PAGE_SIZE);
+    OPURE_REQUIRE(kv->n_pages >= 1 && kv->max_pages_per_seq >= 1, OPURE_E_INVALID, "4-bit attention: the cache has no pages");
+    OPURE_REQUIRE(a->layer < m->n_layers, OPURE_E_INVALID, "4-bit attention: layer %u of %u", a->layer, m->n_layers);
+    OPURE_REQUIRE(a->batch >= 1 && a->batch <= OPURE_MAX_BATCH_ROWS && a->rows >= 1 && a->rows <= OPURE_MAX_PROMPT_ROWS, OPURE_E_CAPACITY,
+                  "4-bit attention: %u rows x %u sequences outside 1..%d x 1..%d", a->rows, a->batch, OPURE_MAX_PROMPT_ROWS, OPURE_MAX_BATCH_ROWS);
+    // the query rows' indexes stay in 32 bits, and a page's bytes
+    OPURE_REQUIRE(static_cast<uint64_t>(m->n_heads) * a->batch * a->rows <= 1u << 25 && m->n_kv_heads <= 1u << 18, OPURE_E_CAPACITY,
+                  "4-bit attention: %u x %u rows of %u heads", a->batch, a->rows, m->n_heads);
+    const uint64_t slots = static_cast<uint64_t>(kv->max_pages_per_seq) * OPURE_PAGE_SIZE;
+    OPURE_REQUIRE(a->max_ctx >= a->rows && a->max_ctx <= slots && a->max_ctx <= 0x7FFFFFFFu - OPURE_MAX_PROMPT_ROWS, OPURE_E_CAPACITY,
+                  "4-bit attention: max_ctx %u below %u rows or beyond the page table's %llu", a->max_ctx, a->rows, (unsigned long long)slots);
+    OPURE_REQUIRE(a->sinks <= 0x7FFFFFFFu, OPURE_E_INVALID, "4-bit attention: %u sinks", a->sinks);
+    OPURE_REQUIRE((reinterpret_cast<uintptr_t>(kv->pool) & 15u) == 0u && (reinterpret_cast<uintptr_t>(kv->page_table) & 3u) == 0u,
+                  OPURE_E_INVALID, "4-bit attention: pool must be 16-byte aligned, page_table 4-byte");
+    return OPURE_OK;
+}
+
+}  // namespace
+
+using namespace opure_hip;
+
+extern "C" int opure_attn_kv4_reserve(opure_dev* dev, const opure_attn_kv4_args* a)
+{
+    OPURE_REQUIRE(dev, OPURE_E_INVALID, "opure_attn_kv4_reserve: null device");
+    const int rc = kv4_validate(a);
+    if (rc) return rc;
+    const DeviceGuard on(dev);
+    Kv4Plan w;
+    const int rp = kv4_plan(dev, a, w);
+    return rp ? rp : ensure_workspace(dev, w.bytes());
+}
+
+extern "C" int opure_attn_kv4_paged(opure_dev* dev, const opure_attn_kv4_args* a)
+{
+    OPURE_REQUIRE(dev && a && a->q && a->out && a->seq_len, OPURE_E_INVALID, "opure_attn_kv4_paged: null argument");
+    int rc = kv4_validate(a);
+    if (rc) return rc;
+    OPURE_REQUIRE((reinterpret_cast<uintptr_t>(a->q) & 15u) == 0u && (reinterpret_cast<uintptr_t>(a->out) & 7u) == 0u &&
+                      (reinterpret_cast<uintptr_t>(a->seq_len) & 3u) == 0u,
+                  OPURE_E_INVALID, "opure_attn_kv4_paged: q must be 16-byte aligned, out 8-byte, seq_len 4-byte");
+    const opure_model* m = a->model;
+    const uint64_t bytes = static_cast<uint64_t>(a->batch) * a->rows * m->n_heads * m->head_dim * act_bytes(m->afmt);
+    OPURE_REQUIRE(!overlaps(a->out, bytes, a->q, bytes), OPURE_E_INVALID, "opure_attn_kv4_paged: out overlaps q");
+    OPURE_REQUIRE(!overlaps(a->out, bytes, a->kv->pool, kv_pool_bytes(m, OPURE_KV_I4, a->kv->n_pages)) &&
+                      !overlaps(a->out, bytes, a->kv->page_table, static_cast<uint64_t>(a->batch) * a->kv->max_pages_per_seq * 4u) &&
+                      !overlaps(a->out, bytes, a->seq_len, a->batch * 4u), OPURE_E_INVALID, "opure_attn_kv4_paged: out overlaps the cache");
+    // the call's parts go to the workspace, which may also move
+    OPURE_REQUIRE(!overlaps(dev->ws, dev->ws_bytes, a->q, bytes) && !overlaps(dev->ws, dev->ws_bytes, a->out, bytes), OPURE_E_INVALID,
+                  "opure_attn_kv4_paged: q or out in the device's workspace");
+    const DeviceGuard on(dev);
+    Kv4Plan w;
+    rc = kv4_plan(dev, a, w);
+    if (rc) return rc;
+    rc = ensure_workspace(dev, w.bytes());
+    if (rc) return rc;
+    WinParams p{};
+    p.q = a->q;
+    p.out = a->out;
+    p.pool = a->kv->pool;
+    p.page_table = a->kv->page_table;
+    p.seq_len = a->seq_len;
+    p.part_acc = static_cast<float*>(dev->ws);
+    p.part_ml = p.part_acc + w.acc / 4u;
+    p.n_heads = m->n_heads;
+    p.n_kv = m->n_kv_heads;
+    p.hd = m->head_dim;
+    p.rows = a->rows;
+    p.n_pages = a->kv->n_pages;
+    p.max_pages = a->kv->max_pages_per_seq;
+    p.layer = a->layer;
+    p.afmt = m->afmt;
+    p.window = a->window == 0u || a->window > 0x7FFFFFFFu ? 0x7FFFFFFFu : a->window;
+    p.sinks = a->sinks;
+    p.cap = a->max_ctx;
+    p.scale = m->attn_scale;
+    p.err = dev->err;
+    p.parts = w.parts;
+    p.blocks = w.blocks;
+    p.block_rows = w.block_rows;
+    p.two = w.two ? 1u : 0u;
+    p.tiles = w.tiles;
+    p.combine_rows = a->batch * a->rows * p.n_heads;
+    const uint32_t wgs = p.n_kv * w.parts * w.blocks * a->batch;
+    rc = split_kernel(dev, p.afmt, p.hd, w.two, w.blocks == 1u, [&](auto kernel, uint32_t lds, uint32_t) {
+        OPURE_LAUNCH(dev, kernel, dim3(wgs), dim3(256), lds, p);
+        OPURE_LAUNCH_CHECK("k_kv4_split");
+        return OPURE_OK;
+    });
+    if (rc) return rc;
+    const bool wide = w.parts > 8u;
+    p.combine_wgs = wide ? p.combine_rows : (p.combine_rows + 3u) / 4u;
+    auto join = [&](auto all) {
+        constexpr bool WIDE = decltype(all)::value;
+        const dim3 grid(p.combine_wgs), block(256);
+        switch ((p.hd + 63u) / 64u)
+        {
+        case 1: OPURE_LAUNCH(dev, (k_kv4_join<WIDE, 1>), grid, block, 0, p); break;
+        case 2: OPURE_LAUNCH(dev, (k_kv4_join<WIDE, 2>), grid, block, 0, p); break;
+        case 3: OPURE_LAUNCH(dev, (k_kv4_join<WIDE, 3>), grid, block, 0, p); break;
+        default: OPURE_LAUNCH(dev, (k_kv4_join<WIDE, 4>), grid, block, 0, p); break;
+        }
+    };
+    if (wide) join(std::true_type{});
+    else join(std::false_type{});
+    OPURE_LAUNCH_CHECK("k_kv4_join");
+    return OPURE_OK;
+}

@@ -19,6 +19,8 @@ OK, E_INVALID, E_NODEVICE, E_HIP, E_OOM, E_UNSUPPORTED, E_CAPACITY, E_DEVICE = 0
 MAX_ROWS, PAGE_SIZE = 16, 16
 W_F32, W_I8PC, W_I4G128 = 0, 1, 2
 A_F32, A_F16, A_BF16 = 0, 1, 2
+KV_ACT, KV_I4 = 0, 1
+MAX_TOP, MAX_LOGPROB_ROWS = 64, 65535
 ROPE_GPU, ROPE_CPUREF = 0, 1
 EPI_STORE, EPI_RESIDUAL, EPI_SWIGLU = 0, 1, 2
 STAGES = ("embed", "qkv", "attention", "o_proj", "gate_up", "down", "lm_head", "accept")
@@ -79,6 +81,27 @@ class AttnWindowArgs(C.Structure):
                 ("max_ctx", C.c_uint32), ("window", C.c_uint32), ("sinks", C.c_uint32), ("q", C.c_void_p),
                 ("out", C.c_void_p), ("weights", C.c_void_p), ("weights_stride", C.c_uint32),
                 ("weights_batch_stride", C.c_uint64)]
+
+
+class KvAppendArgs(C.Structure):
+    _fields_ = [("model", C.POINTER(Model)), ("kv", C.POINTER(KV)), ("kvfmt", C.c_uint32), ("layer", C.c_uint32),
+                ("batch", C.c_uint32), ("rows", C.c_uint32), ("seq_len", C.c_void_p), ("max_ctx", C.c_uint32),
+                ("row_count", C.c_void_p), ("rotate", C.c_uint32), ("xfmt", C.c_uint32), ("q", C.c_void_p),
+                ("k", C.c_void_p), ("v", C.c_void_p), ("q_stride", C.c_uint32), ("k_stride", C.c_uint32),
+                ("v_stride", C.c_uint32), ("q_out", C.c_void_p)]
+
+
+class AttnKv4Args(C.Structure):
+    _fields_ = [("model", C.POINTER(Model)), ("kv", C.POINTER(KV)), ("layer", C.c_uint32),
+                ("batch", C.c_uint32), ("rows", C.c_uint32), ("seq_len", C.c_void_p),
+                ("max_ctx", C.c_uint32), ("window", C.c_uint32), ("sinks", C.c_uint32), ("q", C.c_void_p),
+                ("out", C.c_void_p)]
+
+
+class LogprobsArgs(C.Structure):
+    _fields_ = [("rows", C.c_uint32), ("vocab", C.c_uint32), ("logits", C.c_void_p), ("logits_stride", C.c_uint32),
+                ("temperature", C.c_float), ("tokens", C.c_void_p), ("logprob", C.c_void_p), ("entropy", C.c_void_p),
+                ("top", C.c_uint32), ("top_tokens", C.c_void_p), ("top_logprobs", C.c_void_p)]
 
 
 class AcceptArgs(C.Structure):
@@ -168,6 +191,12 @@ def _declare(L):
         "opure_attn_decode_paged": ([vp, C.POINTER(AttnArgs)], i),
         "opure_attn_window_reserve": ([vp, C.POINTER(AttnWindowArgs)], i),
         "opure_attn_window_paged": ([vp, C.POINTER(AttnWindowArgs)], i),
+        "opure_kv_append": ([vp, C.POINTER(KvAppendArgs)], i),
+        "opure_kv_pool_bytes": ([C.POINTER(Model), u32, u32, C.POINTER(u64)], i),
+        "opure_attn_kv4_reserve": ([vp, C.POINTER(AttnKv4Args)], i),
+        "opure_attn_kv4_paged": ([vp, C.POINTER(AttnKv4Args)], i),
+        "opure_logprobs_reserve": ([vp, C.POINTER(LogprobsArgs)], i),
+        "opure_logprobs": ([vp, C.POINTER(LogprobsArgs)], i),
         "opure_accept_greedy": ([vp, C.POINTER(AcceptArgs)], i),
         "opure_accept_rejection": ([vp, C.POINTER(AcceptArgs)], i),
         "opure_accept_rejection_noalloc": ([vp, C.POINTER(AcceptArgs)], i),
