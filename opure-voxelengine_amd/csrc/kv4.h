@@ -46,14 +46,22 @@ __device__ __forceinline__ uint64_t block_at(uint32_t layer, uint32_t n_pages, u
 
 __device__ __forceinline__ uint32_t half_bits(_Float16 v) { return __builtin_bit_cast(uint16_t, v); }
 
+// A number that is rounded to fp32 before it is rounded to fp16: the compiler would
+// make one instruction of a product and its conversion, which rounds once.
+__device__ __forceinline__ _Float16 round_half(float v)
+{
+    asm volatile("" : "+v"(v));
+    return static_cast<_Float16>(v);
+}
+
 // A group's scale and base from its smallest and largest value.
 struct Scale {
     _Float16 s, b;
     bool bad;
     __device__ __forceinline__ Scale(float lo, float hi, bool nonfinite) : bad(nonfinite)
     {
-        s = static_cast<_Float16>(__fmul_rn(__fsub_rn(hi, lo), static_cast<float>(1.0 / 15.0)));
-        b = static_cast<_Float16>(__fsub_rn(lo, __fmul_rn(16.0f, static_cast<float>(s))));
+        s = round_half(__fmul_rn(__fsub_rn(hi, lo), static_cast<float>(1.0 / 15.0)));
+        b = round_half(__fsub_rn(lo, __fmul_rn(16.0f, static_cast<float>(s))));
     }
     __device__ __forceinline__ uint32_t code(float x) const
     {

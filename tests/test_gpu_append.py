@@ -233,6 +233,27 @@ def test_extremes(dev, i4):
         check(dev, afmt, xfmt, i4, 4, 2, 64, [10], 12, seed=8, edit=edit, rotate=False)
 
 
+def test_scales_between_two_halves(dev):
+    """Ranges whose fifteenth is, rounded to fp32, half way between two fp16 numbers, and is not without that rounding."""
+    say("ties")
+    r = np.random.default_rng(11).uniform(1, 2, 1 << 21).astype(np.float32)
+    f = np.float32(1.0 / 15.0)
+    p = r * f
+    tie = ((p.view(np.uint32) & 0x1FFF) == 0x1000) & (r.astype(np.float64) * np.float64(f) != p)
+    r = r[tie][:160]
+    assert len(r) == 160
+
+    def edit(x):
+        # a group of 32: 0, the range, and numbers between them
+        for which in (1, 2):
+            g = x[:, 128 * which:128 * which + 128].reshape(20, 4, 32)
+            top = r.reshape(2, 20, 4)[which - 1]
+            g[...] = np.abs(g) % 1 * top[..., None]
+            g[..., 3], g[..., 17] = 0, top
+
+    check(dev, BF16, F32, True, 1, 1, 128, [5], 20, seed=3, rotate=False, edit=edit)
+
+
 @pytest.mark.parametrize("spread,offset", [(1.0, 0.0), (30.0, 0.0), (1.0, 40.0), (1e-3, 0.0)])
 def test_error_of_4_bits(dev, spread, offset):
     """A value is off by half a scale, half a step of fp16 in the scale (times 31) and in base and one in the value."""
