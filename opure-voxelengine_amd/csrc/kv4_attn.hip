@@ -108,38 +108,57 @@ __device__ __forceinline__ f4_t mfma(u4v a, u4v b, f4_t c)
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
 }
 
+// A number worked out from all results of a run of matrix instructions, in the block
+// that asked for them: whoever reads them behind a branch finds them written.  (The
+// compiler spaces a read and its matrix instruction by the longest way through the
+// blocks between them, and a short way then reads what was there before.)
+__device__ __forceinline__ float settled(float v)
+{
+    asm volatile("" : "+v"(v));
+    return v;
+}
+// The same after a loop of them: as many clocks as the longest takes.
+__device__ __forceinline__ void settle()
+{
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 15");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 // A query row in fp16: of an fp16 model as it is, else times the power of two that
 // puts its largest magnitude just below 2^9 (bf16's 8 bits fit, and what fp16 cannot
 // hold of its small numbers is 2^-34 of the largest); an fp32 row is the sum of two.
-// Returns the factor of its scores in powers of two.
-template <int AF, int HD>
-__device__ __forceinline__ float load_query(const WinParams& p, uint64_t row, uint32_t g, u4v (&q)[AF == OPURE_A_F32 ? 2 : 1][groups(HD)])
+// A lane takes 8 channels of each step of W = 8 PARTS channels, the `part`-th.  Returns
+// the factor of its scores in powers of two.
+template <int AF, int HD, uint32_t PARTS>
+__device__ __forceinline__ float load_query(const WinParams& p, uint64_t row, uint32_t part,
+                                            u4v (&q)[AF == OPURE_A_F32 ? 2 : 1][(HD + 8u * PARTS - 1u) / (8u * PARTS)])
 {
-    constexpr uint32_t NG = groups(HD);
-    constexpr bool HALF = HD % 32 != 0;
+    constexpr uint32_t W = 8u * PARTS, STEPS = (HD + W - 1u) / W;
     const float c = __fmul_rn(p.scale, LOG2E);
+    auto there = [&](uint32_t s) { return (s + 1u) * W <= HD || s * W + 8u * part < HD; };
     if constexpr (AF == OPURE_A_F16)
     {
-        const uint8_t* at = static_cast<const uint8_t*>(p.q) + row * (HD * 2u) + 16u * g;
+        const uint8_t* at = static_cast<const uint8_t*>(p.q) + row * (HD * 2u) + 16u * part;
 #pragma unroll
-        for (uint32_t s = 0; s < NG; ++s) q[0][s] = HALF && s + 1u == NG && g >= 2u ? u4v{0u, 0u, 0u, 0u} : *reinterpret_cast<const u4v*>(at + 64u * s);
+        for (uint32_t s = 0; s < STEPS; ++s) q[0][s] = there(s) ? *reinterpret_cast<const u4v*>(at + 2u * W * s) : u4v{0u, 0u, 0u, 0u};
         return c;
     }
     else
     {
-        float x[NG][8], top = 0.0f;
+        float x[STEPS][8], top = 0.0f;
 #pragma unroll
-        for (uint32_t s = 0; s < NG; ++s)
+        for (uint32_t s = 0; s < STEPS; ++s)
 #pragma unroll
             for (uint32_t i = 0; i < 8; ++i)
             {
-                const bool there = !(HALF && s + 1u == NG && g >= 2u);
-                x[s][i] = there ? load_act<AF>(p.q, row * HD + 32u * s + 8u * g + i) : 0.0f;
+                x[s][i] = there(s) ? load_act<AF>(p.q, row * HD + W * s + 8u * part + i) : 0.0f;
                 top = fmaxf(top, __builtin_isfinite(x[s][i]) ? __builtin_fabsf(x[s][i]) : 0.0f);
             }
-        const int e = __builtin_amdgcn_frexp_expf(max_xor32(max_xor16(top))) - 9;
+        if constexpr (PARTS == 4u) top = max_xor16(top);
+        const int e = __builtin_amdgcn_frexp_expf(max_xor32(top)) - 9;
 #pragma unroll
-        for (uint32_t s = 0; s < NG; ++s)
+        for (uint32_t s = 0; s < STEPS; ++s)
 #pragma unroll
             for (uint32_t i = 0; i < 4; ++i)
             {
@@ -239,7 +258,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 2 ? 2
     {
         const uint32_t qi = min(q0 + 16u * n + r, Gq - 1u);
         jr[n] = qi / G;
-        c[n] = load_query<AF, HD>(p, (static_cast<uint64_t>(b) * p.rows + jr[n]) * p.n_heads + kh * G + (qi - jr[n] * G), g, q[n]);
+        c[n] = load_query<AF, HD, 4>(p, (static_cast<uint64_t>(b) * p.rows + jr[n]) * p.n_heads + kh * G + (qi - jr[n] * G), g, q[n]);
     }
     const uint32_t j0 = q0 / G, j1 = min(q0 + 16u * NT - 1u, Gq - 1u) / G;    // the block's first and last row
     const WinSpan span = win_span<TT>(p, sq, sq.ctx + j0, sq.ctx + j1 + 1u);
@@ -316,15 +335,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 2 ? 2
                 float s[8];
 #pragma unroll
                 for (uint32_t y = 0; y < 8; ++y) s[y] = __fmul_rn(acc[y >> 2][n][y & 3u], c[n]);
+                auto largest = [&]() {
+                    float v = s[0];
+#pragma unroll
+                    for (uint32_t y = 1; y < 8; ++y) v = fmaxf(v, s[y]);
+                    return v;
+                };
+                float mx = settled(largest());
                 if (!full)
                 {
                     const WinMask mask(p, sq.ctx + jr[n], sq.total, t0 + 4u * g);
 #pragma unroll
                     for (uint32_t y = 0; y < 8; ++y) s[y] = mask.sees(static_cast<int32_t>(16u * (y >> 2) + (y & 3u))) ? s[y] : NEG_INF;
+                    mx = largest();
                 }
-                float mx = s[0];
-#pragma unroll
-                for (uint32_t y = 1; y < 8; ++y) mx = fmaxf(mx, s[y]);
                 mx = fmaxf(m[n], max_xor32(max_xor16(mx)));
                 const float ms = mx == NEG_INF ? 0.0f : mx, a = __builtin_amdgcn_exp2f(__fsub_rn(m[n], ms)), down = __fsub_rn(ms, P_SHIFT);
                 m[n] = mx;
@@ -378,6 +402,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 2 ? 2
             i += 4u;
         }
     }
+    settle();
     // ---- the waves' results through LDS, merged in wave order: wave w takes
     //      channel tiles w, w + 4, ... of every block
 #pragma unroll
@@ -443,7 +468,7 @@ __global__ __launch_bounds__(256) void k_kv4_join(WinParams p)
 {
     __shared__ float sm[4][256];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, G = p.n_heads / p.n_kv;
-    const uint32_t shift = p.two ? 5u : 4u;                // a block's query rows
+    const uint32_t shift = p.two == 2u ? 7u : p.two ? 5u : 4u;   // a block's query rows
     const uint32_t id = WIDE ? blockIdx.x : 4u * blockIdx.x + wave;
     if (id >= p.combine_rows) return;                      // never with WIDE: the barrier below
     const uint32_t row = id / p.n_heads, head = id - row * p.n_heads, b = row / p.rows, j = row - b * p.rows;
@@ -514,6 +539,293 @@ __global__ __launch_bounds__(256) void k_kv4_join(WinParams p)
         if (lane + 64u * i < p.hd) store_act_rt(p.out, at + lane + 64u * i, o[i], p.afmt);
 }
 
+// ---- many query rows -----------------------------------------------------------
+
+typedef float f16_t __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ f16_t mfma_32(u4v a, u4v b, f16_t c)
+{
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, a), __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
+}
+
+template <int HD>
+constexpr uint32_t rows_pages() { return HD <= 128 ? 4u : 2u; }          // pages a tile
+template <int HD>
+constexpr uint32_t rows_stage() { return rows_pages<HD>() * (HD / 16u * 512u + groups(HD) * 1024u); }   // bytes of a tile's values in LDS
+template <int HD>
+constexpr uint32_t rows_lds() { return 2u * rows_stage<HD>(); }
+constexpr uint32_t ROWS_BLOCK = 128;
+constexpr float ROWS_SHIFT = 12.0f, ROWS_LAG = 3.0f;
+
+// A workgroup takes 128 query rows (qi = j group + head) of a KV head, 32 a wave, over
+// tiles of four pages (two past 128 channels) whose values the waves make from the codes
+// once, each its page's, and share in LDS as operands: products are 32x32x16, S^T = K Q^T
+// and O^T = V^T P^T.  A lane (q = lane % 32, h = lane / 32) holds of a page's scores the
+// tokens 4 h .. 4 h + 3 and 8 + 4 h .. 11 + 4 h of row q, its operand P^T, and V of a
+// page lies in LDS in that order of tokens.  Two stages: while one tile is computed the
+// next one's words are on their way.
+//   A row's output is scaled to a new maximum only where that passes the old one by 2^3;
+// weights are held 2^12 higher, so the largest stays in fp16.
+template <int AF, int HD>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 128 ? 2 : 1))) void k_kv4_rows(WinParams p)
+{
+    constexpr uint32_t NG = groups(HD), KS = HD / 16u, NP = rows_pages<HD>(), TT = 16u * NP, QT = AF == OPURE_A_F32 ? 2u : 1u;
+    constexpr bool REST = AF != OPURE_A_BF16, SPLIT = NP == 2u;          // two pages: two waves make K, two V
+    extern __shared__ __align__(16) uint8_t lds[];
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, h = lane >> 5, r = lane & 31u;
+    const uint32_t G = p.n_heads / p.n_kv, Gq = G * p.rows;
+    const uint32_t kh = blockIdx.x % p.n_kv, rest = blockIdx.x / p.n_kv, part = rest % p.parts, b = rest / p.parts / p.blocks;
+    const uint32_t blk = p.blocks - 1u - (rest / p.parts - b * p.blocks), q0 = blk * ROWS_BLOCK;    // the rows that see most first
+    const int32_t* pt = p.page_table + static_cast<uint64_t>(b) * p.max_pages;
+    const WinSeq sq = win_seq(p, p.seq_len[b]);
+    const uint32_t j0 = q0 / G, j1 = min(q0 + ROWS_BLOCK - 1u, Gq - 1u) / G;
+    const WinSpan span = win_span<TT>(p, sq, sq.ctx + j0, sq.ctx + j1 + 1u);
+    const uint32_t first = static_cast<uint32_t>(static_cast<uint64_t>(span.n) * part / p.parts);
+    const uint32_t last = static_cast<uint32_t>(static_cast<uint64_t>(span.n) * (part + 1u) / p.parts);
+    // the wave's rows
+    const uint32_t w0 = min(q0 + 32u * wave, Gq - 1u), w1 = min(q0 + 32u * wave + 31u, Gq - 1u), qi = min(w0 + r, Gq - 1u);
+    const uint32_t j = qi / G, pos = sq.ctx + j, pos0 = sq.ctx + w0 / G, pos1 = sq.ctx + w1 / G;
+    const uint64_t row = (static_cast<uint64_t>(b) * p.rows + j) * p.n_heads + kh * G + (qi - j * G);
+    // scores in powers of two are c times the products: its sign goes to the query
+    u4v q[QT][KS];
+    const float c = __builtin_fabsf(load_query<AF, HD, 2>(p, row, h, q));
+    if (p.scale < 0.0f)
+#pragma unroll
+        for (uint32_t z = 0; z < QT; ++z)
+#pragma unroll
+            for (uint32_t s = 0; s < KS; ++s) q[z][s] ^= u4v{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
+    const uint32_t page_bytes = p.n_kv * (BLOCK * NG);
+    const uint8_t* base = static_cast<const uint8_t*>(p.pool) + block_at(p.layer, p.n_pages, 0u, p.n_kv, kh, NG);
+
+    // ---- a tile's codes to values: wave w has page w (of two: page w % 2, K or V)
+    const uint32_t mine = SPLIT ? wave & 1u : wave;
+    const bool has_k = !SPLIT || wave < 2u, has_v = !SPLIT || wave >= 2u;
+    uint32_t kw[NG], ks[NG], vw[NG];
+    u4v vs[NG];
+    int32_t pg = -1, e = -1;                               // the page, and the next one's entry
+    auto entry = [&](uint32_t i) { e = pt[min(span.tile(min(i, span.n - 1u)) * NP + mine, p.max_pages - 1u)]; };
+    auto fetch = [&](uint32_t i) {
+        const uint32_t col = span.tile(i) * NP + mine;
+        pg = __builtin_amdgcn_readfirstlane(col * OPURE_PAGE_SIZE < sq.total && static_cast<uint32_t>(e) < p.n_pages ? e : -1);
+        const uint8_t* at = base + static_cast<uint64_t>(pg < 0 ? 0u : static_cast<uint32_t>(pg)) * page_bytes;
+        if (has_k)
+        {
+            load_words<NG, false>(reinterpret_cast<const uint32_t*>(at) + lane * NG, kw);
+            load_words<NG, false>(reinterpret_cast<const uint32_t*>(at + k_scales(NG)) + (lane & 15u) * NG, ks);
+        }
+        if (has_v)
+        {
+            load_words<NG, false>(reinterpret_cast<const uint32_t*>(at + v_codes(NG)) + lane * NG, vw);
+#pragma unroll
+            for (uint32_t g = 0; g < NG; ++g) vs[g] = win_load<false>(at + v_scales(NG) + ((lane >> 4) * NG + g) * 16u);
+        }
+    };
+    // K of two pages: [step of 16 channels][lane 32 h + 16 (page of two) + token]; V of a page: [32 channels][lane 32 h + channel]
+    auto k_at = [&](uint32_t stage, uint32_t pair, uint32_t s) {
+        return reinterpret_cast<u4v*>(lds + stage * rows_stage<HD>() + (pair * KS + s) * 1024u);
+    };
+    auto v_at = [&](uint32_t stage, uint32_t page, uint32_t g) {
+        return reinterpret_cast<u4v*>(lds + stage * rows_stage<HD>() + NP * KS * 512u + (page * NG + g) * 1024u);
+    };
+    auto store = [&](uint32_t i) {
+        const uint32_t stage = i & 1u, t0 = span.tile(i) * TT + 16u * mine;
+        if (has_k)
+        {
+            const uint32_t to = (lane >> 4 & 1u) * 32u + (mine & 1u) * 16u + (lane & 15u);
+#pragma unroll
+            for (uint32_t g = 0; g < NG; ++g)
+            {
+                // positions without a page: NaN keys for the rows that see them
+                const half2_t sb = pair(pg < 0 ? 0x7E007E00u : ks[g]), sc = {sb[0], sb[0]}, ba = {sb[1], sb[1]};
+                const u4v k = {values(codes<0>(kw[g]), sc, ba), values(codes<1>(kw[g]), sc, ba), values(codes<2>(kw[g]), sc, ba), values(codes<3>(kw[g]), sc, ba)};
+                if (HD % 32 == 0 || g + 1u < NG || lane < 32u) k_at(stage, mine >> 1, 2u * g + (lane >> 5))[to] = k;
+            }
+        }
+        if (has_v)
+        {
+            const uint32_t x = lane >> 4, t = t0 + 4u * x, n = pg < 0 || t >= sq.total ? 0u : min(sq.total - t, 4u);
+            const uint32_t m0 = n >= 2u ? 0xFFFFFFFFu : n == 1u ? 0xFFFFu : 0u, m1 = n >= 4u ? 0xFFFFFFFFu : n == 3u ? 0xFFFFu : 0u;
+#pragma unroll
+            for (uint32_t g = 0; g < NG; ++g)
+            {
+                // slots past the sequence and pages that are not there hold anything: 0
+                const half2_t s0 = pair(vs[g][0] & m0), s1 = pair(vs[g][1] & m1), b0 = pair(vs[g][2] & m0), b1 = pair(vs[g][3] & m1);
+                u2v* to = reinterpret_cast<u2v*>(v_at(stage, mine, g) + (x & 1u) * 32u + (lane & 15u)) + (x >> 1);
+                to[0] = u2v{values(codes<0>(vw[g]), s0, b0), values(codes<1>(vw[g]), s1, b1)};
+                to[32] = u2v{values(codes<2>(vw[g]), s0, b0), values(codes<3>(vw[g]), s1, b1)};   // 16 channels on
+            }
+        }
+    };
+
+    f16_t o[NG];
+    float m = NEG_INF, l = 0.0f;                            // the maximum in units of the products; this lane's share of the sum
+#pragma unroll
+    for (uint32_t g = 0; g < NG; ++g)
+#pragma unroll
+        for (uint32_t y = 0; y < 16; ++y) o[g][y] = 0.0f;
+    if (first < last)
+    {
+        entry(first);
+        fetch(first);
+        entry(first + 1u);
+        store(first);
+    }
+    __syncthreads();
+    for (uint32_t i = first; i < last; ++i)
+    {
+        const uint32_t stage = i & 1u, t0 = span.tile(i) * TT;
+        const bool more = i + 1u < last;
+        if (more) fetch(i + 1u);
+        entry(i + 2u);
+        // a tile that none of the wave's rows sees is left out
+        const bool none = t0 > pos1 || (t0 >= p.sinks && static_cast<uint64_t>(t0) + TT - 1u + p.window <= pos0);
+        if (!none)
+        {
+            f16_t s[NP / 2u];
+#pragma unroll
+            for (uint32_t x = 0; x < NP / 2u; ++x)
+            {
+#pragma unroll
+                for (uint32_t y = 0; y < 16; ++y) s[x][y] = 0.0f;
+#pragma unroll
+                for (uint32_t d = 0; d < KS; ++d)
+                {
+                    const u4v k = k_at(stage, x, d)[lane];
+#pragma unroll
+                    for (uint32_t z = 0; z < QT; ++z) s[x] = mfma_32(k, q[z][d], s[x]);
+                }
+            }
+            auto largest = [&]() {
+                float v = s[0][0];
+#pragma unroll
+                for (uint32_t x = 0; x < NP / 2u; ++x)
+#pragma unroll
+                    for (uint32_t y = 0; y < 16; ++y) v = fmaxf(v, s[x][y]);
+                return v;
+            };
+            float mx = settled(largest());
+            // every row of the wave sees every position
+            const bool full = t0 + TT <= min(pos0 + 1u, sq.total) && (t0 + TT <= p.sinks || t0 + p.window > pos1);
+            if (!full)
+            {
+                const WinMask mask(p, pos, sq.total, t0 + 4u * h);
+#pragma unroll
+                for (uint32_t x = 0; x < NP / 2u; ++x)
+#pragma unroll
+                    for (uint32_t y = 0; y < 16; ++y) s[x][y] = mask.sees(static_cast<int32_t>(32u * x + 8u * (y >> 2) + (y & 3u))) ? s[x][y] : NEG_INF;
+                mx = largest();
+            }
+            mx = max_xor32(mx);
+            const bool grown = m == NEG_INF ? mx > NEG_INF : __fmul_rn(__fsub_rn(mx, m), c) > ROWS_LAG;
+            if (__any(grown))
+            {
+                const float to = grown ? mx : m, a = m == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(__fmul_rn(__fsub_rn(m, to), c));
+                m = to;
+                l = __fmul_rn(l, a);
+#pragma unroll
+                for (uint32_t g = 0; g < NG; ++g)
+#pragma unroll
+                    for (uint32_t y = 0; y < 16; ++y) o[g][y] = __fmul_rn(o[g][y], a);
+            }
+            const float down = m == NEG_INF ? 0.0f : __fsub_rn(ROWS_SHIFT, __fmul_rn(m, c));
+#pragma unroll
+            for (uint32_t x = 0; x < NP; ++x)
+            {
+                // a page: 8 scores
+                u4v hi, lo;
+                float e[8];
+#pragma unroll
+                for (uint32_t y = 0; y < 8; ++y)
+                {
+                    e[y] = __builtin_amdgcn_exp2f(__fmaf_rn(s[x >> 1][8u * (x & 1u) + y], c, down));
+                    l += e[y];
+                }
+#pragma unroll
+                for (uint32_t y = 0; y < 4; ++y)
+                {
+                    hi[y] = win_pack<OPURE_A_F16>(e[2 * y], e[2 * y + 1]);
+                    if constexpr (REST)
+                        lo[y] = win_pack<OPURE_A_F16>(__fsub_rn(e[2 * y], win_low<OPURE_A_F16>(hi[y])), __fsub_rn(e[2 * y + 1], win_high<OPURE_A_F16>(hi[y])));
+                }
+#pragma unroll
+                for (uint32_t g = 0; g < NG; ++g)
+                {
+                    const u4v v = v_at(stage, x, g)[lane];
+                    if constexpr (REST) o[g] = mfma_32(v, lo, o[g]);
+                    o[g] = mfma_32(v, hi, o[g]);
+                }
+            }
+        }
+        if (more) store(i + 1u);
+        __syncthreads();
+    }
+    settle();
+    l = add_xor32(l);
+    const bool there = q0 + 32u * wave + r < Gq;
+    if (p.parts > 1u)
+    {
+        const uint64_t at = ((((static_cast<uint64_t>(b) * p.n_kv + kh) * p.blocks + blk) * p.parts + part) * p.block_rows) + 32u * wave + r;
+        if (!there) return;
+        if (h == 0u)
+        {
+            // the join takes maxima in powers of two
+            p.part_ml[at * 2u] = m == NEG_INF ? NEG_INF : __fmul_rn(m, c);
+            p.part_ml[at * 2u + 1u] = l;
+        }
+#pragma unroll
+        for (uint32_t g = 0; g < NG; ++g)
+#pragma unroll
+            for (uint32_t y = 0; y < 4; ++y)
+                if (32u * g + 8u * y < HD)
+                    *reinterpret_cast<f4_t*>(p.part_acc + at * HD + 32u * g + 8u * y + 4u * h) = f4_t{o[g][4 * y], o[g][4 * y + 1], o[g][4 * y + 2], o[g][4 * y + 3]};
+        return;
+    }
+    bool fine = true;
+    const float by = l == 0.0f ? 0.0f : __fdiv_rn(1.0f, l);
+    uint8_t* out = static_cast<uint8_t*>(p.out) + row * HD * (AF == OPURE_A_F32 ? 4u : 2u);
+#pragma unroll
+    for (uint32_t g = 0; g < NG; ++g)
+#pragma unroll
+        for (uint32_t y = 0; y < 4; ++y)
+        {
+            if (32u * g + 8u * y >= HD) continue;
+            const uint32_t d = 32u * g + 8u * y + 4u * h;
+            float v[4];
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e)
+            {
+                v[e] = l == 0.0f ? 0.0f : AF == OPURE_A_F32 ? __fdiv_rn(o[g][4 * y + e], l) : __fmul_rn(o[g][4 * y + e], by);
+                fine = fine && __builtin_isfinite(v[e]);
+            }
+            if (!there) continue;
+            if constexpr (AF == OPURE_A_F32)
+            {
+                reinterpret_cast<float2*>(out + d * 4u)[0] = float2{v[0], v[1]};
+                reinterpret_cast<float2*>(out + d * 4u)[1] = float2{v[2], v[3]};
+            }
+            else *reinterpret_cast<u2v*>(out + d * 2u) = u2v{win_pack<AF>(v[0], v[1]), win_pack<AF>(v[2], v[3])};
+        }
+    // rows that are not finite again, position by position; the loop's last barrier freed the stages
+    uint64_t left = __ballot(there && !fine);
+    left = (left | left >> 32) & 0xFFFFFFFFu;
+    float* const qs = reinterpret_cast<float*>(lds) + wave * 256u;
+    while (left)
+    {
+        const uint32_t x = static_cast<uint32_t>(__builtin_ctzll(left)), qx = w0 + x, jx = qx / G;
+        left &= left - 1u;
+        const uint64_t at = ((static_cast<uint64_t>(b) * p.rows + jx) * p.n_heads + kh * G + (qx - jx * G)) * HD;
+        __builtin_amdgcn_wave_barrier();
+        for (uint32_t d = lane; d < HD; d += 64u) qs[d] = load_act<AF>(p.q, at + d);
+        __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        float lx, v[4];
+        kv4_row(p, qs, b, kh, sq.ctx + jx, sq.total, lx, v);
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e)
+            if (lane + 64u * e < HD) store_act_rt(p.out, at + lane + 64u * e, lx == 0.0f ? 0.0f : __fdiv_rn(v[e], lx), AF);
+    }
+}
+
 template <int HD, int NT>
 constexpr uint32_t split_lds() { return 4u * (HD / 16u) * NT * 64u * 16u + 4u * NT * 16u * 2u * 4u; }
 
@@ -554,13 +866,44 @@ int split_kernel(opure_dev* dev, uint32_t afmt, uint32_t hd, bool two, bool once
                                  : by_head(std::integral_constant<int, OPURE_A_BF16>{});
 }
 
+// The same of the kernel of many query rows.
+template <typename F>
+int rows_kernel(opure_dev* dev, uint32_t afmt, uint32_t hd, F&& f)
+{
+    auto by_head = [&](auto af) {
+        return win_by_head(hd, [&](auto h) {
+            constexpr int AF = decltype(af)::value, HD = decltype(h)::value;
+            static std::atomic<uint64_t> done{0};
+            auto* kernel = &k_kv4_rows<AF, HD>;
+            const int rc = win_lds(dev, reinterpret_cast<const void*>(kernel), rows_lds<HD>(), done);
+            return rc ? rc : f(kernel, rows_lds<HD>());
+        });
+    };
+    return afmt == OPURE_A_F32   ? by_head(std::integral_constant<int, OPURE_A_F32>{})
+           : afmt == OPURE_A_F16 ? by_head(std::integral_constant<int, OPURE_A_F16>{})
+                                 : by_head(std::integral_constant<int, OPURE_A_BF16>{});
+}
+
 // How a call is split, and its workspace.
 struct Kv4Plan {
     uint32_t tiles = 0, blocks = 0, block_rows = 0, parts = 0;
-    bool two = false;
+    bool two = false, many = false;                      // blocks of 32 query rows, of 128
     uint64_t acc = 0, ml = 0;                            // bytes
     uint64_t bytes() const { return acc + ml; }
 };
+
+// workspace of `groups` blocks of query rows (`rows` in all) in w.parts parts
+int kv4_slots(const opure_attn_kv4_args* a, uint64_t groups, uint64_t rows, Kv4Plan& w)
+{
+    const uint64_t slots = w.many && w.parts == 1u ? 0u : groups * w.parts * w.block_rows;
+    w.acc = opure_hip::align_up(slots * a->model->head_dim * 4u, 256);
+    w.ml = opure_hip::align_up(slots * 8u, 256);
+    const uint64_t join = w.parts > 8u ? rows : (rows + 3u) / 4u;
+    // a launch's threads, 256 a workgroup, stay in 32 bits
+    OPURE_REQUIRE(std::max(groups * w.parts, join) < 1u << 24, OPURE_E_CAPACITY,
+                  "4-bit attention: %u x %u rows of %u heads over max_ctx %u: too many workgroups", a->batch, a->rows, a->model->n_heads, a->max_ctx);
+    return OPURE_OK;
+}
 
 int kv4_plan(opure_dev* dev, const opure_attn_kv4_args* a, Kv4Plan& w)
 {
@@ -569,6 +912,16 @@ int kv4_plan(opure_dev* dev, const opure_attn_kv4_args* a, Kv4Plan& w)
     // tiles of any block of rows: its sinks', then the window's and the rows', which begin anywhere in a tile
     const uint64_t all = (a->max_ctx + 31u) / 32u, window = a->window ? a->window : 0x7FFFFFFFu;
     w.tiles = static_cast<uint32_t>(std::min<uint64_t>(all, (a->sinks + 31ull) / 32u + (window + a->rows + 30ull) / 32u + 1u));
+    const uint64_t heads = static_cast<uint64_t>(a->batch) * m->n_kv_heads, rows = heads * Gq;
+    const uint64_t cu = dev->n_cu > 0 ? static_cast<uint32_t>(dev->n_cu) : 256u;
+    w.many = Gq > 64u;
+    if (w.many)
+    {
+        w.blocks = (Gq + ROWS_BLOCK - 1u) / ROWS_BLOCK;
+        w.block_rows = std::min(Gq, ROWS_BLOCK);
+        w.parts = static_cast<uint32_t>(std::min<uint64_t>(std::max<uint64_t>(1u, 2u * cu / (heads * w.blocks)), std::min((w.tiles + 7u) / 8u, MAX_PARTS)));
+        return kv4_slots(a, heads * w.blocks, rows, w);
+    }
     w.two = Gq > 16u && m->head_dim <= 128u;
     w.blocks = (Gq + (w.two ? 31u : 15u)) / (w.two ? 32u : 16u);
     w.block_rows = std::min(Gq, w.two ? 32u : 16u);
@@ -578,19 +931,12 @@ int kv4_plan(opure_dev* dev, const opure_attn_kv4_args* a, Kv4Plan& w)
         return OPURE_OK;
     });
     if (rc) return rc;
-    const uint64_t heads = static_cast<uint64_t>(a->batch) * m->n_kv_heads, groups = heads * w.blocks, rows = heads * Gq;
+    const uint64_t groups = heads * w.blocks;
     // Parts of a group: as many as the device holds at a time, each of at least four tiles, one a wave
     const uint32_t least = std::max(4u, w.block_rows / 4u);
     const uint64_t fill = std::max<uint64_t>(1u, room / groups), more = std::min<uint64_t>(3ull * room / groups, w.tiles / 16u);
     w.parts = static_cast<uint32_t>(std::min<uint64_t>(std::max(fill, more), std::min((w.tiles + least - 1u) / least, MAX_PARTS)));
-    const uint64_t slots = groups * w.parts * w.block_rows;
-    w.acc = opure_hip::align_up(slots * m->head_dim * 4u, 256);
-    w.ml = opure_hip::align_up(slots * 8u, 256);
-    const uint64_t join = w.parts > 8u ? rows : (rows + 3u) / 4u;
-    // a launch's threads, 256 a workgroup, stay in 32 bits
-    OPURE_REQUIRE(std::max(groups * w.parts, join) < 1u << 24, OPURE_E_CAPACITY,
-                  "4-bit attention: %u x %u rows of %u heads over max_ctx %u: too many workgroups", a->batch, a->rows, m->n_heads, a->max_ctx);
-    return OPURE_OK;
+    return kv4_slots(a, groups, rows, w);
 }
 
 int kv4_validate(const opure_attn_kv4_args* a)
@@ -682,16 +1028,17 @@ extern "C" int opure_attn_kv4_paged(opure_dev* dev, const opure_attn_kv4_args* a
     p.parts = w.parts;
     p.blocks = w.blocks;
     p.block_rows = w.block_rows;
-    p.two = w.two ? 1u : 0u;
+    p.two = w.many ? 2u : w.two ? 1u : 0u;
     p.tiles = w.tiles;
     p.combine_rows = a->batch * a->rows * p.n_heads;
     const uint32_t wgs = p.n_kv * w.parts * w.blocks * a->batch;
-    rc = split_kernel(dev, p.afmt, p.hd, w.two, w.blocks == 1u, [&](auto kernel, uint32_t lds, uint32_t) {
+    auto launch = [&](auto kernel, uint32_t lds, uint32_t = 0) {
         OPURE_LAUNCH(dev, kernel, dim3(wgs), dim3(256), lds, p);
-        OPURE_LAUNCH_CHECK("k_kv4_split");
+        OPURE_LAUNCH_CHECK("4-bit attention");
         return OPURE_OK;
-    });
-    if (rc) return rc;
+    };
+    rc = w.many ? rows_kernel(dev, p.afmt, p.hd, launch) : split_kernel(dev, p.afmt, p.hd, w.two, w.blocks == 1u, launch);
+    if (rc || (w.many && w.parts == 1u)) return rc;
     const bool wide = w.parts > 8u;
     p.combine_wgs = wide ? p.combine_rows : (p.combine_rows + 3u) / 4u;
     auto join = [&](auto all) {
