@@ -50,33 +50,60 @@ __device__ __forceinline__ float key_value(uint32_t k)
 }
 __device__ __forceinline__ uint64_t make_key(float f, uint32_t at) { return static_cast<uint64_t>(order_key(f)) << 32 | (0xFFFFFFFFu - at); }
 
-__device__ __forceinline__ uint64_t lane_xor(uint64_t v, uint32_t x)
+// Lanes l and l ^ J exchange keys: the larger goes to the lanes of UP.  All moves are
+// the vector unit's (DPP, and the swaps of 16 and 32 lanes, which leave both keys in
+// both lanes): a step is about 8 instructions, a fifth of one through LDS.
+template <uint32_t J, uint64_t UP>
+__device__ __forceinline__ uint64_t exchange(uint64_t v)
 {
-    return static_cast<uint64_t>(__shfl_xor(static_cast<unsigned long long>(v), static_cast<int>(x)));
+    uint32_t lo = static_cast<uint32_t>(v), hi = static_cast<uint32_t>(v >> 32), lo2, hi2;
+    if constexpr (J >= 16u)
+    {
+        const auto l = J == 32u ? __builtin_amdgcn_permlane32_swap(lo, lo, false, false) : __builtin_amdgcn_permlane16_swap(lo, lo, false, false);
+        const auto h = J == 32u ? __builtin_amdgcn_permlane32_swap(hi, hi, false, false) : __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
+        lo = l[0], lo2 = l[1], hi = h[0], hi2 = h[1];
+    }
+    else
+    {
+        // quad_perm [1,0,3,2] and [2,3,0,1], row_ror:8; 4: the half rows mirrored, then the quads
+        constexpr int CTRL = J == 1u ? 0xB1 : J == 2u ? 0x4E : J == 8u ? 0x128 : 0x141;
+        lo2 = __builtin_amdgcn_mov_dpp(static_cast<int>(lo), CTRL, 0xF, 0xF, true);
+        hi2 = __builtin_amdgcn_mov_dpp(static_cast<int>(hi), CTRL, 0xF, 0xF, true);
+        if constexpr (J == 4u)
+        {
+            lo2 = __builtin_amdgcn_mov_dpp(static_cast<int>(lo2), 0x1B, 0xF, 0xF, true);
+            hi2 = __builtin_amdgcn_mov_dpp(static_cast<int>(hi2), 0x1B, 0xF, 0xF, true);
+        }
+    }
+    const uint64_t a = static_cast<uint64_t>(hi) << 32 | lo, b = static_cast<uint64_t>(hi2) << 32 | lo2;
+    return (a > b) == __builtin_amdgcn_inverse_ballot_w64(UP) ? a : b;
 }
-__device__ __forceinline__ uint64_t pick(uint64_t v, uint64_t o, bool larger) { return (v > o) == larger ? v : o; }
 
-// 64 keys, one a lane, into falling order
-__device__ inline uint64_t wave_sort(uint64_t v)
+// lanes whose bit J is 0 where bit K is 0 (K 64: everywhere), and the others
+constexpr uint64_t lanes_up(uint32_t j, uint32_t k)
 {
-    const uint32_t lane = threadIdx.x & 63u;
-#pragma unroll
-    for (uint32_t k = 2; k <= 64u; k <<= 1)
-#pragma unroll
-        for (uint32_t j = k >> 1; j > 0u; j >>= 1)
-            v = pick(v, lane_xor(v, j), ((lane & j) == 0u) == ((lane & k) == 0u || k == 64u));
-    return v;
+    uint64_t m = 0;
+    for (uint32_t l = 0; l < 64u; ++l) m |= static_cast<uint64_t>(((l & j) == 0u) == ((l & k) == 0u)) << l;
+    return m;
 }
-// the 64 largest of two falling sequences, falling
-__device__ inline uint64_t wave_merge(uint64_t a, uint64_t b)
+template <uint32_t J, uint32_t K, bool FALLING>
+__device__ __forceinline__ uint64_t steps(uint64_t v)
 {
-    const uint32_t lane = threadIdx.x & 63u;
-    const uint64_t r = lane_xor(b, 63u);
-    uint64_t v = a > r ? a : r;
-#pragma unroll
-    for (uint32_t j = 32; j > 0u; j >>= 1) v = pick(v, lane_xor(v, j), (lane & j) == 0u);
-    return v;
+    v = exchange<J, FALLING ? lanes_up(J, K) : ~lanes_up(J, K)>(v);
+    if constexpr (J > 1u) return steps<J / 2u, K, FALLING>(v);
+    else return v;
 }
+// 64 keys, one a lane, into rising order
+template <uint32_t K = 2>
+__device__ __forceinline__ uint64_t wave_sort(uint64_t v)
+{
+    v = steps<K / 2u, K, false>(v);
+    if constexpr (K < 64u) return wave_sort<2u * K>(v);
+    else return v;
+}
+// the 64 largest of a falling and a rising sequence, falling
+__device__ __forceinline__ uint64_t wave_merge(uint64_t falling, uint64_t rising) { return steps<32, 64, true>(falling > rising ? falling : rising); }
+
 __device__ __forceinline__ uint64_t key_at(uint64_t v, uint32_t lane)
 {
     const uint32_t lo = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), static_cast<int>(lane)));
@@ -108,8 +135,21 @@ __device__ __forceinline__ Stats wave_stats(Stats a)
     return a;
 }
 
+// A row's token and its logit, asked for before the sums are there.
+struct Given {
+    bool in;
+    float x;
+    __device__ __forceinline__ Given(const LogprobParams& p, uint32_t row) : in(false), x(0.0f)
+    {
+        if (!p.logprob) return;
+        const int32_t t = p.tokens[row];
+        in = t >= 0 && static_cast<uint32_t>(t) < p.vocab;
+        x = p.logits[row * p.stride + (in ? static_cast<uint32_t>(t) : 0u)];
+    }
+};
+
 // A row's results from its sums and its largest keys, by one wave.
-__device__ __forceinline__ void finish(const LogprobParams& p, uint32_t row, Stats a, uint64_t best)
+__device__ __forceinline__ void finish(const LogprobParams& p, uint32_t row, Stats a, uint64_t best, const Given& given)
 {
     const uint32_t lane = threadIdx.x & 63u;
     const float nan = __builtin_nanf("");
@@ -119,10 +159,8 @@ __device__ __forceinline__ void finish(const LogprobParams& p, uint32_t row, Sta
     if (lane == 0u && p.entropy) p.entropy[row] = bad ? nan : __fsub_rn(norm, __fdiv_rn(a.e, a.s));
     if (lane == 0u && p.logprob)
     {
-        const int32_t t = p.tokens[row];
-        const bool in = t >= 0 && static_cast<uint32_t>(t) < p.vocab;
-        if (!in) p.err[ERR_TOKEN] = 1u;
-        p.logprob[row] = in ? of(p.logits[row * p.stride + static_cast<uint32_t>(t)]) : nan;
+        if (!given.in) p.err[ERR_TOKEN] = 1u;
+        p.logprob[row] = given.in ? of(given.x) : nan;
     }
     if (lane < p.top)
     {
@@ -132,14 +170,20 @@ __device__ __forceinline__ void finish(const LogprobParams& p, uint32_t row, Sta
     }
 }
 
-// A slice of a row by a workgroup, its waves every fourth chunk.  A wave keeps its
-// 64 largest keys in order, one a lane; of a logit only a comparison with the
-// top-th of them is needed, and the few that pass wait in LDS until they are 64.
-// The first chunk's lanes' maxima are the first 64.
+// A slice of a row by a workgroup, its waves every fourth chunk.  A wave keeps its 64
+// largest keys in order, one a lane.  The first chunk's lanes' maxima are the first 64, so
+// at most 16 top logits of it follow; of a later chunk only the lanes' maxima are compared
+// with the top-th (an equal logit that comes later loses).  Where one passes, the chunk
+// is left in LDS and looked through behind its sums, four logits a lane at a time; those
+// that pass go to a queue that is sorted and merged 64 at a time.  Neither the chunk's
+// registers nor more than one sort are there for the rare case: with both in the loop the
+// compiler took 64 to 135 registers, and 1,500 rows of 128,256 200 us for 158.
 template <bool TOP, bool ONE>
 __global__ __launch_bounds__(256) void k_logprobs(LogprobParams p)
 {
-    __shared__ uint64_t queue[TOP ? 4 : 1][TOP ? 128 : 1];
+    constexpr uint32_t ROOM = 320;
+    __shared__ uint64_t queue[TOP ? 4 : 1][TOP ? ROOM : 1];
+    __shared__ float4 chunk[TOP ? 4 : 1][TOP ? PER / 4u : 1u][64];
     __shared__ float4 part[4];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u;
     const uint32_t row = blockIdx.x / p.slices, sl = blockIdx.x - row * p.slices;
@@ -150,68 +194,59 @@ __global__ __launch_bounds__(256) void k_logprobs(LogprobParams p)
     uint64_t best = 0, least = 0;                        // the lane's key; the top-th
     float bar = NEG_INF;                                 // its value
     uint32_t waiting = 0;
-    auto take = [&](uint64_t batch) {
-        best = wave_merge(best, wave_sort(batch));
-        least = key_at(best, p.top - 1u);
-        bar = least ? key_value(static_cast<uint32_t>(least >> 32)) : NEG_INF;
-    };
-    for (uint32_t c0 = begin + wave * CHUNK; c0 < end; c0 += 4u * CHUNK)
+    const uint32_t first = begin + wave * CHUNK;
+    for (uint32_t c0 = first; c0 < end; c0 += 4u * CHUNK)
     {
-        float v[PER];
-        const bool whole = c0 + CHUNK <= end;
+        float v[PER], m = NEG_INF;
+        bool bad = false, look = false;
 #pragma unroll
         for (uint32_t i = 0; i < PER; i += 4u)
         {
             const uint32_t at = c0 + 64u * i + 4u * lane;
-            if (whole) __builtin_memcpy(&v[i], x + at, 16);
+            if (c0 + CHUNK <= end) __builtin_memcpy(&v[i], x + at, 16);
             else
 #pragma unroll
                 for (uint32_t e = 0; e < 4; ++e) v[i + e] = at + e < end ? x[at + e] : NEG_INF;
         }
-        auto index = [&](uint32_t i) { return c0 + 64u * (i & ~3u) + 4u * lane + (i & 3u); };
-        if constexpr (TOP)
-        {
-            uint64_t mine = 0;                           // the lane's largest of the first chunk
-            if (c0 < begin + 4u * CHUNK)
-            {
-#pragma unroll
-                for (uint32_t i = 0; i < PER; ++i)
-                {
-                    const uint64_t k = index(i) < end ? make_key(v[i], index(i)) : 0u;
-                    mine = mine > k ? mine : k;
-                }
-                take(mine);
-            }
-#pragma unroll
-            for (uint32_t i = 0; i < PER; ++i)
-            {
-                if (!__any(!(v[i] < bar))) continue;
-                uint64_t k = index(i) < end ? make_key(v[i], index(i)) : 0u;
-                if (k == mine) k = 0u;
-                const uint64_t pass = __ballot(k > least);
-                if (!pass) continue;
-                if (k > least) queue[wave][waiting + __popcll(pass & ((1ull << lane) - 1u))] = k;
-                waiting += static_cast<uint32_t>(__popcll(pass));
-                if (waiting >= 64u)
-                {
-                    __builtin_amdgcn_wave_barrier();
-                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                    const uint64_t batch = queue[wave][lane], rest = queue[wave][64u + lane];
-                    take(batch);
-                    waiting -= 64u;
-                    __builtin_amdgcn_wave_barrier();
-                    if (lane < waiting) queue[wave][lane] = rest;
-                }
-            }
-        }
-        float m = NEG_INF;
 #pragma unroll
         for (uint32_t i = 0; i < PER; ++i)
         {
-            if (tau != 1.0f) v[i] = __fdiv_rn(v[i], tau);
-            a.bad = a.bad || !(v[i] < __builtin_huge_valf());
+            bad = bad || !(v[i] < __builtin_huge_valf());
             m = fmaxf(m, v[i]);
         }
+        auto index = [&](uint32_t q) { return c0 + 256u * q + 4u * lane; };
+        uint32_t taken = PER;                            // the lane's largest of the first chunk: its first NaN, or m
+        float most = m;
+        if constexpr (TOP)
+        {
+            look = c0 == first || __any(bad || m > bar) || (waiting && c0 + 4u * CHUNK >= end);
+            if (look)
+#pragma unroll
+                for (uint32_t q = 0; q < PER / 4u; ++q) chunk[wave][q][lane] = float4{v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]};
+            if (c0 == first)
+            {
+                bool nan = false;
+#pragma unroll
+                for (uint32_t i = PER; i-- > 0u;)
+                {
+                    taken = v[i] == m && !nan ? i : taken;
+                    if (v[i] != v[i]) taken = i, nan = true;
+                }
+                if (nan) most = __builtin_nanf("");
+            }
+        }
+        if (tau != 1.0f)
+        {
+            m = NEG_INF;
+#pragma unroll
+            for (uint32_t i = 0; i < PER; ++i)
+            {
+                v[i] = __fdiv_rn(v[i], tau);
+                bad = bad || !(v[i] < __builtin_huge_valf());
+                m = fmaxf(m, v[i]);
+            }
+        }
+        a.bad = a.bad || bad;
         if (m > a.m) rebase(a, m);
         const float ms = a.m == NEG_INF ? 0.0f : a.m;
 #pragma unroll
@@ -222,25 +257,65 @@ __global__ __launch_bounds__(256) void k_logprobs(LogprobParams p)
             a.s += e;
             a.e = __fmaf_rn(e, d, a.e);
         }
+        if constexpr (TOP)
+            if (look)
+            {
+                // -1: the first chunk's maxima; then four logits of each lane.  Behind them `top` that wait are merged, so that
+                // the next chunks are compared with what is largest now, and at the end all
+                const uint32_t enough = c0 + 4u * CHUNK >= end ? 1u : min(p.top, 64u);
+#pragma unroll 1
+                for (int q = c0 == first ? -1 : 0; q < static_cast<int>(PER / 4u); ++q)
+                {
+                    __builtin_amdgcn_wave_barrier();
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    if (q < 0)
+                    {
+                        const uint32_t at = index(taken >> 2) + (taken & 3u);
+                        queue[wave][lane] = taken < PER && at < end ? make_key(most, at) : 0u;
+                        waiting = 64u;
+                    }
+                    else
+                    {
+                        const float4 w = chunk[wave][q][lane];
+                        const float f[4] = {w.x, w.y, w.z, w.w};
+                        const uint32_t at = index(static_cast<uint32_t>(q));
+#pragma unroll
+                        for (uint32_t e = 0; e < 4; ++e)
+                        {
+                            const uint64_t k = at + e < end && 4u * static_cast<uint32_t>(q) + e != taken ? make_key(f[e], at + e) : 0u;
+                            const uint64_t all = __ballot(k > least);
+                            if (k > least) queue[wave][waiting + __popcll(all & ((1ull << lane) - 1u))] = k;
+                            waiting += static_cast<uint32_t>(__popcll(all));
+                        }
+                    }
+                    __builtin_amdgcn_wave_barrier();
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    while (waiting >= 64u || (waiting >= enough && q + 1 == static_cast<int>(PER / 4u)))
+                    {
+                        const uint32_t n = min(waiting, 64u);
+                        waiting -= n;
+                        best = wave_merge(best, wave_sort(lane < n ? queue[wave][waiting + lane] : 0u));
+                        least = key_at(best, p.top - 1u);
+                        bar = least ? key_value(static_cast<uint32_t>(least >> 32)) : NEG_INF;
+                    }
+                }
+            }
     }
-    a = wave_stats(a);
     if constexpr (TOP)
     {
         __builtin_amdgcn_wave_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        if (waiting) take(lane < waiting ? queue[wave][lane] : 0u);
-        __builtin_amdgcn_wave_barrier();
         queue[wave][lane] = best;
     }
+    a = wave_stats(a);
     if (lane == 0u) part[wave] = float4{a.m, a.s, a.e, a.bad ? 1.0f : 0.0f};
     __syncthreads();
     if (wave != 0u) return;
     const float4 mine = part[lane & 3u];
     a = wave_stats(Stats{lane < 4u ? mine.x : NEG_INF, lane < 4u ? mine.y : 0.0f, lane < 4u ? mine.z : 0.0f, lane < 4u && mine.w != 0.0f});
     if constexpr (TOP)
-#pragma unroll
-        for (uint32_t w = 1; w < 4; ++w) best = wave_merge(best, queue[w][lane]);
-    if constexpr (ONE) finish(p, row, a, best);
+#pragma unroll 1
+        for (uint32_t w = 1; w < 4; ++w) best = wave_merge(best, queue[w][63u - lane]);
+    if constexpr (ONE) finish(p, row, a, best, Given(p, row));
     else
     {
         if (lane == 0u) p.stats[blockIdx.x] = float4{a.m, a.s, a.e, a.bad ? 1.0f : 0.0f};
@@ -248,38 +323,59 @@ __global__ __launch_bounds__(256) void k_logprobs(LogprobParams p)
     }
 }
 
-// Joins a row's slices: each of four waves every fourth slice's keys, then the waves'.
-template <bool TOP>
-__global__ __launch_bounds__(256) void k_logprobs_join(LogprobParams p)
+// Joins a row's slices: each of W waves every W-th slice's keys, then four waves every
+// fourth wave's, then one theirs.
+template <bool TOP, uint32_t W>
+__global__ __launch_bounds__(64 * W) void k_logprobs_join(LogprobParams p)
 {
-    __shared__ uint64_t list[4][64];
+    constexpr uint32_t N = MAX_SLICES / 16u;             // slices a wave at most (W 16; W 4: up to 16 slices)
+    __shared__ uint64_t list[W][64];
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, row = blockIdx.x;
     const uint64_t at = static_cast<uint64_t>(row) * p.slices;
+    const float4 mine = p.stats[at + min(lane, p.slices - 1u)];
+    const Given given(p, row);
     uint64_t best = 0;
     if constexpr (TOP)
     {
-        for (uint32_t s = wave; s < p.slices; s += 4u)
+        uint64_t k[N];
+#pragma unroll
+        for (uint32_t i = 0; i < N; ++i)
         {
-            const uint64_t k = lane < p.top ? p.keys[(at + s) * p.top + lane] : 0u;
-            best = s == wave ? k : wave_merge(best, k);
+            const uint32_t s = wave + i * W, from = i ? 63u - lane : lane;
+            k[i] = p.keys[(at + min(s, p.slices - 1u)) * p.top + min(from, p.top - 1u)];
+            k[i] = s < p.slices && from < p.top ? k[i] : 0u;
         }
+        best = k[0];
+#pragma unroll
+        for (uint32_t i = 1; i < N; ++i) best = wave_merge(best, k[i]);
+        auto join = [&](uint32_t n, uint32_t by) {
+            // wave w and w + by, w + 2 by, ... below n
+#pragma unroll 1
+            for (uint32_t w = wave + by; w < n; w += by) best = wave_merge(best, list[w][63u - lane]);
+        };
         list[wave][lane] = best;
         __syncthreads();
+        if constexpr (W > 4u)
+        {
+            if (wave < 4u)
+            {
+                join(min(W, p.slices), 4u);
+                list[wave][lane] = best;
+            }
+            __syncthreads();
+        }
+        if (wave == 0u) join(4u, 1u);
     }
     if (wave != 0u) return;
-    if constexpr (TOP)
-#pragma unroll
-        for (uint32_t w = 1; w < 4; ++w) best = wave_merge(best, list[w][lane]);
-    const float4 mine = p.stats[at + min(lane, p.slices - 1u)];
     const bool in = lane < p.slices;
-    finish(p, row, wave_stats(Stats{in ? mine.x : NEG_INF, in ? mine.y : 0.0f, in ? mine.z : 0.0f, in && mine.w != 0.0f}), best);
+    finish(p, row, wave_stats(Stats{in ? mine.x : NEG_INF, in ? mine.y : 0.0f, in ? mine.z : 0.0f, in && mine.w != 0.0f}), best, given);
 }
 
-// A row in as many slices as give each CU two workgroups.
+// A row in as many slices as give each CU four workgroups.
 void slices_of(const opure_dev* dev, const opure_logprobs_args* a, uint32_t& slices, uint32_t& slice)
 {
     const uint32_t cu = dev->n_cu > 0 ? static_cast<uint32_t>(dev->n_cu) : 256u, most = (a->vocab + 4u * CHUNK - 1u) / (4u * CHUNK);
-    slices = std::min({std::max(1u, 2u * cu / a->rows), most, MAX_SLICES});
+    slices = std::min({std::max(1u, 4u * cu / a->rows), most, MAX_SLICES});
     slice = ((a->vocab + slices - 1u) / slices + 4u * CHUNK - 1u) / (4u * CHUNK) * (4u * CHUNK);
     slices = (a->vocab + slice - 1u) / slice;
 }
@@ -378,8 +474,9 @@ extern "C" int opure_logprobs(opure_dev* dev, const opure_logprobs_args* a)
     if (p.top) OPURE_LAUNCH(dev, (k_logprobs<true, false>), grid, block, 0, p);
     else OPURE_LAUNCH(dev, (k_logprobs<false, false>), grid, block, 0, p);
     OPURE_LAUNCH_CHECK("k_logprobs");
-    if (p.top) OPURE_LAUNCH(dev, (k_logprobs_join<true>), dim3(p.rows), block, 0, p);
-    else OPURE_LAUNCH(dev, (k_logprobs_join<false>), dim3(p.rows), block, 0, p);
+    if (!p.top) OPURE_LAUNCH(dev, (k_logprobs_join<false, 1>), dim3(p.rows), dim3(64), 0, p);
+    else if (p.slices <= 16u) OPURE_LAUNCH(dev, (k_logprobs_join<true, 4>), dim3(p.rows), block, 0, p);
+    else OPURE_LAUNCH(dev, (k_logprobs_join<true, 16>), dim3(p.rows), dim3(1024), 0, p);
     OPURE_LAUNCH_CHECK("k_logprobs_join");
     return OPURE_OK;
 }
