@@ -74,13 +74,24 @@ struct Scale {
 
 __device__ __forceinline__ half2_t pair(uint32_t w) { return __builtin_bit_cast(half2_t, w); }
 
-// nibble N of both halves of a word as 16 + c
-template <int N>
-__device__ __forceinline__ half2_t codes(uint32_t w)
-{
-    const uint32_t at = N == 0 ? w << 6 : N == 1 ? w << 2 : N == 2 ? w >> 2 : w >> 6;
-    return pair((at & 0x03C003C0u) | 0x4C004C00u);
-}
+// A mask and an exponent that the compiler does not know, a scalar and a vector
+// register: with them a nibble is a shift and one and-or, with constants, of which an
+// instruction has room for one, a shift, an and and an or.
+struct Bits {
+    uint32_t nibble = 0x03C003C0u, sixteen = 0x4C004C00u;
+    __device__ __forceinline__ Bits()
+    {
+        asm volatile("" : "+s"(nibble));
+        asm volatile("" : "+v"(sixteen));
+    }
+    // nibble N of both halves of a word as 16 + c
+    template <int N>
+    __device__ __forceinline__ half2_t codes(uint32_t w) const
+    {
+        const uint32_t at = N == 0 ? w << 6 : N == 1 ? w << 2 : N == 2 ? w >> 2 : w >> 6;
+        return pair((at & nibble) | sixteen);
+    }
+};
 
 __device__ __forceinline__ uint32_t values(half2_t c, half2_t s, half2_t b)
 {

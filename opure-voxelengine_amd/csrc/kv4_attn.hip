@@ -19,9 +19,9 @@ namespace {
 
 constexpr uint32_t MAX_PARTS = 64;                         // of a (sequence, KV head, block of query rows): a lane of the joining wave each
 constexpr float LOG2E = 1.44269504088896340736f;
-// Weights are held times 2^14, which fp16 still has: what fp16 loses at its small end then lies 2^38 below a row's
-// largest weight.
-constexpr float P_SHIFT = 14.0f;
+// A row's output is scaled to a new maximum only where that passes the old one by 2^LAG.  Weights are held times
+// 2^SHIFT, so the largest of 2^15 is still in fp16, and what fp16 loses at its small end lies 2^36 below 1.
+constexpr float SHIFT = 12.0f, LAG = 3.0f;
 
 typedef u4v u4a __attribute__((aligned(4)));
 typedef uint32_t u2v __attribute__((ext_vector_type(2)));
@@ -31,25 +31,31 @@ typedef u2v u2a __attribute__((aligned(4)));
 template <uint32_t N, bool ONCE>
 __device__ __forceinline__ void load_words(const uint32_t* p, uint32_t (&w)[N])
 {
-    auto get = [](auto* q) {
-        if constexpr (ONCE) return __builtin_nontemporal_load(q);
-        else return *q;
-    };
     constexpr uint32_t Q = N / 4u * 4u;
 #pragma unroll
     for (uint32_t i = 0; i < Q; i += 4u)
     {
-        const u4v v = get(reinterpret_cast<const u4a*>(p + i));
+        const u4a* q = reinterpret_cast<const u4a*>(p + i);
+        u4v v;
+        if constexpr (ONCE) v = __builtin_nontemporal_load(q);
+        else v = *q;
 #pragma unroll
         for (uint32_t x = 0; x < 4; ++x) w[i + x] = v[x];
     }
     if constexpr ((N & 2u) != 0u)
     {
-        const u2v v = get(reinterpret_cast<const u2a*>(p + Q));
+        const u2a* q = reinterpret_cast<const u2a*>(p + Q);
+        u2v v;
+        if constexpr (ONCE) v = __builtin_nontemporal_load(q);
+        else v = *q;
         w[Q] = v[0];
         w[Q + 1u] = v[1];
     }
-    if constexpr ((N & 1u) != 0u) w[N - 1u] = get(p + N - 1u);
+    if constexpr ((N & 1u) != 0u)
+    {
+        if constexpr (ONCE) w[N - 1u] = __builtin_nontemporal_load(p + N - 1u);
+        else w[N - 1u] = p[N - 1u];
+    }
 }
 
 // Two pages of a KV head, positions 16 x + 0..15 of page x: lane (r, g) has K codes
@@ -82,22 +88,22 @@ struct Kv4Tile {
         }
     }
     // group p of page x as fp16 numbers
-    __device__ __forceinline__ u4v k(uint32_t x, uint32_t p) const
+    __device__ __forceinline__ u4v k(const Bits& bits, uint32_t x, uint32_t p) const
     {
         const half2_t sb = pair(ks[x][p]), s = {sb[0], sb[0]}, b = {sb[1], sb[1]};
         const uint32_t w = kw[x][p];
-        return u4v{values(codes<0>(w), s, b), values(codes<1>(w), s, b), values(codes<2>(w), s, b), values(codes<3>(w), s, b)};
+        return u4v{values(bits.codes<0>(w), s, b), values(bits.codes<1>(w), s, b), values(bits.codes<2>(w), s, b), values(bits.codes<3>(w), s, b)};
     }
     // channels 32 p + 16 T + r of both pages' tokens
     template <int T>
-    __device__ __forceinline__ u4v v(uint32_t p) const
+    __device__ __forceinline__ u4v v(const Bits& bits, uint32_t p) const
     {
         u4v o;
 #pragma unroll
         for (uint32_t x = 0; x < 2; ++x)
         {
-            o[2 * x] = values(codes<2 * T>(vw[x][p]), pair(vs[x][p][0]), pair(vs[x][p][2]));
-            o[2 * x + 1] = values(codes<2 * T + 1>(vw[x][p]), pair(vs[x][p][1]), pair(vs[x][p][3]));
+            o[2 * x] = values(bits.template codes<2 * T>(vw[x][p]), pair(vs[x][p][0]), pair(vs[x][p][2]));
+            o[2 * x + 1] = values(bits.template codes<2 * T + 1>(vw[x][p]), pair(vs[x][p][1]), pair(vs[x][p][3]));
         }
         return o;
     }
@@ -169,6 +175,19 @@ __device__ __forceinline__ float load_query(const WinParams& p, uint64_t row, ui
             }
         return __builtin_ldexpf(c, e);
     }
+}
+
+// Scores in powers of two are c >= 0 times the products: the scale's sign goes to the query.
+template <int AF, int HD, uint32_t PARTS, uint32_t QT, uint32_t STEPS>
+__device__ __forceinline__ float signed_query(const WinParams& p, uint64_t row, uint32_t part, u4v (&q)[QT][STEPS])
+{
+    const float c = load_query<AF, HD, PARTS>(p, row, part, q);
+    if (p.scale < 0.0f)
+#pragma unroll
+        for (uint32_t z = 0; z < QT; ++z)
+#pragma unroll
+            for (uint32_t s = 0; s < STEPS; ++s) q[z][s] ^= u4v{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
+    return __builtin_fabsf(c);
 }
 
 // One query row by one wave, exactly as the formulas say it; a position that the
@@ -258,8 +277,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 2 ? 2
     {
         const uint32_t qi = min(q0 + 16u * n + r, Gq - 1u);
         jr[n] = qi / G;
-        c[n] = load_query<AF, HD, 4>(p, (static_cast<uint64_t>(b) * p.rows + jr[n]) * p.n_heads + kh * G + (qi - jr[n] * G), g, q[n]);
+        c[n] = signed_query<AF, HD, 4>(p, (static_cast<uint64_t>(b) * p.rows + jr[n]) * p.n_heads + kh * G + (qi - jr[n] * G), g, q[n]);
     }
+    const Bits bits;
     const uint32_t j0 = q0 / G, j1 = min(q0 + 16u * NT - 1u, Gq - 1u) / G;    // the block's first and last row
     const WinSpan span = win_span<TT>(p, sq, sq.ctx + j0, sq.ctx + j1 + 1u);
     const uint32_t first = static_cast<uint32_t>(static_cast<uint64_t>(span.n) * part / p.parts);
@@ -319,7 +339,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 2 ? 2
 #pragma unroll
                 for (uint32_t x = 0; x < 2; ++x)
                 {
-                    const u4v k = tl.k(x, s);
+                    const u4v k = tl.k(bits, x, s);
 #pragma unroll
                     for (uint32_t n = 0; n < NT; ++n)
 #pragma unroll
@@ -334,7 +354,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 2 ? 2
             {
                 float s[8];
 #pragma unroll
-                for (uint32_t y = 0; y < 8; ++y) s[y] = __fmul_rn(acc[y >> 2][n][y & 3u], c[n]);
+                for (uint32_t y = 0; y < 8; ++y) s[y] = acc[y >> 2][n][y & 3u];
                 auto largest = [&]() {
                     float v = s[0];
 #pragma unroll
@@ -349,21 +369,25 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 2 ? 2
                     for (uint32_t y = 0; y < 8; ++y) s[y] = mask.sees(static_cast<int32_t>(16u * (y >> 2) + (y & 3u))) ? s[y] : NEG_INF;
                     mx = largest();
                 }
-                mx = fmaxf(m[n], max_xor32(max_xor16(mx)));
-                const float ms = mx == NEG_INF ? 0.0f : mx, a = __builtin_amdgcn_exp2f(__fsub_rn(m[n], ms)), down = __fsub_rn(ms, P_SHIFT);
-                m[n] = mx;
-                float sum = 0.0f;
+                mx = max_xor32(max_xor16(mx));
+                const bool grown = m[n] == NEG_INF ? mx > NEG_INF : __fmul_rn(__fsub_rn(mx, m[n]), c[n]) > LAG;
+                if (__any(grown))
+                {
+                    const float to = grown ? mx : m[n], a = m[n] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(__fmul_rn(__fsub_rn(m[n], to), c[n]));
+                    m[n] = to;
+                    l[n] = __fmul_rn(l[n], a);
+#pragma unroll
+                    for (uint32_t d = 0; d < DT; ++d)
+#pragma unroll
+                        for (uint32_t y = 0; y < 4; ++y) o[d][n][y] = __fmul_rn(o[d][n][y], a);
+                }
+                const float down = m[n] == NEG_INF ? 0.0f : __fsub_rn(SHIFT, __fmul_rn(m[n], c[n]));
 #pragma unroll
                 for (uint32_t y = 0; y < 8; ++y)
                 {
-                    s[y] = __builtin_amdgcn_exp2f(__fsub_rn(s[y], down));
-                    sum += s[y];
+                    s[y] = __builtin_amdgcn_exp2f(__fmaf_rn(s[y], c[n], down));
+                    l[n] += s[y];                              // this lane's share of the row's sum
                 }
-                l[n] = __fmaf_rn(l[n], a, sum);                // this lane's share of the row's sum
-#pragma unroll
-                for (uint32_t d = 0; d < DT; ++d)
-#pragma unroll
-                    for (uint32_t y = 0; y < 4; ++y) o[d][n][y] = __fmul_rn(o[d][n][y], a);
 #pragma unroll
                 for (uint32_t y = 0; y < 4; ++y)
                 {
@@ -387,7 +411,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 2 ? 2
 #pragma unroll
             for (uint32_t d = 0; d < DT; ++d)
             {
-                const u4v v = d & 1u ? tl.template v<1>(d >> 1) : tl.template v<0>(d >> 1);
+                const u4v v = d & 1u ? tl.template v<1>(bits, d >> 1) : tl.template v<0>(bits, d >> 1);
 #pragma unroll
                 for (uint32_t n = 0; n < NT; ++n)
                 {
@@ -413,7 +437,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 2 ? 2
         for (uint32_t d = 0; d < DT; ++d) cacc[((wave * DT + d) * NT + n) * 64u + lane] = o[d][n];
         if (g == 0u)
         {
-            cml[((wave * NT + n) * 16u + r) * 2u] = m[n];
+            cml[((wave * NT + n) * 16u + r) * 2u] = m[n] == NEG_INF ? NEG_INF : __fmul_rn(m[n], c[n]);   // in powers of two
             cml[((wave * NT + n) * 16u + r) * 2u + 1u] = l[n];
         }
     }
@@ -555,7 +579,6 @@ constexpr uint32_t rows_stage() { return rows_pages<HD>() * (HD / 16u * 512u + g
 template <int HD>
 constexpr uint32_t rows_lds() { return 2u * rows_stage<HD>(); }
 constexpr uint32_t ROWS_BLOCK = 128;
-constexpr float ROWS_SHIFT = 12.0f, ROWS_LAG = 3.0f;
 
 // A workgroup takes 128 query rows (qi = j group + head) of a KV head, 32 a wave, over
 // tiles of four pages (two past 128 channels) whose values the waves make from the codes
@@ -564,8 +587,6 @@ constexpr float ROWS_SHIFT = 12.0f, ROWS_LAG = 3.0f;
 // tokens 4 h .. 4 h + 3 and 8 + 4 h .. 11 + 4 h of row q, its operand P^T, and V of a
 // page lies in LDS in that order of tokens.  Two stages: while one tile is computed the
 // next one's words are on their way.
-//   A row's output is scaled to a new maximum only where that passes the old one by 2^3;
-// weights are held 2^12 higher, so the largest stays in fp16.
 template <int AF, int HD>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 128 ? 2 : 1))) void k_kv4_rows(WinParams p)
 {
@@ -586,14 +607,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 128 ?
     const uint32_t w0 = min(q0 + 32u * wave, Gq - 1u), w1 = min(q0 + 32u * wave + 31u, Gq - 1u), qi = min(w0 + r, Gq - 1u);
     const uint32_t j = qi / G, pos = sq.ctx + j, pos0 = sq.ctx + w0 / G, pos1 = sq.ctx + w1 / G;
     const uint64_t row = (static_cast<uint64_t>(b) * p.rows + j) * p.n_heads + kh * G + (qi - j * G);
-    // scores in powers of two are c times the products: its sign goes to the query
     u4v q[QT][KS];
-    const float c = __builtin_fabsf(load_query<AF, HD, 2>(p, row, h, q));
-    if (p.scale < 0.0f)
-#pragma unroll
-        for (uint32_t z = 0; z < QT; ++z)
-#pragma unroll
-            for (uint32_t s = 0; s < KS; ++s) q[z][s] ^= u4v{0x80008000u, 0x80008000u, 0x80008000u, 0x80008000u};
+    const float c = signed_query<AF, HD, 2>(p, row, h, q);
+    const Bits bits;
     const uint32_t page_bytes = p.n_kv * (BLOCK * NG);
     const uint8_t* base = static_cast<const uint8_t*>(p.pool) + block_at(p.layer, p.n_pages, 0u, p.n_kv, kh, NG);
 
@@ -637,7 +653,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 128 ?
             {
                 // positions without a page: NaN keys for the rows that see them
                 const half2_t sb = pair(pg < 0 ? 0x7E007E00u : ks[g]), sc = {sb[0], sb[0]}, ba = {sb[1], sb[1]};
-                const u4v k = {values(codes<0>(kw[g]), sc, ba), values(codes<1>(kw[g]), sc, ba), values(codes<2>(kw[g]), sc, ba), values(codes<3>(kw[g]), sc, ba)};
+                const u4v k = {values(bits.codes<0>(kw[g]), sc, ba), values(bits.codes<1>(kw[g]), sc, ba), values(bits.codes<2>(kw[g]), sc, ba), values(bits.codes<3>(kw[g]), sc, ba)};
                 if (HD % 32 == 0 || g + 1u < NG || lane < 32u) k_at(stage, mine >> 1, 2u * g + (lane >> 5))[to] = k;
             }
         }
@@ -651,8 +667,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 128 ?
                 // slots past the sequence and pages that are not there hold anything: 0
                 const half2_t s0 = pair(vs[g][0] & m0), s1 = pair(vs[g][1] & m1), b0 = pair(vs[g][2] & m0), b1 = pair(vs[g][3] & m1);
                 u2v* to = reinterpret_cast<u2v*>(v_at(stage, mine, g) + (x & 1u) * 32u + (lane & 15u)) + (x >> 1);
-                to[0] = u2v{values(codes<0>(vw[g]), s0, b0), values(codes<1>(vw[g]), s1, b1)};
-                to[32] = u2v{values(codes<2>(vw[g]), s0, b0), values(codes<3>(vw[g]), s1, b1)};   // 16 channels on
+                to[0] = u2v{values(bits.codes<0>(vw[g]), s0, b0), values(bits.codes<1>(vw[g]), s1, b1)};
+                to[32] = u2v{values(bits.codes<2>(vw[g]), s0, b0), values(bits.codes<3>(vw[g]), s1, b1)};   // 16 channels on
             }
         }
     };
@@ -716,7 +732,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 128 ?
                 mx = largest();
             }
             mx = max_xor32(mx);
-            const bool grown = m == NEG_INF ? mx > NEG_INF : __fmul_rn(__fsub_rn(mx, m), c) > ROWS_LAG;
+            const bool grown = m == NEG_INF ? mx > NEG_INF : __fmul_rn(__fsub_rn(mx, m), c) > LAG;
             if (__any(grown))
             {
                 const float to = grown ? mx : m, a = m == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(__fmul_rn(__fsub_rn(m, to), c));
@@ -727,7 +743,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 128 ?
 #pragma unroll
                     for (uint32_t y = 0; y < 16; ++y) o[g][y] = __fmul_rn(o[g][y], a);
             }
-            const float down = m == NEG_INF ? 0.0f : __fsub_rn(ROWS_SHIFT, __fmul_rn(m, c));
+            const float down = m == NEG_INF ? 0.0f : __fsub_rn(SHIFT, __fmul_rn(m, c));
 #pragma unroll
             for (uint32_t x = 0; x < NP; ++x)
             {
