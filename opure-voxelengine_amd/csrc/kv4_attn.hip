@@ -245,15 +245,102 @@ __device__ inline void kv4_row(const WinParams& p, const float* qs, uint32_t b, 
     }
 }
 
-// A workgroup takes a part of the tiles that a sequence's rows see, for 16 NT query
+// How the tiles are shared out: those of all sequences, one sequence's behind the
+// other's, in pieces of one size, so that all workgroups that the device holds have as
+// much to do whatever the lengths are.  A piece is a workgroup of each KV head and block
+// of rows; it may hold the end of a sequence, whole ones and the begin of one.  Piece w's
+// part of sequence b has slot w + b: going on to the next part is going on to the next
+// piece or to the next sequence.
+//   32 sequences of 1,024 to 16,384 positions (8 KV heads of 128): a sixth of each
+// sequence a workgroup 68 us, pieces that end with their sequence 62 to 65.
+struct Share {
+    uint32_t size, total;                                  // tiles of a piece, of all
+    uint32_t b, before;                                    // a sequence, tiles before it
+};
+
+__device__ __forceinline__ WinSpan seq_span(const WinParams& p, const WinSeq& sq) { return win_span<32u>(p, sq, sq.ctx, sq.ctx + p.rows); }
+
+// a sequence's tiles; one at least, so that it has a part
+__device__ __forceinline__ uint32_t seq_tiles(const WinParams& p, uint32_t b)
+{
+    const int32_t len = p.seq_len[b];
+    WinSeq sq;
+    sq.ctx = len < 0 ? 0u : static_cast<uint32_t>(len);
+    sq.total = min(sq.ctx + p.rows, p.cap);
+    return max(seq_span(p, sq).n, 1u);
+}
+
+__device__ __forceinline__ uint32_t sum_lanes(uint32_t v)
+{
+    v += static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0xB1, 0xF, 0xF, true));
+    v += static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x4E, 0xF, 0xF, true));
+    v += static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x141, 0xF, 0xF, true));
+    v += static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(v), 0x140, 0xF, 0xF, true));
+    return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), 0) + __builtin_amdgcn_readlane(static_cast<int>(v), 16) +
+                                 __builtin_amdgcn_readlane(static_cast<int>(v), 32) + __builtin_amdgcn_readlane(static_cast<int>(v), 48));
+}
+
+// n / p.parts, n < 2^31; of n p.parts itself n
+__device__ __forceinline__ uint32_t part_of(const WinParams& p, uint32_t n) { return p.parts == 1u ? n : __umulhi(n, p.by_parts); }
+
+// The shares, and of `u` a piece the sequence that it begins in (PIECE), else sequence u.
+template <bool PIECE>
+__device__ __forceinline__ Share share_out(const WinParams& p, uint32_t u)
+{
+    const uint32_t lane = threadIdx.x & 63u;               // has sequences 4 lane .. 4 lane + 3
+    uint32_t n[4], mine = 0, most = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) n[i] = seq_tiles(p, min(4u * lane + i, p.batch - 1u));
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+    {
+        most = max(most, n[i]);
+        n[i] = 4u * lane + i < p.batch ? n[i] : 0u;
+        mine += n[i];
+    }
+    // as fp32: off by 2^-24 of it, which the room for two more parts covers
+    most = static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(wave_max64(static_cast<float>(most)))));
+    Share s;
+    s.total = sum_lanes(mine);
+    // a sequence's parts, one a piece that it meets, are 64 at most
+    s.size = max(max(part_of(p, s.total) + 1u, most / (MAX_PARTS - 2u) + 1u), p.least);
+    uint32_t before = mine;
+#pragma unroll
+    for (uint32_t o = 1; o < 64u; o <<= 1)
+    {
+        const uint32_t x = __shfl_up(before, o);
+        if (lane >= o) before += x;
+    }
+    before -= mine;
+    const uint32_t at = PIECE ? min(u * s.size, s.total - 1u) : 0u;
+    const uint32_t l = PIECE ? static_cast<uint32_t>(__popcll(__ballot(before <= at && mine != 0u))) - 1u : u >> 2;
+    auto of = [&](uint32_t v) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), static_cast<int>(l))); };
+    s.b = 4u * l;
+    s.before = of(before);
+#pragma unroll
+    for (uint32_t i = 0; i < 3; ++i)
+    {
+        const uint32_t c = of(n[i]);
+        if (s.b == 4u * l + i && (PIECE ? at >= s.before + c : (u & 3u) > i))
+        {
+            s.before += c;
+            ++s.b;
+        }
+    }
+    return s;
+}
+
+// A workgroup takes a piece of the tiles that the sequences' rows see, for 16 NT query
 // rows of a KV head (row qi = j group + head), a wave every fourth tile of 32
-// positions with a running maximum, sum and output of its own in registers.  Lane
+// positions of a sequence's part with a running maximum, sum and output of its own in registers.  Lane
 // (r, g) holds scores of query row r and the tokens 4 g .. 4 g + 3 of both pages,
 // which is its operand P^T in the order that the V codes have.  Each tile's words are
 // asked for when the last one's are used up.  The four waves are merged in LDS, the
 // parts by k_kv4_join.
-template <int AF, int HD, int NT, bool ONCE>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 2 ? 2 : 1))) void k_kv4_split(WinParams p)
+//   PIECES: of one size over all sequences, where they are long; else a workgroup has a
+// part of one sequence, as many of each.
+template <int AF, int HD, int NT, bool ONCE, bool PIECES>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 2 ? 2 : HD > 128 ? 1 : AF == OPURE_A_F32 ? 2 : 3))) void k_kv4_split(WinParams p)
 {
     typedef Kv4Tile<HD, ONCE> T;
     constexpr uint32_t TT = 32u, DT = HD / 16u, NG = T::NG, QT = AF == OPURE_A_F32 ? 2u : 1u;
@@ -263,30 +350,67 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 2 ? 2
     float* cml = reinterpret_cast<float*>(lds + 4u * DT * NT * 64u * 16u);   // [wave][NT][16][2]
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63u, g = lane >> 4, r = lane & 15u;
     const uint32_t G = p.n_heads / p.n_kv, Gq = G * p.rows;
-    // KV heads next to each other, then parts, blocks and sequences
-    const uint32_t kh = blockIdx.x % p.n_kv, rest = blockIdx.x / p.n_kv, part = rest % p.parts;
-    const uint32_t b = rest / p.parts / p.blocks, blk = rest / p.parts - b * p.blocks, q0 = blk * 16u * NT;
-    const int32_t* pt = p.page_table + static_cast<uint64_t>(b) * p.max_pages;
-    const int32_t len = p.seq_len[b];
-    const WinSeq sq = win_seq(p, len);
-    u4v q[NT][QT][NG];
-    uint32_t jr[NT];
-    float c[NT];
-#pragma unroll
-    for (uint32_t n = 0; n < NT; ++n)
+    // KV heads next to each other, then pieces, or parts, blocks of rows and sequences
+    const uint32_t kh = blockIdx.x % p.n_kv, rest = blockIdx.x / p.n_kv, part = PIECES ? rest : rest % p.parts, group = PIECES ? 0u : rest / p.parts;
+    uint32_t b = ONCE ? group : group / p.blocks;
+    const uint32_t blk = ONCE ? 0u : group - b * p.blocks, q0 = blk * 16u * NT;
+    uint32_t before = 0, at0 = 0, at1 = 0;                 // tiles at0 .. at1 - 1 of all, those before sequence b
+    if constexpr (PIECES)
     {
-        const uint32_t qi = min(q0 + 16u * n + r, Gq - 1u);
-        jr[n] = qi / G;
-        c[n] = signed_query<AF, HD, 4>(p, (static_cast<uint64_t>(b) * p.rows + jr[n]) * p.n_heads + kh * G + (qi - jr[n] * G), g, q[n]);
+        const Share share = share_out<true>(p, part);
+        at0 = part * share.size;
+        if (at0 >= share.total) return;                    // pieces that the lengths leave over
+        at1 = min(at0 + share.size, share.total);
+        b = share.b;
+        before = share.before;
     }
     const Bits bits;
     const uint32_t j0 = q0 / G, j1 = min(q0 + 16u * NT - 1u, Gq - 1u) / G;    // the block's first and last row
-    const WinSpan span = win_span<TT>(p, sq, sq.ctx + j0, sq.ctx + j1 + 1u);
-    const uint32_t first = static_cast<uint32_t>(static_cast<uint64_t>(span.n) * part / p.parts);
-    const uint32_t last = static_cast<uint32_t>(static_cast<uint64_t>(span.n) * (part + 1u) / p.parts);
     const uint32_t page_bytes = p.n_kv * (BLOCK * NG);
     const uint8_t* base = static_cast<const uint8_t*>(p.pool) + block_at(p.layer, p.n_pages, 0u, p.n_kv, kh, NG);
-
+    // ---- the piece's part of sequence b: the wave's tiles i, i + 4, .. below last of its list, its queries and first words
+    const int32_t* pt;
+    WinSeq sq;
+    WinSpan span;
+    u4v q[NT][QT][NG];
+    uint32_t jr[NT], i, last, has;
+    float c[NT];
+    int32_t e = -1, pa = -1, pb = -1;
+    T tl;
+    // pages of tile i of the list: -1 past the sequence, missing or not in the pool
+    auto entry = [&](uint32_t i) { return pt[min(span.tile(min(i, span.n - 1u)) * 2u + (lane & 1u), p.max_pages - 1u)]; };
+    auto page = [&](int32_t e, uint32_t i, uint32_t which) -> int32_t {
+        const int32_t pg = __builtin_amdgcn_readlane(e, which);
+        return (span.tile(i) * 2u + which) * OPURE_PAGE_SIZE < sq.total && static_cast<uint32_t>(pg) < p.n_pages ? pg : -1;
+    };
+    auto at = [&](int32_t pg) { return base + static_cast<uint64_t>(pg < 0 ? 0u : static_cast<uint32_t>(pg)) * page_bytes; };
+    auto start = [&]() {
+        pt = p.page_table + static_cast<uint64_t>(b) * p.max_pages;
+        sq = win_seq(p, p.seq_len[b]);
+        span = seq_span(p, sq);
+        has = max(span.n, 1u);
+        i = (PIECES ? at0 - before : part_of(p, span.n * part)) + wave;
+        last = PIECES ? min(min(at1 - before, has), span.n) : part_of(p, span.n * (part + 1u));
+        if (i < last)
+        {
+            e = entry(i);
+            pa = page(e, i, 0u);
+            pb = page(e, i, 1u);
+            tl.load_k(at(pa), at(pb), lane);
+            tl.load_v(at(pa), at(pb), lane);
+            e = entry(i + 4u);
+        }
+#pragma unroll
+        for (uint32_t n = 0; n < NT; ++n)
+        {
+            const uint32_t qi = min(q0 + 16u * n + r, Gq - 1u);
+            jr[n] = qi / G;
+            c[n] = signed_query<AF, HD, 4>(p, (static_cast<uint64_t>(b) * p.rows + jr[n]) * p.n_heads + kh * G + (qi - jr[n] * G), g, q[n]);
+        }
+    };
+    start();
+    while (true)
+    {
     f4_t o[DT][NT];
     float m[NT], l[NT];
 #pragma unroll
@@ -297,22 +421,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 2 ? 2
 #pragma unroll
         for (uint32_t d = 0; d < DT; ++d) o[d][n] = f4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    // pages of tile i of the list: -1 past the sequence, missing or not in the pool
-    auto entry = [&](uint32_t i) { return pt[min(span.tile(min(i, span.n - 1u)) * 2u + (lane & 1u), p.max_pages - 1u)]; };
-    auto page = [&](int32_t e, uint32_t i, uint32_t which) -> int32_t {
-        const int32_t pg = __builtin_amdgcn_readlane(e, which);
-        return (span.tile(i) * 2u + which) * OPURE_PAGE_SIZE < sq.total && static_cast<uint32_t>(pg) < p.n_pages ? pg : -1;
-    };
-    T tl;
-    uint32_t i = first + wave;
     if (i < last)
-    {
-        int32_t e = entry(i);
-        int32_t pa = page(e, i, 0u), pb = page(e, i, 1u);
-        auto at = [&](int32_t pg) { return base + static_cast<uint64_t>(pg < 0 ? 0u : static_cast<uint32_t>(pg)) * page_bytes; };
-        tl.load_k(at(pa), at(pb), lane);
-        tl.load_v(at(pa), at(pb), lane);
-        e = entry(i + 4u);
         while (true)
         {
             const uint32_t t0 = span.tile(i) * TT;
@@ -425,7 +534,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 2 ? 2
             pb = nb;
             i += 4u;
         }
-    }
     settle();
     // ---- the waves' results through LDS, merged in wave order: wave w takes
     //      channel tiles w, w + 4, ... of every block
@@ -441,8 +549,22 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 2 ? 2
             cml[((wave * NT + n) * 16u + r) * 2u + 1u] = l[n];
         }
     }
+    const uint64_t slot = PIECES ? static_cast<uint64_t>(part + b) * p.n_kv + kh : ((static_cast<uint64_t>(b) * p.n_kv + kh) * p.blocks + blk) * p.parts + part;
+    const uint64_t pbase = slot * p.block_rows;
+    bool on = false;
+    if constexpr (PIECES)
+    {
+        // the next sequence's loads on their way while this one's results are merged
+        before += has;
+        at0 = before;
+        on = at0 < at1;
+        if (on)
+        {
+            ++b;
+            start();
+        }
+    }
     __syncthreads();
-    const uint64_t pbase = (((static_cast<uint64_t>(b) * p.n_kv + kh) * p.blocks + blk) * p.parts + part) * p.block_rows;
 #pragma unroll
     for (uint32_t n = 0; n < NT; ++n)
     {
@@ -481,6 +603,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 2 ? 2
             *reinterpret_cast<f4_t*>(p.part_acc + (pbase + qi) * HD + 16u * d + 4u * g) = acc;
         }
     }
+    if (!on) return;
+    __syncthreads();                                       // the merge has read the waves' results
+    }
 }
 
 // Joins the parts: a workgroup a query row (WIDE: many parts, a wave every fourth
@@ -497,9 +622,20 @@ __global__ __launch_bounds__(256) void k_kv4_join(WinParams p)
     if (id >= p.combine_rows) return;                      // never with WIDE: the barrier below
     const uint32_t row = id / p.n_heads, head = id - row * p.n_heads, b = row / p.rows, j = row - b * p.rows;
     const uint32_t kh = head / G, qi = j * G + (head - kh * G), blk = qi >> shift, qb = qi - (blk << shift);
-    const uint32_t parts = p.parts, end = parts - 1u;
-    const uint64_t slot = ((static_cast<uint64_t>(b) * p.n_kv + kh) * p.blocks + blk) * parts;
-    const uint64_t ml = ((slot + min(lane, end)) * p.block_rows + qb) * 2u;
+    // part x's slot is slot + x * step
+    uint32_t parts = p.parts;
+    uint64_t step = 1u, slot = ((static_cast<uint64_t>(b) * p.n_kv + kh) * p.blocks + blk) * parts;
+    if (p.pieces)
+    {
+        // the pieces that hold the sequence's first and last tile
+        const Share share = share_out<false>(p, b);
+        const uint32_t piece = share.before / share.size;
+        parts = (share.before + seq_tiles(p, b) - 1u) / share.size - piece + 1u;
+        step = p.n_kv;
+        slot = (piece + b) * step + kh;
+    }
+    const uint32_t end = parts - 1u;
+    const uint64_t ml = ((slot + min(lane, end) * step) * p.block_rows + qb) * 2u;
     const float pm = p.part_ml[ml], pl = p.part_ml[ml + 1u];
     constexpr uint32_t U = WIDE ? 8u : 4u, BY = WIDE ? 4u : 1u;
     const uint32_t x0 = WIDE ? wave : 0u;
@@ -509,7 +645,7 @@ __global__ __launch_bounds__(256) void k_kv4_join(WinParams p)
         for (uint32_t u = 0; u < U; ++u)
 #pragma unroll
             for (uint32_t i = 0; i < DPL; ++i)
-                v[u][i] = p.part_acc[((slot + min(x + BY * u, end)) * p.block_rows + qb) * p.hd + min(lane + 64u * i, p.hd - 1u)];
+                v[u][i] = p.part_acc[((slot + min(x + BY * u, end) * step) * p.block_rows + qb) * p.hd + min(lane + 64u * i, p.hd - 1u)];
     };
     fetch(x0);
     const float M = wave_max64(lane < parts ? pm : NEG_INF);
@@ -601,8 +737,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 128 ?
     const WinSeq sq = win_seq(p, p.seq_len[b]);
     const uint32_t j0 = q0 / G, j1 = min(q0 + ROWS_BLOCK - 1u, Gq - 1u) / G;
     const WinSpan span = win_span<TT>(p, sq, sq.ctx + j0, sq.ctx + j1 + 1u);
-    const uint32_t first = static_cast<uint32_t>(static_cast<uint64_t>(span.n) * part / p.parts);
-    const uint32_t last = static_cast<uint32_t>(static_cast<uint64_t>(span.n) * (part + 1u) / p.parts);
+    const uint32_t first = span.n * part / p.parts;
+    const uint32_t last = span.n * (part + 1u) / p.parts;
     // the wave's rows
     const uint32_t w0 = min(q0 + 32u * wave, Gq - 1u), w1 = min(q0 + 32u * wave + 31u, Gq - 1u), qi = min(w0 + r, Gq - 1u);
     const uint32_t j = qi / G, pos = sq.ctx + j, pos0 = sq.ctx + w0 / G, pos1 = sq.ctx + w1 / G;
@@ -848,14 +984,14 @@ constexpr uint32_t split_lds() { return 4u * (HD / 16u) * NT * 64u * 16u + 4u * 
 // f(kernel, dynamic LDS, workgroups of it that the device holds at a time) for a head size and format.
 // What a CU holds is asked once a kernel: it is the same on every device that the code is built for.
 template <typename F>
-int split_kernel(opure_dev* dev, uint32_t afmt, uint32_t hd, bool two, bool once, F&& f)
+int split_kernel(opure_dev* dev, uint32_t afmt, uint32_t hd, bool two, bool once, bool pieces, F&& f)
 {
-    auto one = [&](auto af, auto h, auto nt, auto alone) {
+    auto one = [&](auto af, auto h, auto nt, auto alone, auto pc) {
         constexpr int AF = decltype(af)::value, HD = decltype(h)::value, NT = decltype(nt)::value;
-        constexpr bool ONCE = decltype(alone)::value;
+        constexpr bool ONCE = decltype(alone)::value, PIECES = decltype(pc)::value;
         static std::atomic<uint64_t> done{0};
         static std::atomic<int> a_cu{0};
-        auto* kernel = &k_kv4_split<AF, HD, NT, ONCE>;
+        auto* kernel = &k_kv4_split<AF, HD, NT, ONCE, PIECES>;
         const int rc = win_lds(dev, reinterpret_cast<const void*>(kernel), split_lds<HD, NT>(), done);
         if (rc) return rc;
         int n = a_cu.load(std::memory_order_relaxed);
@@ -867,14 +1003,15 @@ int split_kernel(opure_dev* dev, uint32_t afmt, uint32_t hd, bool two, bool once
         }
         return f(kernel, split_lds<HD, NT>(), static_cast<uint32_t>(n) * (dev->n_cu > 0 ? static_cast<uint32_t>(dev->n_cu) : 256u));
     };
+    typedef std::integral_constant<int, 1> One;
     auto by_head = [&](auto af) {
         return win_by_head(hd, [&](auto h) {
             if constexpr (decltype(h)::value <= 128)
             {
-                if (two) return one(af, h, std::integral_constant<int, 2>{}, std::false_type{});
+                if (two) return one(af, h, std::integral_constant<int, 2>{}, std::false_type{}, std::false_type{});
             }
-            else if (!once) return one(af, h, std::integral_constant<int, 1>{}, std::false_type{});
-            return one(af, h, std::integral_constant<int, 1>{}, std::true_type{});
+            else if (!once) return one(af, h, One{}, std::false_type{}, std::false_type{});
+            return pieces ? one(af, h, One{}, std::true_type{}, std::true_type{}) : one(af, h, One{}, std::true_type{}, std::false_type{});
         });
     };
     return afmt == OPURE_A_F32   ? by_head(std::integral_constant<int, OPURE_A_F32>{})
@@ -902,22 +1039,20 @@ int rows_kernel(opure_dev* dev, uint32_t afmt, uint32_t hd, F&& f)
 
 // How a call is split, and its workspace.
 struct Kv4Plan {
-    uint32_t tiles = 0, blocks = 0, block_rows = 0, parts = 0;
-    bool two = false, many = false;                      // blocks of 32 query rows, of 128
+    uint32_t tiles = 0, blocks = 0, block_rows = 0, parts = 0, least = 1;
+    bool two = false, many = false, pieces = false;      // blocks of 32 query rows, of 128; pieces of one size
     uint64_t acc = 0, ml = 0;                            // bytes
     uint64_t bytes() const { return acc + ml; }
 };
 
-// workspace of `groups` blocks of query rows (`rows` in all) in w.parts parts
-int kv4_slots(const opure_attn_kv4_args* a, uint64_t groups, uint64_t rows, Kv4Plan& w)
+// workspace of `slots` parts' outputs, and what a launch can have
+int kv4_slots(const opure_attn_kv4_args* a, uint64_t slots, uint64_t wgs, uint64_t rows, Kv4Plan& w)
 {
-    const uint64_t slots = w.many && w.parts == 1u ? 0u : groups * w.parts * w.block_rows;
-    w.acc = opure_hip::align_up(slots * a->model->head_dim * 4u, 256);
-    w.ml = opure_hip::align_up(slots * 8u, 256);
-    const uint64_t join = w.parts > 8u ? rows : (rows + 3u) / 4u;
-    // a launch's threads, 256 a workgroup, stay in 32 bits
-    OPURE_REQUIRE(std::max(groups * w.parts, join) < 1u << 24, OPURE_E_CAPACITY,
-                  "4-bit attention: %u x %u rows of %u heads over max_ctx %u: too many workgroups", a->batch, a->rows, a->model->n_heads, a->max_ctx);
+    w.acc = opure_hip::align_up(slots * w.block_rows * a->model->head_dim * 4u, 256);
+    w.ml = opure_hip::align_up(slots * w.block_rows * 8u, 256);
+    // a launch's threads, 256 a workgroup (the join's: a row at most), stay in 32 bits
+    OPURE_REQUIRE(std::max(wgs, rows) < 1u << 24, OPURE_E_CAPACITY, "4-bit attention: %u x %u rows of %u heads over max_ctx %u: too many workgroups",
+                  a->batch, a->rows, a->model->n_heads, a->max_ctx);
     return OPURE_OK;
 }
 
@@ -936,23 +1071,42 @@ int kv4_plan(opure_dev* dev, const opure_attn_kv4_args* a, Kv4Plan& w)
         w.blocks = (Gq + ROWS_BLOCK - 1u) / ROWS_BLOCK;
         w.block_rows = std::min(Gq, ROWS_BLOCK);
         w.parts = static_cast<uint32_t>(std::min<uint64_t>(std::max<uint64_t>(1u, 2u * cu / (heads * w.blocks)), std::min((w.tiles + 7u) / 8u, MAX_PARTS)));
-        return kv4_slots(a, heads * w.blocks, rows, w);
+        const uint64_t wgs = heads * w.blocks * w.parts;
+        return kv4_slots(a, w.parts == 1u ? 0u : wgs, wgs, rows, w);
     }
     w.two = Gq > 16u && m->head_dim <= 128u;
     w.blocks = (Gq + (w.two ? 31u : 15u)) / (w.two ? 32u : 16u);
     w.block_rows = std::min(Gq, w.two ? 32u : 16u);
     uint32_t room = 0;
-    const int rc = split_kernel(dev, m->afmt, m->head_dim, w.two, w.blocks == 1u, [&](auto, uint32_t, uint32_t n) {
+    auto holds = [&](auto, uint32_t, uint32_t n) {
         room = n;
         return OPURE_OK;
-    });
-    if (rc) return rc;
+    };
     const uint64_t groups = heads * w.blocks;
-    // Parts of a group: as many as the device holds at a time, each of at least four tiles, one a wave
+    if (w.blocks == 1u && a->batch > 1u)
+    {
+        int rc = split_kernel(dev, m->afmt, m->head_dim, w.two, true, true, holds);
+        if (rc) return rc;
+        const uint64_t hold = std::max<uint64_t>(1u, room / m->n_kv_heads), all = static_cast<uint64_t>(a->batch) * w.tiles;
+        w.pieces = !w.two && all >= 32u * hold;
+        if (w.pieces)
+        {
+            // the sum of the sequences' tiles stays in 31 bits
+            OPURE_REQUIRE(all < 1u << 31, OPURE_E_CAPACITY, "4-bit attention: %u sequences of max_ctx %u", a->batch, a->max_ctx);
+            w.least = 4u;
+            w.parts = static_cast<uint32_t>(hold);
+            return kv4_slots(a, (hold + a->batch - 1u) * m->n_kv_heads, hold * m->n_kv_heads, rows, w);
+        }
+    }
+    const int rc = split_kernel(dev, m->afmt, m->head_dim, w.two, w.blocks == 1u, false, holds);
+    if (rc) return rc;
+    // Parts of a group: as many as the device holds at a time, each of at least four tiles (one a wave), or of so many
+    // that the part's outputs, written and read again, stay a quarter of its keys and values; three times as many where
+    // a wave still has four tiles, which evens out ragged sequences
     const uint32_t least = std::max(4u, w.block_rows / 4u);
     const uint64_t fill = std::max<uint64_t>(1u, room / groups), more = std::min<uint64_t>(3ull * room / groups, w.tiles / 16u);
     w.parts = static_cast<uint32_t>(std::min<uint64_t>(std::max(fill, more), std::min((w.tiles + least - 1u) / least, MAX_PARTS)));
-    return kv4_slots(a, groups, rows, w);
+    return kv4_slots(a, groups * w.parts, groups * w.parts, rows, w);
 }
 
 int kv4_validate(const opure_attn_kv4_args* a)
@@ -1047,15 +1201,19 @@ extern "C" int opure_attn_kv4_paged(opure_dev* dev, const opure_attn_kv4_args* a
     p.two = w.many ? 2u : w.two ? 1u : 0u;
     p.tiles = w.tiles;
     p.combine_rows = a->batch * a->rows * p.n_heads;
-    const uint32_t wgs = p.n_kv * w.parts * w.blocks * a->batch;
+    p.least = w.least;
+    p.pieces = w.pieces ? 1u : 0u;
+    p.by_parts = w.parts > 1u ? static_cast<uint32_t>(((1ull << 32) + w.parts - 1u) / w.parts) : 0u;
+    p.batch = a->batch;
+    const uint32_t wgs = p.n_kv * w.parts * (w.pieces ? 1u : w.blocks * a->batch);
     auto launch = [&](auto kernel, uint32_t lds, uint32_t = 0) {
         OPURE_LAUNCH(dev, kernel, dim3(wgs), dim3(256), lds, p);
         OPURE_LAUNCH_CHECK("4-bit attention");
         return OPURE_OK;
     };
-    rc = w.many ? rows_kernel(dev, p.afmt, p.hd, launch) : split_kernel(dev, p.afmt, p.hd, w.two, w.blocks == 1u, launch);
+    rc = w.many ? rows_kernel(dev, p.afmt, p.hd, launch) : split_kernel(dev, p.afmt, p.hd, w.two, w.blocks == 1u, w.pieces, launch);
     if (rc || (w.many && w.parts == 1u)) return rc;
-    const bool wide = w.parts > 8u;
+    const bool wide = w.parts > (w.pieces ? 8u * a->batch : 8u);
     p.combine_wgs = wide ? p.combine_rows : (p.combine_rows + 3u) / 4u;
     auto join = [&](auto all) {
         constexpr bool WIDE = decltype(all)::value;

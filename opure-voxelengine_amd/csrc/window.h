@@ -35,6 +35,7 @@ struct WinParams {
     uint32_t two;                 // blocks of 32 query rows, not 16
     uint32_t parts;               // parts of each (sequence, KV head, block): slot part + parts * its index
     uint32_t tiles;               // most tiles a sequence's rows see
+    uint32_t pieces, least, by_parts;   // 4-bit attention: parts are pieces of one size, its least; 2^32 / parts, rounded up
     uint32_t combine_rows;        // query rows of the call
     uint32_t combine_wgs;         // k_win_join: its first workgroups join the parts, the others add the weights
     float scale;
