@@ -35,9 +35,10 @@ struct AppendParams {
     uint32_t k_first;                        // the row's first thread of k: q_units to the next four, whose lanes share a group
     uint32_t per_head;                       // 2^32 / (a head's threads among the k_units), rounded up; q_units': q_per_head
     uint32_t q_per_head, v_per_head;
-    uint32_t row_wgs, v_wgs;                 // workgroups a row, a piece
-    uint32_t pieces;                         // most pieces that a sequence's rows touch: pages, or with 4 bits quarters of a page
-    uint32_t row_total;                      // workgroups of all rows; the others are the values'
+    uint32_t batch;
+    uint32_t row_cols, v_cols;               // waves a row, a piece
+    uint32_t pieces;                         // most pieces that a sequence's rows touch: pages, or quarters of one
+    uint32_t v_waves;                        // waves of all pieces; the others are the rows'
     uint32_t* err;
 };
 
@@ -131,86 +132,126 @@ __device__ __forceinline__ int32_t append_page(const AppendParams& p, uint32_t b
     return -1;
 }
 
-// The first workgroups take a row's queries and keys, 8 channels a thread, the
-// others values: with a model's format a page's slots of a channel a thread, which
-// lie next to each other, in 4 bits the four tokens of two channels that share a
-// word.  A word that also holds tokens of before keeps those: each word is written
-// by one thread, whatever rows of the call meet in it.
+// 8 channels of a key from d on to 4 bits: four lanes a group, of half a group the last two
+// have no channels (`there`)
+__device__ __forceinline__ void put_k4(const AppendParams& p, f8_t x, bool there, uint32_t pg, uint32_t h, uint32_t i, uint32_t slot)
+{
+    float lo = __builtin_huge_valf(), hi = -__builtin_huge_valf();
+    bool bad = false;
+    if (there)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+        {
+            bad = bad || !__builtin_isfinite(x[e]);
+            x[e] = fminf(fmaxf(x[e], -MOST), MOST);
+            lo = fminf(lo, x[e]);
+            hi = fmaxf(hi, x[e]);
+        }
+    lo = fminf(lo, dpp_f<0xB1>(lo));
+    lo = fminf(lo, dpp_f<0x4E>(lo));
+    hi = fmaxf(hi, dpp_f<0xB1>(hi));
+    hi = fmaxf(hi, dpp_f<0x4E>(hi));
+    const uint64_t any = __ballot(bad);
+    const Scale sc(lo, hi, (any >> (threadIdx.x & 60u) & 15u) != 0u);
+    uint32_t w = 0;
+    float c[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c[e] = x[e];
+    sc.codes(c);
+    if (there)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w |= static_cast<uint32_t>(c[e]) << (16 * (e & 1) + 4 * (e >> 1));
+    uint8_t* block = static_cast<uint8_t*>(p.pool) + block_at(p.layer, p.n_pages, pg, p.n_kv, h, p.ng);
+    reinterpret_cast<uint32_t*>(block)[((i & 3u) * 16u + slot) * p.ng + (i >> 2)] = w;
+    if ((i & 3u) == 0u) reinterpret_cast<uint32_t*>(block + k_scales(p.ng))[slot * p.ng + (i >> 2)] = sc.scale_bits() | sc.base_bits() << 16;
+}
+
+// Two channels, c and c + 16 of group g (`both`: the second is there), of the tokens t0 .. t0 + 3 to 4
+// bits: sixteen lanes a group.  Tokens outside lo .. hi - 1 keep theirs.
+__device__ __forceinline__ void put_v4(const AppendParams& p, const float (&x)[4][2], bool both, uint32_t pg, uint32_t h, uint32_t g, uint32_t c,
+                                       uint32_t t0, uint32_t lo, uint32_t hi)
+{
+    uint8_t* block = static_cast<uint8_t*>(p.pool) + block_at(p.layer, p.n_pages, pg, p.n_kv, h, p.ng);
+    const uint32_t j = t0 / 4u % 4u;
+    uint32_t* to = reinterpret_cast<uint32_t*>(block + v_codes(p.ng)) + (j * 16u + c) * p.ng + g;
+    uint16_t* sb = reinterpret_cast<uint16_t*>(block + v_scales(p.ng)) + (j * p.ng + g) * 8u;
+    uint32_t w = 0, mine = 0;
+#pragma unroll
+    for (uint32_t t = 0; t < 4; ++t)
+    {
+        const bool bad = !__builtin_isfinite(x[t][0]) || !__builtin_isfinite(x[t][1]);
+        const float y0 = fminf(fmaxf(x[t][0], -MOST), MOST), y1 = fminf(fmaxf(x[t][1], -MOST), MOST);
+        float mn = fminf(y0, y1), mx = fmaxf(y0, y1);
+        mn = fminf(mn, dpp_f<0xB1>(mn));
+        mn = fminf(mn, dpp_f<0x4E>(mn));
+        mn = fminf(mn, dpp_f<0x141>(mn));
+        mn = fminf(mn, dpp_f<0x140>(mn));
+        mx = fmaxf(mx, dpp_f<0xB1>(mx));
+        mx = fmaxf(mx, dpp_f<0x4E>(mx));
+        mx = fmaxf(mx, dpp_f<0x141>(mx));
+        mx = fmaxf(mx, dpp_f<0x140>(mx));
+        const Scale sc(mn, mx, (__ballot(bad) >> (threadIdx.x & 48u) & 0xFFFFu) != 0u);
+        if (t0 + t < lo || t0 + t >= hi) continue;
+        const uint32_t shift = 16u * (t & 1u) + 4u * (t >> 1);
+        float y[2] = {y0, y1};
+        sc.codes(y);
+        w |= static_cast<uint32_t>(y[0]) << shift;
+        if (both) w |= static_cast<uint32_t>(y[1]) << (shift + 8u);
+        mine |= 0x0F0Fu << shift;
+        if (c == 0u)
+        {
+            sb[t] = static_cast<uint16_t>(sc.scale_bits());
+            sb[4u + t] = static_cast<uint16_t>(sc.base_bits());
+        }
+    }
+    *to = mine == 0xFFFFFFFFu ? w : w | (*to & ~mine);
+}
+
+// The first waves take values: with a model's format a page's slots of a channel a
+// thread, which lie next to each other, in 4 bits the four tokens of two channels that
+// share a word.  A word that also holds tokens of before keeps those: each word is
+// written by one thread, whatever rows of the call meet in it.  The others take queries
+// and keys, 8 channels of a row a thread.  Many short waves: with four rows a wave 2,874
+// rows of 32 + 16 heads of 64 take 14.8 us for 12.4, and the values' longer waves at the
+// end, behind the others, cost 4.
 template <int XF, int AF, bool I4>
 __global__ __launch_bounds__(256) void k_kv_append(AppendParams p)
 {
-    const uint32_t tid = threadIdx.x;
-    if (blockIdx.x < p.row_total)
+    const uint32_t lane = threadIdx.x & 63u;
+    const uint32_t id = __builtin_amdgcn_readfirstlane(4u * blockIdx.x + (threadIdx.x >> 6));
+    if (id >= p.v_waves)
     {
-        const uint32_t row = blockIdx.x / p.row_wgs, b = row / p.rows, j = row - b * p.rows;
-        uint32_t u = (blockIdx.x - row * p.row_wgs) * 256u + tid;
+        const uint32_t row_id = id - p.v_waves, row = row_id / p.row_cols, b = row / p.rows;
+        uint32_t u = (row_id - row * p.row_cols) * 64u + lane;
+        if (b >= p.batch) return;                         // the last workgroup's waves past the end
         const AppendSeq sq(p, b);
-        if (sq.bad && tid == 0u) p.err[ERR_POSITION] = 1u;
-        const uint32_t pos = sq.first + j;
+        if (sq.bad && lane == 0u) p.err[ERR_POSITION] = 1u;
+        const uint32_t pos = sq.first + (row - b * p.rows);
         if (pos >= sq.end) return;
         if (u < p.q_units)
         {
-            const uint32_t h = div_by(u, p.q_per_head), d = 8u * u - h * p.hd;
-            store8<AF>(p.q_out, static_cast<uint64_t>(row) * p.heads * p.hd + 8u * u,
-                       turn8(p, load8<XF>(p.q, row * p.q_stride + 8u * u), pos, d));
+            const uint32_t d = 8u * u - div_by(u, p.q_per_head) * p.hd;
+            store8<AF>(p.q_out, static_cast<uint64_t>(row) * p.heads * p.hd + 8u * u, turn8(p, load8<XF>(p.q, row * p.q_stride + 8u * u), pos, d));
             return;
         }
         u -= p.k_first;                                   // wraps between q_units and k_first
         if (u >= p.k_units) return;
         const int32_t pg = append_page(p, b, pos);
         if (pg < 0) return;
-        const uint32_t h = div_by(u, p.per_head), slot = pos % OPURE_PAGE_SIZE;
-        if constexpr (!I4)
-        {
-            const uint32_t d = 8u * u - h * p.hd;
-            store8<AF>(p.pool, kv_elem(p.layer, p.n_pages, static_cast<uint32_t>(pg), 0u, p.n_kv, h, p.hd, slot, d),
-                       turn8(p, load8<XF>(p.k, row * p.k_stride + 8u * u), pos, d));
-        }
-        else
-        {
-            // four lanes a group; of half a group the last two have no channels
-            const uint32_t i = u - h * 4u * p.ng, d = 8u * i;
-            const bool there = d < p.hd;
-            f8_t x = {};
-            float lo = __builtin_huge_valf(), hi = -__builtin_huge_valf();
-            bool bad = false;
-            if (there)
-            {
-                x = turn8(p, load8<XF>(p.k, row * p.k_stride + h * p.hd + d), pos, d);
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                {
-                    bad = bad || !__builtin_isfinite(x[e]);
-                    x[e] = fminf(fmaxf(x[e], -MOST), MOST);
-                    lo = fminf(lo, x[e]);
-                    hi = fmaxf(hi, x[e]);
-                }
-            }
-            lo = fminf(lo, dpp_f<0xB1>(lo));
-            lo = fminf(lo, dpp_f<0x4E>(lo));
-            hi = fmaxf(hi, dpp_f<0xB1>(hi));
-            hi = fmaxf(hi, dpp_f<0x4E>(hi));
-            const uint64_t any = __ballot(bad);
-            const Scale sc(lo, hi, (any >> (tid & 60u) & 15u) != 0u);
-            uint32_t w = 0;
-            if (there)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) w |= sc.code(x[e]) << (16 * (e & 1) + 4 * (e >> 1));
-            uint8_t* block = static_cast<uint8_t*>(p.pool) + block_at(p.layer, p.n_pages, static_cast<uint32_t>(pg), p.n_kv, h, p.ng);
-            reinterpret_cast<uint32_t*>(block)[((i & 3u) * 16u + slot) * p.ng + (i >> 2)] = w;
-            if ((i & 3u) == 0u)
-                reinterpret_cast<uint32_t*>(block + k_scales(p.ng))[slot * p.ng + (i >> 2)] = sc.scale_bits() | sc.base_bits() << 16;
-        }
+        const uint32_t h = div_by(u, p.per_head), i = u - h * (I4 ? 4u * p.ng : p.hd / 8u), d = 8u * i, slot = pos % OPURE_PAGE_SIZE;
+        const bool there = !I4 || d < p.hd;
+        f8_t x = {};
+        if (there) x = turn8(p, load8<XF>(p.k, row * p.k_stride + h * p.hd + d), pos, d);
+        if constexpr (I4) put_k4(p, x, there, static_cast<uint32_t>(pg), h, i, slot);
+        else store8<AF>(p.pool, kv_elem(p.layer, p.n_pages, static_cast<uint32_t>(pg), 0u, p.n_kv, h, p.hd, slot, d), x);
         return;
     }
-    const uint32_t id = blockIdx.x - p.row_total, piece = id / p.v_wgs, u = (id - piece * p.v_wgs) * 256u + tid;
-    const uint32_t b = piece / p.pieces, i = piece - b * p.pieces;
+    const uint32_t piece = id / p.v_cols, u = (id - piece * p.v_cols) * 64u + lane, b = piece / p.pieces, i = piece - b * p.pieces;
     const AppendSeq sq(p, b);
-    constexpr uint32_t N = I4 ? 4u : OPURE_PAGE_SIZE;    // positions of a piece
-    const uint32_t t0 = (sq.first / N + i) * N;          // its first
-    const uint32_t lo = max(t0, sq.first), hi = min(t0 + N, sq.end);
+    constexpr uint32_t N = I4 ? 4u : OPURE_PAGE_SIZE;     // positions of a piece
+    const uint32_t first = (sq.first / N + i) * N, lo = max(first, sq.first), hi = min(first + N, sq.end);
     if (lo >= hi || u >= p.v_units) return;
-    const int32_t pg = append_page(p, b, t0);
+    const int32_t pg = append_page(p, b, first);
     if (pg < 0) return;
     const uint64_t row0 = static_cast<uint64_t>(b) * p.rows - sq.first;     // a position's row, modulo 2^64
     if constexpr (!I4)
@@ -221,12 +262,12 @@ __global__ __launch_bounds__(256) void k_kv_append(AppendParams p)
         {
             float x[N];
 #pragma unroll
-            for (uint32_t t = 0; t < N; ++t) x[t] = load_act<XF>(p.v, (row0 + t0 + t) * p.v_stride + u);
+            for (uint32_t t = 0; t < N; ++t) x[t] = load_act<XF>(p.v, (row0 + first + t) * p.v_stride + u);
 #pragma unroll
             for (uint32_t t = 0; t < N; t += 8u) store8<AF>(p.pool, at + t, f8_t{x[t], x[t + 1], x[t + 2], x[t + 3], x[t + 4], x[t + 5], x[t + 6], x[t + 7]});
         }
         else
-            for (uint32_t t = lo; t < hi; ++t) store_act_rt(p.pool, at + (t - t0), load_act<XF>(p.v, (row0 + t) * p.v_stride + u), AF);
+            for (uint32_t t = lo; t < hi; ++t) store_act_rt(p.pool, at + (t - first), load_act<XF>(p.v, (row0 + t) * p.v_stride + u), AF);
     }
     else
     {
@@ -237,42 +278,11 @@ __global__ __launch_bounds__(256) void k_kv_append(AppendParams p)
 #pragma unroll
         for (uint32_t t = 0; t < 4; ++t)
         {
-            const uint64_t at = (row0 + min(max(t0 + t, lo), hi - 1u)) * p.v_stride + h * p.hd + d;
+            const uint64_t at = (row0 + min(max(first + t, lo), hi - 1u)) * p.v_stride + h * p.hd + d;
             x[t][0] = load_act<XF>(p.v, at);
             x[t][1] = both ? load_act<XF>(p.v, at + 16u) : x[t][0];
         }
-        uint8_t* block = static_cast<uint8_t*>(p.pool) + block_at(p.layer, p.n_pages, static_cast<uint32_t>(pg), p.n_kv, h, p.ng);
-        const uint32_t j = t0 / 4u % 4u;
-        uint32_t* to = reinterpret_cast<uint32_t*>(block + v_codes(p.ng)) + (j * 16u + c) * p.ng + g;
-        uint16_t* sb = reinterpret_cast<uint16_t*>(block + v_scales(p.ng)) + (j * p.ng + g) * 8u;
-        uint32_t w = 0, mine = 0;
-#pragma unroll
-        for (uint32_t t = 0; t < 4; ++t)
-        {
-            const bool bad = !__builtin_isfinite(x[t][0]) || !__builtin_isfinite(x[t][1]);
-            const float y0 = fminf(fmaxf(x[t][0], -MOST), MOST), y1 = fminf(fmaxf(x[t][1], -MOST), MOST);
-            float mn = fminf(y0, y1), mx = fmaxf(y0, y1);
-            mn = fminf(mn, dpp_f<0xB1>(mn));
-            mn = fminf(mn, dpp_f<0x4E>(mn));
-            mn = fminf(mn, dpp_f<0x141>(mn));
-            mn = fminf(mn, dpp_f<0x140>(mn));
-            mx = fmaxf(mx, dpp_f<0xB1>(mx));
-            mx = fmaxf(mx, dpp_f<0x4E>(mx));
-            mx = fmaxf(mx, dpp_f<0x141>(mx));
-            mx = fmaxf(mx, dpp_f<0x140>(mx));
-            const Scale sc(mn, mx, (__ballot(bad) >> (tid & 48u) & 0xFFFFu) != 0u);
-            if (t0 + t < lo || t0 + t >= hi) continue;
-            const uint32_t shift = 16u * (t & 1u) + 4u * (t >> 1);
-            w |= sc.code(y0) << shift;
-            if (both) w |= sc.code(y1) << (shift + 8u);
-            mine |= 0x0F0Fu << shift;
-            if (c == 0u)
-            {
-                sb[t] = static_cast<uint16_t>(sc.scale_bits());
-                sb[4u + t] = static_cast<uint16_t>(sc.base_bits());
-            }
-        }
-        *to = mine == 0xFFFFFFFFu ? w : w | (*to & ~mine);
+        put_v4(p, x, both, static_cast<uint32_t>(pg), h, g, c, first, lo, hi);
     }
 }
 
@@ -394,15 +404,16 @@ extern "C" int opure_kv_append(opure_dev* dev, const opure_kv_append_args* a)
     p.per_head = i4 ? magic(4u * p.ng) : p.q_per_head;
     p.v_units = p.n_kv * (i4 ? 16u * p.ng : p.hd);
     p.v_per_head = magic(i4 ? 16u * p.ng : p.hd);
-    p.row_wgs = up_div(p.k_first + p.k_units, 256u);
-    p.v_wgs = up_div(p.v_units, 256u);
+    p.row_cols = up_div(p.k_first + p.k_units, 64u);
+    p.batch = a->batch;
+    p.v_cols = up_div(p.v_units, 64u);
     p.pieces = i4 ? (a->rows + 2u) / 4u + 1u : (a->rows + 14u) / 16u + 1u;
-    p.row_total = static_cast<uint32_t>(n) * p.row_wgs;
-    const uint64_t wgs = p.row_total + static_cast<uint64_t>(a->batch) * p.pieces * p.v_wgs;
-    OPURE_REQUIRE(n * p.row_wgs < 1u << 24 && wgs < 1u << 24, OPURE_E_CAPACITY, "opure_kv_append: too many workgroups");
+    const uint64_t v_waves = static_cast<uint64_t>(a->batch) * p.pieces * p.v_cols, waves = v_waves + static_cast<uint64_t>(a->batch) * a->rows * p.row_cols;
+    OPURE_REQUIRE(waves < 1u << 26, OPURE_E_CAPACITY, "opure_kv_append: too many workgroups");
+    p.v_waves = static_cast<uint32_t>(v_waves);
     auto go = [&](auto xf, auto af) {
         constexpr int XF = decltype(xf)::value, AF = decltype(af)::value;
-        const dim3 grid(static_cast<uint32_t>(wgs)), block(256);
+        const dim3 grid(up_div(waves, 4u)), block(256);
         if (i4) OPURE_LAUNCH(dev, (k_kv_append<XF, AF, true>), grid, block, 0, p);
         else OPURE_LAUNCH(dev, (k_kv_append<XF, AF, false>), grid, block, 0, p);
     };

@@ -63,10 +63,28 @@ struct Scale {
         s = round_half(__fmul_rn(__fsub_rn(hi, lo), static_cast<float>(1.0 / 15.0)));
         b = round_half(__fsub_rn(lo, __fmul_rn(16.0f, static_cast<float>(s))));
     }
-    __device__ __forceinline__ uint32_t code(float x) const
+    // The group's values to their codes: rint((x - base) / scale - 16).  A product with the scale's reciprocal is off
+    // by 2^-18 at most (t < 32: three roundings of 2^-24 of it each), so it decides but for what lies nearer to the
+    // middle of two codes; there the quotient does (2,874 rows of 16 heads of 64: 12.4 us with quotients alone).
+    template <int N>
+    __device__ __forceinline__ void codes(float (&x)[N]) const
     {
-        const float c = __builtin_rintf(__fsub_rn(__fdiv_rn(__fsub_rn(x, static_cast<float>(b)), static_cast<float>(s)), 16.0f));
-        return bad || s == static_cast<_Float16>(0) ? 0u : static_cast<uint32_t>(fminf(fmaxf(c, 0.0f), 15.0f));
+        const float sf = static_cast<float>(s), bf = static_cast<float>(b), inv = __fdiv_rn(1.0f, sf);
+        float c[N];
+        bool near = false;
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+        {
+            const float f = __fmaf_rn(__fsub_rn(x[i], bf), inv, -16.0f);
+            c[i] = __builtin_rintf(f);
+            near = near || __builtin_fabsf(__fsub_rn(f, c[i])) > 0.5f - 0x1p-16f;
+        }
+        if (__any(near))
+#pragma unroll
+            for (int i = 0; i < N; ++i) c[i] = __builtin_rintf(__fsub_rn(__fdiv_rn(__fsub_rn(x[i], bf), sf), 16.0f));
+        const bool none = bad || s == static_cast<_Float16>(0);
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] = none ? 0.0f : fminf(fmaxf(c[i], 0.0f), 15.0f);
     }
     __device__ __forceinline__ uint32_t scale_bits() const { return bad ? 0x7E00u : half_bits(s); }
     __device__ __forceinline__ uint32_t base_bits() const { return bad ? 0x7E00u : half_bits(b); }
