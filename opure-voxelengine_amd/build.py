@@ -25,7 +25,7 @@ ENGINE_LIB = os.path.join(LIB, "libopure_engine.so")
 
 ARCH = "gfx950"
 HIP_SOURCES = ["runtime.hip", "gemv.hip", "gemv_f32.hip", "gemv_i8.hip", "gemv_i4h.hip", "gemv_i4b.hip",
-               "attention.hip", "window.hip", "window_prompt.hip", "evict.hip", "append.hip", "kv4_attn.hip", "logprobs.hip", "accept.hip", "verify.hip"]
+               "attention.hip", "window.hip", "window_prompt.hip", "evict.hip", "append.hip", "kv4_attn.hip", "kv4_one.hip", "kv4_rows.hip", "logprobs.hip", "accept.hip", "verify.hip"]
 # -ffp-contract=off: every float expression rounds as written (fmas are
 # explicit __fmaf_rn), like the CPU oracle.  Packed-fp32 instructions stay
 # off: they are emitted only from plain float
