@@ -145,7 +145,10 @@ def attention(cache, layer, q, afmt, heads, seq, rows, window, sinks, scale):
     The bound counts, for each score, its 32-bit sum (hd + 2 roundings of its terms' magnitudes) and what the
     row's fp16 form leaves out (bf16: 2^-34 of the row's largest magnitude; fp32, as two numbers: 2^-22 of each
     and that), entering the weight twice (itself and the sum), 2^-20 for the exponential and the sums of
-    positive terms, the weight's rounding (2^-11 as one fp16 number, 2^-22 as two) and one rounding of the result."""
+    positive terms, the weight's rounding (2^-11 as one fp16 number, 2^-22 as two) and one rounding of the result;
+    and fp16's smallest step, 2^-24: a weight is held as 2^12 e^(s - m), m at least the largest score seen less
+    3 ln 2, so that half a step is 2^-37 of a weight whose row sums to 1 or more.  A sum in which all that
+    counts lies there (the larger weights' values are 0 exactly) is off by as much of the values' magnitudes."""
     B, hd, G = len(seq), cache.hd, heads // cache.n_kv
     out = np.zeros((B, rows, heads, hd))
     tol = np.zeros_like(out)
@@ -173,12 +176,13 @@ def attention(cache, layer, q, afmt, heads, seq, rows, window, sinks, scale):
                         ds = ds + 2.0 ** -22 * size
                     ds = np.where(m & np.isfinite(ds), ds, 0).max(1, keepdims=True)
                     if np.isfinite(v).all():
-                        out[b, :, h * G + g], mag = w @ v, w @ np.abs(v)
+                        out[b, :, h * G + g], mag, least = w @ v, w @ np.abs(v), m @ np.abs(v)
                     else:
                         vz = np.where(m[:, :, None], v[None], 0.0)
                         out[b, :, h * G + g], mag = np.einsum("rt,rtd->rd", w, vz), np.einsum("rt,rtd->rd", w, np.abs(vz))
+                        least = np.abs(vz).sum(1)
                 rel = 2 * ds + 2.0 ** -20 + (2.0 ** -11 if afmt == H.A_BF16 else 2.0 ** -22)
-                tol[b, :, h * G + g] = u * np.abs(out[b, :, h * G + g]) * (1 + u) + rel * mag + 1e-30
+                tol[b, :, h * G + g] = u * np.abs(out[b, :, h * G + g]) * (1 + u) + rel * mag + 2.0 ** -37 * least + 1e-30
                 if afmt == H.A_F16:
                     tol[b, :, h * G + g] += 2.0 ** -24        # half a step of fp16's smallest values
     return out, tol
