@@ -84,36 +84,36 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 128 ?
     auto v_at = [&](uint32_t stage, uint32_t page, uint32_t g) {
         return reinterpret_cast<u4v*>(lds + stage * rows_stage<HD>() + NP * KS * 512u + (page * NG + g) * 1024u);
     };
+    // K's and V's group g of tile i
+    auto store_k = [&](uint32_t i, uint32_t g) {
+        const uint32_t to = (lane >> 4 & 1u) * 32u + (mine & 1u) * 16u + (lane & 15u);
+        // positions without a page: NaN keys for the rows that see them
+        const half2_t sb = pair(pg < 0 ? 0x7E007E00u : ks[g]), sc = {sb[0], sb[0]}, ba = {sb[1], sb[1]};
+        const u4v k = {values(bits.codes<0>(kw[g]), sc, ba), values(bits.codes<1>(kw[g]), sc, ba), values(bits.codes<2>(kw[g]), sc, ba), values(bits.codes<3>(kw[g]), sc, ba)};
+        if (HD % 32 == 0 || g + 1u < NG || lane < 32u) k_at(i & 1u, mine >> 1, 2u * g + (lane >> 5))[to] = k;
+    };
+    auto store_v = [&](uint32_t i, uint32_t g) {
+        const uint32_t x = lane >> 4, t = span.tile(i) * TT + 16u * mine + 4u * x, n = pg < 0 || t >= sq.total ? 0u : min(sq.total - t, 4u);
+        const uint32_t m0 = n >= 2u ? 0xFFFFFFFFu : n == 1u ? 0xFFFFu : 0u, m1 = n >= 4u ? 0xFFFFFFFFu : n == 3u ? 0xFFFFu : 0u;
+        // slots past the sequence and pages that are not there hold anything: 0
+        const half2_t s0 = pair(vs[g][0] & m0), s1 = pair(vs[g][1] & m1), b0 = pair(vs[g][2] & m0), b1 = pair(vs[g][3] & m1);
+        u2v* to = reinterpret_cast<u2v*>(v_at(i & 1u, mine, g) + (x & 1u) * 32u + (lane & 15u)) + (x >> 1);
+        to[0] = u2v{values(bits.codes<0>(vw[g]), s0, b0), values(bits.codes<1>(vw[g]), s1, b1)};
+        to[32] = u2v{values(bits.codes<2>(vw[g]), s0, b0), values(bits.codes<3>(vw[g]), s1, b1)};   // 16 channels on
+    };
     auto store = [&](uint32_t i) {
-        const uint32_t stage = i & 1u, t0 = span.tile(i) * TT + 16u * mine;
         if (has_k)
-        {
-            const uint32_t to = (lane >> 4 & 1u) * 32u + (mine & 1u) * 16u + (lane & 15u);
 #pragma unroll
-            for (uint32_t g = 0; g < NG; ++g)
-            {
-                // positions without a page: NaN keys for the rows that see them
-                const half2_t sb = pair(pg < 0 ? 0x7E007E00u : ks[g]), sc = {sb[0], sb[0]}, ba = {sb[1], sb[1]};
-                const u4v k = {values(bits.codes<0>(kw[g]), sc, ba), values(bits.codes<1>(kw[g]), sc, ba), values(bits.codes<2>(kw[g]), sc, ba), values(bits.codes<3>(kw[g]), sc, ba)};
-                if (HD % 32 == 0 || g + 1u < NG || lane < 32u) k_at(stage, mine >> 1, 2u * g + (lane >> 5))[to] = k;
-            }
-        }
+            for (uint32_t g = 0; g < NG; ++g) store_k(i, g);
         if (has_v)
-        {
-            const uint32_t x = lane >> 4, t = t0 + 4u * x, n = pg < 0 || t >= sq.total ? 0u : min(sq.total - t, 4u);
-            const uint32_t m0 = n >= 2u ? 0xFFFFFFFFu : n == 1u ? 0xFFFFu : 0u, m1 = n >= 4u ? 0xFFFFFFFFu : n == 3u ? 0xFFFFu : 0u;
 #pragma unroll
-            for (uint32_t g = 0; g < NG; ++g)
-            {
-                // slots past the sequence and pages that are not there hold anything: 0
-                const half2_t s0 = pair(vs[g][0] & m0), s1 = pair(vs[g][1] & m1), b0 = pair(vs[g][2] & m0), b1 = pair(vs[g][3] & m1);
-                u2v* to = reinterpret_cast<u2v*>(v_at(stage, mine, g) + (x & 1u) * 32u + (lane & 15u)) + (x >> 1);
-                to[0] = u2v{values(bits.codes<0>(vw[g]), s0, b0), values(bits.codes<1>(vw[g]), s1, b1)};
-                to[32] = u2v{values(bits.codes<2>(vw[g]), s0, b0), values(bits.codes<3>(vw[g]), s1, b1)};   // 16 channels on
-            }
-        }
+            for (uint32_t g = 0; g < NG; ++g) store_v(i, g);
     };
 
+    // what is written on its two sides stays there
+    auto apart = []() {
+        if constexpr (!SPLIT) __builtin_amdgcn_sched_barrier(0);
+    };
     f16_t o[NG];
     float m = NEG_INF, l = 0.0f;                            // the maximum in units of the products; this lane's share of the sum
 #pragma unroll
@@ -126,94 +126,127 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 128 ?
         fetch(first);
         entry(first + 1u);
         store(first);
+        if constexpr (!SPLIT)
+        {
+            fetch(min(first + 1u, last - 1u));
+            entry(first + 2u);
+        }
     }
     __syncthreads();
     for (uint32_t i = first; i < last; ++i)
     {
         const uint32_t stage = i & 1u, t0 = span.tile(i) * TT;
-        const bool more = i + 1u < last;
-        if (more) fetch(i + 1u);
-        entry(i + 2u);
-        // a tile that none of the wave's rows sees is left out
-        const bool none = t0 > pos1 || (t0 >= p.sinks && static_cast<uint64_t>(t0) + TT - 1u + p.window <= pos0);
-        if (!none)
+        if constexpr (SPLIT)
         {
-            f16_t s[NP / 2u];
+            if (i + 1u < last) fetch(i + 1u);
+            entry(i + 2u);
+        }
+        f16_t s[NP / 2u];
+#pragma unroll
+        for (uint32_t x = 0; x < NP / 2u; ++x)
+#pragma unroll
+            for (uint32_t y = 0; y < 16; ++y) s[x][y] = 0.0f;
+        u4v k[2][NP / 2u];
+        auto read_k = [&](uint32_t d) {
+#pragma unroll
+            for (uint32_t x = 0; x < NP / 2u; ++x) k[d & 1u][x] = k_at(stage, x, d)[lane];
+        };
+        read_k(0u);
+        apart();
+#pragma unroll
+        for (uint32_t d = 0; d < 2u * NG; ++d)
+        {
+            if (d + 1u < KS) read_k(d + 1u);
+            if (d < KS)
+#pragma unroll
+                for (uint32_t x = 0; x < NP / 2u; ++x)
+#pragma unroll
+                    for (uint32_t z = 0; z < QT; ++z) s[x] = mfma_32(k[d & 1u][x], q[z][d], s[x]);
+            if constexpr (!SPLIT)
+            {
+                if (d & 1u) store_v(i + 1u, d >> 1);
+                else store_k(i + 1u, d >> 1);
+            }
+            apart();
+        }
+        auto largest = [&]() {
+            float v = s[0][0];
 #pragma unroll
             for (uint32_t x = 0; x < NP / 2u; ++x)
+#pragma unroll
+                for (uint32_t y = 0; y < 16; ++y) v = fmaxf(v, s[x][y]);
+            return v;
+        };
+        float mx = settled(largest());
+        if constexpr (!SPLIT)
+        {
+            if (i + 2u < last) fetch(i + 2u);
+            entry(i + 3u);
+        }
+        // every row of the wave sees every position
+        const bool full = t0 + TT <= min(pos0 + 1u, sq.total) && (t0 + TT <= p.sinks || t0 + p.window > pos1);
+        if (!full)
+        {
+            const WinMask mask(p, pos, sq.total, t0 + 4u * h);
+#pragma unroll
+            for (uint32_t x = 0; x < NP / 2u; ++x)
+#pragma unroll
+                for (uint32_t y = 0; y < 16; ++y) s[x][y] = mask.sees(static_cast<int32_t>(32u * x + 8u * (y >> 2) + (y & 3u))) ? s[x][y] : NEG_INF;
+            mx = largest();
+        }
+        mx = max_xor32(mx);
+        const bool grown = m == NEG_INF ? mx > NEG_INF : __fmul_rn(__fsub_rn(mx, m), c) > LAG;
+        if (__any(grown))
+        {
+            const float to = grown ? mx : m, a = m == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(__fmul_rn(__fsub_rn(m, to), c));
+            m = to;
+            l = __fmul_rn(l, a);
+#pragma unroll
+            for (uint32_t g = 0; g < NG; ++g)
+#pragma unroll
+                for (uint32_t y = 0; y < 16; ++y) o[g][y] = __fmul_rn(o[g][y], a);
+        }
+        const float down = m == NEG_INF ? 0.0f : __fsub_rn(SHIFT, __fmul_rn(m, c));
+        u4v hi[2], lo[2], v[2][NG];
+        auto read_v = [&](uint32_t x) {
+#pragma unroll
+            for (uint32_t g = 0; g < NG; ++g) v[x & 1u][g] = v_at(stage, x, g)[lane];
+        };
+        // two of a page's eight weights
+        auto weigh = [&](uint32_t x, uint32_t y) {
+            const float e0 = __builtin_amdgcn_exp2f(__fmaf_rn(s[x >> 1][8u * (x & 1u) + 2u * y], c, down));
+            const float e1 = __builtin_amdgcn_exp2f(__fmaf_rn(s[x >> 1][8u * (x & 1u) + 2u * y + 1u], c, down));
+            l += e0;
+            l += e1;
+            const uint32_t w = win_pack<OPURE_A_F16>(e0, e1);
+            hi[x & 1u][y] = w;
+            if constexpr (REST) lo[x & 1u][y] = win_pack<OPURE_A_F16>(__fsub_rn(e0, win_low<OPURE_A_F16>(w)), __fsub_rn(e1, win_high<OPURE_A_F16>(w)));
+        };
+        read_v(0u);
+        apart();
+#pragma unroll
+        for (uint32_t y = 0; y < 4; ++y) weigh(0u, y);
+#pragma unroll
+        for (uint32_t x = 0; x < NP; ++x)
+        {
+            if (x + 1u < NP) read_v(x + 1u);
+            apart();
+#pragma unroll
+            for (uint32_t g = 0; g < std::max(NG, 4u); ++g)
             {
-#pragma unroll
-                for (uint32_t y = 0; y < 16; ++y) s[x][y] = 0.0f;
-#pragma unroll
-                for (uint32_t d = 0; d < KS; ++d)
+                if (g < NG)
                 {
-                    const u4v k = k_at(stage, x, d)[lane];
-#pragma unroll
-                    for (uint32_t z = 0; z < QT; ++z) s[x] = mfma_32(k, q[z][d], s[x]);
+                    if constexpr (REST) o[g] = mfma_32(v[x & 1u][g], lo[x & 1u], o[g]);
+                    o[g] = mfma_32(v[x & 1u][g], hi[x & 1u], o[g]);
                 }
-            }
-            auto largest = [&]() {
-                float v = s[0][0];
-#pragma unroll
-                for (uint32_t x = 0; x < NP / 2u; ++x)
-#pragma unroll
-                    for (uint32_t y = 0; y < 16; ++y) v = fmaxf(v, s[x][y]);
-                return v;
-            };
-            float mx = settled(largest());
-            // every row of the wave sees every position
-            const bool full = t0 + TT <= min(pos0 + 1u, sq.total) && (t0 + TT <= p.sinks || t0 + p.window > pos1);
-            if (!full)
-            {
-                const WinMask mask(p, pos, sq.total, t0 + 4u * h);
-#pragma unroll
-                for (uint32_t x = 0; x < NP / 2u; ++x)
-#pragma unroll
-                    for (uint32_t y = 0; y < 16; ++y) s[x][y] = mask.sees(static_cast<int32_t>(32u * x + 8u * (y >> 2) + (y & 3u))) ? s[x][y] : NEG_INF;
-                mx = largest();
-            }
-            mx = max_xor32(mx);
-            const bool grown = m == NEG_INF ? mx > NEG_INF : __fmul_rn(__fsub_rn(mx, m), c) > LAG;
-            if (__any(grown))
-            {
-                const float to = grown ? mx : m, a = m == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(__fmul_rn(__fsub_rn(m, to), c));
-                m = to;
-                l = __fmul_rn(l, a);
-#pragma unroll
-                for (uint32_t g = 0; g < NG; ++g)
-#pragma unroll
-                    for (uint32_t y = 0; y < 16; ++y) o[g][y] = __fmul_rn(o[g][y], a);
-            }
-            const float down = m == NEG_INF ? 0.0f : __fsub_rn(SHIFT, __fmul_rn(m, c));
-#pragma unroll
-            for (uint32_t x = 0; x < NP; ++x)
-            {
-                // a page: 8 scores
-                u4v hi, lo;
-                float e[8];
-#pragma unroll
-                for (uint32_t y = 0; y < 8; ++y)
-                {
-                    e[y] = __builtin_amdgcn_exp2f(__fmaf_rn(s[x >> 1][8u * (x & 1u) + y], c, down));
-                    l += e[y];
-                }
-#pragma unroll
-                for (uint32_t y = 0; y < 4; ++y)
-                {
-                    hi[y] = win_pack<OPURE_A_F16>(e[2 * y], e[2 * y + 1]);
-                    if constexpr (REST)
-                        lo[y] = win_pack<OPURE_A_F16>(__fsub_rn(e[2 * y], win_low<OPURE_A_F16>(hi[y])), __fsub_rn(e[2 * y + 1], win_high<OPURE_A_F16>(hi[y])));
-                }
-#pragma unroll
-                for (uint32_t g = 0; g < NG; ++g)
-                {
-                    const u4v v = v_at(stage, x, g)[lane];
-                    if constexpr (REST) o[g] = mfma_32(v, lo, o[g]);
-                    o[g] = mfma_32(v, hi, o[g]);
-                }
+                if (x + 1u < NP && g < 4u) weigh(x + 1u, g);
+                apart();
             }
         }
-        if (more) store(i + 1u);
+        if constexpr (SPLIT)
+        {
+            if (i + 1u < last) store(i + 1u);
+        }
         __syncthreads();
     }
     settle();
