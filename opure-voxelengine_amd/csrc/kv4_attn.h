@@ -254,7 +254,7 @@ __device__ inline void kv4_row(const WinParams& p, const float* qs, uint32_t b, 
 // part of sequence b has slot w + b: going on to the next part is going on to the next
 // piece or to the next sequence.
 //   32 sequences of 1,024 to 16,384 positions (8 KV heads of 128): a sixth of each
-// sequence a workgroup 68 us, pieces that end with their sequence 62 to 65.
+// sequence a workgroup 68 us, pieces that end with their sequence 62 to 65, these 53 to 56.
 struct Share {
     uint32_t size, total;                                  // tiles of a piece, of all
     uint32_t b, before;                                    // a sequence, tiles before it

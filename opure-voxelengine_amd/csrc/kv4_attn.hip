@@ -18,6 +18,12 @@ namespace {
 // parts by k_kv4_join.
 //   PIECES: of one size over all sequences, where they are long; else a workgroup has a
 // part of one sequence, as many of each.
+//   Bound by memory and, close behind, the vector unit (3 instructions a pair of codes, the
+// softmax; half of the clocks): 32 sequences of 1,024 to 16,384 positions, 8 KV heads of 128,
+// 232 MB in 53 us with the join, 4.4 TB/s (49 us this kernel, 4.7 TB/s, a large copy's rate).
+// A single sequence of 2,000 is launches and round trips, 4.4 and 3.3 us.  Three waves a SIMD
+// at up to 128 channels, which have 168 registers each (a form that spilled some took 66 us for
+// 57), one past that.
 template <int AF, int HD, int NT, bool ONCE, bool PIECES>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 2 ? 2 : HD > 128 ? 1 : AF == OPURE_A_F32 ? 2 : 3))) void k_kv4_split(WinParams p)
 {

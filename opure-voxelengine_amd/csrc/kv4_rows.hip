@@ -27,7 +27,20 @@ constexpr uint32_t rows_lds() { return 2u * rows_stage<HD>(); }
 // and O^T = V^T P^T.  A lane (q = lane % 32, h = lane / 32) holds of a page's scores the
 // tokens 4 h .. 4 h + 3 and 8 + 4 h .. 11 + 4 h of row q, its operand P^T, and V of a
 // page lies in LDS in that order of tokens.  Two stages: while one tile is computed the
-// next one's words are on their way.
+// next one's values are made, each group's conversions between two products of K, and
+// the words of the one after are on their way; a page's weights are made between the
+// products of the page before, its values read a page ahead.  Left to itself the compiler
+// takes few registers and waits for LDS before every product.
+//   A tile that none of a wave's rows sees is computed all the same (two of a block's at
+// most): with a branch round it and this order the outputs are copied twice a tile, 128
+// moves beside 300 instructions, and 148 registers spill.
+//   2,048 rows of 32 heads over 6,000 positions and themselves (8 KV heads of 128, bf16):
+// 277 to 285 us by the device, 825 to 850 TFLOP/s of the 1,250 that a product of 8,192
+// squared reaches; 291 to 298 in the compiler's order, 483 where each wave makes its own
+// values.  Bound by the matrix units (44% of the clocks), the vector unit (63%) and LDS, of
+// which products of 32 rows a wave read 56 bytes a clock of 128.  Two pages past 128
+// channels, with a wave a SIMD and 512 registers, where the compiler's order is the better
+// one (256 channels, 2,048 rows of 16 heads: 115 us, in this order 124).
 template <int AF, int HD>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 128 ? 2 : 1))) void k_kv4_rows(WinParams p)
 {
