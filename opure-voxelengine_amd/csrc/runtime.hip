@@ -52,7 +52,7 @@ int ensure_workspace(opure_dev* dev, uint64_t bytes)
     {
         OPURE_REQUIRE(!dev->capturing, OPURE_E_CAPACITY,
                       "workspace too small during graph capture (%llu < %llu bytes): call "
-                      "opure_verify_reserve (opure_attn_window_reserve) before capturing", (unsigned long long)dev->ws_bytes,
+                      "opure_verify_reserve (opure_attn_window_reserve, opure_attn_kv4_reserve, opure_logprobs_reserve) before capturing", (unsigned long long)dev->ws_bytes,
                       (unsigned long long)bytes);
         OPURE_HIP_TRY(hipStreamSynchronize(dev->stream));
         void* ws = nullptr;
