@@ -392,7 +392,8 @@ struct Kv4Wave {
         r = lane & 15u;
         pt = p.page_table + static_cast<uint64_t>(b) * p.max_pages;
         sq = win_seq(p, p.seq_len[b]);
-        span = seq_span(p, sq);
+        // what the block's rows see (of all rows: 859 of 8 heads of 192 behind a window of 96 34.7 us, so 18.3)
+        span = win_span<TT>(p, sq, sq.ctx + j0, sq.ctx + j1 + 1u);
     }
     // tiles first .. end - 1 of the list, the wave's from `mine` on
     __device__ __forceinline__ void start(uint32_t b, uint32_t mine, uint32_t end)

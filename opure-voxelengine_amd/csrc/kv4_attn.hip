@@ -298,14 +298,15 @@ int kv4_plan(opure_dev* dev, const opure_attn_kv4_args* a, Kv4Plan& w)
 {
     const opure_model* m = a->model;
     const uint32_t Gq = m->n_heads / m->n_kv_heads * a->rows;
-    // tiles of any block of rows: its sinks', then the window's and the rows', which begin anywhere in a tile
-    const uint64_t all = (a->max_ctx + 31u) / 32u, window = a->window ? a->window : 0x7FFFFFFFu;
-    w.tiles = static_cast<uint32_t>(std::min<uint64_t>(all, (a->sinks + 31ull) / 32u + (window + a->rows + 30ull) / 32u + 1u));
     const uint64_t heads = static_cast<uint64_t>(a->batch) * m->n_kv_heads, rows = heads * Gq;
     const uint64_t cu = dev->n_cu > 0 ? static_cast<uint32_t>(dev->n_cu) : 256u;
     w.two = Gq > 16u && m->head_dim <= 128u;
     w.blocks = (Gq + (w.two ? 31u : 15u)) / (w.two ? 32u : 16u);
     w.block_rows = std::min(Gq, w.two ? 32u : 16u);
+    // tiles of any block of rows: its sinks', then the window's and the rows', which begin anywhere in a tile
+    const uint32_t G = m->n_heads / m->n_kv_heads, seen = std::min(a->rows, (w.block_rows + G - 2u) / G + 1u);
+    const uint64_t all = (a->max_ctx + 31u) / 32u, window = a->window ? a->window : 0x7FFFFFFFu;
+    w.tiles = static_cast<uint32_t>(std::min<uint64_t>(all, (a->sinks + 31ull) / 32u + (window + seen + 30ull) / 32u + 1u));
     const uint64_t groups = heads * w.blocks;
     kv4_choose(a, Gq, cu, w);
     if (w.many)
