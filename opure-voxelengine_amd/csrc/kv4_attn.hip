@@ -274,9 +274,10 @@ int kv4_slots(const opure_attn_kv4_args* a, uint64_t slots, uint64_t wgs, uint64
 //     0.4 + channels / 85 (blocks of 32 rows 1.75; 16 waves 2.2; fp32 past 192 channels, whose waves are a few registers
 //     short, half as much again: 256 channels over 300 positions in 12 sequences 16.4, split 11.9), times the workgroups a CU;
 //   k_kv4_split + k_kv4_join: 7.2 + channels / 100 and 0.06 a query row, 0.9 ns a tile, block of rows and 100 channels
-//     (1.6 of 32 rows).
+//     (1.6 of 32 rows), and for the join 0.33 ns a query row.  Tiles are the blocks' mean.
 // Measured, one / split: one row of 64 channels over 300 positions 6.0 / 8.2, 700 7.3 / 7.8, 2,000 13.4 / 7.8; of 128 over
-// 300 7.1 / 8.3, 700 10.5 / 9.0; 32 sequences of 1,000 positions 10.0 / 13.7 (64 channels), 14.8 / 17.5 (128).
+// 300 7.1 / 8.3, 700 10.5 / 9.0; 32 sequences of 1,000 positions 10.0 / 13.7 (64 channels), 14.8 / 17.5 (128); 410 rows
+// of 64 heads of 16 over themselves 13.2 / 21.8.
 //   k_kv4_rows makes a tile's values once for 128 query rows, but is four waves where the others are many: from 12,000 tiles
 // and blocks of 32 rows of 64 query rows or more on, past 128 channels, where its waves have a SIMD each, of 1,024.  Rows /
 // split: 256 query rows of 8 KV heads of 128 channels over 500 positions 15.9 / 11.9, over 8,000 35.1 / 41.0; 64 over 8,000
@@ -288,8 +289,10 @@ void kv4_choose(const opure_attn_kv4_args* a, uint32_t Gq, uint64_t cu, Kv4Plan&
     const uint32_t waves = kv4_one_waves(a->model->head_dim, w.two);
     const double wide = a->model->afmt == OPURE_A_F32 && hd > 192.0 ? 1.5 : 1.0;
     const double turn = w.two ? 1.75 : waves == 16u ? 2.2 : wide * (0.4 + hd / 85.0), rows = std::min(Gq, 32u);
-    const double one = 4.7 + hd / 150.0 + 0.05 * rows + w.tiles * turn / waves * std::max(1.0, groups / static_cast<double>(cu));
-    const double split = 7.2 + hd / 100.0 + 0.06 * rows + groups * w.tiles * hd * (w.two ? 1.6e-5 : 0.9e-5);
+    // tiles of a block: a prompt's first ones see less
+    const double mean = std::min<double>(w.tiles, (a->max_ctx - a->rows / 2u) / 32u + 1u);
+    const double one = 4.7 + hd / 150.0 + 0.05 * rows + turn / waves * std::max<double>(w.tiles, mean * groups / static_cast<double>(cu));
+    const double split = 7.2 + hd / 100.0 + 0.06 * rows + groups * mean * hd * (w.two ? 1.6e-5 : 0.9e-5) + 3.3e-4 * heads * Gq;
     // (past 64 tiles a long sequence among short ones is what such a call waits for)
     w.one = !w.many && w.tiles <= 64u && one < split;
 }
@@ -313,7 +316,10 @@ int kv4_plan(opure_dev* dev, const opure_attn_kv4_args* a, Kv4Plan& w)
     {
         w.blocks = (Gq + ROWS_BLOCK - 1u) / ROWS_BLOCK;
         w.block_rows = std::min(Gq, ROWS_BLOCK);
-        w.parts = static_cast<uint32_t>(std::min<uint64_t>(std::max<uint64_t>(1u, 2u * cu / (heads * w.blocks)), std::min((w.tiles + 7u) / 8u, MAX_PARTS)));
+        // Two workgroups a CU; but one part, and no join, where a short walk takes half the CUs as it is (779 rows of 24 heads of
+        // 112 over themselves 24.2 us, in three parts 30.4; 1,500 of 16 of 192 over 1,000 and themselves 167 and 131)
+        const uint64_t fill = 2u * heads * w.blocks >= cu && w.tiles <= 32u ? 1u : std::max<uint64_t>(1u, 2u * cu / (heads * w.blocks));
+        w.parts = static_cast<uint32_t>(std::min<uint64_t>(fill, std::min((w.tiles + 7u) / 8u, MAX_PARTS)));
         const uint64_t wgs = heads * w.blocks * w.parts;
         return kv4_slots(a, w.parts == 1u ? 0u : wgs, wgs, rows, w);
     }
