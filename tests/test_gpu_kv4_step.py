@@ -271,3 +271,47 @@ def test_two_handles_at_once(dev):
         s.check(s.pool0, *call[1:])
         s.free()
     second.close()
+
+
+def test_workspace_grows_behind_a_graph(dev):
+    """A larger call is refused in a capture that has too little workspace, which goes on; run eagerly it replaces
+    the workspace, and the graph's calls keep theirs."""
+    own = H.Dev(0)
+    rng = np.random.default_rng(6)
+    calls = []
+    for batch, rows, n in ((1, 1, 2000), (6, 4, 2500)):     # both in parts, which are joined from the workspace
+        cache = K.Kv4Cache(rng, 1, KV, HD, [n] * batch)
+        q = rng.standard_normal((batch, rows, HEADS, HD), dtype=np.float32)
+        c = K.Call(own, cache, q, H.A_F32, HEADS, [n - rows] * batch, rows, 0, 0, 0.1)
+        calls.append((c, *K.attention(cache, 0, q, H.A_F32, HEADS, [n - rows] * batch, rows, 0, 0, 0.1)))
+    (small, *want), (big, *want_big) = calls
+    H.check(H.lib().opure_attn_kv4_reserve(own.h, C.byref(small.args)))
+    own.graph_begin()
+    small.run(sync=False)
+    assert H.lib().opure_attn_kv4_paged(own.h, C.byref(big.args)) == H.E_CAPACITY
+    g = own.graph_end()
+    for _ in range(3):
+        own.graph_launch(g)
+        P.compare(big.run().result(), *want_big)
+        P.compare(small.result(), *want)
+        own.fill_u32(small.out, 0x7FC00000, HEADS * HD)
+    own.graph_destroy(g)
+    P.compare(small.run().result(), *want)
+    small.free()
+    big.free()
+    own.close()
+
+
+@pytest.mark.parametrize("rows", [1, 9, 40])
+def test_sequences_that_share_pages(dev, rows):
+    """One cache read through three rows of the page table, its pages in the same places: the same bits in each."""
+    rng = np.random.default_rng(rows)
+    cache = K.Kv4Cache(rng, 1, KV, HD, [900 + rows] * 3)
+    cache.table[1:] = cache.table[0]
+    q = np.repeat(rng.standard_normal((1, rows, HEADS, HD), dtype=np.float32), 3, 0)
+    c = K.Call(dev, cache, q, H.A_F32, HEADS, [900] * 3, rows, 0, 0, 0.1)
+    got = c.run().result()
+    assert np.array_equal(got[0], got[1]) and np.array_equal(got[0], got[2])
+    ref, tol = K.attention(cache, 0, q, H.A_F32, HEADS, [900] * 3, rows, 0, 0, 0.1)
+    assert (np.abs(got - ref) <= tol).all()
+    c.free()
