@@ -116,11 +116,13 @@ struct Stats {
     bool bad;
 };
 
-// f (S and E) to a maximum m2 >= m
+constexpr float LEAST = -1e30f;                      // of y - m: e^(y - m) is 0 long before, and 2^24 of them have a finite sum
+
+// f (S and E) to a maximum m2 >= m.  Logits that a mask has at the type's lowest value are such a step below.
 __device__ __forceinline__ void rebase(Stats& a, float m2)
 {
     const bool none = a.m == NEG_INF;
-    const float d = none ? 0.0f : __fsub_rn(a.m, m2), f = __builtin_amdgcn_exp2f(__fmul_rn(d, 1.44269504088896340736f));
+    const float d = none ? 0.0f : fmaxf(__fsub_rn(a.m, m2), LEAST), f = __builtin_amdgcn_exp2f(__fmul_rn(d, 1.44269504088896340736f));
     a.e = __fmul_rn(__fmaf_rn(a.s, d, a.e), f);
     a.s = __fmul_rn(a.s, f);
     a.m = m2;
@@ -256,7 +258,7 @@ __global__ __launch_bounds__(256) void k_logprobs(LogprobParams p)
         for (uint32_t i = 0; i < PER; ++i)
         {
             // of a masked logit e is 0 and d finite
-            const float d = fmaxf(__fsub_rn(v[i], ms), -1e30f), e = __builtin_amdgcn_exp2f(__fmul_rn(d, 1.44269504088896340736f));
+            const float d = fmaxf(__fsub_rn(v[i], ms), LEAST), e = __builtin_amdgcn_exp2f(__fmul_rn(d, 1.44269504088896340736f));
             a.s += e;
             a.e = __fmaf_rn(e, d, a.e);
         }
