@@ -2,11 +2,13 @@
 //  logprobs.hip -- log probabilities of given tokens, the entropy and the most
 //  probable tokens of rows of logits.
 //
-//  With y = x / temperature, m = max y, S = sum e^(y - m), E = sum e^(y - m) (y - m):
-//    log p(t) = (y_t - m) - log S,   entropy = log S - E / S
-//  (both terms of the entropy are positive: nothing cancels).  One pass: a lane
-//  holds m, S and E of what it has read; past a new maximum m',
-//    S' = S f,  E' = (E + S (m - m')) f,  f = e^(m - m').
+//  With m = max x, d = (x - m) / temperature, S = sum e^d, E = sum e^d d:
+//    log p(t) = d_t - log S,   entropy = log S - E / S
+//  (both terms of the entropy are positive: nothing cancels).  x / temperature itself
+//  may pass fp32's numbers below a temperature of 1, of a row's largest or of all of a
+//  row that a mask has at the type's lowest value.  One pass: a lane
+//  holds m, S and E of what it has read; past a new maximum m', c = (m - m') / temperature,
+//    S' = S f,  E' = (E + S c) f,  f = e^c.
 //  The largest logits go by a 64-bit key, the value's bits in order above the
 //  index's complement, so no two are equal and ties fall to the lowest index.
 // ============================================================================
@@ -116,21 +118,23 @@ struct Stats {
     bool bad;
 };
 
-constexpr float LEAST = -1e30f;                      // of y - m: e^(y - m) is 0 long before, and 2^24 of them have a finite sum
+constexpr float LEAST = -1e30f;                      // of d: e^d is 0 long before, and 2^24 of them have a finite sum
+
+__device__ __forceinline__ float over(float d, float tau) { return __builtin_expect(tau == 1.0f, 1) ? d : __fdiv_rn(d, tau); }
 
 // f (S and E) to a maximum m2 >= m.  Logits that a mask has at the type's lowest value are such a step below.
-__device__ __forceinline__ void rebase(Stats& a, float m2)
+__device__ __forceinline__ void rebase(Stats& a, float m2, float tau)
 {
     const bool none = a.m == NEG_INF;
-    const float d = none ? 0.0f : fmaxf(__fsub_rn(a.m, m2), LEAST), f = __builtin_amdgcn_exp2f(__fmul_rn(d, 1.44269504088896340736f));
+    const float d = none ? 0.0f : fmaxf(over(__fsub_rn(a.m, m2), tau), LEAST), f = __builtin_amdgcn_exp2f(__fmul_rn(d, 1.44269504088896340736f));
     a.e = __fmul_rn(__fmaf_rn(a.s, d, a.e), f);
     a.s = __fmul_rn(a.s, f);
     a.m = m2;
 }
 
-__device__ __forceinline__ Stats wave_stats(Stats a)
+__device__ __forceinline__ Stats wave_stats(Stats a, float tau)
 {
-    rebase(a, wave_max64(a.m));
+    rebase(a, wave_max64(a.m), tau);
     a.s = wave_sum64(a.s);
     a.e = wave_sum64(a.e);
     a.bad = __any(a.bad);
@@ -157,7 +161,8 @@ __device__ __forceinline__ void finish(const LogprobParams& p, uint32_t row, Sta
     const float nan = __builtin_nanf("");
     const bool bad = a.bad || a.s == 0.0f;
     const float norm = logf(a.s);
-    auto of = [&](float x) { return bad ? nan : __fsub_rn(__fsub_rn(p.temperature == 1.0f ? x : __fdiv_rn(x, p.temperature), a.m), norm); };
+    // of halves: a temperature brings a difference past fp32's numbers back
+    auto of = [&](float x) { return bad ? nan : __fmaf_rn(2.0f, over(__fsub_rn(__fmul_rn(0.5f, x), __fmul_rn(0.5f, a.m)), p.temperature), -norm); };
     if (lane == 0u && p.entropy) p.entropy[row] = bad ? nan : __fsub_rn(norm, __fdiv_rn(a.e, a.s));
     if (lane == 0u && p.logprob)
     {
@@ -240,20 +245,15 @@ __global__ __launch_bounds__(256) void k_logprobs(LogprobParams p)
                 if (nan) most = __builtin_nanf("");
             }
         }
-        if (tau != 1.0f)
-        {
-            m = NEG_INF;
-#pragma unroll
-            for (uint32_t i = 0; i < PER; ++i)
-            {
-                v[i] = __fdiv_rn(v[i], tau);
-                bad = bad || !(v[i] < __builtin_huge_valf());
-                m = fmaxf(m, v[i]);
-            }
-        }
         a.bad = a.bad || bad;
-        if (m > a.m) rebase(a, m);
-        const float ms = a.m == NEG_INF ? 0.0f : a.m;
+        if (m > a.m) rebase(a, m, tau);
+        float ms = a.m == NEG_INF ? 0.0f : a.m;
+        if (__builtin_expect(tau != 1.0f, 0))
+        {
+#pragma unroll
+            for (uint32_t i = 0; i < PER; ++i) v[i] = __fdiv_rn(__fsub_rn(v[i], ms), tau);
+            ms = 0.0f;
+        }
 #pragma unroll
         for (uint32_t i = 0; i < PER; ++i)
         {
@@ -311,12 +311,12 @@ __global__ __launch_bounds__(256) void k_logprobs(LogprobParams p)
         __builtin_amdgcn_wave_barrier();
         queue[wave][lane] = best;
     }
-    a = wave_stats(a);
+    a = wave_stats(a, tau);
     if (lane == 0u) part[wave] = float4{a.m, a.s, a.e, a.bad ? 1.0f : 0.0f};
     __syncthreads();
     if (wave != 0u) return;
     const float4 mine = part[lane & 3u];
-    a = wave_stats(Stats{lane < 4u ? mine.x : NEG_INF, lane < 4u ? mine.y : 0.0f, lane < 4u ? mine.z : 0.0f, lane < 4u && mine.w != 0.0f});
+    a = wave_stats(Stats{lane < 4u ? mine.x : NEG_INF, lane < 4u ? mine.y : 0.0f, lane < 4u ? mine.z : 0.0f, lane < 4u && mine.w != 0.0f}, tau);
     if constexpr (TOP)
 #pragma unroll 1
         for (uint32_t w = 1; w < 4; ++w) best = wave_merge(best, queue[w][63u - lane]);
@@ -373,7 +373,7 @@ __global__ __launch_bounds__(64 * W) void k_logprobs_join(LogprobParams p)
     }
     if (wave != 0u) return;
     const bool in = lane < p.slices;
-    finish(p, row, wave_stats(Stats{in ? mine.x : NEG_INF, in ? mine.y : 0.0f, in ? mine.z : 0.0f, in && mine.w != 0.0f}), best, given);
+    finish(p, row, wave_stats(Stats{in ? mine.x : NEG_INF, in ? mine.y : 0.0f, in ? mine.z : 0.0f, in && mine.w != 0.0f}, p.temperature), best, given);
 }
 
 // A row in as many slices as give each CU four workgroups.

@@ -21,19 +21,16 @@ def dev():
 
 
 def reference(x, tokens, top, temperature):
-    """(log p of tokens, entropy, top tokens, theirs) in 64 bits, and bounds of the errors.  Logits over a temperature
-    of 1 or more are rounded quotients y, below 1 the difference x - m is what is divided: y - m is off by 2 u |y - m| and,
-    over 1, by the two roundings of y and m (none where they are equal).  Each e^(y - m) is relatively off by that, by u |y - m|
-    for its argument's product and by 2^-21 (the hardware's exponential); a term below 2^-126 may be lost.  Sums of
+    """(log p of tokens, entropy, top tokens, theirs) in 64 bits, and bounds of the errors.  With d = (x - m) /
+    temperature, off by 2 u |d|, each e^d is relatively off by that, by u |d| for its argument's product and by 2^-21 (the
+    hardware's exponential); a term below 2^-126 may be lost.  Sums of
     positive terms are off by 2^-24 times the longest chain: a lane's share of the vocabulary and 64 joins."""
     x = x.astype(np.float64)
-    y = x / temperature
-    m = y.max(1, keepdims=True)
-    d = y - m
+    d = (x - x.max(1, keepdims=True)) / temperature
     e = np.exp(d)
     s = e.sum(1)
     chain = (-(-x.shape[1] // 256) + 16 + 64) * U
-    off = 2 * U * np.abs(d) + (np.where(d == 0, 0, U * (np.abs(y) + np.abs(m))) if temperature > 1 else 0)
+    off = 2 * U * np.abs(d)
     de = off + U * np.abs(d) + 2.0 ** -21
     count = e > 0
     rel = np.where(count, e * de, 0).sum(1) / s + chain
@@ -102,3 +99,28 @@ def test_fills_mixed(dev):
         x[5] = np.sort(x[5])[::-1]
         got = check(dev, x, 20)
         assert np.isfinite(got[1]).all()
+
+
+@pytest.mark.parametrize("temperature", [0.05, 0.7, 0.999, 1.9, 60.0])
+@pytest.mark.parametrize("rows,vocab", [(9, 700), (4, 9000), (1, 128256), (530, 6001)])
+def test_low_fills_over_a_temperature(dev, rows, vocab, temperature):
+    """A logit's quotient by the temperature may pass fp32's numbers where the differences that count do not."""
+    say("temperature", rows, vocab, temperature)
+    rng = np.random.default_rng(vocab)
+    for fill, left in ((LOWEST, 0.05), (-3e38, 0.3), (-1e38, 0.001), (-1e30, 0.01)):
+        got = check(dev, masked(rng, rows, vocab, np.float32(fill), left), 20, temperature)
+        assert np.isfinite(got[1]).all()
+
+
+@pytest.mark.parametrize("temperature", [0.05, 0.7, 1.0, 1.9, 60.0])
+def test_rows_of_one_size(dev, temperature):
+    """Nothing but masked logits: as likely as each other; and logits near fp32's largest."""
+    say("rows", temperature)
+    for vocab in (1, 700, 9000, 128256):
+        x = np.full((3, vocab), LOWEST, np.float32)
+        x[1], x[2] = -LOWEST, -1e38
+        got = check(dev, x, min(vocab, 20), temperature, tokens=[0, vocab - 1, vocab // 2])
+        assert np.allclose(got[1], np.log(vocab), rtol=1e-5)
+    x = np.full((2, 9000), 3e38, np.float32)
+    x[0, 8000], x[1, :5000] = 3.2e38, LOWEST
+    check(dev, x, 20, temperature)
