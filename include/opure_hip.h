@@ -370,8 +370,10 @@ int opure_kv_pool_bytes(const opure_model* model, uint32_t kvfmt, uint32_t n_pag
  *      maxima and sums are fp32.  A query row enters as fp16 numbers of a power of
  *      two of it (fp32 rows as two each, 22 bits), a softmax weight as one fp16
  *      number (bf16 models) or two (its rounding and the rest, 22 bits), in steps of no
- *      less than 2^-36 of the row's largest.  The same call gives the same bits; a row
- *      alone and in a batch may differ in its last ones.
+ *      less than 2^-36 of the row's largest.  Scores may be as large as fp32 holds; a
+ *      row whose largest passes 2^22 ln 2 either way is computed position by position,
+ *      which is slow.  The same call gives the same bits; a row alone and in a batch
+ *      may differ in its last ones.
  *        opure_kv_rollback without poison and the page tables work on such a cache as
  *      on any other; opure_verify_step, opure_prompt_step, the other attention calls
  *      and opure_kv_evict read a cache in the model's format. */

@@ -13,9 +13,23 @@ using namespace opure_win;
 
 constexpr uint32_t MAX_PARTS = 64;                         // of a (sequence, KV head, block of query rows): a lane of the joining wave each
 constexpr float LOG2E = 1.44269504088896340736f;
-// A row's output is scaled to a new maximum only where that passes the old one by 2^LAG.  Weights are held times
-// 2^SHIFT, so the largest of 2^15 is still in fp16, and what fp16 loses at its small end lies 2^36 below 1.
-constexpr float SHIFT = 12.0f, LAG = 3.0f;
+// With the products s of a row and c = scale log2 e, weights are 2^(s c - M) by one fused multiply-add, M the largest
+// s c rounded down to a whole number: M, what it is told apart by and 2^(M - M') are exact, so a weight is off by its
+// exponent's own rounding alone, however large the scores.  (With M = m c rounded, the rounding, 2^5 at 2^29, stood in
+// every weight's exponent.)  A row is scaled to a new M only where s c passes the old one by LAG.  Weights are held
+// times 2^SHIFT, so the largest of 2^15 is still in fp16, and what fp16 loses at its small end lies 2^36 below 1.  Past
+// FAR, where SHIFT - M would be rounded in the end, a row's sum is NaN, and it is computed position by position.
+constexpr float SHIFT = 12.0f, LAG = 3.0f, FAR = 0x1p22f;
+__device__ __forceinline__ bool has_grown(float m, float mx, float c) { return m == NEG_INF ? mx > NEG_INF : __fmaf_rn(mx, c, -m) > LAG; }
+// m, and the row's sum l, to a new maximum mx where it has grown; returns the factor of what is there already
+__device__ __forceinline__ float grow(bool grown, float mx, float c, float& m, float& l)
+{
+    const float to = grown ? __builtin_floorf(__fmul_rn(mx, c)) : m, a = m == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(__fsub_rn(m, to));
+    m = to;
+    // a NaN whose bits an instruction has room for: another one takes two registers, and a workgroup a CU of three kernels (96 channels 8.3 us, so 10.6)
+    l = grown && !(__builtin_fabsf(to) <= FAR) ? __uint_as_float(0xFFFFFFFFu) : __fmul_rn(l, a);
+    return a;
+}
 
 typedef u4v u4a __attribute__((aligned(4)));
 typedef uint32_t u2v __attribute__((ext_vector_type(2)));
@@ -364,7 +378,7 @@ struct Kv4Wave {
     float c[NT];
     int32_t e = -1, pa = -1, pb = -1;
     T tl;
-    // a row's maximum in units of the products, this lane's share of its sum, its output
+    // a row's M, this lane's share of its sum, its output
     f4_t o[DT][NT];
     float m[NT], l[NT];
 
@@ -485,18 +499,16 @@ struct Kv4Wave {
                     mx = largest();
                 }
                 mx = max_xor32(max_xor16(mx));
-                const bool grown = m[n] == NEG_INF ? mx > NEG_INF : __fmul_rn(__fsub_rn(mx, m[n]), c[n]) > LAG;
+                const bool grown = has_grown(m[n], mx, c[n]);
                 if (__any(grown))
                 {
-                    const float to = grown ? mx : m[n], a = m[n] == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(__fmul_rn(__fsub_rn(m[n], to), c[n]));
-                    m[n] = to;
-                    l[n] = __fmul_rn(l[n], a);
+                    const float a = grow(grown, mx, c[n], m[n], l[n]);
 #pragma unroll
                     for (uint32_t d = 0; d < DT; ++d)
 #pragma unroll
                         for (uint32_t y = 0; y < 4; ++y) o[d][n][y] = __fmul_rn(o[d][n][y], a);
                 }
-                const float down = m[n] == NEG_INF ? 0.0f : __fsub_rn(SHIFT, __fmul_rn(m[n], c[n]));
+                const float down = m[n] == NEG_INF ? 0.0f : __fsub_rn(SHIFT, m[n]);
 #pragma unroll
                 for (uint32_t y = 0; y < 8; ++y)
                 {
@@ -542,7 +554,7 @@ struct Kv4Wave {
         }
         settle();
     }
-    // to LDS for the workgroup's merge: acc [wave][DT][NT][64], ml [wave][NT][16][2], maxima in powers of two
+    // to LDS for the workgroup's merge: acc [wave][DT][NT][64], ml [wave][NT][16][2]
     __device__ __forceinline__ void leave(uint32_t wave, f4_t* acc, float* ml)
     {
 #pragma unroll
@@ -553,7 +565,7 @@ struct Kv4Wave {
             for (uint32_t d = 0; d < DT; ++d) acc[((wave * DT + d) * NT + n) * 64u + lane] = o[d][n];
             if (g == 0u)
             {
-                ml[((wave * NT + n) * 16u + r) * 2u] = m[n] == NEG_INF ? NEG_INF : __fmul_rn(m[n], c[n]);
+                ml[((wave * NT + n) * 16u + r) * 2u] = m[n];
                 ml[((wave * NT + n) * 16u + r) * 2u + 1u] = l[n];
             }
         }

@@ -128,7 +128,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 128 ?
         if constexpr (!SPLIT) __builtin_amdgcn_sched_barrier(0);
     };
     f16_t o[NG];
-    float m = NEG_INF, l = 0.0f;                            // the maximum in units of the products; this lane's share of the sum
+    float m = NEG_INF, l = 0.0f;                            // the row's M; this lane's share of the sum
 #pragma unroll
     for (uint32_t g = 0; g < NG; ++g)
 #pragma unroll
@@ -208,18 +208,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 128 ?
             mx = largest();
         }
         mx = max_xor32(mx);
-        const bool grown = m == NEG_INF ? mx > NEG_INF : __fmul_rn(__fsub_rn(mx, m), c) > LAG;
+        const bool grown = has_grown(m, mx, c);
         if (__any(grown))
         {
-            const float to = grown ? mx : m, a = m == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(__fmul_rn(__fsub_rn(m, to), c));
-            m = to;
-            l = __fmul_rn(l, a);
+            const float a = grow(grown, mx, c, m, l);
 #pragma unroll
             for (uint32_t g = 0; g < NG; ++g)
 #pragma unroll
                 for (uint32_t y = 0; y < 16; ++y) o[g][y] = __fmul_rn(o[g][y], a);
         }
-        const float down = m == NEG_INF ? 0.0f : __fsub_rn(SHIFT, __fmul_rn(m, c));
+        const float down = m == NEG_INF ? 0.0f : __fsub_rn(SHIFT, m);
         u4v hi[2], lo[2], v[2][NG];
         auto read_v = [&](uint32_t x) {
 #pragma unroll
@@ -271,8 +269,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(HD <= 128 ?
         if (!there) return;
         if (h == 0u)
         {
-            // the join takes maxima in powers of two
-            p.part_ml[at * 2u] = m == NEG_INF ? NEG_INF : __fmul_rn(m, c);
+            p.part_ml[at * 2u] = m;
             p.part_ml[at * 2u + 1u] = l;
         }
 #pragma unroll
