@@ -257,13 +257,13 @@ struct Kv4Plan {
     uint64_t bytes() const { return acc + ml; }
 };
 
-// workspace of `slots` parts' outputs, and what a launch can have
-int kv4_slots(const opure_attn_kv4_args* a, uint64_t slots, uint64_t wgs, uint64_t rows, Kv4Plan& w)
+// workspace of `slots` parts' outputs, and what a launch of `wgs` workgroups can have
+int kv4_slots(const opure_attn_kv4_args* a, uint64_t slots, uint64_t wgs, uint64_t rows, Kv4Plan& w, uint32_t threads = 256u)
 {
     w.acc = opure_hip::align_up(slots * w.block_rows * a->model->head_dim * 4u, 256);
     w.ml = opure_hip::align_up(slots * w.block_rows * 8u, 256);
-    // a launch's threads, 256 a workgroup (the join's: a row at most), stay in 32 bits
-    OPURE_REQUIRE(std::max(wgs, rows) < 1u << 24, OPURE_E_CAPACITY, "4-bit attention: %u x %u rows of %u heads over max_ctx %u: too many workgroups",
+    // a launch's threads stay in 32 bits (the join's workgroups, of 256, have a row at least)
+    OPURE_REQUIRE(wgs * threads < 1ull << 32 && rows < 1u << 24, OPURE_E_CAPACITY, "4-bit attention: %u x %u rows of %u heads over max_ctx %u: too many workgroups",
                   a->batch, a->rows, a->model->n_heads, a->max_ctx);
     return OPURE_OK;
 }
@@ -326,7 +326,7 @@ int kv4_plan(opure_dev* dev, const opure_attn_kv4_args* a, Kv4Plan& w)
     if (w.one)
     {
         w.parts = 1u;
-        return kv4_slots(a, 0u, groups, rows, w);
+        return kv4_slots(a, 0u, groups, rows, w, 64u * kv4_one_waves(m->head_dim, w.two));
     }
     uint32_t room = 0;
     auto holds = [&](auto, uint32_t, uint32_t n) {
