@@ -697,6 +697,16 @@ int opure_debug_set_rejection_launches(opure_dev* dev, uint32_t mode);
  * lengths and rollback. */
 enum { OPURE_GREEDY_IN_LM_HEAD = 0, OPURE_GREEDY_SEPARATE = 1 };
 int opure_debug_set_greedy_acceptance(opure_dev* dev, uint32_t mode);
+/* Kernels of opure_attn_kv4_paged (and of its reserve): by what each would take
+ * (default), or one of them, so that tests reach each at every shape: a workgroup
+ * for all tiles of a sequence, parts of each sequence and a join, pieces of one
+ * size over all sequences and a join (one block of up to 16 query rows a KV head,
+ * else OPURE_E_UNSUPPORTED at the call), or 128 query rows a workgroup, in one
+ * part or several and a join.  The second call tells which a call takes, and the
+ * parts of a sequence (the pieces of all). */
+enum { OPURE_KV4_BEST = 0, OPURE_KV4_ONE = 1, OPURE_KV4_SPLIT = 2, OPURE_KV4_PIECES = 3, OPURE_KV4_ROWS = 4 };
+int opure_debug_set_kv4_kernels(opure_dev* dev, uint32_t kernels);
+int opure_debug_kv4_kernels(opure_dev* dev, const opure_attn_kv4_args* a, uint32_t* kernels, uint32_t* parts);
 /* Evaluates the SwiGLU epilogue's branch-free exponential and the oracle-order
  * exponential the other kernels use on every one of the 2^32 fp32 bit
  * patterns and counts the results that differ (bit for bit; 0 expected). */

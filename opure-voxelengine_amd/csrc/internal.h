@@ -66,6 +66,8 @@ struct opure_dev {
     uint32_t    wait_limit = 1u << 22;
     // GEMV engine of opure_gemv_batched_i8pc for M <= 8 (opure_debug_set_gemv_engine)
     uint32_t    gemv_engine = OPURE_GEMV_MFMA;
+    // kernels of 4-bit attention (opure_debug_set_kv4_kernels)
+    uint32_t    kv4_kernels = OPURE_KV4_BEST;
     // launches of the rejection step (opure_debug_set_rejection_launches)
     uint32_t    rej_mode = OPURE_REJ_ONE_LAUNCH;
     // captured graphs still alive: a workspace they point into is kept, not

@@ -312,6 +312,14 @@ int kv4_plan(opure_dev* dev, const opure_attn_kv4_args* a, Kv4Plan& w)
     w.tiles = static_cast<uint32_t>(std::min<uint64_t>(all, (a->sinks + 31ull) / 32u + (window + seen + 30ull) / 32u + 1u));
     const uint64_t groups = heads * w.blocks;
     kv4_choose(a, Gq, cu, w);
+    const uint32_t asked = dev->kv4_kernels;
+    if (asked != OPURE_KV4_BEST)
+    {
+        w.many = asked == OPURE_KV4_ROWS;
+        w.one = asked == OPURE_KV4_ONE;
+        OPURE_REQUIRE(asked != OPURE_KV4_PIECES || (w.blocks == 1u && !w.two), OPURE_E_UNSUPPORTED,
+                      "4-bit attention: pieces of one size have up to 16 query rows a KV head, not %u", Gq);
+    }
     if (w.many)
     {
         w.blocks = (Gq + ROWS_BLOCK - 1u) / ROWS_BLOCK;
@@ -333,12 +341,12 @@ int kv4_plan(opure_dev* dev, const opure_attn_kv4_args* a, Kv4Plan& w)
         room = n;
         return OPURE_OK;
     };
-    if (w.blocks == 1u && a->batch > 1u)
+    if (w.blocks == 1u && (a->batch > 1u || asked == OPURE_KV4_PIECES))
     {
         int rc = split_kernel(dev, m->afmt, m->head_dim, w.two, true, true, holds);
         if (rc) return rc;
         const uint64_t hold = std::max<uint64_t>(1u, room / m->n_kv_heads), all = static_cast<uint64_t>(a->batch) * w.tiles;
-        w.pieces = !w.two && all >= 32u * hold;
+        w.pieces = asked == OPURE_KV4_BEST ? !w.two && all >= 32u * hold : asked == OPURE_KV4_PIECES;
         if (w.pieces)
         {
             // the sum of the sequences' tiles stays in 31 bits
@@ -399,6 +407,20 @@ extern "C" int opure_attn_kv4_reserve(opure_dev* dev, const opure_attn_kv4_args*
     Kv4Plan w;
     const int rp = kv4_plan(dev, a, w);
     return rp ? rp : ensure_workspace(dev, w.bytes());
+}
+
+extern "C" int opure_debug_kv4_kernels(opure_dev* dev, const opure_attn_kv4_args* a, uint32_t* kernels, uint32_t* parts)
+{
+    OPURE_REQUIRE(dev && kernels && parts, OPURE_E_INVALID, "opure_debug_kv4_kernels: null argument");
+    const int rc = kv4_validate(a);
+    if (rc) return rc;
+    const DeviceGuard on(dev);
+    Kv4Plan w;
+    const int rp = kv4_plan(dev, a, w);
+    if (rp) return rp;
+    *kernels = w.many ? OPURE_KV4_ROWS : w.one ? OPURE_KV4_ONE : w.pieces ? OPURE_KV4_PIECES : OPURE_KV4_SPLIT;
+    *parts = w.parts;
+    return OPURE_OK;
 }
 
 extern "C" int opure_attn_kv4_paged(opure_dev* dev, const opure_attn_kv4_args* a)

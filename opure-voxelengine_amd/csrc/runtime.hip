@@ -381,6 +381,14 @@ int opure_debug_set_gemv_engine(opure_dev* dev, uint32_t engine)
     return OPURE_OK;
 }
 
+int opure_debug_set_kv4_kernels(opure_dev* dev, uint32_t kernels)
+{
+    OPURE_REQUIRE(dev, OPURE_E_INVALID, "opure_debug_set_kv4_kernels: null device");
+    OPURE_REQUIRE(kernels <= OPURE_KV4_ROWS, OPURE_E_INVALID, "opure_debug_set_kv4_kernels: kernels %u", kernels);
+    dev->kv4_kernels = kernels;
+    return OPURE_OK;
+}
+
 int opure_debug_set_rejection_launches(opure_dev* dev, uint32_t mode)
 {
     OPURE_REQUIRE(dev, OPURE_E_INVALID, "opure_debug_set_rejection_launches: null device");

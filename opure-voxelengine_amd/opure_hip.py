@@ -29,6 +29,7 @@ BW_READ, BW_COPY = 0, 1
 GEMV_MFMA, GEMV_VALU = 0, 1
 REJ_ONE_LAUNCH, REJ_STAGED = 0, 1
 GREEDY_IN_LM_HEAD, GREEDY_SEPARATE = 0, 1
+KV4_BEST, KV4_ONE, KV4_SPLIT, KV4_PIECES, KV4_ROWS = 0, 1, 2, 3, 4
 
 
 class OpureError(RuntimeError):
@@ -212,6 +213,8 @@ def _declare(L):
         "opure_debug_workspace": ([vp, C.POINTER(vp), C.POINTER(u64)], i),
         "opure_debug_set_wait_limit": ([vp, u32], i),
         "opure_debug_set_gemv_engine": ([vp, u32], i),
+        "opure_debug_set_kv4_kernels": ([vp, u32], i),
+        "opure_debug_kv4_kernels": ([vp, C.POINTER(AttnKv4Args), C.POINTER(u32), C.POINTER(u32)], i),
         "opure_debug_set_rejection_launches": ([vp, u32], i),
         "opure_debug_set_greedy_acceptance": ([vp, u32], i),
         "opure_debug_exp_check": ([vp, C.POINTER(u64)], i),
