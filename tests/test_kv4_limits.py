@@ -1,5 +1,6 @@
-"""Calls of 4-bit attention whose launches have too many threads are refused (no kernel
-is launched: the device handle is a block of zeros, which sizing such a call only reads)."""
+"""Calls of 4-bit attention whose launches have too many threads are refused, and kernels that
+are none (no kernel is launched: the device handle is a block of zeros, which sizing such a
+call only reads)."""
 import ctypes as C
 
 import pytest
@@ -23,3 +24,14 @@ def test_threads_of_one_launch(heads, hd, batch, fits):
     assert (rc == H.E_CAPACITY) != fits                     # one that fits goes on to ask the device for its workspace
     if not fits:
         assert b"workgroups" in H.lib().opure_last_error()
+
+
+def test_kernels_that_are_none():
+    L, zeros, n = H.lib(), C.create_string_buffer(8192), C.c_uint32()
+    dev = (C.addressof(zeros) + 255) // 256 * 256
+    assert L.opure_debug_set_kv4_kernels(None, H.KV4_ONE) == H.E_INVALID
+    assert L.opure_debug_set_kv4_kernels(dev, H.KV4_ROWS + 1) == H.E_INVALID
+    a = H.AttnKv4Args()
+    for args in ((None, C.byref(a), C.byref(n), C.byref(n)), (dev, None, C.byref(n), C.byref(n)), (dev, C.byref(a), None, C.byref(n)), (dev, C.byref(a), C.byref(n), None),
+                 (dev, C.byref(a), C.byref(n), C.byref(n))):
+        assert L.opure_debug_kv4_kernels(*args) == H.E_INVALID
