@@ -328,8 +328,10 @@ int opure_attn_window_paged(opure_dev* dev, const opure_attn_window_args* a);
  *      straight from fp32.
  *        4 bits (OPURE_KV_I4): of a token's 32 channels scale = fp16((hi - lo) / 15),
  *      base = fp16(lo - 16 scale), codes to the nearest value, so a value is off by
- *      half a scale and base's and the value's roundings to fp16 at most; magnitudes
- *      past 2^14 are held as 2^14; a group with a NaN or an infinity reads NaN.
+ *      half a scale, 15 times the scale's rounding to fp16 (2^-11 of it, 2^-25 where it
+ *      is least) and base's and the value's roundings at most: a group whose range is
+ *      not far above 2^-20 is held in few steps or as its base alone.  Magnitudes past
+ *      2^14 are held as 2^14; a group with a NaN or an infinity reads NaN.
  *        row_count (or NULL: all) gives each sequence's rows that are there, 0 to
  *      `rows` (what lies outside counts as the nearest): the others of a padded
  *      batch are not read and nothing of them is written, q_out's rows included.

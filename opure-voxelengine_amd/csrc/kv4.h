@@ -63,8 +63,9 @@ struct Scale {
         s = round_half(__fmul_rn(__fsub_rn(hi, lo), static_cast<float>(1.0 / 15.0)));
         b = round_half(__fsub_rn(lo, __fmul_rn(16.0f, static_cast<float>(s))));
     }
-    // The group's values to their codes: rint((x - base) / scale - 16).  A product with the scale's reciprocal is off
-    // by 2^-18 at most (t < 32: three roundings of 2^-24 of it each), so it decides but for what lies nearer to the
+    // The group's values to their codes: rint((x - base) / scale - 16).  Where the quotient is 15.5 to 31.5 (past it both
+    // ways clamp) a product with the scale's reciprocal is off from it by the two roundings, 2^-24 of it each, and those
+    // of the two differences, 2^-20 each: under 2^-17 in all.  So it decides but for what lies nearer than 2^-16 to the
     // middle of two codes; there the quotient does (2,874 rows of 16 heads of 64: 12.4 us with quotients alone).
     template <int N>
     __device__ __forceinline__ void codes(float (&x)[N]) const
