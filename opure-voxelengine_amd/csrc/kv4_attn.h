@@ -363,7 +363,9 @@ template <int AF, int HD, int NT, bool ONCE, uint32_t W>
 struct Kv4Wave {
     typedef Kv4Tile<HD, ONCE> T;
     static constexpr uint32_t TT = 32u, DT = HD / 16u, NG = T::NG, QT = AF == OPURE_A_F32 ? 2u : 1u;
-    static constexpr bool REST = AF != OPURE_A_BF16;       // a weight's rounding rest counts: bf16 results are rounded 2^3 more coarsely than a weight
+    // a weight's rounding rest counts: bf16 results are rounded 2^3 more coarsely than a weight (with it their error is 1.66e-3
+    // for 1.67e-3, and a prompt of 2,048 rows over 6,000 takes 357 us for 276, a long batch of single rows 54.7 for 52.6)
+    static constexpr bool REST = AF != OPURE_A_BF16;
     const WinParams& p;
     const Bits bits;
     uint32_t lane, g, r;

@@ -19,11 +19,11 @@ namespace {
 //   PIECES: of one size over all sequences, where they are long; else a workgroup has a
 // part of one sequence, as many of each.
 //   Bound by memory and, close behind, the vector unit (3 instructions a pair of codes, the
-// softmax; half of the clocks): 32 sequences of 1,024 to 16,384 positions, 8 KV heads of 128,
+// softmax; 63% of the clocks): 32 sequences of 1,024 to 16,384 positions, 8 KV heads of 128,
 // 232 MB in 53 us with the join, 4.4 TB/s (49 us this kernel, 4.7 TB/s, a large copy's rate).
 // A single sequence of 2,000 is launches and round trips, 4.4 and 3.3 us.  Three waves a SIMD
 // at up to 128 channels, which have 168 registers each (a form that spilled some took 66 us for
-// 57), one past that.
+// 57), one past that; of fp32 rows, which are two numbers each, two (that batch 57 us).
 template <int AF, int HD, int NT, bool ONCE, bool PIECES>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(NT == 2 ? 2 : HD > 128 ? 1 : AF == OPURE_A_F32 ? 2 : 3))) void k_kv4_split(WinParams p)
 {
@@ -269,7 +269,7 @@ int kv4_slots(const opure_attn_kv4_args* a, uint64_t slots, uint64_t wgs, uint64
 }
 
 // Which kernels take a call, by what each would take (us; measured on 8 KV heads of 64, 80 and 128 channels, 4 of 256,
-// 4 to 32 query rows each, 1 to 32 sequences of 100 to 8,000 positions):
+// 4 to 32 query rows each, 1 to 32 sequences of 100 to 8,000 positions; fp16 and bf16 but where fp32 is named):
 //   k_kv4_one walks a sequence's tiles in one workgroup: 4.7 + channels / 150 and 0.05 a query row, and for each W tiles
 //     0.4 + channels / 85 (blocks of 32 rows 1.75; 16 waves 2.2; fp32 past 192 channels, whose waves are a few registers
 //     short, half as much again: 256 channels over 300 positions in 12 sequences 16.4, split 11.9), times the workgroups a CU;
