@@ -374,8 +374,10 @@ int opure_kv_pool_bytes(const opure_model* model, uint32_t kvfmt, uint32_t n_pag
  *      number (bf16 models) or two (its rounding and the rest, 22 bits), in steps of no
  *      less than 2^-36 of the row's largest.  Scores may be as large as fp32 holds; a
  *      row whose largest passes 2^22 ln 2 either way is computed position by position,
- *      which is slow.  The same call gives the same bits; a row alone and in a batch
- *      may differ in its last ones.
+ *      which is slow, as is one near whose positions values are NaN that it does not see
+ *      (slots that a padded batch's rows past their count reach into: a pool cleared
+ *      before its first use has none).  The same call gives the same bits; a row alone
+ *      and in a batch may differ in its last ones.
  *        opure_kv_rollback without poison and the page tables work on such a cache as
  *      on any other; opure_verify_step, opure_prompt_step, the other attention calls
  *      and opure_kv_evict read a cache in the model's format. */

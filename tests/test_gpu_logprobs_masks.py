@@ -124,3 +124,25 @@ def test_rows_of_one_size(dev, temperature):
     x = np.full((2, 9000), 3e38, np.float32)
     x[0, 8000], x[1, :5000] = 3.2e38, LOWEST
     check(dev, x, 20, temperature)
+
+
+@pytest.mark.parametrize("temperature", [0.3, 2.5])
+def test_numbers_that_are_not_finite_over_a_temperature(dev, temperature):
+    """A NaN, a +inf or nothing but -inf make a row NaN, and no other; -inf among others has probability 0."""
+    say("not finite", temperature)
+    rng = np.random.default_rng(3)
+    for vocab in (700, 9000):
+        x = P.logits(rng, 7, vocab)
+        x[1, vocab - 1], x[2, 5], x[3], x[4, ::2], x[5, :600] = np.nan, np.inf, -np.inf, -np.inf, LOWEST
+        x[6, :600] = -np.inf
+        c = P.Call(dev, x, [0] * 7, 9, float(np.float32(temperature)))
+        got = c.run().result()
+        c.free()
+        assert np.array_equal(np.isnan(got[1]), [False, True, True, True, False, False, False])
+        assert np.array_equal(got[2], np.stack([P.order(r)[:9] for r in x]))
+        fine = [0, 4, 5, 6]
+        finite = np.where(np.isneginf(x), -3e38, x).astype(np.float32)     # -inf as a number of probability 0
+        want, tol = reference(finite[fine], [0] * 4, 9, float(np.float32(temperature)))
+        P.compare(got[1][fine], want[1], tol[1])
+        P.compare(got[3][fine], want[3], tol[3])
+        assert np.isneginf(got[0][[4, 6]]).all() and np.isnan(got[0][[1, 2, 3]]).all()
