@@ -254,14 +254,18 @@ __global__ __launch_bounds__(256) void k_logprobs(LogprobParams p)
             for (uint32_t i = 0; i < PER; ++i) v[i] = __fdiv_rn(__fsub_rn(v[i], ms), tau);
             ms = 0.0f;
         }
+        // a chunk's by themselves: errors of 5.6e-8 on rows of 128,256, of one chain through a lane's 501 logits 2.1e-7
+        float cs = 0.0f, ce = 0.0f;
 #pragma unroll
         for (uint32_t i = 0; i < PER; ++i)
         {
             // of a masked logit e is 0 and d finite
             const float d = fmaxf(__fsub_rn(v[i], ms), LEAST), e = __builtin_amdgcn_exp2f(__fmul_rn(d, 1.44269504088896340736f));
-            a.s += e;
-            a.e = __fmaf_rn(e, d, a.e);
+            cs += e;
+            ce = __fmaf_rn(e, d, ce);
         }
+        a.s += cs;
+        a.e += ce;
         if constexpr (TOP)
             if (look)
             {
